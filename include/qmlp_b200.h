@@ -37,6 +37,8 @@ enum {
 
 /* qmlp::Tensor::Precision, src_cpp/include/qmlp/tensor.h:25-30 */
 enum { QMLP_FLOAT = 0, QMLP_HALF = 1, QMLP_DOUBLE = 2 };
+/* further element types, of the operators on feature rows only (networks, encodings and activations refuse them) */
+enum { QMLP_BFLOAT16 = 3, QMLP_INT32 = 4, QMLP_INT64 = 5 };
 /* qmlp::Tensor::Usage, src_cpp/include/qmlp/tensor.h:35-38 */
 enum { QMLP_INFERENCE = 0, QMLP_GRADIENTS = 1 };
 /* qmlp::FusedNetwork::AdjointMode, src_cpp/include/qmlp/fused_network.h:22-34 */
@@ -325,6 +327,80 @@ QMLP_API int qmlp_trainer_scatter_levels(qmlp_trainer_t* tr, int max_levels, int
 /* Adam over the fused buffer (gradient scaled by grad_scale first, e.g. 1 for a summed all-reduce of gradients
  * already normalised by global_points), refresh of the half copy, gradient buffer zeroed. step is 1-based. */
 QMLP_API int qmlp_trainer_update(qmlp_trainer_t* tr, int64_t step, float grad_scale, qmlp_stream_t stream);
+
+/* ---- operators on feature rows ------------------------------------------------------------------
+ * What a user of the reference writes in PyTorch between an encoding and a network, or around several networks (no
+ * counterpart in the reference): layer norm, lookup of latent codes, routing of rows to experts, matrix products grouped by
+ * expert. Feature matrices are (rows, channels) views of float, half or bfloat16 elements; the elements of a row lie side by
+ * side, rows may be any distance apart (16-byte aligned rows are read and written 16 bytes at a time). Sums and statistics are fp32,
+ * results are rounded once. Results are written, not accumulated, and do not change from run to run. Scratch memory is 256-byte
+ * aligned, its contents irrelevant; a *_memory function gives its size (0: none is needed, pass NULL). */
+
+/* output = (input - mean) / sqrt(variance + epsilon) * weight + bias, over the channels of each row. weight and bias: vectors
+ * of float or of the input's type; NULL or undefined: 1 and 0. stats (2 x rows floats: means, then reciprocal deviations) is what the
+ * adjoint needs; may be NULL. */
+QMLP_API int qmlp_layer_norm_forward(const qmlp_tensor_t* input, const qmlp_tensor_t* weight, const qmlp_tensor_t* bias, float epsilon,
+                                     qmlp_tensor_t* output, float* stats, qmlp_stream_t stream);
+/* Gradients of what is given: adj_input, adj_weight, adj_bias may be NULL or undefined. */
+QMLP_API int qmlp_layer_norm_adjoint_memory(int64_t rows, int channels, int precision, size_t* bytes);
+QMLP_API int qmlp_layer_norm_adjoint(const qmlp_tensor_t* input, const qmlp_tensor_t* adj_output, const qmlp_tensor_t* weight, const float* stats,
+                                     qmlp_tensor_t* adj_input, qmlp_tensor_t* adj_weight, qmlp_tensor_t* adj_bias, qmlp_stream_t stream,
+                                     void* tmp_memory, size_t tmp_bytes);
+
+/* output[t] = scale * table[tokens[t]]; tokens: int32 or int64. A token outside the table (-1, say) is masked: its row is
+ * zeros, and it contributes to no gradient. */
+QMLP_API int qmlp_embedding_forward(const qmlp_tensor_t* tokens, const qmlp_tensor_t* table, float scale, qmlp_tensor_t* output,
+                                    qmlp_stream_t stream);
+/* adj_table[v] = scale * sum of adj_output[t] over the tokens t that name row v, in the order of the tokens; every row is
+ * written. */
+QMLP_API int qmlp_embedding_adjoint_memory(int64_t tokens, int64_t rows, int channels, int precision, size_t* bytes);
+QMLP_API int qmlp_embedding_adjoint(const qmlp_tensor_t* tokens, const qmlp_tensor_t* adj_output, float scale, qmlp_tensor_t* adj_table,
+                                    qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes);
+
+/* The choice of `chosen` (at most 32) of `num_experts` (at most 1024) experts by each of `tokens` rows: contiguous device arrays that the
+ * caller owns. Slot s = row * chosen + j is a row's j-th choice. */
+typedef struct qmlp_routing {
+    int64_t tokens;
+    int32_t num_experts, chosen;
+    float* weights;       /* (tokens, chosen) weight of a choice; 0 in a slot without an expert */
+    int32_t* experts;     /* (tokens, chosen) expert; -1: none */
+    int32_t* order;       /* (tokens * chosen) slots, expert by expert, ascending within one; -1 behind the last expert's */
+    int32_t* positions;   /* (tokens, chosen) place of a slot in order; -1: none */
+    int32_t* offsets;     /* (num_experts + 1) where the slots of an expert begin in order */
+} qmlp_routing_t;
+/* Fills the arrays of `routing` from the rows' logits (tokens, num_experts): the largest logits first, ties to the lowest
+ * expert; NaN counts as the largest, an expert with -inf is never chosen (a row with too few others has slots without an
+ * expert). weights: softmax over the chosen experts (normalize != 0) or over all of the row. */
+QMLP_API int qmlp_route_memory(const qmlp_routing_t* routing, size_t* bytes);
+QMLP_API int qmlp_route_forward(const qmlp_tensor_t* logits, int normalize, qmlp_routing_t* routing, qmlp_stream_t stream, void* tmp_memory,
+                                size_t tmp_bytes);
+/* Gradient of the weights by the logits (the choice itself is constant); adj_weights: (tokens, chosen) floats. */
+QMLP_API int qmlp_route_adjoint(const qmlp_tensor_t* logits, int normalize, const qmlp_routing_t* routing, const float* adj_weights,
+                                qmlp_tensor_t* adj_logits, qmlp_stream_t stream);
+/* rows[r] = input[order[r] / chosen], zeros where order[r] is -1; adjoint: adj_input[t] = sum of adj_rows over t's slots. */
+QMLP_API int qmlp_dispatch_forward(const qmlp_tensor_t* input, const qmlp_routing_t* routing, qmlp_tensor_t* rows, qmlp_stream_t stream);
+QMLP_API int qmlp_dispatch_adjoint(const qmlp_tensor_t* adj_rows, const qmlp_routing_t* routing, qmlp_tensor_t* adj_input, qmlp_stream_t stream);
+/* output[t] = sum over t's slots of weights[s] * rows[positions[s]]; gradients of what is given (adj_rows, adj_weights may be
+ * NULL). */
+QMLP_API int qmlp_combine_forward(const qmlp_tensor_t* rows, const qmlp_routing_t* routing, qmlp_tensor_t* output, qmlp_stream_t stream);
+QMLP_API int qmlp_combine_adjoint(const qmlp_tensor_t* rows, const qmlp_tensor_t* adj_output, const qmlp_routing_t* routing, qmlp_tensor_t* adj_rows,
+                                  float* adj_weights, qmlp_stream_t stream);
+
+/* output[r] = weight[e] input[r] + bias[e] for the rows r in [offsets[e], offsets[e + 1]) of expert e; rows of no expert are
+ * zeros. Half or bfloat16, one type for all; weight: (num_experts * channels out, channels in), bias: (num_experts, channels
+ * out) or undefined, both contiguous; offsets: num_experts + 1 ascending int32 on the device (at most 2048 experts), which never travel to the
+ * host. A kernel that gives up a bounded wait sets bit 0 of qmlp_device_status. */
+QMLP_API int qmlp_expert_linear_forward_memory(const qmlp_tensor_t* input, const qmlp_tensor_t* weight, int num_experts, size_t* bytes);
+QMLP_API int qmlp_expert_linear_forward(const qmlp_tensor_t* input, const qmlp_tensor_t* weight, const int32_t* offsets, int num_experts,
+                                        const qmlp_tensor_t* bias, qmlp_tensor_t* output, qmlp_stream_t stream, void* tmp_memory,
+                                        size_t tmp_bytes);
+/* Gradients of what is given (adj_input, adj_weight, adj_bias may be NULL or undefined). adjoint_flags of the size:
+ * QMLP_GRADIENTS_INPUT, QMLP_GRADIENTS_NETWORK_WEIGHTS. */
+QMLP_API int qmlp_expert_linear_adjoint_memory(const qmlp_tensor_t* input, const qmlp_tensor_t* adj_output, const qmlp_tensor_t* weight,
+                                               int num_experts, int adjoint_flags, size_t* bytes);
+QMLP_API int qmlp_expert_linear_adjoint(const qmlp_tensor_t* input, const qmlp_tensor_t* adj_output, const qmlp_tensor_t* weight,
+                                        const int32_t* offsets, int num_experts, qmlp_tensor_t* adj_input, qmlp_tensor_t* adj_weight,
+                                        qmlp_tensor_t* adj_bias, qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes);
 
 #ifdef __cplusplus
 }

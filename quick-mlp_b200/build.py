@@ -9,12 +9,15 @@ import hashlib
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libqmlp_b200.so")
-SOURCES = ["host.cpp", "jit.cpp", "capi.cpp", "generic_kernels.cu", "static_scratch.cu"]
+SOURCES = ["host.cpp", "jit.cpp", "capi.cpp", "capi_operators.cpp", "generic_kernels.cu", "static_scratch.cu",
+           "operators/layer_norm.cu", "operators/embedding.cu", "operators/routing.cu", "operators/expert_linear.cu"]
 NVCC = os.environ.get("QMLP_NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -25,7 +28,7 @@ def _digest():
         if os.path.basename(root) == "kernels":
             continue  # template headers only enter the per-spec instantiations
         for f in sorted(files):
-            if f.endswith((".cpp", ".cu", ".h", ".hpp")):
+            if f.endswith((".cpp", ".cu", ".cuh", ".h", ".hpp")):
                 h.update(f.encode())
                 h.update(open(os.path.join(root, f), "rb").read())
     h.update(open(os.path.join(CSRC, "kernels", "launch_args.h"), "rb").read())
@@ -39,11 +42,18 @@ def build_library(force=False, verbose=True):
     digest = _digest()
     if not force and os.path.exists(LIB) and os.path.exists(stamp) and open(stamp).read() == digest:
         return LIB
-    cmd = [NVCC, "-std=c++17", "-O3", "-lineinfo", *ARCH, "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
-           "-o", LIB] + [os.path.join(CSRC, s) for s in SOURCES] + ["-ldl"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+    flags = ["-std=c++17", "-O3", "-lineinfo", *ARCH, "-Xcompiler", "-fPIC,-fvisibility=hidden"]
+    with tempfile.TemporaryDirectory() as objects:
+        def compile_one(source):
+            out = os.path.join(objects, source.replace("/", "_") + ".o")
+            cmd = [NVCC, *flags, "-c", os.path.join(CSRC, source), "-o", out]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            subprocess.check_call(cmd)
+            return out
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            linked = list(pool.map(compile_one, SOURCES))
+        subprocess.check_call([NVCC, *flags, "-shared", "-o", LIB, *linked, "-ldl"])
     with open(stamp, "w") as f:
         f.write(digest)
     return LIB

@@ -14,7 +14,7 @@ def _build(name, source, ldflags, verbose):
     from torch.utils import cpp_extension
     src = os.path.join(HERE, "csrc", "torch", source)
     out = os.path.join(OUTDIR, name + ".so")
-    deps = [src, os.path.join(INCLUDE, "qmlp_b200.h")] + [os.path.join(INCLUDE, "qmlp", f) for f in os.listdir(os.path.join(INCLUDE, "qmlp"))]
+    deps = [src, os.path.join(os.path.dirname(src), "operator_calls.h"), os.path.join(INCLUDE, "qmlp_b200.h")] + [os.path.join(INCLUDE, "qmlp", f) for f in os.listdir(os.path.join(INCLUDE, "qmlp"))]
     if os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(p) for p in deps):
         return out
     os.makedirs(OUTDIR, exist_ok=True)

@@ -1,6 +1,6 @@
 // extern "C" entry points of libqmlp_b200.so: argument checks in the style of the reference's CHECK_* macros
 // (src_cpp/include/qmlp/errors.h:78-90), launch-argument marshalling, and exception -> status-code translation.
-#include "host.hpp"
+#include "entry.hpp"
 #include "generic_kernels.h"
 
 #include <algorithm>
@@ -15,58 +15,6 @@ using namespace qmlp;
 namespace {
 
 thread_local std::string g_lastError;
-
-int fail(int code, const std::string& msg)
-{
-    g_lastError = msg;
-    return code;
-}
-
-#define QMLP_TRY try {
-#define QMLP_CATCH                                                                         \
-    }                                                                                      \
-    catch (const qmlp::configuration_error& e) { return fail(QMLP_ERROR_CONFIGURATION, e.what()); } \
-    catch (const qmlp::cuda_error& e) { return fail(QMLP_ERROR_CUDA, e.what()); }          \
-    catch (const qmlp::compile_error& e) { return fail(QMLP_ERROR_COMPILE, e.what()); }    \
-    catch (const std::exception& e) { return fail(QMLP_ERROR_RUNTIME, e.what()); }         \
-    catch (...) { return fail(QMLP_ERROR_RUNTIME, "unknown error"); }                      \
-    return QMLP_OK;
-
-void checkCuda(cudaError_t e, const char* what)
-{
-    if (e == cudaSuccess) return;
-    (void)cudaGetLastError();   // reported here: the check after the next launch must not find it again
-    throw cuda_error(std::string(what) + ": " + cudaGetErrorString(e));
-}
-void checkLaunch(int e, const char* what)
-{
-    if (e != 0) throw cuda_error(std::string(what) + ": " + cudaGetErrorString(static_cast<cudaError_t>(e)));
-}
-
-void checkDefined(const qmlp_tensor_t* t, const char* name)
-{
-    if (t == nullptr || t->ndim <= 0) throw std::runtime_error(std::string(name) + " is undefined");
-    bool empty = false;
-    for (int i = 0; i < t->ndim && i < 2; ++i) empty = empty || t->sizes[i] == 0;
-    if (t->data == nullptr && !empty) throw std::runtime_error(std::string(name) + " is undefined");
-}
-void checkDim(const qmlp_tensor_t* t, int dim, const char* name)
-{
-    checkDefined(t, name);
-    if (t->ndim != dim) throw std::runtime_error(format("%s has the wrong dimension, expected %d but got %d", name, dim, t->ndim));
-}
-void checkSize(const qmlp_tensor_t* t, int d, int64_t size, const char* name)
-{
-    if (t->sizes[d] != size)
-        throw std::runtime_error(format("%s has the wrong size at dimension %d, expected %lld but got %lld", name, d,
-                                        static_cast<long long>(size), static_cast<long long>(t->sizes[d])));
-}
-void checkDtype(const qmlp_tensor_t* t, int precision, const char* name)
-{
-    static const char* names[] = {"float", "half", "double"};
-    if (t->precision != precision)
-        throw std::runtime_error(format("%s has the wrong data type, expected %s", name, names[precision]));
-}
 
 void fillCommon(Network& n, kernel::LaunchArgs& a, const qmlp_tensor_t* input)
 {
@@ -104,35 +52,7 @@ void checkIO(Network& n, const qmlp_tensor_t* input, const qmlp_tensor_t* output
     checkDtype(output, QMLP_FLOAT, outName);
 }
 
-// Optional per-kernel device timing (qmlp_set_kernel_timing): an event pair around every launch the library makes,
-// read back and summed per kernel by qmlp_read_kernel_timing. Off by default: the events cost a little.
-struct KernelTimer {
-    struct Record { int id; cudaEvent_t begin, end; };
-    std::mutex mutex;
-    bool enabled = false;
-    std::vector<Record> records;
-} g_timer;
-
 constexpr int KERNEL_ID_ADAM = 100, KERNEL_ID_REFRESH_HALF = 101;
-
-struct TimedLaunch {
-    int id;
-    cudaStream_t stream;
-    cudaEvent_t begin = nullptr, end = nullptr;
-    TimedLaunch(int kernelId, cudaStream_t s) : id(kernelId), stream(s)
-    {
-        if (!g_timer.enabled) return;
-        if (cudaEventCreate(&begin) != cudaSuccess || cudaEventCreate(&end) != cudaSuccess) { begin = end = nullptr; return; }
-        cudaEventRecord(begin, stream);
-    }
-    ~TimedLaunch()
-    {
-        if (!begin) return;
-        cudaEventRecord(end, stream);
-        std::lock_guard<std::mutex> lock(g_timer.mutex);
-        g_timer.records.push_back({id, begin, end});
-    }
-};
 
 // The launch arguments with the sizes of the scratch buffers they point to, for bounds-checking instantiations: the stash
 // (of the encoded input alone, for the recomputing pair) and the delta stash hold n32 rows of the network's widths, the planes
@@ -243,7 +163,14 @@ void bindReplicas(const Network& n, kernel::LaunchArgs& a, void* memory)
 
 namespace qmlp {
 
-int reportError(int code, const char* message) { return fail(code, message ? message : ""); }
+KernelTimer g_timer;
+
+int reportError(int code, const char* message)
+{
+    g_lastError = message ? message : "";
+    return code;
+}
+
 
 void forwardWithStashAt(Network& n, const qmlp_tensor_t* input, qmlp_tensor_t* output, void* tmp, qmlp_stream_t stream)
 {

@@ -1,4 +1,4 @@
-// Native call path of the Python package: the tensor-facing half of qmlp/bindings.py, qmlp/ops.py and qmlp/trainer.py.
+// Native call path of the Python package: the tensor-facing half of qmlp/bindings.py, qmlp/ops.py, qmlp/rows.py and qmlp/trainer.py.
 //
 // A small batch is bound by what the host does per call (a thousand points through a 64-wide network are 8 us of kernel).
 // Argument checks, tensor views, output allocation, stream lookup and the autograd nodes therefore live here; Python only
@@ -35,7 +35,11 @@ using OptTensor = std::optional<Tensor>;
     X(network_forward) X(network_adjoint_memory) X(network_adjoint) X(network_recompute_memory) X(network_forward_recompute) X(network_adjoint_recompute) X(network_parameter_count) X(encoding_create)         \
     X(encoding_num_output_channels) X(encoding_has_parameters) X(encoding_set_parameter) X(encoding_forward_memory) X(encoding_forward_with_memory)              \
     X(encoding_adjoint_memory) X(encoding_adjoint_with_memory) X(activation_create) X(activation_forward) X(activation_adjoint) X(trainer_workspace_bytes)       \
-    X(trainer_gradients_part) X(trainer_update) X(convert_half)
+    X(trainer_gradients_part) X(trainer_update) X(convert_half)                                                            \
+    X(layer_norm_forward) X(layer_norm_adjoint_memory) X(layer_norm_adjoint) X(embedding_forward) X(embedding_adjoint_memory)  \
+    X(embedding_adjoint) X(route_memory) X(route_forward) X(route_adjoint) X(dispatch_forward) X(dispatch_adjoint)         \
+    X(combine_forward) X(combine_adjoint) X(expert_linear_forward_memory) X(expert_linear_forward)                         \
+    X(expert_linear_adjoint_memory) X(expert_linear_adjoint)
 
 struct Api {
 #define QMLP_MEMBER(name) decltype(&qmlp_##name) name = nullptr;
@@ -505,6 +509,8 @@ void trainerUpdate(intptr_t trainer, int64_t step, double gradScale)
     check(api.trainer_update(reinterpret_cast<qmlp_trainer_t*>(trainer), step, static_cast<float>(gradScale), currentStream()));
 }
 
+#include "operator_calls.h"
+
 // Resolves the C ABI, then registers the kernels of the operators that qmlp/ops.py defines (in this order: another thread may
 // call an operator as soon as it is registered). The devices' own autograd keys are used: the alias key holds the entry that
 // loads this module.
@@ -533,6 +539,8 @@ void load(const std::string& path, py::object error, py::object configurationErr
     kernels(c10::DispatchKey::Meta, encodingForwardMeta, encodingAdjointMeta, activationForwardMeta, activationAdjointMeta);
     for (auto key : {c10::DispatchKey::AutogradCUDA, c10::DispatchKey::AutogradMeta, c10::DispatchKey::AutogradOther})   // (Other: functorch)
         kernels(key, encodingForwardAutograd, encodingAdjointAutograd, activationForwardAutograd, activationAdjointAutograd);
+    for (auto key : {c10::DispatchKey::CUDA, c10::DispatchKey::Meta, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::AutogradMeta, c10::DispatchKey::AutogradOther})
+        registerRowOperators(key);
 }
 
 } // namespace
@@ -552,4 +560,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("trainer_workspace_bytes", wrap_pybind_function_no_gil(trainerWorkspaceBytes));
     m.def("trainer_gradients", wrap_pybind_function_no_gil(trainerGradients));
     m.def("trainer_update", wrap_pybind_function_no_gil(trainerUpdate));
+    m.def("layer_norm", wrap_pybind_function_no_gil(layerNorm));
+    m.def("embedding", wrap_pybind_function_no_gil(embedding));
+    m.def("route", wrap_pybind_function_no_gil(route));
+    m.def("dispatch", wrap_pybind_function_no_gil(dispatchRows));
+    m.def("combine", wrap_pybind_function_no_gil(combineRows));
+    m.def("expert_linear", wrap_pybind_function_no_gil(expertLinear));
 }

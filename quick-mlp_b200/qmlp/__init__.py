@@ -5,6 +5,8 @@ from .import_library import load_library, load_torch_classes
 from .activation import FusedActivation
 from .encoding import FusedEncoding
 from .network import SimulatedNetwork, FusedNetwork, copy_torch_to_fused
+from .rows import (FusedEmbedding, FusedExperts, FusedLayerNorm, Routing, combine, dispatch, embedding, expert_linear,
+                   layer_norm, route)
 from .trainer import FusedTrainer, shard_points
 
 __all__ = [
@@ -18,4 +20,14 @@ __all__ = [
     "copy_torch_to_fused",
     "FusedTrainer",
     "shard_points",
+    "FusedEmbedding",
+    "FusedExperts",
+    "FusedLayerNorm",
+    "Routing",
+    "combine",
+    "dispatch",
+    "embedding",
+    "expert_linear",
+    "layer_norm",
+    "route",
 ]

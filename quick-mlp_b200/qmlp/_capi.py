@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "..", "lib", "libqmlp_b200.so")
 
 QMLP_FLOAT, QMLP_HALF, QMLP_DOUBLE = 0, 1, 2
+QMLP_BFLOAT16, QMLP_INT32, QMLP_INT64 = 3, 4, 5    # operators on feature rows only
 QMLP_INFERENCE, QMLP_GRADIENTS = 0, 1
 GRADIENTS_INPUT, GRADIENTS_NETWORK_WEIGHTS, GRADIENTS_INPUT_ENCODINGS = 1, 2, 4
 ENCODING_INPUT_GRADIENTS, ENCODING_PARAM_GRADIENTS = 1, 2
@@ -32,6 +33,12 @@ class TrainerConfig(C.Structure):
                 ("grid_half_copy", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Routing(C.Structure):
+    """qmlp_routing_t"""
+    _fields_ = [("tokens", C.c_int64), ("num_experts", C.c_int32), ("chosen", C.c_int32), ("weights", C.c_void_p),
+                ("experts", C.c_void_p), ("order", C.c_void_p), ("positions", C.c_void_p), ("offsets", C.c_void_p)]
+
+
 class QmlpError(RuntimeError):
     pass
 
@@ -45,6 +52,8 @@ _lib = None
 # name -> (restype, argtypes); every symbol include/qmlp_b200.h declares
 _P = C.c_void_p
 _TP = C.POINTER(Tensor)
+_RP = C.POINTER(Routing)
+_SIZE = C.POINTER(C.c_size_t)
 SIGNATURES = {
     "qmlp_last_error": (C.c_char_p, []),
     "qmlp_is_cuda_available": (C.c_int, []),
@@ -129,6 +138,23 @@ SIGNATURES = {
     "qmlp_trainer_gradients_part": (C.c_int, [_P, _TP, _TP, C.c_int64, _P, C.c_size_t, _P, C.c_int, _P]),
     "qmlp_trainer_scatter_levels": (C.c_int, [_P, C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "qmlp_trainer_update": (C.c_int, [_P, C.c_int64, C.c_float, _P]),
+    "qmlp_layer_norm_forward": (C.c_int, [_TP, _TP, _TP, C.c_float, _TP, _P, _P]),
+    "qmlp_layer_norm_adjoint_memory": (C.c_int, [C.c_int64, C.c_int, C.c_int, _SIZE]),
+    "qmlp_layer_norm_adjoint": (C.c_int, [_TP, _TP, _TP, _P, _TP, _TP, _TP, _P, _P, C.c_size_t]),
+    "qmlp_embedding_forward": (C.c_int, [_TP, _TP, C.c_float, _TP, _P]),
+    "qmlp_embedding_adjoint_memory": (C.c_int, [C.c_int64, C.c_int64, C.c_int, C.c_int, _SIZE]),
+    "qmlp_embedding_adjoint": (C.c_int, [_TP, _TP, C.c_float, _TP, _P, _P, C.c_size_t]),
+    "qmlp_route_memory": (C.c_int, [_RP, _SIZE]),
+    "qmlp_route_forward": (C.c_int, [_TP, C.c_int, _RP, _P, _P, C.c_size_t]),
+    "qmlp_route_adjoint": (C.c_int, [_TP, C.c_int, _RP, _P, _TP, _P]),
+    "qmlp_dispatch_forward": (C.c_int, [_TP, _RP, _TP, _P]),
+    "qmlp_dispatch_adjoint": (C.c_int, [_TP, _RP, _TP, _P]),
+    "qmlp_combine_forward": (C.c_int, [_TP, _RP, _TP, _P]),
+    "qmlp_combine_adjoint": (C.c_int, [_TP, _TP, _RP, _TP, _P, _P]),
+    "qmlp_expert_linear_forward_memory": (C.c_int, [_TP, _TP, C.c_int, _SIZE]),
+    "qmlp_expert_linear_forward": (C.c_int, [_TP, _TP, _P, C.c_int, _TP, _TP, _P, _P, C.c_size_t]),
+    "qmlp_expert_linear_adjoint_memory": (C.c_int, [_TP, _TP, _TP, C.c_int, C.c_int, _SIZE]),
+    "qmlp_expert_linear_adjoint": (C.c_int, [_TP, _TP, _TP, _P, C.c_int, _TP, _TP, _TP, _P, _P, C.c_size_t]),
 }
 
 

@@ -13,6 +13,9 @@ and loading it needs nothing but this package imported. The operator looks the c
     encoding_adjoint(Tensor input, Tensor? parameters, Tensor adj_output, bool want_input, bool want_parameters,
                      str cfg) -> (Tensor, Tensor)
 
+The operators on feature rows (qmlp/rows.py: layer norm, embedding lookup, routing to experts, products grouped by expert)
+are registered in the same way: X_forward, differentiable, and X_adjoint, its gradients.
+
 The schemas are registered here; the kernels and the autograd nodes come with the native call path (csrc/torch/calls.cpp),
 which registers them for CUDA and meta tensors when it is loaded. The first object of the package loads it, not the import:
 the package's plain Python (configurations, the stock PyTorch modules) works without any of the native libraries. A graph
@@ -30,6 +33,18 @@ SCHEMAS = {
     "activation_adjoint": "(Tensor input, Tensor adj_output, str cfg) -> Tensor",
     "encoding_forward": "(Tensor input, Tensor? parameters, str cfg) -> Tensor",
     "encoding_adjoint": "(Tensor input, Tensor? parameters, Tensor adj_output, bool want_input, bool want_parameters, str cfg) -> (Tensor, Tensor)",
+    "layer_norm_forward": "(Tensor input, Tensor? weight, Tensor? bias, float epsilon) -> (Tensor, Tensor)",
+    "layer_norm_adjoint": "(Tensor input, Tensor adj_output, Tensor? weight, Tensor? bias, Tensor stats, bool want_input, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)",
+    "embedding_forward": "(Tensor tokens, Tensor table, float scale) -> Tensor",
+    "embedding_adjoint": "(Tensor tokens, Tensor adj_output, int rows, float scale) -> Tensor",
+    "route_forward": "(Tensor logits, int chosen, bool normalize) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "route_adjoint": "(Tensor logits, bool normalize, Tensor weights, Tensor experts, Tensor adj_weights) -> Tensor",
+    "dispatch_forward": "(Tensor input, Tensor order, Tensor positions) -> Tensor",
+    "dispatch_adjoint": "(Tensor adj_rows, Tensor positions) -> Tensor",
+    "combine_forward": "(Tensor rows, Tensor weights, Tensor order, Tensor positions) -> Tensor",
+    "combine_adjoint": "(Tensor rows, Tensor adj_output, Tensor weights, Tensor order, Tensor positions, bool want_rows, bool want_weights) -> (Tensor, Tensor)",
+    "expert_linear_forward": "(Tensor input, Tensor weight, Tensor offsets, Tensor? bias) -> Tensor",
+    "expert_linear_adjoint": "(Tensor input, Tensor adj_output, Tensor weight, Tensor offsets, bool want_input, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)",
 }
 
 _library = torch.library.Library("qmlp_b200", "DEF")
