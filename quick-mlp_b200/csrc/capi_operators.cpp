@@ -179,6 +179,7 @@ int qmlp_layer_norm_forward(const qmlp_tensor_t* input, const qmlp_tensor_t* wei
     a.y = rowsOf(output);
     a.stats = stats;
     a.numSMs = Library::instance().smCount();
+    a.status = Library::instance().statusWord();
     launch(KERNEL_ID_LAYER_NORM_FORWARD, stream, [&](cudaStream_t s) { return kernel::launchLayerNormForward(a, s); });
     QMLP_CATCH
 }
@@ -215,6 +216,7 @@ int qmlp_layer_norm_adjoint(const qmlp_tensor_t* input, const qmlp_tensor_t* adj
         a.partial = static_cast<float*>(tmp_memory);
     }
     a.numSMs = Library::instance().smCount();
+    a.status = Library::instance().statusWord();
     launch(KERNEL_ID_LAYER_NORM_ADJOINT, stream, [&](cudaStream_t s) { return kernel::launchLayerNormAdjoint(a, s); });
     QMLP_CATCH
 }

@@ -33,20 +33,68 @@ template <class T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
     T v[VEC];
 };
+// two 16-bit elements at once: one conversion instruction per pair where there is one
+__device__ __forceinline__ float2 toPair(const __half* v) { return __half22float2(*reinterpret_cast<const __half2*>(v)); }
+__device__ __forceinline__ float2 toPair(const __nv_bfloat16* v)
+{
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(v);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ void fromPair(__half* v, float a, float b) { *reinterpret_cast<__half2*>(v) = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void fromPair(__nv_bfloat16* v, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(v) = __floats2bfloat162_rn(a, b); }
+
 template <class T, int VEC>
 __device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&f)[VEC])
 {
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = Element<T>::to(p.v[i]);
+        for (int i = 0; i < VEC; i += 2) {
+            const float2 v = toPair(&p.v[i]);
+            f[i] = v.x;
+            f[i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = Element<T>::to(p.v[i]);
+    }
 }
 template <class T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> pack(const float (&f)[VEC])
 {
     Pack<T, VEC> p;
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p.v[i] = Element<T>::from(f[i]);
+        for (int i = 0; i < VEC; i += 2) fromPair(&p.v[i], f[i], f[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) p.v[i] = Element<T>::from(f[i]);
+    }
     return p;
 }
+
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // 16-byte accesses go through uint4, so that they stay one instruction
 template <class T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> load(const T* at)
@@ -92,12 +140,50 @@ __device__ __forceinline__ float groupSum(float v)
     return v;
 }
 
+// ---- mbarriers and bulk copies ---------------------------------------------------------------------------------------
+constexpr uint32_t WAIT_LIMIT = 1u << 22;   // polls of an mbarrier before a kernel gives up
+
+__device__ __forceinline__ uint32_t smemAddress(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void barrierInit(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void barrierInitDone()
+{
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ bool barrierTest(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool barrierWait(uint32_t bar, uint32_t parity)
+{
+    for (uint32_t i = 0; i < WAIT_LIMIT; ++i)
+        if (barrierTest(bar, parity)) return true;
+    return false;
+}
+__device__ __forceinline__ void barrierArrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void barrierExpect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// global -> shared, both addresses and the size multiples of 16 bytes; completes on the mbarrier
+__device__ __forceinline__ void bulkLoad(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
+}
+
 // whether rows can be read and written 16 bytes at a time
 inline bool wide(const Rows& r, int type, int channels)
 {
     const int n = 16 / typeBytes(type);
     return r.data == nullptr || ((reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.stride % n == 0 && channels % n == 0);
 }
+
+// lets a kernel use up to `bytes` of dynamic shared memory on the current device; asked for once per kernel and device
+cudaError_t allowShared(const void* kernel, int bytes);
 
 } // namespace ops
 } // namespace kernel

@@ -21,7 +21,6 @@
 #include "common.cuh"
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include <cuda.h>
@@ -32,23 +31,7 @@ namespace {
 
 using namespace ops;
 
-constexpr uint32_t WAIT_LIMIT = 1u << 22;   // polls of an mbarrier before a kernel gives up
-
 // ---- PTX ---------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smemAddress(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void barrierInit(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
-__device__ __forceinline__ bool barrierTest(uint32_t bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ void barrierArrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void barrierExpect(uint32_t bar, uint32_t bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void tmaLoad2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
 {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -260,8 +243,7 @@ __global__ void __launch_bounds__(BLOCK, 1)
         }
         barrierInit(drain, 1);
         *failed = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fenceProxyAsync();
+        barrierInitDone();
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddress(tmemBase)), "r"(L::TMEM) : "memory");
@@ -615,15 +597,8 @@ template <class T, int MODE, int BN>
 cudaError_t launchProduct(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, int blocks, cudaStream_t stream)
 {
     auto* kernel = expert_product_kernel<T, MODE, BN>;
-    static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may use its shared memory
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
+    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), Layout<BN>::bytes(EXPERTS_MAX));
     if (e != cudaSuccess) return e;
-    if (device >= 64 || (allowed.load(std::memory_order_relaxed) >> device & 1) == 0) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<BN>::bytes(EXPERTS_MAX));
-        if (e != cudaSuccess) return e;
-        if (device < 64) allowed.fetch_or(1ull << device);
-    }
     kernel<<<blocks, BLOCK, Layout<BN>::bytes(p.experts), stream>>>(a, b, p);
     return cudaGetLastError();
 }

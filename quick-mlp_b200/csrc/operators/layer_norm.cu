@@ -5,6 +5,10 @@
 //
 // A row is held in the registers of G threads (8 or 32 lanes of a warp, or a block of 64 to 1024), EPT elements each, so that it
 // is read once: the variance is summed from the centred values, not from a difference of squares. All sums are fp32.
+// Rows of a block of their own (more than 512 channels) come through a ring of bulk copies in shared memory. What bounds the kernels is DRAM;
+// on the way there it was instructions (two fp32 operations per instruction, pairs converted at once), L1 (parameters in
+// registers) and the latency of a row's sums (one exchange through shared memory per row, the row's statistics fetched ahead).
+// 32768 x 4096 bfloat16: forward 87 us, 6.2 TB/s; adjoint 134 us + 4 us for the parameters' sums, 5.8 TB/s.
 // The gradients of the parameters are sums over rows: a block walks its share of the rows with one fp32 sum per column in
 // registers, adds up its row groups in shared memory and leaves one row of partial sums; a second kernel adds those up in a
 // fixed order, so the result does not change from run to run. Rows wider than 16384 take three passes over memory instead.
@@ -45,128 +49,391 @@ __device__ __forceinline__ void rowSum(float (&v)[N], float* shared, int& half)
 
 __host__ __device__ constexpr int threadsFor(int g) { return g <= 32 ? 256 : g; }
 
+// The elements of a thread: EPT of a row, VEC side by side; number k (in pairs: k, k + 1) is element (k / VEC * G + lane) * VEC + k % VEC.
 template <class T, int VEC, int G, int EPT>
-__global__ void __launch_bounds__(threadsFor(G)) layer_norm_forward_kernel(const __grid_constant__ LayerNormArgs a)
+__device__ __forceinline__ void fetchRow(const T* row, int lane, int channels, bool active, float2 (&v)[EPT / 2])
 {
-    constexpr int NV = EPT / VEC, THREADS = threadsFor(G), GROUPS = THREADS / G;
-    __shared__ float shared[2 * 32];
-    int half = 0;
-    const int lane = threadIdx.x % G, group = threadIdx.x / G;
-    const float invC = 1.f / static_cast<float>(a.channels);
-    // the parameters stay in registers where a block walks many rows
-    float w[EPT], b[EPT];
+    Pack<T, VEC> p[EPT / VEC];
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const int c = (i / VEC * G + lane) * VEC + i % VEC;
-        w[i] = a.weight.data != nullptr && c < a.channels ? element(a.weight, c) : 1.f;
-        b[i] = a.bias.data != nullptr && c < a.channels ? element(a.bias, c) : 0.f;
+    for (int n = 0; n < EPT / VEC; ++n) {
+        const int c = (n * G + lane) * VEC;
+        p[n] = {};
+        if (active && c < channels) p[n] = load<T, VEC>(row + c);
     }
+#pragma unroll
+    for (int n = 0; n < EPT / VEC; ++n) unpack<T, VEC>(p[n], reinterpret_cast<float (*)[VEC]>(&v[0])[n]);
+}
+template <class T, int VEC, int G, int EPT>
+__device__ __forceinline__ void storeRow(T* row, int lane, int channels, const float2 (&v)[EPT / 2])
+{
+#pragma unroll
+    for (int n = 0; n < EPT / VEC; ++n) {
+        const int c = (n * G + lane) * VEC;
+        if (c < channels) store<T, VEC>(row + c, pack<T, VEC>(reinterpret_cast<const float (*)[VEC]>(&v[0])[n]));
+    }
+}
+// zero where an element lies behind the row's last
+template <int VEC, int G, int EPT>
+__device__ __forceinline__ void clearBehind(int lane, int channels, float2 (&v)[EPT / 2])
+{
+#pragma unroll
+    for (int n = 0; n < EPT / VEC; ++n)
+        if ((n * G + lane) * VEC >= channels) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) reinterpret_cast<float*>(&v[0])[n * VEC + i] = 0.f;
+        }
+}
+template <int N>
+__device__ __forceinline__ float pairSum(const float2 (&v)[N])
+{
+    float2 s = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) s = add2(s, v[i]);
+    return s.x + s.y;
+}
+
+// Mean and variance of a row whose elements `v` are centred on the way. Each warp has its own mean first, so that one exchange through
+// shared memory does for both: sum (x - mean)^2 = sum over warps of (squares about the warp's mean + count * (warp's mean - mean)^2).
+template <int VEC, int G, int EPT>
+struct Moments {
+    static constexpr int LANES = G < 32 ? G : 32, WARPS = G > 32 ? G / 32 : 1;
+    float invC, invCount;        // elements of the row; of this warp (group of lanes), 0 if it has none
+    float otherCount = 0.f, otherInv = 0.f;   // of warp `lane`
+    float* shared;               // 2 x 64 floats
+    int half = 0;
+    __device__ __forceinline__ Moments(int lane, int channels, float* memory) : shared(memory)
+    {
+        float count = 0.f;
+#pragma unroll
+        for (int n = 0; n < EPT / VEC; ++n) count += (n * G + lane) * VEC < channels ? static_cast<float>(VEC) : 0.f;
+        count = groupSum<LANES>(count);
+        invC = 1.f / static_cast<float>(channels);
+        invCount = count > 0.f ? 1.f / count : 0.f;
+        if constexpr (G > 32) {
+            const int l = threadIdx.x & 31;
+            if (l == 0) shared[threadIdx.x >> 5] = count;
+            __syncthreads();
+            otherCount = l < WARPS ? shared[l] : 0.f;
+            otherInv = otherCount > 0.f ? 1.f / otherCount : 0.f;
+            __syncthreads();
+        }
+    }
+    __device__ __forceinline__ void operator()(int lane, int channels, float2 (&v)[EPT / 2], float& mean, float& variance)
+    {
+        const float sum = groupSum<LANES>(pairSum(v)), own = sum * invCount;
+        float2 s = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < EPT / 2; ++i) v[i] = add2(v[i], both(-own));
+        clearBehind<VEC, G, EPT>(lane, channels, v);
+#pragma unroll
+        for (int i = 0; i < EPT / 2; ++i) s = fma2(v[i], v[i], s);
+        float squares = groupSum<LANES>(s.x + s.y);
+        mean = own;
+        if constexpr (G > 32) {
+            float* at = shared + half * 64;
+            half ^= 1;
+            const int l = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            if (l == 0) *reinterpret_cast<float2*>(at + 2 * warp) = make_float2(sum, squares);
+            __syncthreads();
+            const float2 other = l < WARPS ? *reinterpret_cast<const float2*>(at + 2 * l) : make_float2(0.f, 0.f);
+            mean = groupSum<WARPS>(other.x) * invC;
+            if constexpr (WARPS < 32) mean = __shfl_sync(0xffffffffu, mean, 0);
+            const float d = fmaf(other.x, otherInv, -mean);
+            squares = groupSum<WARPS>(fmaf(d * d, otherCount, other.y));
+            if constexpr (WARPS < 32) squares = __shfl_sync(0xffffffffu, squares, 0);
+#pragma unroll
+            for (int i = 0; i < EPT / 2; ++i) v[i] = add2(v[i], both(own - mean));
+        }
+        variance = squares * invC;
+    }
+};
+
+// The parameters of a thread's elements: kept in registers where these allow it, or read from L1 when they are used. (Reading both
+// vectors for every row of 4096 bfloat16 keeps L1 82 % busy and was slower: 131 us for 32768 rows.)
+template <int VEC, int G, int EPT>
+struct Parameters {
+    static constexpr bool KEEP = G <= 256;
+    float kept[KEEP ? EPT : 1];
+    Vector source;
+    float otherwise;
+    int lane, channels;
+    bool wide;
+    __device__ __forceinline__ Parameters(const Vector& v, float none, int l, int c) : source(v), otherwise(none), lane(l), channels(c)
+    {
+        wide = VEC % 4 == 0 && v.type == TYPE_FLOAT && (reinterpret_cast<uintptr_t>(v.data) & 15) == 0;
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int n = 0; n < EPT / VEC; ++n) read(n, *reinterpret_cast<float (*)[VEC]>(&kept[n * VEC]));
+        }
+    }
+    __device__ __forceinline__ void read(int n, float (&f)[VEC]) const
+    {
+        const int c = (n * G + lane) * VEC;
+        if (source.data != nullptr && c < channels) {
+            if (wide) {   // (channels is a multiple of VEC)
+#pragma unroll
+                for (int i = 0; i + 3 < VEC; i += 4) *reinterpret_cast<float4*>(&f[i]) = *reinterpret_cast<const float4*>(static_cast<const float*>(source.data) + c + i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[i] = element(source, c + i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = otherwise;
+        }
+    }
+    __device__ __forceinline__ void get(int n, float (&f)[VEC]) const
+    {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = kept[n * VEC + i];
+        } else {
+            read(n, f);
+        }
+    }
+    __device__ __forceinline__ void get(float2 (&f)[EPT / 2]) const
+    {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int i = 0; i < EPT / 2; ++i) f[i] = make_float2(kept[2 * i], kept[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < EPT / VEC; ++n) read(n, reinterpret_cast<float (*)[VEC]>(&f[0])[n]);
+        }
+    }
+};
+
+// Rows on their way to a block of one row: bulk copies ahead of the row that is worked on, into a ring of `stages` slots in
+// shared memory. What is in flight then does not depend on what the threads are doing, nor on their registers.
+struct Ring {
+    uint32_t slots, bars, slotBytes, rowBytes;
+    int stages, stage = 0, phase = 0;
+    bool ok = true;
+    __device__ __forceinline__ Ring() {}
+    // `matrices` rows per slot; called by all threads, ends in a barrier
+    __device__ __forceinline__ Ring(unsigned char* memory, int count, int matrices, uint32_t bytes)
+        : slots(smemAddress(memory) + 128), bars(smemAddress(memory)), slotBytes(matrices * bytes), rowBytes(bytes), stages(count)
+    {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < stages; ++i) barrierInit(bars + i * 8, 1);
+            barrierInitDone();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void issue(int at, const void* first, const void* second) const
+    {
+        barrierExpect(bars + at * 8, slotBytes);
+        bulkLoad(slots + at * slotBytes, first, rowBytes, bars + at * 8);
+        if (second != nullptr) bulkLoad(slots + at * slotBytes + rowBytes, second, rowBytes, bars + at * 8);
+    }
+    // offset of the slot whose row is there now
+    __device__ __forceinline__ uint32_t await()
+    {
+        ok = barrierWait(bars + stage * 8, phase) && ok;
+        return 128 + stage * slotBytes;
+    }
+    __device__ __forceinline__ void advance()
+    {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+};
+constexpr int RING_MAX = 8;
+
+// blocks per SM that the registers have to allow
+__host__ __device__ constexpr int perSM(int g) { return g <= 32 ? 2 : g <= 256 ? 512 / g : 1; }
+__host__ __device__ constexpr int forwardPerSM(int g) { return g <= 32 ? 3 : g <= 256 ? 768 / g : 1024 / g; }
+
+template <class T, int VEC, int G, int EPT, bool RINGED>
+__global__ void __launch_bounds__(threadsFor(G), forwardPerSM(G)) layer_norm_forward_kernel(const __grid_constant__ LayerNormArgs a)
+{
+    constexpr int GROUPS = threadsFor(G) / G;
+    extern __shared__ __align__(128) unsigned char dynamic[];
+    __shared__ __align__(8) float shared[2 * 64];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const T* x = static_cast<const T*>(a.x.data);
     T* y = static_cast<T*>(a.y.data);
-    for (long long first = static_cast<long long>(blockIdx.x) * GROUPS; first < a.rows; first += static_cast<long long>(gridDim.x) * GROUPS) {
-        const long long row = first + group;
+    const long long step = static_cast<long long>(gridDim.x) * GROUPS;
+    long long row = static_cast<long long>(blockIdx.x) * GROUPS + group;
+    Ring ring = [&] {
+        if constexpr (RINGED) return Ring(dynamic, a.ringStages, 1, a.channels * sizeof(T));
+        else return Ring();
+    }();
+    if (RINGED && threadIdx.x == 0)
+        for (int i = 0; i < a.ringStages && row + i * step < a.rows; ++i) ring.issue(i, x + (row + i * step) * a.x.stride, nullptr);
+    const Parameters<VEC, G, EPT> w(a.weight, 1.f, lane, a.channels), b(a.bias, 0.f, lane, a.channels);
+    Moments<VEC, G, EPT> moments(lane, a.channels, shared);
+    for (; row - group < a.rows; row += step) {
         const bool active = row < a.rows;
-        float v[EPT];
-        float sum[1] = {0.f};
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + lane) * VEC;
-            float f[VEC] = {};
-            if (active && c < a.channels) unpack<T, VEC>(load<T, VEC>(x + row * a.x.stride + c), f);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) { v[n * VEC + i] = f[i]; sum[0] += f[i]; }
+        float2 v[EPT / 2], f[EPT / 2];
+        fetchRow<T, VEC, G, EPT>(RINGED ? reinterpret_cast<const T*>(dynamic + ring.await()) : x + row * a.x.stride, lane, a.channels, active, v);
+        float mean, variance;
+        moments(lane, a.channels, v, mean, variance);
+        if constexpr (RINGED) {   // (behind the barrier of the sums: the slot has been read)
+            if (threadIdx.x == 0 && row + a.ringStages * step < a.rows) ring.issue(ring.stage, x + (row + a.ringStages * step) * a.x.stride, nullptr);
+            ring.advance();
         }
-        rowSum<G, 1>(sum, shared, half);
-        const float mean = sum[0] * invC;
-        float square[1] = {0.f};
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const bool inside = (n * G + lane) * VEC < a.channels;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                v[n * VEC + i] -= mean;
-                square[0] += inside ? v[n * VEC + i] * v[n * VEC + i] : 0.f;
-            }
-        }
-        rowSum<G, 1>(square, shared, half);
-        const float rstd = rsqrtf(square[0] * invC + a.epsilon);
+        const float rstd = rsqrtf(variance + a.epsilon);
         if (!active) continue;   // (whole rows: the lanes of a row leave together, the row's sums are complete)
         if (a.stats != nullptr && lane == 0) {
             a.stats[row] = mean;
             a.stats[a.rows + row] = rstd;
         }
+        w.get(f);
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + lane) * VEC;
-            if (c >= a.channels) continue;
-            float f[VEC];
+        for (int i = 0; i < EPT / 2; ++i) v[i] = mul2(mul2(v[i], both(rstd)), f[i]);
+        b.get(f);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = fmaf(v[n * VEC + i] * rstd, w[n * VEC + i], b[n * VEC + i]);
-            store<T, VEC>(y + row * a.y.stride + c, pack<T, VEC>(f));
-        }
+        for (int i = 0; i < EPT / 2; ++i) v[i] = add2(v[i], f[i]);
+        storeRow<T, VEC, G, EPT>(y + row * a.y.stride, lane, a.channels, v);
     }
+    if (RINGED && !ring.ok) atomicOr(a.status, 1);
 }
 
-template <class T, int VEC, int G, int EPT>
-__global__ void __launch_bounds__(threadsFor(G)) layer_norm_adjoint_kernel(const __grid_constant__ LayerNormArgs a)
+// VEC elements of a row in the adjoint, from the packed x and dy: u = (x - mean) / deviation, d = dy, g = dy w
+template <class T, int VEC>
+struct Piece {
+    static constexpr int N = (VEC + 1) / 2;
+    float2 u[N], d[N], g[N];
+    __device__ __forceinline__ Piece(const Pack<T, VEC>& x, const Pack<T, VEC>& dy, const float* w, float mean, float rstd)
+    {
+        float fx[2 * N] = {}, fd[2 * N] = {};
+        unpack<T, VEC>(x, *reinterpret_cast<float (*)[VEC]>(fx));
+        unpack<T, VEC>(dy, *reinterpret_cast<float (*)[VEC]>(fd));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            u[i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), both(-mean)), both(rstd));   // (elements behind the row: whatever, their dy is zero)
+            d[i] = make_float2(fd[2 * i], fd[2 * i + 1]);
+            g[i] = mul2(d[i], make_float2(w[2 * i], VEC > 1 ? w[2 * i + 1] : 0.f));
+        }
+    }
+};
+
+// Between its sums and its result a row is held packed, and u and g are formed a second time: unpacked they would take twice the registers.
+// Blocks of 1024 threads have 64 registers each: they read the row a second time instead.
+// 32768 x 4096 bfloat16: 134 us, 6.0 TB/s (blocks that take two rows per step and share the barrier were slower: 159 us against 143 then).
+template <class T, int VEC, int G, int EPT, bool RINGED>
+__global__ void __launch_bounds__(threadsFor(G), perSM(G)) layer_norm_adjoint_kernel(const __grid_constant__ LayerNormArgs a)
 {
-    constexpr int NV = EPT / VEC, THREADS = threadsFor(G), GROUPS = THREADS / G;
+    constexpr int THREADS = threadsFor(G), GROUPS = THREADS / G, NV = EPT / VEC;
+    constexpr bool TWICE = G == 1024;
+    extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ float shared[2 * 32 * 2];
     int half = 0;
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float invC = 1.f / static_cast<float>(a.channels);
-    float w[EPT], dw[EPT], db[EPT];
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const int c = (i / VEC * G + lane) * VEC + i % VEC;
-        w[i] = a.weight.data != nullptr && c < a.channels ? element(a.weight, c) : 1.f;
-        dw[i] = db[i] = 0.f;
-    }
     const T *x = static_cast<const T*>(a.x.data), *dy = static_cast<const T*>(a.gradY.data);
     T* dx = static_cast<T*>(a.gradX.data);
-    for (long long first = static_cast<long long>(blockIdx.x) * GROUPS; first < a.rows; first += static_cast<long long>(gridDim.x) * GROUPS) {
-        const long long row = first + group;
-        const bool active = row < a.rows;
-        const float mean = active ? a.stats[row] : 0.f, rstd = active ? a.stats[a.rows + row] : 0.f;
-        float u[EPT], g[EPT];
-        float sums[2] = {0.f, 0.f};
+    const long long step = static_cast<long long>(gridDim.x) * GROUPS;
+    long long row = static_cast<long long>(blockIdx.x) * GROUPS + group;
+    Ring ring = [&] {
+        if constexpr (RINGED) return Ring(dynamic, a.ringStages, 2, a.channels * sizeof(T));
+        else return Ring();
+    }();
+    if (RINGED && threadIdx.x == 0)
+        for (int i = 0; i < a.ringStages && row + i * step < a.rows; ++i) ring.issue(i, x + (row + i * step) * a.x.stride, dy + (row + i * step) * a.gradY.stride);
+    const Parameters<VEC, G, EPT> w(a.weight, 1.f, lane, a.channels);
+    float2 dw[EPT / 2] = {}, db[EPT / 2] = {};
+    float nextMean, nextRstd;   // on their way for the row after: their latency would be every row's
+    auto fetchStats = [&](long long r) {
+        nextMean = r < a.rows ? a.stats[r] : 0.f;
+        nextRstd = r < a.rows ? a.stats[a.rows + r] : 0.f;
+    };
+    fetchStats(row);
+    for (; row - group < a.rows; row += step) {
+        const bool active = row < a.rows;   // (rows behind the last: zeros, which add nothing)
+        const float mean = nextMean, rstd = nextRstd;
+        fetchStats(row + step);
+        const T *rowX = x + row * a.x.stride, *rowY = dy + row * a.gradY.stride;
+        if constexpr (RINGED) {
+            const unsigned char* slot = dynamic + ring.await();
+            rowX = reinterpret_cast<const T*>(slot);
+            rowY = reinterpret_cast<const T*>(slot + ring.rowBytes);
+        }
+        Pack<T, VEC> px[NV], py[NV];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int c = (n * G + lane) * VEC;
-            const bool inside = active && c < a.channels;
-            float f[VEC] = {}, d[VEC] = {};
-            if (inside) {
-                unpack<T, VEC>(load<T, VEC>(x + row * a.x.stride + c), f);
-                unpack<T, VEC>(load<T, VEC>(dy + row * a.gradY.stride + c), d);
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int k = n * VEC + i;
-                u[k] = inside ? (f[i] - mean) * rstd : 0.f;
-                dw[k] = fmaf(d[i], u[k], dw[k]);
-                db[k] += d[i];
-                g[k] = d[i] * w[k];
-                sums[0] += g[k];
-                sums[1] = fmaf(g[k], u[k], sums[1]);
+            px[n] = py[n] = {};
+            if (active && c < a.channels) {
+                px[n] = load<T, VEC>(rowX + c);
+                py[n] = load<T, VEC>(rowY + c);
             }
         }
-        if (dx == nullptr) continue;
-        rowSum<G, 2>(sums, shared, half);
-        if (!active) continue;
-        const float m0 = sums[0] * invC, m1 = sums[1] * invC;
+        float2 s0 = {0.f, 0.f}, s1 = {0.f, 0.f};
+        if constexpr (VEC > 1) {
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + lane) * VEC;
-            if (c >= a.channels) continue;
-            float f[VEC];
+            for (int n = 0; n < NV; ++n) {
+                float fw[VEC];
+                w.get(n, fw);
+                const Piece<T, VEC> p(px[n], py[n], fw, mean, rstd);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int k = n * VEC + i;
-                f[i] = rstd * (g[k] - m0 - u[k] * m1);
+                for (int i = 0; i < VEC / 2; ++i) {
+                    float2 &sw = dw[n * VEC / 2 + i], &sb = db[n * VEC / 2 + i];
+                    sw = fma2(p.d[i], p.u[i], sw);
+                    sb = add2(sb, p.d[i]);
+                    s0 = add2(s0, p.g[i]);
+                    s1 = fma2(p.g[i], p.u[i], s1);
+                }
             }
-            store<T, VEC>(dx + row * a.gradX.stride + c, pack<T, VEC>(f));
+        } else {
+            float *sw = reinterpret_cast<float*>(dw), *sb = reinterpret_cast<float*>(db);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                float fw[1];
+                w.get(n, fw);
+                const float d = Element<T>::to(py[n].v[0]), u = (Element<T>::to(px[n].v[0]) - mean) * rstd, g = d * fw[0];
+                sw[n] = fmaf(d, u, sw[n]);
+                sb[n] += d;
+                s0.x += g;
+                s1.x = fmaf(g, u, s1.x);
+            }
+        }
+        float sums[2] = {s0.x + s0.y, s1.x + s1.y};
+        if (dx != nullptr) rowSum<G, 2>(sums, shared, half);
+        else if (RINGED) __syncthreads();
+        auto release = [&] {   // behind a barrier: the slot has been read
+            const long long after = row + a.ringStages * step;
+            if (threadIdx.x == 0 && after < a.rows) ring.issue(ring.stage, x + after * a.x.stride, dy + after * a.gradY.stride);
+            ring.advance();
+        };
+        if constexpr (RINGED && !TWICE) release();
+        if (dx != nullptr && active) {
+            const float m0 = sums[0] * invC, m1 = sums[1] * invC;
+            T* out = dx + row * a.gradX.stride;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int c = (n * G + lane) * VEC;
+                if (c >= a.channels) continue;
+                if constexpr (TWICE) {
+                    px[n] = load<T, VEC>(rowX + c);
+                    py[n] = load<T, VEC>(rowY + c);
+                }
+                float f[VEC], fw[VEC];
+                w.get(n, fw);
+                if constexpr (VEC > 1) {
+                    const Piece<T, VEC> p(px[n], py[n], fw, mean, rstd);
+#pragma unroll
+                    for (int i = 0; i < VEC / 2; ++i) {
+                        const float2 v = mul2(add2(fma2(p.u[i], both(-m1), p.g[i]), both(-m0)), both(rstd));
+                        f[2 * i] = v.x;
+                        f[2 * i + 1] = v.y;
+                    }
+                } else {
+                    const float u = (Element<T>::to(px[n].v[0]) - mean) * rstd;
+                    f[0] = (fmaf(-u, m1, Element<T>::to(py[n].v[0]) * fw[0]) - m0) * rstd;
+                }
+                store<T, VEC>(out + c, pack<T, VEC>(f));
+            }
+        }
+        if constexpr (RINGED && TWICE) {
+            __syncthreads();
+            release();
         }
     }
+    if (RINGED && !ring.ok) atomicOr(a.status, 1);
     if (a.partial == nullptr) return;
     float* out = a.partial + static_cast<long long>(blockIdx.x) * 2 * a.channels;
     if constexpr (GROUPS == 1) {
@@ -174,8 +441,8 @@ __global__ void __launch_bounds__(threadsFor(G)) layer_norm_adjoint_kernel(const
         for (int i = 0; i < EPT; ++i) {
             const int c = (i / VEC * G + lane) * VEC + i % VEC;
             if (c < a.channels) {
-                out[c] = dw[i];
-                out[a.channels + c] = db[i];
+                out[c] = reinterpret_cast<const float*>(dw)[i];
+                out[a.channels + c] = reinterpret_cast<const float*>(db)[i];
             }
         }
     } else {
@@ -186,8 +453,8 @@ __global__ void __launch_bounds__(threadsFor(G)) layer_norm_adjoint_kernel(const
 #pragma unroll
                 for (int i = 0; i < EPT; ++i) {
                     const int k = i * G + lane;
-                    sumW[k] = r == 0 ? dw[i] : sumW[k] + dw[i];
-                    sumB[k] = r == 0 ? db[i] : sumB[k] + db[i];
+                    sumW[k] = (r == 0 ? 0.f : sumW[k]) + reinterpret_cast<const float*>(dw)[i];
+                    sumB[k] = (r == 0 ? 0.f : sumB[k]) + reinterpret_cast<const float*>(db)[i];
                 }
             }
             __syncthreads();
@@ -309,8 +576,6 @@ unsigned blocksFor(long long rows, int groups, int numSMs, int perSM)
     const long long wanted = (rows + groups - 1) / groups, most = static_cast<long long>(numSMs) * perSM;
     return static_cast<unsigned>(std::max<long long>(1, std::min(wanted, most)));
 }
-// blocks per SM of a kernel of one row per G threads: what the registers allow
-constexpr int perSM(int g) { return g <= 32 ? 2 : g <= 256 ? 512 / g : 1; }
 constexpr int groupsOf(int g) { return g <= 32 ? 256 / g : 1; }
 
 // calls f<G, EPT>() for a row of `channels` elements
@@ -346,6 +611,21 @@ unsigned adjointBlocks(long long rows, int channels, int numSMs)
     return blocks;
 }
 
+// A kernel with a ring of rows: as many slots as `perSM` blocks on an SM have room for, at least one (a slot of two rows of 16384
+// floats takes 128 KB).
+template <class K>
+cudaError_t launchRinged(K kernel, LayerNormArgs a, int matrices, unsigned blocks, int threads, int perSM, cudaStream_t stream)
+{
+    constexpr int SHARED = 224 * 1024;
+    const int slot = matrices * a.channels * typeBytes(a.type);
+    a.ringStages = std::max(1, std::min(RING_MAX, (SHARED / perSM - 2048) / slot));
+    const int bytes = 128 + a.ringStages * slot;
+    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), SHARED);
+    if (e != cudaSuccess) return e;
+    kernel<<<blocks, threads, bytes, stream>>>(a);
+    return cudaGetLastError();
+}
+
 } // namespace
 
 int layerNormPartials(long long rows, int channels, int, int numSMs) { return static_cast<int>(adjointBlocks(rows, channels, numSMs)); }
@@ -362,9 +642,12 @@ cudaError_t launchLayerNormForward(const LayerNormArgs& a, cudaStream_t stream)
         const bool vec = wide(a.x, a.type, a.channels) && wide(a.y, a.type, a.channels);
         return byWidth(a.channels, [&](auto g, auto e) {
             constexpr int G = decltype(g)::value, EPT = decltype(e)::value;
-            const unsigned blocks = blocksFor(a.rows, groupsOf(G), a.numSMs, 2048 / threadsFor(G));
-            if (vec) layer_norm_forward_kernel<T, WIDE<T>, G, EPT><<<blocks, threadsFor(G), 0, stream>>>(a);
-            else layer_norm_forward_kernel<T, 1, G, EPT><<<blocks, threadsFor(G), 0, stream>>>(a);
+            if constexpr (G > 32) {
+                if (vec) return launchRinged(layer_norm_forward_kernel<T, WIDE<T>, G, EPT, true>, a, 1, blocksFor(a.rows, 1, a.numSMs, forwardPerSM(G)), G, forwardPerSM(G), stream);
+            }
+            const unsigned blocks = blocksFor(a.rows, groupsOf(G), a.numSMs, 2 * forwardPerSM(G));
+            if (vec && G <= 32) layer_norm_forward_kernel<T, WIDE<T>, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
+            else layer_norm_forward_kernel<T, 1, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
             return cudaGetLastError();
         });
     });
@@ -391,8 +674,11 @@ cudaError_t launchLayerNormAdjoint(const LayerNormArgs& a, cudaStream_t stream)
             const bool vec = wide(a.x, a.type, a.channels) && wide(a.gradY, a.type, a.channels) && wide(a.gradX, a.type, a.channels);
             return byWidth(a.channels, [&](auto g, auto n) {
                 constexpr int G = decltype(g)::value, EPT = decltype(n)::value;
-                if (vec) layer_norm_adjoint_kernel<T, WIDE<T>, G, EPT><<<blocks, threadsFor(G), 0, stream>>>(a);
-                else layer_norm_adjoint_kernel<T, 1, G, EPT><<<blocks, threadsFor(G), 0, stream>>>(a);
+                if constexpr (G > 32) {
+                    if (vec) return launchRinged(layer_norm_adjoint_kernel<T, WIDE<T>, G, EPT, true>, a, 2, blocks, G, perSM(G), stream);
+                }
+                if (vec && G <= 32) layer_norm_adjoint_kernel<T, WIDE<T>, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
+                else layer_norm_adjoint_kernel<T, 1, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
                 return cudaGetLastError();
             });
         });

@@ -35,6 +35,8 @@ struct LayerNormArgs {
     void *gradWeight, *gradBias;   // of type weight.type / gradBiasType, may be null
     int gradWeightType, gradBiasType;
     float* partial;       // scratch: layerNormPartials() rows of 2 x channels sums
+    int* status;          // the library's status word
+    int ringStages;       // set by the launcher
 };
 // blocks whose partial sums of the parameters' gradients the adjoint leaves in its scratch (an upper bound)
 int layerNormPartials(long long rows, int channels, int type, int numSMs);

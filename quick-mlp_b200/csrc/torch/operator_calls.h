@@ -324,10 +324,12 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
         auto r = QMLP_CALL("layer_norm_forward", layerNormForward).call(input, weight, bias, epsilon);
         ctx->save_for_backward({input, weight.value_or(Tensor()), bias.value_or(Tensor()), std::get<1>(r)});
         ctx->mark_non_differentiable({std::get<1>(r)});
+        ctx->set_materialize_grads(false);   // (a fill kernel for every output nobody differentiates)
         return {std::get<0>(r), std::get<1>(r)};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grad)
     {
+        if (!grad[0].defined()) return variable_list(4);
         const auto s = ctx->get_saved_variables();
         const bool wx = ctx->needs_input_grad(0), ww = s[1].defined() && ctx->needs_input_grad(1), wb = s[2].defined() && ctx->needs_input_grad(s[1].defined() ? 2 : 1);
         auto g = QMLP_CALL("layer_norm_adjoint", layerNormAdjoint).call(s[0], grad[0], optional(s[1]), optional(s[2]), s[3], wx, ww, wb);
@@ -396,10 +398,12 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
         ctx->save_for_backward({logits, weights, experts});
         ctx->saved_data["normalize"] = normalize;
         ctx->mark_non_differentiable({experts, order, positions, offsets});
+        ctx->set_materialize_grads(false);
         return {weights, experts, order, positions, offsets};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grad)
     {
+        if (!grad[0].defined()) return variable_list(3);
         const auto s = ctx->get_saved_variables();
         return {QMLP_CALL("route_adjoint", routeAdjoint).call(s[0], ctx->saved_data["normalize"].toBool(), s[1], s[2], grad[0]), Tensor(), Tensor()};
     }
