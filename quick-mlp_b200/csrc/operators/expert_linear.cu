@@ -14,13 +14,19 @@
 // products those only fill rows of D that are not stored; in the third they are zeroed in shared memory before the tensor core
 // reads them (a zero in one operand would not do: another expert's infinity times zero is NaN).
 //
-// One persistent block per SM: a TMA warp, an MMA warp, four epilogue warps; a ring of operand stages between the first two, two
-// accumulators between the last two, so that the products of a tile run under the epilogue of the one before. Which tile is
-// whose follows from the offsets, which every block adds up for itself: the group sizes never travel to the host.
+// One persistent block per SM, or a pair of blocks that share tiles of 256 x 256 (cta_group::2; each block loads half of either operand):
+// a TMA warp, an MMA warp, two groups of four epilogue warps, one per accumulator, so that the products of a tile run under the
+// epilogues of the two before; in the weight product four more warps add up the columns of dy for the bias gradient, from the
+// stages that are in shared memory anyway. Which tile is whose follows from the offsets, which every block adds up for itself: the group
+// sizes never travel to the host. 16 experts, 131072 rows, 1024 -> 1024 bfloat16: 226, 226 and 244 us for the three products, 12 us more
+// with the bias gradient (1.1 to 1.2 PFLOP/s; a library product of one matrix of that size 194 us; 128 x 256 tiles of single blocks
+// 254, 239 and 346 us: operands at 192 bytes a clock ask for more than shared memory has). 512 experts, 1000003 rows, 64 -> 64 half: 54, 55
+// and 69 us, bound by memory (40 us each at the copy rate) and the latency of an epilogue.
 // Waits are bounded: on a timeout the block drains, gives its tensor memory back and sets the library's status word.
 #include "common.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include <cuda.h>
@@ -32,29 +38,86 @@ namespace {
 using namespace ops;
 
 // ---- PTX ---------------------------------------------------------------------------------------------------------------
+// ---- pairs of blocks: the leader (rank 0) issues the products of both, its barriers are reached from the other by their cluster address
+__device__ __forceinline__ uint32_t clusterRank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t inBlock(uint32_t address, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void clusterArriveBarrier(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void clusterSync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int CTAS>
 __device__ __forceinline__ void tmaLoad2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+    // (.cta_group::2: the barrier may be the other block's; the destination is this block's own, nothing is multicast)
+    if constexpr (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+template <int CTAS>
 __device__ __forceinline__ void tmaLoad3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar)
 {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void fenceProxyAsync() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <int CTAS>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)) : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)) : "memory");
 }
+// arrives on the barrier (of both blocks, at the same place) when the products issued so far are done
+template <int CTAS>
 __device__ __forceinline__ void mmaCommit(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
-// 32 consecutive fp32 columns of this thread's lane of tensor memory
+template <int CTAS>
+__device__ __forceinline__ void tmemAlloc(uint32_t at, uint32_t columns)
+{
+    if constexpr (CTAS == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void tmemFree(uint32_t at, uint32_t columns)
+{
+    if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+}
+// 32 consecutive fp32 columns of this thread's lane of tensor memory; there after tmemWait
 __device__ __forceinline__ void tmemLoad32(uint32_t at, float (&v)[32])
 {
     uint32_t r[32];
@@ -65,9 +128,15 @@ __device__ __forceinline__ void tmemLoad32(uint32_t at, float (&v)[32])
                    "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
                    "=r"(r[30]), "=r"(r[31])
                  : "r"(at) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// (the values are operands: nothing that uses them may move in front of the wait)
+__device__ __forceinline__ void tmemWait(float (&v)[32], float (&w)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]), "+f"(w[i]));
 }
 // descriptor of a 128-byte swizzled operand: groups of 8 rows of 128 bytes lie 1024 bytes apart. K-major: the rows are rows of the
 // operand. MN-major: the rows run along the sum, and blocks of 64 rows of the operand lie `lead` bytes apart.
@@ -78,19 +147,25 @@ __device__ __forceinline__ uint64_t operandDescriptor(uint32_t address, uint32_t
 
 // ---- plan ------------------------------------------------------------------------------------------------------------------
 enum Product : int { FORWARD = 0, INPUT = 1, WEIGHTS = 2 };
-constexpr int BM = 128, BK = 64, BOX = 64 * 128;   // tile of D, block along the sum, bytes of a box of 64 x 64 elements
-constexpr int EPILOGUE_WARPS = 4, BLOCK = (2 + EPILOGUE_WARPS) * 32;
+constexpr int BM = 128, BK = 64, BOX = 64 * 128;   // rows of D per block, step along the sum, bytes of a box of 64 x 64 elements
+constexpr int EPILOGUE_GROUPS = 2, EPILOGUE_WARPS = 4 * EPILOGUE_GROUPS, SUM_WARPS = 4;
+constexpr int EPILOGUE_BYTES = 32 * 64 + 128;      // per warp: 32 rows x 32 elements of 16 bits, 32 floats of bias
+// producer, products, epilogue; the weight gradient with a bias gradient: warps that sum the columns of dy
+__host__ __device__ constexpr int blockThreads(bool sums) { return (2 + EPILOGUE_WARPS + (sums ? SUM_WARPS : 0)) * 32; }
 
-template <int BN>
+// BN: columns of D; CTAS: blocks that share a tile, each with BM rows of D and BN / CTAS of the columns of B
+template <int BN, int CTAS>
 struct Layout {
-    static constexpr int ABYTES = BM * 128, BBYTES = BN * 128, STAGE = ABYTES + BBYTES;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int ACC = BN;                    // columns of an accumulator
-    static constexpr int TMEM = 2 * ACC < 32 ? 32 : 2 * ACC;
-    static constexpr int OUT = EPILOGUE_WARPS * 32 * 128;   // 32 rows x 64 elements of 16 bits per epilogue warp
-    static constexpr int BARS = 16 * 8 + 4 * 8 + 32;
+    static constexpr int BCOLS = BN / CTAS, ABYTES = BM * 128, BBYTES = BCOLS * 128, STAGE = ABYTES + BBYTES;
+    static constexpr int STAGES = 192 * 1024 / STAGE;
+    static constexpr int TMEM = 2 * BN;
+    static constexpr int OUT = EPILOGUE_WARPS * EPILOGUE_BYTES;
+    // barriers: full, empty, landed (STAGES each, at most 8), accumulator full, empty (2 each), tail, drain; then flag and tensor memory
+    static constexpr int FULL = 0, EMPTY = 64, LANDED = 128, ACC_FULL = 192, ACC_EMPTY = 208, TAIL = 224, DRAIN = 232, FAILED = 240, BASE = 244, BARS = 256;
     // 1 KB for the alignment of the ring
     static constexpr int bytes(int experts) { return 1024 + STAGES * STAGE + OUT + BARS + 2 * (experts + 1) * 4; }
+    static_assert(STAGES <= 8, "barriers");
+    static_assert(bytes(EXPERTS_MAX) <= 227 * 1024, "shared memory");
 };
 
 struct ProductArgs {
@@ -98,6 +173,7 @@ struct ProductArgs {
     int experts, columns, sum;    // columns of D; length of the sum (forward, input), channels out (weights)
     int rowTiles, columnTiles;    // weights: tiles of D; else columnTiles alone
     int chunk;                    // weights: rows of an expert per item
+    int tileRows;                 // rows of D per tile: BM x CTAS
     const int* offsets;
     void* out;
     long long outStride;          // elements between rows of D in memory
@@ -105,6 +181,8 @@ struct ProductArgs {
     int* plan;                    // weights: units of the experts before, written for the join; null where no expert can have two
     float* partial;               // weights: items x tiles x 128 x BN sums of experts with more than one item
     int* status;
+    void* gradBias;               // weights: (experts, channels out) or null
+    float* partialBias;           // weights: items x tiles of rows x tileRows sums of experts with more than one item
     bool wideStore;               // rows of D can be written 16 bytes at a time
 };
 
@@ -117,7 +195,7 @@ __device__ __forceinline__ int clampOffset(const ProductArgs& p, int e)
 template <int MODE>
 __device__ __forceinline__ int unitsOf(const ProductArgs& p, int rows)
 {
-    return MODE == WEIGHTS ? max(1, (rows + p.chunk - 1) / p.chunk) : (rows + BM - 1) / BM;
+    return MODE == WEIGHTS ? max(1, (rows + p.chunk - 1) / p.chunk) : (rows + p.tileRows - 1) / p.tileRows;
 }
 // One warp: bounds[e] = first row of expert e, bounds[experts] the end of the last one; before[e] = units of the experts before.
 template <int MODE>
@@ -158,19 +236,27 @@ __device__ __forceinline__ void planExperts(const ProductArgs& p, int* bounds, i
 struct Tile {
     int expert, unit, units, begin, end, row, column;
 };
-// Walks the tiles of a block. All threads of a warp call next() together: 32 experts are looked at in one step.
-template <int MODE, int BN>
+// Walks every stride-th tile from `first` on. All threads of a warp call next() together: 32 experts are looked at in one step.
+template <int MODE, int BN, int CTAS>
 struct Walk {
-    const ProductArgs& p;
+    const ProductArgs* args;
     const int *bounds, *before;   // planExperts
-    long long tile;
-    int expert = 0;
-    __device__ __forceinline__ Walk(const ProductArgs& args, const int* rows, const int* units) : p(args), bounds(rows), before(units), tile(blockIdx.x) {}
+    long long tile, total;
+    int perUnit, stride, expert = 0;
+    __device__ __forceinline__ Walk(const ProductArgs& p, const int* rows, const int* units, int first, int step)
+        : args(&p), bounds(rows), before(units), tile(first), stride(step)
+    {
+        perUnit = MODE == WEIGHTS ? p.rowTiles * p.columnTiles : p.columnTiles;
+        total = static_cast<long long>(before[p.experts]) * perUnit;
+    }
     __device__ __forceinline__ bool next(Tile& t)
     {
-        const long long perUnit = MODE == WEIGHTS ? static_cast<long long>(p.rowTiles) * p.columnTiles : p.columnTiles;
-        if (tile >= before[p.experts] * perUnit) return false;
-        const int unit = static_cast<int>(tile / perUnit), at = static_cast<int>(tile - unit * perUnit);
+        const ProductArgs& p = *args;
+        if (tile >= total) return false;
+        const int unit = perUnit == 1          ? static_cast<int>(tile)
+                         : total <= 0x7fffffff ? static_cast<int>(static_cast<unsigned>(tile) / static_cast<unsigned>(perUnit))
+                                               : static_cast<int>(tile / perUnit);
+        const int at = static_cast<int>(tile - static_cast<long long>(unit) * perUnit);
         const int lane = threadIdx.x & 31;
         for (;;) {   // first expert whose units reach behind `unit`
             const int e = expert + 1 + lane;
@@ -183,21 +269,22 @@ struct Walk {
         t.unit = unit - before[expert];
         t.units = before[expert + 1] - before[expert];
         if constexpr (MODE == WEIGHTS) {
+            const int row = at / p.columnTiles;
             t.begin = first + t.unit * p.chunk;
             t.end = min(last, t.begin + p.chunk);
-            t.row = at / p.columnTiles * BM;
-            t.column = at % p.columnTiles * BN;
+            t.row = row * (BM * CTAS);
+            t.column = (at - row * p.columnTiles) * BN;
         } else {
-            t.begin = first + t.unit * BM;
-            t.end = min(last, t.begin + BM);
+            t.begin = first + t.unit * (BM * CTAS);
+            t.end = min(last, t.begin + BM * CTAS);
             t.row = t.begin;
             t.column = at * BN;
         }
-        tile += gridDim.x;
+        tile += stride;
         return true;
     }
-    // blocks along the sum
-    __device__ __forceinline__ int steps(const Tile& t) const { return MODE == WEIGHTS ? (t.end - t.begin + BK - 1) / BK : (p.sum + BK - 1) / BK; }
+    // steps along the sum
+    __device__ __forceinline__ int steps(const Tile& t) const { return MODE == WEIGHTS ? (t.end - t.begin + BK - 1) / BK : (args->sum + BK - 1) / BK; }
 };
 
 // A wait that ends, for a whole warp: on success, when another warp of the block has given up, or after WAIT_LIMIT polls. False: leave.
@@ -216,111 +303,140 @@ __device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, volatile in
 // operand format in the instruction descriptor
 template <class T> constexpr uint32_t FORMAT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
 
-template <class T, int MODE, int BN>
-__global__ void __launch_bounds__(BLOCK, 1)
+// boxes of 64 that `n` elements fill, 0 to `most`
+__device__ __forceinline__ int boxes(int n, int most) { return max(0, min(most, (n + 63) / 64)); }
+
+template <class T, int MODE, int BN, int CTAS, bool SUMS>
+__global__ void __launch_bounds__(blockThreads(SUMS), 1)
     expert_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ ProductArgs p)
 {
-    using L = Layout<BN>;
+    using L = Layout<BN, CTAS>;
     extern __shared__ unsigned char dynamic[];
     const uint32_t raw = smemAddress(dynamic), ring = (raw + 1023u) & ~1023u;
     unsigned char* base = dynamic + (ring - raw);
     unsigned char* outStage = base + L::STAGES * L::STAGE;
     const uint32_t bars = ring + L::STAGES * L::STAGE + L::OUT;
-    const uint32_t full = bars, empty = bars + 8 * 8, accFull = bars + 16 * 8, accEmpty = accFull + 16, drain = bars + 16 * 8 + 4 * 8 + 16;
-    volatile int* failed = reinterpret_cast<volatile int*>(outStage + L::OUT + 16 * 8 + 4 * 8);
-    uint32_t* tmemBase = reinterpret_cast<uint32_t*>(outStage + L::OUT + 16 * 8 + 4 * 8 + 8);
+    const uint32_t full = bars + L::FULL, empty = bars + L::EMPTY, landed = bars + L::LANDED, accFull = bars + L::ACC_FULL, accEmpty = bars + L::ACC_EMPTY;
+    volatile int* failed = reinterpret_cast<volatile int*>(outStage + L::OUT + L::FAILED);
+    uint32_t* tmemBase = reinterpret_cast<uint32_t*>(outStage + L::OUT + L::BASE);
     int *bounds = reinterpret_cast<int*>(outStage + L::OUT + L::BARS), *before = bounds + p.experts + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CTAS == 1 ? 0u : clusterRank();
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::STAGES; ++s) {
-            barrierInit(full + s * 8, 1);
+            barrierInit(full + s * 8, CTAS);
             barrierInit(empty + s * 8, 1);
+            barrierInit(landed + s * 8, 1);
         }
         for (int i = 0; i < 2; ++i) {
             barrierInit(accFull + i * 8, 1);
-            barrierInit(accEmpty + i * 8, EPILOGUE_WARPS);
+            barrierInit(accEmpty + i * 8, 4 * CTAS);
         }
-        barrierInit(drain, 1);
+        barrierInit(bars + L::TAIL, 1);
+        barrierInit(bars + L::DRAIN, 1);
         *failed = 0;
         barrierInitDone();
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddress(tmemBase)), "r"(L::TMEM) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmemAlloc<CTAS>(smemAddress(tmemBase), L::TMEM);
     if (warp == 2) planExperts<MODE>(p, bounds, before);
     fenceBefore();
     __syncthreads();
+    if constexpr (CTAS > 1) clusterSync();   // the other block's barriers are set
     fenceAfter();
     const uint32_t tmem = *tmemBase;
     if (MODE == WEIGHTS && p.plan != nullptr && blockIdx.x == 0)   // for the kernel that joins the partial sums
-        for (int e = threadIdx.x; e <= p.experts; e += BLOCK) p.plan[e] = before[e];
-    Walk<MODE, BN> walk(p, bounds, before);
+        for (int e = threadIdx.x; e <= p.experts; e += blockThreads(SUMS)) p.plan[e] = before[e];
+    const int tile0 = blockIdx.x / CTAS, tileStep = gridDim.x / CTAS;
+    Walk<MODE, BN, CTAS> walk(p, bounds, before, tile0, tileStep);
     Tile t;
 
     if (warp == 0) {
         // ---- operands -------------------------------------------------------------------------------------------------
-        uint32_t stage = 0, phase = 0;
+        uint32_t stage = 0, phase = 0, tailPhase = 0;
         long long issued = 0;
         bool ok = true;
         while (ok && walk.next(t)) {
             const int steps = walk.steps(t);
+            const int row = t.row + rank * BM, column = t.column + rank * L::BCOLS, rowEnd = MODE == WEIGHTS ? p.sum : t.end;
+            const int boxesA = boxes(rowEnd - row, BM / 64), boxesB = boxes(p.columns - column, L::BCOLS / 64);
+            const uint32_t bytes = (boxesA + boxesB) * BOX;   // of this block; of both blocks:
+            const uint32_t allBytes = CTAS == 1 ? bytes : bytes + (boxes(rowEnd - row - BM, BM / 64) + boxes(p.columns - column - L::BCOLS, L::BCOLS / 64)) * BOX;
             for (int k = 0; k < steps; ++k) {
                 if (!await(empty + stage * 8, phase ^ 1, failed)) { ok = false; break; }
+                const uint32_t a = ring + stage * L::STAGE, b = a + L::ABYTES;
+                const uint32_t ready = CTAS == 1 ? full + stage * 8 : inBlock(full + stage * 8, 0);
+                // the last rows of an expert's last step belong to another expert: a pair of blocks clears them before it hands the step on
+                const int left = t.end - t.begin - k * BK, tail = MODE == WEIGHTS && CTAS > 1 && left < BK ? (16 - left % 16) % 16 : 0;
+                const uint32_t bar = tail > 0 ? bars + L::TAIL : ready;
                 if (lane == 0) {
-                    const uint32_t a = ring + stage * L::STAGE, b = a + L::ABYTES, bar = full + stage * 8;
-                    barrierExpect(bar, L::STAGE);
-                    if constexpr (MODE == WEIGHTS) {
-                        const int row = t.begin + k * BK;
-#pragma unroll
-                        for (int i = 0; i < BM / 64; ++i) tmaLoad2(a + i * BOX, &mapA, t.row + i * 64, row, bar);
-#pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tmaLoad2(b + i * BOX, &mapB, t.column + i * 64, row, bar);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < BM / 64; ++i) tmaLoad2(a + i * BOX, &mapA, k * BK, t.begin + i * 64, bar);
-#pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) {
-                            if constexpr (MODE == FORWARD) tmaLoad3(b + i * BOX, &mapB, k * BK, t.column + i * 64, t.expert, bar);
-                            else tmaLoad3(b + i * BOX, &mapB, t.column + i * 64, k * BK, t.expert, bar);
-                        }
+                    // the leader expects the bytes of both blocks, and arrives for both (an arrival from the other block at every step costs more
+                    // than the step: its release takes about a microsecond)
+                    if (tail > 0) barrierExpect(bar, bytes);
+                    else if (rank == 0) {
+                        barrierExpect(full + stage * 8, allBytes);
+                        if (CTAS > 1) barrierArrive(full + stage * 8);
+                    }
+                    for (int i = 0; i < boxesA; ++i) {
+                        if constexpr (MODE == WEIGHTS) tmaLoad2<CTAS>(a + i * BOX, &mapA, row + i * 64, t.begin + k * BK, bar);
+                        else tmaLoad2<CTAS>(a + i * BOX, &mapA, k * BK, row + i * 64, bar);
+                    }
+                    for (int i = 0; i < boxesB; ++i) {
+                        if constexpr (MODE == WEIGHTS) tmaLoad2<CTAS>(b + i * BOX, &mapB, column + i * 64, t.begin + k * BK, bar);
+                        else if constexpr (MODE == FORWARD) tmaLoad3<CTAS>(b + i * BOX, &mapB, k * BK, column + i * 64, t.expert, bar);
+                        else tmaLoad3<CTAS>(b + i * BOX, &mapB, column + i * 64, k * BK, t.expert, bar);
                     }
                 }
                 __syncwarp();
+                if constexpr (MODE == WEIGHTS && CTAS > 1) {
+                    if (tail > 0) {
+                        if (!await(bar, tailPhase, failed)) { ok = false; break; }
+                        tailPhase ^= 1;
+                        for (int i = lane; i < tail * (L::STAGE / BOX) * 8; i += 32) {
+                            const int box = i / (tail * 8), r = left + i / 8 % tail, chunk = i % 8;
+                            *reinterpret_cast<uint4*>(base + stage * L::STAGE + box * BOX + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fenceProxyAsync();
+                        __syncwarp();
+                        if (lane == 0) clusterArriveBarrier(ready);
+                        __syncwarp();
+                    }
+                }
                 ++issued;
                 if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
             }
         }
-        if (!ok) {   // copies in flight land before the block's shared memory is given back
+        if (!ok && rank == 0) {   // copies in flight land before the blocks' shared memory is given back
             const int outstanding = static_cast<int>(min(issued, static_cast<long long>(L::STAGES)));
             for (int i = 0; i < outstanding; ++i) {
                 if (stage == 0) { stage = L::STAGES; phase ^= 1; }
                 --stage;
-                for (uint32_t n = 0; n < WAIT_LIMIT && !barrierTest(full + stage * 8, phase); ++n) {}
+                barrierWait(full + stage * 8, phase);
             }
         }
     } else if (warp == 1) {
         // ---- products -------------------------------------------------------------------------------------------------
-        constexpr uint32_t instruction = (1u << 4) | (FORMAT<T> << 7) | (FORMAT<T> << 10) | (MODE == WEIGHTS ? 1u << 15 : 0u) |
-                                         (MODE != FORWARD ? 1u << 16 : 0u) | (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
-        uint32_t stage = 0, phase = 0, acc = 0, accPhase = 0;
-        bool ok = true;
+        constexpr uint32_t instruction = (1u << 4) | (FORMAT<T> << 7) | (FORMAT<T> << 10) | (MODE == WEIGHTS ? 1u << 15 : 0u) | (MODE != FORWARD ? 1u << 16 : 0u) |
+                                         (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>((BM * CTAS) >> 4) << 24);
+        uint32_t stage = 0, phase = 0, acc = 1, accPhases = 0;   // accPhases: one bit per accumulator
+        bool ok = rank == 0;
         while (ok && walk.next(t)) {
             const int steps = walk.steps(t);
+            acc ^= 1;                   // the tiles' numbers alternate between the accumulators
             if (steps == 0) continue;   // an expert without rows: the epilogue writes zeros
-            if (!await(accEmpty + acc * 8, accPhase ^ 1, failed)) break;
+            if (!await(accEmpty + acc * 8, (accPhases >> acc & 1) ^ 1, failed)) break;
+            accPhases ^= 1u << acc;
             fenceAfter();
-            const uint32_t d = tmem + acc * L::ACC;
+            const uint32_t d = tmem + acc * BN;
             for (int k = 0; k < steps; ++k) {
                 if (!await(full + stage * 8, phase, failed)) { ok = false; break; }
                 fenceAfter();
                 const uint32_t a = ring + stage * L::STAGE, b = a + L::ABYTES;
                 const int left = MODE == WEIGHTS ? t.end - t.begin - k * BK : p.sum - k * BK, parts = min(BK, left + 15) / 16;
-                if (MODE == WEIGHTS && left < parts * 16) {
+                if (MODE == WEIGHTS && CTAS == 1 && left < parts * 16) {
                     // the last rows of the step belong to another expert
                     const int rows = parts * 16 - left;
-                    for (int i = lane; i < rows * ((BM + BN) / 64) * 8; i += 32) {
+                    for (int i = lane; i < rows * (L::STAGE / BOX) * 8; i += 32) {
                         const int box = i / (rows * 8), r = left + i / 8 % rows, chunk = i % 8;
                         *reinterpret_cast<uint4*>(base + stage * L::STAGE + box * BOX + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
                     }
@@ -330,93 +446,120 @@ __global__ void __launch_bounds__(BLOCK, 1)
                 if (lane == 0) {
                     const uint64_t descA = operandDescriptor(a, MODE == WEIGHTS ? BOX : 16), descB = operandDescriptor(b, MODE == FORWARD ? 16 : BOX);
                     // 16 along the sum: 32 bytes of a K-major row, 16 rows of an MN-major block
-                    for (int i = 0; i < parts; ++i)
-                        mma(d, descA + i * (MODE == WEIGHTS ? 2048 >> 4 : 32 >> 4), descB + i * (MODE == FORWARD ? 32 >> 4 : 2048 >> 4), instruction, k + i > 0);
-                    mmaCommit(empty + stage * 8);
-                    if (k == steps - 1) mmaCommit(accFull + acc * 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < parts)
+                            mma<CTAS>(d, descA + i * (MODE == WEIGHTS ? 2048 >> 4 : 32 >> 4), descB + i * (MODE == FORWARD ? 32 >> 4 : 2048 >> 4), instruction, k + i > 0);
+                    mmaCommit<CTAS>((SUMS && t.column == 0 ? landed : empty) + stage * 8);   // (the warps that sum come between)
+                    if (k == steps - 1) mmaCommit<CTAS>(accFull + acc * 8);
                 }
                 __syncwarp();
                 if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
             }
-            if (++acc == 2) { acc = 0; accPhase ^= 1; }
         }
-    } else {
-        // ---- epilogue --------------------------------------------------------------------------------------------------
-        const int quarter = warp & 3;   // lanes of tensor memory this warp may read
-        unsigned char* mine = outStage + (warp - 2) * 32 * 128;
+    } else if (warp < 2 + EPILOGUE_WARPS) {
+        // ---- epilogue: two groups of four warps, one per accumulator -------------------------------------------------------
+        const int group = (warp - 2) / 4, quarter = warp & 3;   // quarter: lanes of tensor memory this warp may read
+        unsigned char* mine = outStage + (warp - 2) * EPILOGUE_BYTES;
+        float* mineBias = reinterpret_cast<float*>(mine + 32 * 64);
+        const uint32_t released = CTAS == 1 ? accEmpty + group * 8 : inBlock(accEmpty + group * 8, 0);
         T* out = static_cast<T*>(p.out);
-        uint32_t acc = 0, accPhase = 0;
+        uint32_t accPhase = 0;
+        walk = Walk<MODE, BN, CTAS>(p, bounds, before, tile0 + group * tileStep, EPILOGUE_GROUPS * tileStep);
         while (walk.next(t)) {
             const int steps = walk.steps(t);
+            const int tileRow = t.row + rank * BM;
+            float bias[BN / 32];   // of column c * 32 + lane
+            if constexpr (MODE == FORWARD) {
+                const T* row = static_cast<const T*>(p.bias) + static_cast<long long>(t.expert) * p.columns + t.column;
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) bias[i] = p.bias != nullptr && t.column + i * 32 + lane < p.columns ? Element<T>::to(row[i * 32 + lane]) : 0.f;
+            }
             if (steps > 0) {
-                if (!await(accFull + acc * 8, accPhase, failed)) break;
+                if (!await(accFull + group * 8, accPhase, failed)) break;
+                accPhase ^= 1;
                 fenceAfter();
             }
-            const uint32_t from = tmem + acc * L::ACC + (static_cast<uint32_t>(quarter * 32) << 16);
+            const uint32_t from = tmem + group * BN + (static_cast<uint32_t>(quarter * 32) << 16);
             // rows of D in memory: expert by expert, channels out (weights); the tile's own rows (else)
-            const int rowsLeft = (MODE == WEIGHTS ? p.sum - t.row : t.end - t.row) - quarter * 32;
-            const long long firstRow = (MODE == WEIGHTS ? static_cast<long long>(t.expert) * p.sum : 0ll) + t.row + quarter * 32;
+            const int rowsLeft = (MODE == WEIGHTS ? p.sum : t.end) - tileRow - quarter * 32;
+            const long long firstRow = (MODE == WEIGHTS ? static_cast<long long>(t.expert) * p.sum : 0ll) + tileRow + quarter * 32;
             const bool split = MODE == WEIGHTS && t.units > 1;
             float* partial = nullptr;
             if constexpr (MODE == WEIGHTS) {
-                const long long item = before[t.expert] + t.unit, tileAt = static_cast<long long>(t.row / BM) * p.columnTiles + t.column / BN;
-                partial = p.partial + ((item * p.rowTiles * p.columnTiles + tileAt) * BM + quarter * 32 + lane) * BN;
+                const long long item = before[t.expert] + t.unit, tileAt = static_cast<long long>(t.row / (BM * CTAS)) * p.columnTiles + t.column / BN;
+                partial = p.partial + ((item * p.rowTiles * p.columnTiles + tileAt) * (BM * CTAS) + rank * BM + quarter * 32 + lane) * BN;
             }
-            for (int c0 = 0; c0 < BN && t.column + c0 < p.columns; c0 += 64) {
+            // 64 columns of the accumulator at a time, 32 through shared memory
+#pragma unroll
+            for (int pair = 0; pair < BN / 64; ++pair) {
+                if (t.column + pair * 64 >= p.columns || rowsLeft <= 0) break;
+                float v[2][32];
+                if (steps > 0) {
+                    tmemLoad32(from + pair * 64, v[0]);
+                    tmemLoad32(from + pair * 64 + 32, v[1]);
+                    tmemWait(v[0], v[1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0.f;
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float v[32];
-                    if (steps > 0) tmemLoad32(from + c0 + h * 32, v);
-                    else {
+                    const int c0 = pair * 64 + h * 32;
+                    if (t.column + c0 >= p.columns) break;
+                    if (split) {
+                        if (lane < rowsLeft) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-                    }
-                    if (MODE == WEIGHTS && split) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(partial + c0 + h * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(partial + c0 + i) = make_float4(v[h][i], v[h][i + 1], v[h][i + 2], v[h][i + 3]);
+                        }
                         continue;
                     }
-                    if (MODE == FORWARD && p.bias != nullptr) {
-                        const T* bias = static_cast<const T*>(p.bias) + static_cast<long long>(t.expert) * p.columns;
+                    if constexpr (MODE == FORWARD) {
+                        if (p.bias != nullptr) {
+                            mineBias[lane] = bias[pair * 2 + h];
+                            __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int c = t.column + c0 + h * 32 + i;
-                            v[i] += c < p.columns ? Element<T>::to(bias[c]) : 0.f;
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 f = *reinterpret_cast<const float4*>(mineBias + i);
+                                v[h][i] += f.x;
+                                v[h][i + 1] += f.y;
+                                v[h][i + 2] += f.z;
+                                v[h][i + 3] += f.w;
+                            }
                         }
                     }
+                    // rows of 64 bytes, their 16-byte chunks exchanged so that neither side meets a bank twice
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float f[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) f[k] = v[i * 8 + k];
-                        store<T, 8>(reinterpret_cast<T*>(mine + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)), pack<T, 8>(f));
+                        for (int k = 0; k < 8; ++k) f[k] = v[h][i * 8 + k];
+                        store<T, 8>(reinterpret_cast<T*>(mine + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)), pack<T, 8>(f));
                     }
-                }
-                if (MODE == WEIGHTS && split) continue;
-                __syncwarp();
-                if (p.wideStore) {
+                    __syncwarp();
+                    if (p.wideStore) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + (lane >> 3), chunk = lane & 7, c = t.column + c0 + chunk * 8;
-                        if (r < rowsLeft && c < p.columns)
-                            store<T, 8>(out + (firstRow + r) * p.outStride + c, load<T, 8>(reinterpret_cast<const T*>(mine + r * 128 + ((chunk ^ (r & 7)) << 4))));
-                    }
-                } else {
-                    for (int r = 0; r < 32 && r < rowsLeft; ++r)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int k = h * 32 + lane, c = t.column + c0 + k;
-                            if (c < p.columns)
-                                out[(firstRow + r) * p.outStride + c] = *reinterpret_cast<const T*>(mine + r * 128 + (((k >> 3) ^ (r & 7)) << 4) + (k & 7) * 2);
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = i * 8 + (lane >> 2), chunk = lane & 3, column = t.column + c0 + chunk * 8;
+                            if (r < rowsLeft && column < p.columns)
+                                store<T, 8>(out + (firstRow + r) * p.outStride + column, load<T, 8>(reinterpret_cast<const T*>(mine + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4))));
                         }
+                    } else {
+                        const int column = t.column + c0 + lane;
+                        for (int r = 0; r < 32 && r < rowsLeft; ++r)
+                            if (column < p.columns)
+                                out[(firstRow + r) * p.outStride + column] = *reinterpret_cast<const T*>(mine + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             if (steps > 0) {
                 fenceBefore();
                 __syncwarp();
-                if (lane == 0) barrierArrive(accEmpty + acc * 8);
-                if (++acc == 2) { acc = 0; accPhase ^= 1; }
+                if (lane == 0) {
+                    if constexpr (CTAS == 1) barrierArrive(released);
+                    else clusterArriveBarrier(released);
+                }
             }
         }
         if constexpr (MODE != WEIGHTS) {
@@ -428,25 +571,79 @@ __global__ void __launch_bounds__(BLOCK, 1)
                 for (int c = lane; c < p.columns; c += 32) row[c] = Element<T>::from(0.f);
             }
         }
+    } else if constexpr (SUMS) {
+        // ---- bias gradient: the columns of dy, summed where they lie for the products ----------------------------------------
+        // A thread takes 8 columns (a 16-byte chunk) of every eighth row of a step, when the products of the step are done and before its
+        // stage is handed back; only tiles of the first columns count.
+        const int thread = threadIdx.x - (2 + EPILOGUE_WARPS) * 32;
+        const int chunk = thread >> 3, first = thread & 7;   // chunk of the 16 chunks of 128 columns; 8 neighbouring lanes share one
+        uint32_t stage = 0, phases = 0;                      // phases: one bit per stage
+        bool ok = true;
+        while (ok && walk.next(t)) {
+            const int steps = walk.steps(t);
+            if (t.column != 0) {
+                stage = (stage + steps) % L::STAGES;
+                continue;
+            }
+            const int tileRow = t.row + rank * BM;
+            float2 sum[4] = {};
+            for (int k = 0; k < steps; ++k) {
+                if (!await(landed + stage * 8, phases >> stage & 1, failed)) { ok = false; break; }
+                phases ^= 1u << stage;
+                const int left = t.end - t.begin - k * BK;
+                const unsigned char* box = base + stage * L::STAGE + (chunk >> 3) * BOX;
+                Pack<T, 8> v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * 8 + first;
+                    v[i] = load<T, 8>(reinterpret_cast<const T*>(box + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)));
+                }
+                if (left < BK) {   // rows of another expert
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i * 8 + first >= left) v[i] = {};
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[j] = add2(sum[j], toPair(&v[i].v[2 * j]));
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (thread == 0) barrierArrive(empty + stage * 8);
+                if (++stage == L::STAGES) stage = 0;
+            }
+            if (ok) {
+                float mine = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float all = groupSum<8>(j % 2 == 0 ? sum[j / 2].x : sum[j / 2].y);
+                    mine = first == j ? all : mine;
+                }
+                const int channel = tileRow + chunk * 8 + first;
+                if (channel < p.sum) {
+                    if (t.units > 1) p.partialBias[(static_cast<long long>(before[t.expert]) + t.unit) * p.sum + channel] = mine;
+                    else static_cast<T*>(p.gradBias)[static_cast<long long>(t.expert) * p.sum + channel] = Element<T>::from(mine);
+                }
+            }
+        }
     }
     fenceBefore();
     __syncthreads();
     fenceAfter();
-    if (warp == 1) {
-        if (*failed != 0) {
-            // products that were issued end before the tensor memory is given back
-            if (lane == 0) {
-                mmaCommit(drain);
-                for (uint32_t n = 0; n < WAIT_LIMIT && !barrierTest(drain, 0); ++n) {}
-                atomicOr(p.status, 1);
-            }
-            __syncwarp();
+    if (*failed != 0 && warp == 1 && rank == 0) {
+        // products that were issued end before the tensor memory is given back
+        if (lane == 0) {
+            mmaCommit<CTAS>(bars + L::DRAIN);
+            barrierWait(bars + L::DRAIN, 0);
+            atomicOr(p.status, 1);
         }
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM) : "memory");
+        __syncwarp();
     }
+    if constexpr (CTAS > 1) clusterSync();   // nothing reaches the other block any more
+    if (warp == 1) tmemFree<CTAS>(tmem, L::TMEM);
 }
 
-// adds up the partial sums of the weight gradients of experts with more than one item: a block per 16 rows of a tile of an expert
+// adds up the partial sums of the weight gradients (and, behind the tiles, of the bias gradients) of experts with more than one item:
+// a block per 16 rows of a tile of an expert
 template <class T, int BN>
 __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant__ ProductArgs p)
 {
@@ -454,20 +651,29 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
     const int expert = blockIdx.x / tiles, tile = blockIdx.x % tiles;
     const int before = p.plan[expert], units = p.plan[expert + 1] - before;
     if (units == 1) return;
-    const long long unitStride = static_cast<long long>(tiles) * BM * BN;
-    const float* from = p.partial + before * unitStride + static_cast<long long>(tile) * BM * BN;
-    const int row0 = tile / p.columnTiles * BM, column0 = tile % p.columnTiles * BN;
+    const long long unitStride = static_cast<long long>(tiles) * p.tileRows * BN;
+    const float* from = p.partial + before * unitStride + static_cast<long long>(tile) * p.tileRows * BN;
+    const int row0 = tile / p.columnTiles * p.tileRows, column0 = tile % p.columnTiles * BN;
     for (int i = threadIdx.x; i < 16 * BN; i += 256) {
         const int r = blockIdx.y * 16 + i / BN, c = i % BN;
         if (row0 + r >= p.sum || column0 + c >= p.columns) continue;
         float sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int u = 0; u < units; ++u) sum += from[u * unitStride + r * BN + c];
         static_cast<T*>(p.out)[(static_cast<long long>(expert) * p.sum + row0 + r) * p.outStride + column0 + c] = Element<T>::from(sum);
     }
+    if (p.gradBias != nullptr && column0 == 0 && threadIdx.x < 16) {
+        const int channel = row0 + blockIdx.y * 16 + threadIdx.x;
+        if (channel < p.sum) {
+            float sum = 0.f;
+#pragma unroll 8
+            for (int u = 0; u < units; ++u) sum += p.partialBias[static_cast<long long>(before + u) * p.sum + channel];
+            static_cast<T*>(p.gradBias)[static_cast<long long>(expert) * p.sum + channel] = Element<T>::from(sum);
+        }
+    }
 }
 
-// ---- bias gradient: column sums of an expert's rows ------------------------------------------------------------------------
+// ---- bias gradient without a weight gradient: column sums of an expert's rows ----------------------------------------------------
 // blockIdx.x: expert, blockIdx.y: 32 x 8 columns. 8 warps take strided rows, then join.
 template <class T>
 __global__ void __launch_bounds__(256) expert_bias_kernel(const __grid_constant__ ProductArgs p, const T* __restrict__ dy, long long stride, T* __restrict__ out)
@@ -532,9 +738,18 @@ cudaError_t encodeMap(CUtensorMap& map, int type, const void* data, long long ma
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(matrices)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride) * 2, static_cast<cuuint64_t>(stride) * 2 * rows};
     const cuuint32_t box[3] = {64, 64, 1}, one[3] = {1, 1, 1};
-    const CUresult r = encode(&map, type == TYPE_HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, matrices > 0 ? 3 : 2, const_cast<void*>(data),
-                              dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto run = [&] {
+        return encode(&map, type == TYPE_HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, matrices > 0 ? 3 : 2, const_cast<void*>(data), dims,
+                      strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = run();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {   // a thread's first call (a backward pass runs in a thread of its own): the driver wants a context, which the runtime binds
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e == cudaSuccess) e = cudaSetDevice(device);
+        if (e != cudaSuccess) return e;
+        r = run();
+    }
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
@@ -543,19 +758,46 @@ int pad8(int n) { return (n + 7) / 8 * 8; }
 // rows the TMA can read where they lie
 bool direct(const void* data, long long stride, int columns) { return (reinterpret_cast<uintptr_t>(data) & 15) == 0 && stride % 8 == 0 && stride >= columns; }
 
-int tileWidth(int columns) { return columns <= 64 ? 64 : columns <= 128 ? 128 : 256; }
-
-// rows per item of the weight gradient: enough items that every SM gets a few
-int weightChunk(const ExpertArgs& a, int tiles)
+// Shape of the tiles. Pairs of blocks (256 x 256) read a third less shared memory per product, but cut rows into coarser pieces: taken where
+// D is wide and an expert has rows enough for two such tiles on average.
+struct Shape {
+    int width, ctas;
+};
+Shape shapeOf(long long rows, int columns)
 {
-    const long long items = std::max<long long>(1, 4ll * a.numSMs / tiles);
-    return static_cast<int>(std::min<long long>(std::max<long long>((a.rows / items + 63) / 64 * 64, 512), 1ll << 30));
+    if (columns <= 64) return {64, 1};
+    if (columns <= 128) return {128, 1};
+    return {256, rows >= 512 ? 2 : 1};
+}
+Shape rowShape(const ExpertArgs& a, int columns) { return shapeOf(a.rows / a.experts, columns); }                       // forward, input gradient
+Shape weightShape(const ExpertArgs& a) { return shapeOf(a.channelsOut > 128 ? 512 : 0, a.channelsIn); }                 // weight gradient
+
+// Rows per item of the weight gradient. Cutting an expert's rows fills the blocks where its tiles alone do not, at the price of a write and
+// a read of an fp32 tile per item. The estimate below weighs the two for runs of average length: a step of 64 rows takes about 0.3 us
+// (256 x 256 tiles at the tensor core's rate, narrow ones at the memory's), partial sums move at about 5 TB/s. 64 experts of 4096 rows of
+// 256 x 256: whole runs 49 us, cut into 320 items 74 us and 44 us for their sums. An expert with more than twice the average is cut in any case.
+int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
+{
+    const double run = static_cast<double>(a.rows) / a.experts;
+    double best = 0;
+    int pieces = 1;
+    for (int k = 1; k <= 1024 && (k == 1 || run / k >= 256); k *= 2) {
+        const double items = static_cast<double>(a.experts) * k * tiles;
+        const double time = std::ceil(items / blocks) * std::ceil(run / k / BK) * 0.3 + (k > 1 ? 5.0 + items * tileElements * 8 / 5e6 : 0.0);
+        if (k == 1 || time < best) {
+            best = time;
+            pieces = k;
+        }
+    }
+    const double rows = pieces == 1 ? 2 * run : run / pieces;
+    return static_cast<int>(std::min<double>(std::max<double>(std::ceil(rows / BK) * BK, 512), 1 << 30));
 }
 
-// scratch: [x | weight | dy in a form the TMA reads, where needed | partial sums of the weight gradients]
+// scratch: [x | weight | dy in a form the TMA reads, where needed | partial sums of the weight and bias gradients | their plan]
 struct Scratch {
-    size_t x, weight, gradY, partial, plan, bytes;
-    int chunk, rowTiles, columnTiles, width;
+    size_t x, weight, gradY, partial, partialBias, plan, bytes;
+    int chunk, rowTiles, columnTiles, tileRows;
+    Shape shape;
     Scratch(const ExpertArgs& a, bool adjoint)
     {
         const bool forward = !adjoint;
@@ -570,13 +812,15 @@ struct Scratch {
         x = take((forward || weights) && !direct(a.x.data, a.x.stride, a.channelsIn), rows * pad8(a.channelsIn) * 2);
         weight = take((forward || a.gradX.data != nullptr) && !direct(a.weight, a.channelsIn, a.channelsIn), matrices * pad8(a.channelsIn) * 2);
         gradY = take(adjoint && !direct(a.gradY.data, a.gradY.stride, a.channelsOut), rows * pad8(a.channelsOut) * 2);
-        width = tileWidth(a.channelsIn);
-        rowTiles = (a.channelsOut + BM - 1) / BM;
-        columnTiles = (a.channelsIn + width - 1) / width;
+        shape = weightShape(a);
+        tileRows = BM * shape.ctas;
+        rowTiles = (a.channelsOut + tileRows - 1) / tileRows;
+        columnTiles = (a.channelsIn + shape.width - 1) / shape.width;
         const int tiles = rowTiles * columnTiles;
-        chunk = weightChunk(a, tiles);
+        chunk = weightChunk(a, tiles, tileRows * shape.width, a.numSMs / shape.ctas);
         const size_t items = a.rows > chunk ? a.experts + rows / chunk : 0;
-        partial = take(weights && items > 0, items * tiles * BM * width * 4);
+        partial = take(weights, items * tiles * tileRows * shape.width * 4);
+        partialBias = take(weights, items * a.channelsOut * 4);
         plan = take(weights && items > 0, (static_cast<size_t>(a.experts) + 1) * 4);
     }
 };
@@ -593,23 +837,32 @@ cudaError_t readable(const void*& data, long long& stride, long long rows, int c
     return cudaGetLastError();
 }
 
-template <class T, int MODE, int BN>
-cudaError_t launchProduct(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, int blocks, cudaStream_t stream)
+template <class T, int MODE, int BN, int CTAS, bool SUMS>
+cudaError_t launchProduct(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, int numSMs, cudaStream_t stream)
 {
-    auto* kernel = expert_product_kernel<T, MODE, BN>;
-    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), Layout<BN>::bytes(EXPERTS_MAX));
+    auto* kernel = expert_product_kernel<T, MODE, BN, CTAS, SUMS>;
+    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), Layout<BN, CTAS>::bytes(EXPERTS_MAX));
     if (e != cudaSuccess) return e;
-    kernel<<<blocks, BLOCK, Layout<BN>::bytes(p.experts), stream>>>(a, b, p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(numSMs / CTAS * CTAS);
+    config.blockDim = dim3(blockThreads(SUMS));
+    config.dynamicSmemBytes = Layout<BN, CTAS>::bytes(p.experts);
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = CTAS;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = CTAS > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, a, b, p);
 }
-template <class T, int MODE>
-cudaError_t launchWidth(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, int blocks, cudaStream_t stream)
+template <class T, int MODE, bool SUMS = false>
+cudaError_t launchShape(const Shape& shape, const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, int numSMs, cudaStream_t stream)
 {
-    switch (tileWidth(p.columns)) {
-    case 64: return launchProduct<T, MODE, 64>(a, b, p, blocks, stream);
-    case 128: return launchProduct<T, MODE, 128>(a, b, p, blocks, stream);
-    default: return launchProduct<T, MODE, 256>(a, b, p, blocks, stream);
-    }
+    if (shape.width == 64) return launchProduct<T, MODE, 64, 1, SUMS>(a, b, p, numSMs, stream);
+    if (shape.width == 128) return launchProduct<T, MODE, 128, 1, SUMS>(a, b, p, numSMs, stream);
+    if (shape.ctas == 1) return launchProduct<T, MODE, 256, 1, SUMS>(a, b, p, numSMs, stream);
+    return launchProduct<T, MODE, 256, 2, SUMS>(a, b, p, numSMs, stream);
 }
 
 ProductArgs common(const ExpertArgs& a)
@@ -639,12 +892,14 @@ cudaError_t forward(const ExpertArgs& a, cudaStream_t stream)
     ProductArgs p = common(a);
     p.columns = a.channelsOut;
     p.sum = a.channelsIn;
-    p.columnTiles = (p.columns + tileWidth(p.columns) - 1) / tileWidth(p.columns);
+    const Shape shape = rowShape(a, p.columns);
+    p.columnTiles = (p.columns + shape.width - 1) / shape.width;
+    p.tileRows = BM * shape.ctas;
     p.out = a.y.data;
     p.outStride = a.y.stride;
     p.bias = a.bias;
     p.wideStore = wideOut(p.out, p.outStride, p.columns);
-    return launchWidth<T, FORWARD>(mapX, mapW, p, a.numSMs, stream);
+    return launchShape<T, FORWARD>(shape, mapX, mapW, p, a.numSMs, stream);
 }
 
 template <class T>
@@ -653,7 +908,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
     const Scratch s(a, true);
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
     cudaError_t e = cudaSuccess;
-    if (a.gradBias != nullptr) {
+    if (a.gradBias != nullptr && (a.gradWeight == nullptr || a.rows == 0)) {
         ProductArgs p = common(a);
         p.columns = a.channelsOut;
         expert_bias_kernel<T><<<dim3(a.experts, (a.channelsOut + 31) / 32), 256, 0, stream>>>(p, static_cast<const T*>(a.gradY.data), a.gradY.stride, static_cast<T*>(a.gradBias));
@@ -676,11 +931,13 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         ProductArgs p = common(a);
         p.columns = a.channelsIn;
         p.sum = a.channelsOut;
-        p.columnTiles = (p.columns + tileWidth(p.columns) - 1) / tileWidth(p.columns);
+        const Shape shape = rowShape(a, p.columns);
+        p.columnTiles = (p.columns + shape.width - 1) / shape.width;
+        p.tileRows = BM * shape.ctas;
         p.out = a.gradX.data;
         p.outStride = a.gradX.stride;
         p.wideStore = wideOut(p.out, p.outStride, p.columns);
-        e = launchWidth<T, INPUT>(mapY, mapW, p, a.numSMs, stream);
+        e = launchShape<T, INPUT>(shape, mapY, mapW, p, a.numSMs, stream);
     }
     if (e == cudaSuccess && a.gradWeight != nullptr) {
         e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, a.numSMs, stream);
@@ -697,11 +954,15 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         p.partial = reinterpret_cast<float*>(base + s.partial);
         p.plan = a.rows > s.chunk ? reinterpret_cast<int*>(base + s.plan) : nullptr;
         p.wideStore = wideOut(p.out, p.outStride, p.columns);
-        e = launchWidth<T, WEIGHTS>(mapY, mapX, p, a.numSMs, stream);
+        p.tileRows = s.tileRows;
+        p.gradBias = a.gradBias;
+        p.partialBias = reinterpret_cast<float*>(base + s.partialBias);
+        e = a.gradBias != nullptr ? launchShape<T, WEIGHTS, true>(s.shape, mapY, mapX, p, a.numSMs, stream)
+                                  : launchShape<T, WEIGHTS, false>(s.shape, mapY, mapX, p, a.numSMs, stream);
         if (e == cudaSuccess && a.rows > s.chunk) {
-            const dim3 grid(a.experts * s.rowTiles * s.columnTiles, BM / 16);
-            if (s.width == 64) expert_join_kernel<T, 64><<<grid, 256, 0, stream>>>(p);
-            else if (s.width == 128) expert_join_kernel<T, 128><<<grid, 256, 0, stream>>>(p);
+            const dim3 grid(a.experts * s.rowTiles * s.columnTiles, s.tileRows / 16);
+            if (s.shape.width == 64) expert_join_kernel<T, 64><<<grid, 256, 0, stream>>>(p);
+            else if (s.shape.width == 128) expert_join_kernel<T, 128><<<grid, 256, 0, stream>>>(p);
             else expert_join_kernel<T, 256><<<grid, 256, 0, stream>>>(p);
             e = cudaGetLastError();
         }

@@ -96,7 +96,7 @@ __device__ __forceinline__ float pairSum(const float2 (&v)[N])
 // shared memory does for both: sum (x - mean)^2 = sum over warps of (squares about the warp's mean + count * (warp's mean - mean)^2).
 template <int VEC, int G, int EPT>
 struct Moments {
-    static constexpr int LANES = G < 32 ? G : 32, WARPS = G > 32 ? G / 32 : 1;
+    static constexpr int LANES = G < 32 ? G : 32;
     float invC, invCount;        // elements of the row; of this warp (group of lanes), 0 if it has none
     float otherCount = 0.f, otherInv = 0.f;   // of warp `lane`
     float* shared;               // 2 x 64 floats
@@ -110,6 +110,7 @@ struct Moments {
         invC = 1.f / static_cast<float>(channels);
         invCount = count > 0.f ? 1.f / count : 0.f;
         if constexpr (G > 32) {
+            constexpr int WARPS = G / 32;
             const int l = threadIdx.x & 31;
             if (l == 0) shared[threadIdx.x >> 5] = count;
             __syncthreads();
@@ -130,6 +131,7 @@ struct Moments {
         float squares = groupSum<LANES>(s.x + s.y);
         mean = own;
         if constexpr (G > 32) {
+            constexpr int WARPS = G / 32;
             float* at = shared + half * 64;
             half ^= 1;
             const int l = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -296,7 +296,7 @@ def experts_case(qmlp, x, weight, offsets, bias, grad):
 SHAPES = [  # counts of rows, channels in, channels out
     ([1], 8, 8), ([1, 0, 1], 64, 64), ([5, 0, 3, 0], 16, 24), ([128], 64, 64), ([127, 1, 129, 256], 64, 128), ([130, 0, 0, 70, 64], 128, 64),
     ([300, 5], 200, 136), ([64, 64], 72, 264), ([33] * 40, 64, 64), ([1000, 1], 256, 256), ([513, 2000], 64, 64), ([3000], 32, 48), ([700, 20], 520, 300),
-    ([2, 1, 3], 13, 5), ([200, 17], 77, 65), ([90], 1, 1), ([10, 140], 31, 257), ([40, 0, 30], 130, 7),
+    ([2, 1, 3], 13, 5), ([200, 17], 77, 65), ([1500, 0, 300], 264, 320), ([600, 1029], 144, 392), ([700, 513], 200, 130), ([90], 1, 1), ([10, 140], 31, 257), ([40, 0, 30], 130, 7),
 ]
 
 
@@ -366,6 +366,16 @@ def test_expert_linear_offsets(qmlp):
     x, w, g = rand(95, (300, 32), torch.float16), rand(96, (5, 40, 32), torch.float16), rand(97, (300, 40), torch.float16)
     for bad in ([-5, 100, 50, 400, 200, 1000], [300, 200, 100, 0, 0, 0], [0, 300, 0, 300, 0, 300], [2 ** 31 - 1] * 6, [-2 ** 31] * 6):
         experts_case(qmlp, x, w, torch.tensor(bad, dtype=torch.int32, device="cuda"), None, g)
+
+
+def test_expert_linear_threads(qmlp):
+    """the first call of a thread of its own: nothing has bound the device's context to it yet"""
+    import threading
+    x, w, offsets, got = rand(98, (40, 16), torch.float16), rand(99, (2, 24, 16), torch.float16), offsets_of([25, 15]), []
+    thread = threading.Thread(target=lambda: got.append(qmlp.expert_linear(x, w, offsets)))
+    thread.start()
+    thread.join()
+    assert torch.equal(got[0], qmlp.expert_linear(x, w, offsets))
 
 
 def test_expert_linear_empty(qmlp):
