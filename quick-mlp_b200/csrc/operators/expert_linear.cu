@@ -153,6 +153,11 @@ constexpr int EPILOGUE_BYTES = 32 * 64 + 128;      // per warp: 32 rows x 32 ele
 // producer, products, epilogue; the weight gradient with a bias gradient: warps that sum the columns of dy
 __host__ __device__ constexpr int blockThreads(bool sums) { return (2 + EPILOGUE_WARPS + (sums ? SUM_WARPS : 0)) * 32; }
 
+// Lists in shared memory: bounds, before, and for up to SORTED_MAX experts their order, with room to sort them in
+constexpr int SORTED_MAX = 512;
+__host__ __device__ constexpr int listStride(int experts) { return (experts + 4) / 4 * 4; }
+__host__ __device__ constexpr int listInts(int experts) { return experts <= SORTED_MAX ? 2 * listStride(experts) + SORTED_MAX : 2 * listStride(experts); }
+
 // BN: columns of D; CTAS: blocks that share a tile, each with BM rows of D and BN / CTAS of the columns of B
 template <int BN, int CTAS>
 struct Layout {
@@ -163,7 +168,7 @@ struct Layout {
     // barriers: full, empty, landed (STAGES each, at most 8), accumulator full, empty (2 each), tail, drain; then flag and tensor memory
     static constexpr int FULL = 0, EMPTY = 64, LANDED = 128, ACC_FULL = 192, ACC_EMPTY = 208, TAIL = 224, DRAIN = 232, FAILED = 240, BASE = 244, BARS = 256;
     // 1 KB for the alignment of the ring
-    static constexpr int bytes(int experts) { return 1024 + STAGES * STAGE + OUT + BARS + 2 * (experts + 1) * 4; }
+    static constexpr int bytes(int experts) { return 1024 + STAGES * STAGE + OUT + BARS + listInts(experts) * 4; }
     static_assert(STAGES <= 8, "barriers");
     static_assert(bytes(EXPERTS_MAX) <= 227 * 1024, "shared memory");
 };
@@ -178,7 +183,7 @@ struct ProductArgs {
     void* out;
     long long outStride;          // elements between rows of D in memory
     const void* bias;             // forward: (experts, columns) or null
-    int* plan;                    // weights: units of the experts before, written for the join; null where no expert can have two
+    int2* plan;                   // weights: first item and items of an expert, written for the join; null where no expert can have two
     float* partial;               // weights: items x tiles x 128 x BN sums of experts with more than one item
     int* status;
     void* gradBias;               // weights: (experts, channels out) or null
@@ -197,54 +202,87 @@ __device__ __forceinline__ int unitsOf(const ProductArgs& p, int rows)
 {
     return MODE == WEIGHTS ? max(1, (rows + p.chunk - 1) / p.chunk) : (rows + p.tileRows - 1) / p.tileRows;
 }
-// One warp: bounds[e] = first row of expert e, bounds[experts] the end of the last one; before[e] = units of the experts before.
+// The experts' runs and units of work, for all threads of a block: bounds[e] = first row of expert e, bounds[experts] the end of the last one;
+// before[i] = units of the experts in front of the i-th in `order`. The weight product takes the longest runs first (up to SORTED_MAX
+// experts): its tiles cost what their runs are long, and the blocks' shares come out even. (Offsets are fetched at once: one
+// after the other, 512 experts' cost the kernel 8 us.)
 template <int MODE>
-__device__ __forceinline__ void planExperts(const ProductArgs& p, int* bounds, int* before)
+__device__ __forceinline__ void planExperts(const ProductArgs& p, int* bounds, int* before, int* order, int threads)
 {
-    const int lane = threadIdx.x & 31;
-    int reached = clampOffset(p, 0), carry = 0;
-    if (lane == 0) {
-        bounds[0] = reached;
-        before[0] = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e <= p.experts; e += threads) bounds[e] = clampOffset(p, e);
+    __syncthreads();
+    if (warp == 2) {   // running maximum
+        int reached = bounds[0];
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + lane;
+            int end = e < p.experts ? bounds[e + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end = max(end, up);
+            }
+            end = max(end, reached);
+            if (e < p.experts) bounds[e + 1] = end;
+            reached = __shfl_sync(0xffffffffu, end, 31);
+        }
     }
-    for (int e0 = 0; e0 < p.experts; e0 += 32) {
-        const int e = e0 + lane;
-        int end = e < p.experts ? clampOffset(p, e + 1) : 0;
+    const bool sorted = MODE == WEIGHTS && order != nullptr;
+    if (sorted) {
+        // bitonic, of keys (length, number) that differ, the length cut to 22 bits
+        __syncthreads();
+        const int size = p.experts <= 1 ? 1 : 1 << (32 - __clz(p.experts - 1)), cut = max(0, 10 - __clzll(p.rows) + 32);
+        unsigned* keys = reinterpret_cast<unsigned*>(before);   // (has room for SORTED_MAX, and is not needed yet)
+        for (int e = threadIdx.x; e < size; e += threads) keys[e] = e < p.experts ? static_cast<unsigned>((bounds[e + 1] - bounds[e]) >> cut) << 10 | (e + 1) : 0u;
+        for (int length = 2; length <= size; length *= 2)
+            for (int apart = length / 2; apart > 0; apart /= 2) {
+                __syncthreads();
+                const int i = (threadIdx.x / apart * 2) * apart + threadIdx.x % apart;
+                if (threadIdx.x < size / 2) {
+                    const unsigned x = keys[i], y = keys[i + apart];
+                    if ((x < y) == ((i & length) == 0)) {
+                        keys[i] = y;
+                        keys[i + apart] = x;
+                    }
+                }
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.experts; i += threads) order[i] = static_cast<int>(keys[i] & 1023) - 1;
+        __syncthreads();
+    }
+    if (warp == 2) {
+        __syncwarp();
+        int carry = 0;
+        for (int i0 = 0; i0 < p.experts; i0 += 32) {
+            const int i = i0 + lane, e = i < p.experts ? (sorted ? order[i] : i) : 0;
+            int units = i < p.experts ? unitsOf<MODE>(p, bounds[e + 1] - bounds[e]) : 0;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int up = __shfl_up_sync(0xffffffffu, end, o);
-            if (lane >= o) end = max(end, up);
+            for (int o = 1; o < 32; o *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, units, o);
+                if (lane >= o) units += up;
+            }
+            if (i < p.experts) before[i + 1] = carry + units;
+            carry += __shfl_sync(0xffffffffu, units, 31);
         }
-        end = max(end, reached);
-        const int left = __shfl_up_sync(0xffffffffu, end, 1), begin = lane == 0 ? reached : left;
-        int units = e < p.experts ? unitsOf<MODE>(p, end - begin) : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int up = __shfl_up_sync(0xffffffffu, units, o);
-            if (lane >= o) units += up;
-        }
-        if (e < p.experts) {
-            bounds[e + 1] = end;
-            before[e + 1] = carry + units;
-        }
-        reached = __shfl_sync(0xffffffffu, end, 31);
-        carry += __shfl_sync(0xffffffffu, units, 31);
+        if (lane == 0) before[0] = 0;
     }
 }
 
-// One tile of D: its expert, the run of rows it reads (forward, input: its own rows) and where it lies.
+// One tile of D: its expert (-1: no tile), the unit it belongs to, the expert's units, the run of rows it reads (forward, input: its own rows)
+// and where it lies.
 struct Tile {
-    int expert, unit, units, begin, end, row, column;
+    int expert, item, units, begin, end, row, column;
 };
-// Walks every stride-th tile from `first` on. All threads of a warp call next() together: 32 experts are looked at in one step.
+// Walks the tiles of a block or pair of blocks: one of every round, from alternating ends, so that with the longest first the shares come out
+// even; rounds `round`, `round` + `stride`, ... All threads of a warp call next() together: 32 experts are looked at in one step.
 template <int MODE, int BN, int CTAS>
 struct Walk {
     const ProductArgs* args;
-    const int *bounds, *before;   // planExperts
-    long long tile, total;
-    int perUnit, stride, expert = 0;
-    __device__ __forceinline__ Walk(const ProductArgs& p, const int* rows, const int* units, int first, int step)
-        : args(&p), bounds(rows), before(units), tile(first), stride(step)
+    const int *bounds, *before, *order;   // planExperts
+    long long total;
+    int perUnit, round, stride, at = 0;   // at: place in `order` (the expert itself without one)
+    __device__ __forceinline__ Walk(const ProductArgs& p, const int* rows, const int* units, const int* list, int first, int step)
+        : args(&p), bounds(rows), before(units), order(MODE == WEIGHTS ? list : nullptr), round(first), stride(step)
     {
         perUnit = MODE == WEIGHTS ? p.rowTiles * p.columnTiles : p.columnTiles;
         total = static_cast<long long>(before[p.experts]) * perUnit;
@@ -252,39 +290,44 @@ struct Walk {
     __device__ __forceinline__ bool next(Tile& t)
     {
         const ProductArgs& p = *args;
-        if (tile >= total) return false;
+        const int blocks = gridDim.x / CTAS, block = blockIdx.x / CTAS;
+        const long long tile = static_cast<long long>(round) * blocks + (round & 1 ? blocks - 1 - block : block);
+        if (static_cast<long long>(round) * blocks >= total) return false;
+        round += stride;
+        t.expert = -1;
+        if (tile >= total) return true;   // (the last round may have no tile for this block)
         const int unit = perUnit == 1          ? static_cast<int>(tile)
                          : total <= 0x7fffffff ? static_cast<int>(static_cast<unsigned>(tile) / static_cast<unsigned>(perUnit))
                                                : static_cast<int>(tile / perUnit);
-        const int at = static_cast<int>(tile - static_cast<long long>(unit) * perUnit);
+        const int within = static_cast<int>(tile - static_cast<long long>(unit) * perUnit);
         const int lane = threadIdx.x & 31;
         for (;;) {   // first expert whose units reach behind `unit`
-            const int e = expert + 1 + lane;
-            const unsigned passed = __ballot_sync(0xffffffffu, e <= p.experts && before[e] <= unit);
-            expert += __popc(passed);
+            const int i = at + 1 + lane;
+            const unsigned passed = __ballot_sync(0xffffffffu, i <= p.experts && before[i] <= unit);
+            at += __popc(passed);
             if (passed != 0xffffffffu) break;
         }
-        const int first = bounds[expert], last = bounds[expert + 1];
-        t.expert = expert;
-        t.unit = unit - before[expert];
-        t.units = before[expert + 1] - before[expert];
+        t.expert = order != nullptr ? order[at] : at;
+        const int first = bounds[t.expert], last = bounds[t.expert + 1];
+        t.item = unit;
+        t.units = before[at + 1] - before[at];
+        const int part = unit - before[at];
         if constexpr (MODE == WEIGHTS) {
-            const int row = at / p.columnTiles;
-            t.begin = first + t.unit * p.chunk;
+            const int row = within / p.columnTiles;
+            t.begin = first + part * p.chunk;
             t.end = min(last, t.begin + p.chunk);
             t.row = row * (BM * CTAS);
-            t.column = (at - row * p.columnTiles) * BN;
+            t.column = (within - row * p.columnTiles) * BN;
         } else {
-            t.begin = first + t.unit * (BM * CTAS);
+            t.begin = first + part * (BM * CTAS);
             t.end = min(last, t.begin + BM * CTAS);
             t.row = t.begin;
-            t.column = at * BN;
+            t.column = within * BN;
         }
-        tile += stride;
         return true;
     }
     // steps along the sum
-    __device__ __forceinline__ int steps(const Tile& t) const { return MODE == WEIGHTS ? (t.end - t.begin + BK - 1) / BK : (args->sum + BK - 1) / BK; }
+    __device__ __forceinline__ int steps(const Tile& t) const { return t.expert < 0 ? 0 : MODE == WEIGHTS ? (t.end - t.begin + BK - 1) / BK : (args->sum + BK - 1) / BK; }
 };
 
 // A wait that ends, for a whole warp: on success, when another warp of the block has given up, or after WAIT_LIMIT polls. False: leave.
@@ -319,7 +362,8 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     const uint32_t full = bars + L::FULL, empty = bars + L::EMPTY, landed = bars + L::LANDED, accFull = bars + L::ACC_FULL, accEmpty = bars + L::ACC_EMPTY;
     volatile int* failed = reinterpret_cast<volatile int*>(outStage + L::OUT + L::FAILED);
     uint32_t* tmemBase = reinterpret_cast<uint32_t*>(outStage + L::OUT + L::BASE);
-    int *bounds = reinterpret_cast<int*>(outStage + L::OUT + L::BARS), *before = bounds + p.experts + 1;
+    int *bounds = reinterpret_cast<int*>(outStage + L::OUT + L::BARS), *before = bounds + listStride(p.experts);
+    int* order = p.experts <= SORTED_MAX ? before + listStride(p.experts) : nullptr;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CTAS == 1 ? 0u : clusterRank();
 
@@ -339,16 +383,15 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         barrierInitDone();
     }
     if (warp == 1) tmemAlloc<CTAS>(smemAddress(tmemBase), L::TMEM);
-    if (warp == 2) planExperts<MODE>(p, bounds, before);
+    planExperts<MODE>(p, bounds, before, order, blockThreads(SUMS));
     fenceBefore();
     __syncthreads();
     if constexpr (CTAS > 1) clusterSync();   // the other block's barriers are set
     fenceAfter();
     const uint32_t tmem = *tmemBase;
     if (MODE == WEIGHTS && p.plan != nullptr && blockIdx.x == 0)   // for the kernel that joins the partial sums
-        for (int e = threadIdx.x; e <= p.experts; e += blockThreads(SUMS)) p.plan[e] = before[e];
-    const int tile0 = blockIdx.x / CTAS, tileStep = gridDim.x / CTAS;
-    Walk<MODE, BN, CTAS> walk(p, bounds, before, tile0, tileStep);
+        for (int i = threadIdx.x; i < p.experts; i += blockThreads(SUMS)) p.plan[order != nullptr ? order[i] : i] = make_int2(before[i], before[i + 1] - before[i]);
+    Walk<MODE, BN, CTAS> walk(p, bounds, before, order, 0, 1);
     Tile t;
 
     if (warp == 0) {
@@ -465,9 +508,10 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         const uint32_t released = CTAS == 1 ? accEmpty + group * 8 : inBlock(accEmpty + group * 8, 0);
         T* out = static_cast<T*>(p.out);
         uint32_t accPhase = 0;
-        walk = Walk<MODE, BN, CTAS>(p, bounds, before, tile0 + group * tileStep, EPILOGUE_GROUPS * tileStep);
+        walk = Walk<MODE, BN, CTAS>(p, bounds, before, order, group, EPILOGUE_GROUPS);
         while (walk.next(t)) {
             const int steps = walk.steps(t);
+            if (t.expert < 0) break;
             const int tileRow = t.row + rank * BM;
             float bias[BN / 32];   // of column c * 32 + lane
             if constexpr (MODE == FORWARD) {
@@ -487,7 +531,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
             const bool split = MODE == WEIGHTS && t.units > 1;
             float* partial = nullptr;
             if constexpr (MODE == WEIGHTS) {
-                const long long item = before[t.expert] + t.unit, tileAt = static_cast<long long>(t.row / (BM * CTAS)) * p.columnTiles + t.column / BN;
+                const long long item = t.item, tileAt = static_cast<long long>(t.row / (BM * CTAS)) * p.columnTiles + t.column / BN;
                 partial = p.partial + ((item * p.rowTiles * p.columnTiles + tileAt) * (BM * CTAS) + rank * BM + quarter * 32 + lane) * BN;
             }
             // 64 columns of the accumulator at a time, 32 through shared memory
@@ -581,6 +625,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         bool ok = true;
         while (ok && walk.next(t)) {
             const int steps = walk.steps(t);
+            if (t.expert < 0) break;
             if (t.column != 0) {
                 stage = (stage + steps) % L::STAGES;
                 continue;
@@ -620,7 +665,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                 }
                 const int channel = tileRow + chunk * 8 + first;
                 if (channel < p.sum) {
-                    if (t.units > 1) p.partialBias[(static_cast<long long>(before[t.expert]) + t.unit) * p.sum + channel] = mine;
+                    if (t.units > 1) p.partialBias[static_cast<long long>(t.item) * p.sum + channel] = mine;
                     else static_cast<T*>(p.gradBias)[static_cast<long long>(t.expert) * p.sum + channel] = Element<T>::from(mine);
                 }
             }
@@ -649,7 +694,7 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
 {
     const int tiles = p.rowTiles * p.columnTiles;
     const int expert = blockIdx.x / tiles, tile = blockIdx.x % tiles;
-    const int before = p.plan[expert], units = p.plan[expert + 1] - before;
+    const int before = p.plan[expert].x, units = p.plan[expert].y;
     if (units == 1) return;
     const long long unitStride = static_cast<long long>(tiles) * p.tileRows * BN;
     const float* from = p.partial + before * unitStride + static_cast<long long>(tile) * p.tileRows * BN;
@@ -671,6 +716,102 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
             static_cast<T*>(p.gradBias)[static_cast<long long>(expert) * p.sum + channel] = Element<T>::from(sum);
         }
     }
+}
+
+// ---- few rows: matrix-vector products -----------------------------------------------------------------------------------------
+// The forward product of a handful of rows is bound by reading their experts' matrices once. blockIdx.y is a row; a block of 4 warps takes up
+// to 4 consecutive rows of one expert (the first of every 4 does the work) and 16 channels out, 4 per warp, the lanes side by side along the
+// channels in. No tiles of 128 rows to fill, no copies where the channels in are odd, and enough blocks to fill the machine.
+constexpr int FEW_ROWS = 4, FEW_OUT = 4, FEW_WARPS = 4;
+template <class T, int VEC>
+__global__ void __launch_bounds__(FEW_WARPS * 32) expert_few_rows_kernel(const __grid_constant__ ExpertArgs a)
+{
+    extern __shared__ __align__(16) float rowsIn[];   // FEW_ROWS x channels in, rounded up to whole accesses of a warp
+    __shared__ int found[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
+    const int n0 = (blockIdx.x * FEW_WARPS + warp) * FEW_OUT;
+    if (threadIdx.x == 0) {
+        found[0] = a.experts + 1;
+        found[1] = 0;
+    }
+    __syncthreads();
+    // the first offset behind the row ends its expert's run (see clampOffset): that expert is the one before it
+    int behind = a.experts + 1;
+    for (int e = threadIdx.x; e <= a.experts; e += FEW_WARPS * 32)
+        if (a.offsets[e] > row) { behind = e; break; }
+    if (behind <= a.experts) atomicMin(&found[0], behind);
+    __syncthreads();
+    behind = found[0];
+    T* y = static_cast<T*>(a.y.data);
+    if (behind == 0 || behind > a.experts) {   // nobody's row
+        for (int n = n0 + lane; n < min(n0 + FEW_OUT, a.channelsOut); n += 32) y[row * a.y.stride + n] = Element<T>::from(0.f);
+        return;
+    }
+    int begin = 0;
+    for (int e = threadIdx.x; e < behind; e += FEW_WARPS * 32) begin = max(begin, a.offsets[e]);
+    if (begin > 0) atomicMax(&found[1], begin);
+    __syncthreads();
+    begin = found[1];
+    const int expert = behind - 1, end = static_cast<int>(min(a.rows, static_cast<long long>(a.offsets[behind])));
+    if ((row - begin) % FEW_ROWS != 0) return;
+    const int count = min(FEW_ROWS, end - row);
+    const int stride = (a.channelsIn + 32 * VEC - 1) / (32 * VEC) * (32 * VEC);
+    for (int r = 0; r < count; ++r) {
+        const T* x = static_cast<const T*>(a.x.data) + (row + r) * a.x.stride;
+        for (int k = threadIdx.x; k < stride; k += FEW_WARPS * 32) rowsIn[r * stride + k] = k < a.channelsIn ? Element<T>::to(x[k]) : 0.f;
+    }
+    __syncthreads();
+    const T* w = static_cast<const T*>(a.weight) + (static_cast<long long>(expert) * a.channelsOut + n0) * a.channelsIn;
+    float sum[FEW_OUT][FEW_ROWS] = {};
+    auto step = [&](int k0, auto unroll) {
+        constexpr int U = decltype(unroll)::value;
+        Pack<T, VEC> v[U][FEW_OUT];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int o = 0; o < FEW_OUT; ++o) {
+                const int k = k0 + (u * 32 + lane) * VEC;
+                v[u][o] = {};
+                if (k < a.channelsIn && n0 + o < a.channelsOut) v[u][o] = load<T, VEC>(w + static_cast<long long>(o) * a.channelsIn + k);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + (u * 32 + lane) * VEC;
+            float f[FEW_OUT][VEC];
+#pragma unroll
+            for (int o = 0; o < FEW_OUT; ++o) unpack<T, VEC>(v[u][o], f[o]);
+#pragma unroll
+            for (int r = 0; r < FEW_ROWS; ++r) {
+                if (r >= count) break;
+                float x[VEC];
+                if constexpr (VEC % 4 == 0) {
+#pragma unroll
+                    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(&x[i]) = *reinterpret_cast<const float4*>(rowsIn + r * stride + k + i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) x[i] = rowsIn[r * stride + k + i];
+                }
+#pragma unroll
+                for (int o = 0; o < FEW_OUT; ++o)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) sum[o][r] = fmaf(f[o][i], x[i], sum[o][r]);
+            }
+        }
+    };
+    int k0 = 0;
+    for (; k0 + 4 * 32 * VEC <= stride; k0 += 4 * 32 * VEC) step(k0, std::integral_constant<int, 4>());
+    for (; k0 < stride; k0 += 32 * VEC) step(k0, std::integral_constant<int, 1>());
+#pragma unroll
+    for (int o = 0; o < FEW_OUT; ++o)
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; ++r) {
+            if (r >= count) break;
+            const float all = groupSum<32>(sum[o][r]);
+            if (lane == 0 && n0 + o < a.channelsOut) {
+                const float b = a.bias != nullptr ? Element<T>::to(static_cast<const T*>(a.bias)[static_cast<long long>(expert) * a.channelsOut + n0 + o]) : 0.f;
+                y[(row + r) * a.y.stride + n0 + o] = Element<T>::from(all + b);
+            }
+        }
 }
 
 // ---- bias gradient without a weight gradient: column sums of an expert's rows ----------------------------------------------------
@@ -821,7 +962,7 @@ struct Scratch {
         const size_t items = a.rows > chunk ? a.experts + rows / chunk : 0;
         partial = take(weights, items * tiles * tileRows * shape.width * 4);
         partialBias = take(weights, items * a.channelsOut * 4);
-        plan = take(weights && items > 0, (static_cast<size_t>(a.experts) + 1) * 4);
+        plan = take(weights && items > 0, static_cast<size_t>(a.experts) * sizeof(int2));
     }
 };
 
@@ -876,9 +1017,34 @@ ProductArgs common(const ExpertArgs& a)
 }
 bool wideOut(const void* out, long long stride, int columns) { return (reinterpret_cast<uintptr_t>(out) & 15) == 0 && stride % 8 == 0 && columns % 8 == 0; }
 
+// Rows that the matrix-vector kernel takes. Its time goes with the rows, the tensor kernel's hardly; half, us of the two: 64 experts of 1024 -> 2048,
+// 2 rows 4.1 / 13, 16 rows 17 / 18, 64 rows 59 / 50; 512 experts of 256 -> 256, 64 rows 6.3 / 15; one of 4096 -> 4096, 4 rows 19 / 33, 16 rows 55 / 34.
+bool fewRows(const ExpertArgs& a)
+{
+    return a.rows <= 64 && a.rows * a.channelsIn * a.channelsOut <= 1ll << 26 && FEW_ROWS * (a.channelsIn + 256) * 4 <= 200 * 1024;
+}
+
+template <class T>
+cudaError_t forwardFewRows(const ExpertArgs& a, cudaStream_t stream)
+{
+    const dim3 grid((a.channelsOut + FEW_WARPS * FEW_OUT - 1) / (FEW_WARPS * FEW_OUT), static_cast<unsigned>(a.rows));
+    const bool vec = (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0 && a.channelsIn % 8 == 0;
+    auto go = [&](auto* kernel, int width) {
+        const int bytes = FEW_ROWS * ((a.channelsIn + 32 * width - 1) / (32 * width) * (32 * width)) * 4;
+        if (bytes > 48 * 1024) {
+            const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), 200 * 1024);
+            if (e != cudaSuccess) return e;
+        }
+        kernel<<<grid, FEW_WARPS * 32, bytes, stream>>>(a);
+        return cudaGetLastError();
+    };
+    return vec ? go(expert_few_rows_kernel<T, 8>, 8) : go(expert_few_rows_kernel<T, 1>, 1);
+}
+
 template <class T>
 cudaError_t forward(const ExpertArgs& a, cudaStream_t stream)
 {
+    if (fewRows(a)) return forwardFewRows<T>(a, stream);
     const Scratch s(a, false);
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
     const void *x = a.x.data, *w = a.weight;
@@ -952,7 +1118,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         p.out = a.gradWeight;
         p.outStride = a.channelsIn;
         p.partial = reinterpret_cast<float*>(base + s.partial);
-        p.plan = a.rows > s.chunk ? reinterpret_cast<int*>(base + s.plan) : nullptr;
+        p.plan = a.rows > s.chunk ? reinterpret_cast<int2*>(base + s.plan) : nullptr;
         p.wideStore = wideOut(p.out, p.outStride, p.columns);
         p.tileRows = s.tileRows;
         p.gradBias = a.gradBias;
@@ -972,7 +1138,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
 
 } // namespace
 
-size_t expertBytes(const ExpertArgs& a, bool adjoint) { return a.rows == 0 ? 0 : Scratch(a, adjoint).bytes; }
+size_t expertBytes(const ExpertArgs& a, bool adjoint) { return a.rows == 0 || (!adjoint && fewRows(a)) ? 0 : Scratch(a, adjoint).bytes; }
 
 cudaError_t launchExpertForward(const ExpertArgs& a, cudaStream_t stream)
 {

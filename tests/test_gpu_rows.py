@@ -308,6 +308,16 @@ def test_expert_linear(qmlp, counts, n_in, n_out, dtype):
                  rand(72, (experts, n_out), dtype) if rows % 2 else None, rand(73, (rows, n_out), dtype))
 
 
+@pytest.mark.parametrize("experts", [3, 37, 512, 513])
+def test_expert_linear_ragged(qmlp, experts):
+    """runs of all lengths in no order, one far longer than the others, many empty: sums of cut runs, experts by length"""
+    counts = [int(c) for c in ints(110, (experts,), -20, 90).clamp(min=0)]
+    counts[experts // 2] = 3000
+    rows = sum(counts)
+    experts_case(qmlp, rand(111, (rows, 40), torch.float16), rand(112, (experts, 24, 40), torch.float16, 0.2), offsets_of(counts),
+                 rand(113, (experts, 24), torch.float16), rand(114, (rows, 24), torch.float16))
+
+
 def test_expert_linear_many(qmlp):
     """as many experts as are supported, most of them without a row"""
     counts = [0] * 2048
