@@ -18,10 +18,10 @@
 // a TMA warp, an MMA warp, two groups of four epilogue warps, one per accumulator, so that the products of a tile run under the
 // epilogues of the two before; in the weight product four more warps add up the columns of dy for the bias gradient, from the
 // stages that are in shared memory anyway. Which tile is whose follows from the offsets, which every block adds up for itself: the group
-// sizes never travel to the host. 16 experts, 131072 rows, 1024 -> 1024 bfloat16: 226, 226 and 244 us for the three products, 12 us more
-// with the bias gradient (1.1 to 1.2 PFLOP/s; a library product of one matrix of that size 194 us; 128 x 256 tiles of single blocks
-// 254, 239 and 346 us: operands at 192 bytes a clock ask for more than shared memory has). 512 experts, 1000003 rows, 64 -> 64 half: 54, 55
-// and 69 us, bound by memory (40 us each at the copy rate) and the latency of an epilogue.
+// sizes never travel to the host. 16 experts, 131072 rows, 1024 -> 1024 bfloat16: 200, 196 and 205 us for the three products, 3 us more
+// with the bias gradient (1.34 to 1.40 PFLOP/s; a library product of one matrix of that size 198 us, at clocks that the power limit holds
+// down; 128 x 256 tiles of single blocks 254, 239 and 346 us: their operands ask for more bytes a clock than shared memory has).
+// 512 experts, 1000003 rows, 64 -> 64 half: 49, 49 and 56 us, bound by memory (40 us each at the copy rate).
 // Waits are bounded: on a timeout the block drains, gives its tensor memory back and sets the library's status word.
 #include "common.cuh"
 
@@ -57,48 +57,66 @@ __device__ __forceinline__ void clusterSync()
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The issuing warps run their loops as a whole, with branches that are the same for all lanes, so that descriptors and addresses live in uniform
+// registers; only the elected lane's instruction (`lead`) takes effect. (Behind a `lane == 0` branch every operand is moved to a
+// uniform register first: four products and a commit took 500 clocks to issue, whatever their size.)
+__device__ __forceinline__ uint32_t electOne()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
 template <int CTAS>
-__device__ __forceinline__ void tmaLoad2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+__device__ __forceinline__ void tmaLoad2(uint32_t lead, uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
 {
     // (.cta_group::2: the barrier may be the other block's; the destination is this block's own, nothing is multicast)
     if constexpr (CTAS == 1)
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                     "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
     else
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                     "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];\n\t}"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
 }
 template <int CTAS>
-__device__ __forceinline__ void tmaLoad3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar)
+__device__ __forceinline__ void tmaLoad3(uint32_t lead, uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar)
 {
     if constexpr (CTAS == 1)
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+                     "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(lead) : "memory");
     else
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
-                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+                     "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];\n\t}"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void fenceProxyAsync() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 template <int CTAS>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate)
+__device__ __forceinline__ void mma(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t accumulate)
 {
     if constexpr (CTAS == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)) : "memory");
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                     "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(accumulate), "r"(lead) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(static_cast<uint32_t>(accumulate)) : "memory");
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                     "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(accumulate), "r"(lead) : "memory");
 }
 // arrives on the barrier (of both blocks, at the same place) when the products issued so far are done
 template <int CTAS>
-__device__ __forceinline__ void mmaCommit(uint32_t bar)
+__device__ __forceinline__ void mmaCommit(uint32_t lead, uint32_t bar)
 {
     if constexpr (CTAS == 1)
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+                     ::"r"(bar), "h"(static_cast<uint16_t>(3)), "r"(lead) : "memory");
 }
 template <int CTAS>
 __device__ __forceinline__ void tmemAlloc(uint32_t at, uint32_t columns)
@@ -170,7 +188,7 @@ struct Layout {
     // 1 KB for the alignment of the ring
     static constexpr int bytes(int experts) { return 1024 + STAGES * STAGE + OUT + BARS + listInts(experts) * 4; }
     static_assert(STAGES <= 8, "barriers");
-    static_assert(bytes(EXPERTS_MAX) <= 227 * 1024, "shared memory");
+    static_assert(bytes(EXPERTS_MAX) + 512 <= 227 * 1024, "shared memory");
 };
 
 struct ProductArgs {
@@ -204,33 +222,36 @@ __device__ __forceinline__ int unitsOf(const ProductArgs& p, int rows)
 }
 // The experts' runs and units of work, for all threads of a block: bounds[e] = first row of expert e, bounds[experts] the end of the last one;
 // before[i] = units of the experts in front of the i-th in `order`. The weight product takes the longest runs first (up to SORTED_MAX
-// experts): its tiles cost what their runs are long, and the blocks' shares come out even. (Offsets are fetched at once: one
-// after the other, 512 experts' cost the kernel 8 us.)
+// experts): its tiles cost what their runs are long, and the blocks' shares come out even. (Segments
+// of 32 experts side by side: one warp that took them one after the other cost a kernel of 512 experts 8 us.)
 template <int MODE>
 __device__ __forceinline__ void planExperts(const ProductArgs& p, int* bounds, int* before, int* order, int threads)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int e = threadIdx.x; e <= p.experts; e += threads) bounds[e] = clampOffset(p, e);
-    __syncthreads();
-    if (warp == 2) {   // running maximum
-        int reached = bounds[0];
-        for (int e0 = 0; e0 < p.experts; e0 += 32) {
-            const int e = e0 + lane;
-            int end = e < p.experts ? bounds[e + 1] : 0;
+    __shared__ int segment[64];   // of 32 experts: their largest offset, then their units
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = threads / 32, segments = (p.experts + 31) / 32;
+    const int start = clampOffset(p, 0);
+    for (int s = warp; s < segments; s += warps) {   // running maximum
+        const int e = s * 32 + lane;
+        int end = e < p.experts ? max(start, clampOffset(p, e + 1)) : start;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int up = __shfl_up_sync(0xffffffffu, end, o);
-                if (lane >= o) end = max(end, up);
-            }
-            end = max(end, reached);
-            if (e < p.experts) bounds[e + 1] = end;
-            reached = __shfl_sync(0xffffffffu, end, 31);
+        for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end = max(end, up);
         }
+        if (e < p.experts) bounds[e + 1] = end;
+        if (lane == 31) segment[s] = end;
     }
+    if (threadIdx.x == 0) bounds[0] = start;
+    __syncthreads();
+    for (int s = warp; s < segments; s += warps) {
+        const int e = s * 32 + lane;
+        const int reached = __reduce_max_sync(0xffffffffu, max(lane < s ? segment[lane] : 0, lane + 32 < s ? segment[lane + 32] : 0));
+        if (e < p.experts) bounds[e + 1] = max(bounds[e + 1], reached);
+    }
+    __syncthreads();
     const bool sorted = MODE == WEIGHTS && order != nullptr;
     if (sorted) {
         // bitonic, of keys (length, number) that differ, the length cut to 22 bits
-        __syncthreads();
         const int size = p.experts <= 1 ? 1 : 1 << (32 - __clz(p.experts - 1)), cut = max(0, 10 - __clzll(p.rows) + 32);
         unsigned* keys = reinterpret_cast<unsigned*>(before);   // (has room for SORTED_MAX, and is not needed yet)
         for (int e = threadIdx.x; e < size; e += threads) keys[e] = e < p.experts ? static_cast<unsigned>((bounds[e + 1] - bounds[e]) >> cut) << 10 | (e + 1) : 0u;
@@ -250,22 +271,25 @@ __device__ __forceinline__ void planExperts(const ProductArgs& p, int* bounds, i
         for (int i = threadIdx.x; i < p.experts; i += threads) order[i] = static_cast<int>(keys[i] & 1023) - 1;
         __syncthreads();
     }
-    if (warp == 2) {
-        __syncwarp();
-        int carry = 0;
-        for (int i0 = 0; i0 < p.experts; i0 += 32) {
-            const int i = i0 + lane, e = i < p.experts ? (sorted ? order[i] : i) : 0;
-            int units = i < p.experts ? unitsOf<MODE>(p, bounds[e + 1] - bounds[e]) : 0;
+    for (int s = warp; s < segments; s += warps) {
+        const int i = s * 32 + lane, e = i < p.experts ? (sorted ? order[i] : i) : 0;
+        int units = i < p.experts ? unitsOf<MODE>(p, bounds[e + 1] - bounds[e]) : 0;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int up = __shfl_up_sync(0xffffffffu, units, o);
-                if (lane >= o) units += up;
-            }
-            if (i < p.experts) before[i + 1] = carry + units;
-            carry += __shfl_sync(0xffffffffu, units, 31);
+        for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, units, o);
+            if (lane >= o) units += up;
         }
-        if (lane == 0) before[0] = 0;
+        if (i < p.experts) before[i + 1] = units;
+        if (lane == 31) segment[s] = units;
     }
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    for (int s = warp; s < segments; s += warps) {
+        const int i = s * 32 + lane;
+        const int carry = __reduce_add_sync(0xffffffffu, (lane < s ? segment[lane] : 0) + (lane + 32 < s ? segment[lane + 32] : 0));
+        if (i < p.experts) before[i + 1] += carry;
+    }
+    // (the caller's barrier follows)
 }
 
 // One tile of D: its expert (-1: no tile), the unit it belongs to, the expert's units, the run of rows it reads (forward, input: its own rows)
@@ -364,7 +388,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     uint32_t* tmemBase = reinterpret_cast<uint32_t*>(outStage + L::OUT + L::BASE);
     int *bounds = reinterpret_cast<int*>(outStage + L::OUT + L::BARS), *before = bounds + listStride(p.experts);
     int* order = p.experts <= SORTED_MAX ? before + listStride(p.experts) : nullptr;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = CTAS == 1 ? 0u : clusterRank();
 
     if (threadIdx.x == 0) {
@@ -396,6 +420,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
 
     if (warp == 0) {
         // ---- operands -------------------------------------------------------------------------------------------------
+        const uint32_t lead = electOne();
         uint32_t stage = 0, phase = 0, tailPhase = 0;
         long long issued = 0;
         bool ok = true;
@@ -405,14 +430,14 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
             const int boxesA = boxes(rowEnd - row, BM / 64), boxesB = boxes(p.columns - column, L::BCOLS / 64);
             const uint32_t bytes = (boxesA + boxesB) * BOX;   // of this block; of both blocks:
             const uint32_t allBytes = CTAS == 1 ? bytes : bytes + (boxes(rowEnd - row - BM, BM / 64) + boxes(p.columns - column - L::BCOLS, L::BCOLS / 64)) * BOX;
-            for (int k = 0; k < steps; ++k) {
+            for (int k = 0; __all_sync(0xffffffffu, k < steps); ++k) {
                 if (!await(empty + stage * 8, phase ^ 1, failed)) { ok = false; break; }
                 const uint32_t a = ring + stage * L::STAGE, b = a + L::ABYTES;
                 const uint32_t ready = CTAS == 1 ? full + stage * 8 : inBlock(full + stage * 8, 0);
                 // the last rows of an expert's last step belong to another expert: a pair of blocks clears them before it hands the step on
                 const int left = t.end - t.begin - k * BK, tail = MODE == WEIGHTS && CTAS > 1 && left < BK ? (16 - left % 16) % 16 : 0;
                 const uint32_t bar = tail > 0 ? bars + L::TAIL : ready;
-                if (lane == 0) {
+                if (lead) {
                     // the leader expects the bytes of both blocks, and arrives for both (an arrival from the other block at every step costs more
                     // than the step: its release takes about a microsecond)
                     if (tail > 0) barrierExpect(bar, bytes);
@@ -420,17 +445,19 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                         barrierExpect(full + stage * 8, allBytes);
                         if (CTAS > 1) barrierArrive(full + stage * 8);
                     }
-                    for (int i = 0; i < boxesA; ++i) {
-                        if constexpr (MODE == WEIGHTS) tmaLoad2<CTAS>(a + i * BOX, &mapA, row + i * 64, t.begin + k * BK, bar);
-                        else tmaLoad2<CTAS>(a + i * BOX, &mapA, k * BK, row + i * 64, bar);
-                    }
-                    for (int i = 0; i < boxesB; ++i) {
-                        if constexpr (MODE == WEIGHTS) tmaLoad2<CTAS>(b + i * BOX, &mapB, column + i * 64, t.begin + k * BK, bar);
-                        else if constexpr (MODE == FORWARD) tmaLoad3<CTAS>(b + i * BOX, &mapB, k * BK, column + i * 64, t.expert, bar);
-                        else tmaLoad3<CTAS>(b + i * BOX, &mapB, column + i * 64, k * BK, t.expert, bar);
-                    }
                 }
                 __syncwarp();
+#pragma unroll
+                for (int i = 0; i < BM / 64; ++i) {
+                    if constexpr (MODE == WEIGHTS) tmaLoad2<CTAS>(lead && i < boxesA, a + i * BOX, &mapA, row + i * 64, t.begin + k * BK, bar);
+                    else tmaLoad2<CTAS>(lead && i < boxesA, a + i * BOX, &mapA, k * BK, row + i * 64, bar);
+                }
+#pragma unroll
+                for (int i = 0; i < L::BCOLS / 64; ++i) {
+                    if constexpr (MODE == WEIGHTS) tmaLoad2<CTAS>(lead && i < boxesB, b + i * BOX, &mapB, column + i * 64, t.begin + k * BK, bar);
+                    else if constexpr (MODE == FORWARD) tmaLoad3<CTAS>(lead && i < boxesB, b + i * BOX, &mapB, k * BK, column + i * 64, t.expert, bar);
+                    else tmaLoad3<CTAS>(lead && i < boxesB, b + i * BOX, &mapB, column + i * 64, k * BK, t.expert, bar);
+                }
                 if constexpr (MODE == WEIGHTS && CTAS > 1) {
                     if (tail > 0) {
                         if (!await(bar, tailPhase, failed)) { ok = false; break; }
@@ -461,17 +488,18 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         // ---- products -------------------------------------------------------------------------------------------------
         constexpr uint32_t instruction = (1u << 4) | (FORMAT<T> << 7) | (FORMAT<T> << 10) | (MODE == WEIGHTS ? 1u << 15 : 0u) | (MODE != FORWARD ? 1u << 16 : 0u) |
                                          (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>((BM * CTAS) >> 4) << 24);
+        const uint32_t lead = electOne();
         uint32_t stage = 0, phase = 0, acc = 1, accPhases = 0;   // accPhases: one bit per accumulator
         bool ok = rank == 0;
         while (ok && walk.next(t)) {
             const int steps = walk.steps(t);
             acc ^= 1;                   // the tiles' numbers alternate between the accumulators
-            if (steps == 0) continue;   // an expert without rows: the epilogue writes zeros
+            if (__all_sync(0xffffffffu, steps == 0)) continue;   // an expert without rows: the epilogue writes zeros
             if (!await(accEmpty + acc * 8, (accPhases >> acc & 1) ^ 1, failed)) break;
             accPhases ^= 1u << acc;
             fenceAfter();
             const uint32_t d = tmem + acc * BN;
-            for (int k = 0; k < steps; ++k) {
+            for (int k = 0; __all_sync(0xffffffffu, k < steps); ++k) {
                 if (!await(full + stage * 8, phase, failed)) { ok = false; break; }
                 fenceAfter();
                 const uint32_t a = ring + stage * L::STAGE, b = a + L::ABYTES;
@@ -486,17 +514,14 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                     fenceProxyAsync();
                     __syncwarp();
                 }
-                if (lane == 0) {
-                    const uint64_t descA = operandDescriptor(a, MODE == WEIGHTS ? BOX : 16), descB = operandDescriptor(b, MODE == FORWARD ? 16 : BOX);
-                    // 16 along the sum: 32 bytes of a K-major row, 16 rows of an MN-major block
+                const uint64_t descA = operandDescriptor(a, MODE == WEIGHTS ? BOX : 16), descB = operandDescriptor(b, MODE == FORWARD ? 16 : BOX);
+                // 16 along the sum: 32 bytes of a K-major row, 16 rows of an MN-major block
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (i < parts)
-                            mma<CTAS>(d, descA + i * (MODE == WEIGHTS ? 2048 >> 4 : 32 >> 4), descB + i * (MODE == FORWARD ? 32 >> 4 : 2048 >> 4), instruction, k + i > 0);
-                    mmaCommit<CTAS>((SUMS && t.column == 0 ? landed : empty) + stage * 8);   // (the warps that sum come between)
-                    if (k == steps - 1) mmaCommit<CTAS>(accFull + acc * 8);
-                }
-                __syncwarp();
+                for (int i = 0; i < 4; ++i)
+                    mma<CTAS>(lead && i < parts, d, descA + i * (MODE == WEIGHTS ? 2048 >> 4 : 32 >> 4), descB + i * (MODE == FORWARD ? 32 >> 4 : 2048 >> 4), instruction,
+                              i > 0 ? 1u : k > 0 ? 1u : 0u);
+                mmaCommit<CTAS>(lead, (SUMS && t.column == 0 ? landed : empty) + stage * 8);   // (the warps that sum come between)
+                mmaCommit<CTAS>(lead && k == steps - 1, accFull + acc * 8);
                 if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
             }
         }
@@ -676,8 +701,8 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     fenceAfter();
     if (*failed != 0 && warp == 1 && rank == 0) {
         // products that were issued end before the tensor memory is given back
+        mmaCommit<CTAS>(electOne(), bars + L::DRAIN);   // (elects the lane that issued the products)
         if (lane == 0) {
-            mmaCommit<CTAS>(bars + L::DRAIN);
             barrierWait(bars + L::DRAIN, 0);
             atomicOr(p.status, 1);
         }
@@ -687,11 +712,13 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     if (warp == 1) tmemFree<CTAS>(tmem, L::TMEM);
 }
 
-// adds up the partial sums of the weight gradients (and, behind the tiles, of the bias gradients) of experts with more than one item:
-// a block per 16 rows of a tile of an expert
+// Adds up the partial sums of the weight gradients (and, behind the tiles, of the bias gradients) of experts with more than one item. blockIdx.x: tile
+// of an expert, blockIdx.y: JOIN_ELEMENTS of it. Most blocks find one item and leave, so there are few of them.
+constexpr int JOIN_ELEMENTS = 8192;
 template <class T, int BN>
 __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant__ ProductArgs p)
 {
+    constexpr int ROWS = JOIN_ELEMENTS / BN;
     const int tiles = p.rowTiles * p.columnTiles;
     const int expert = blockIdx.x / tiles, tile = blockIdx.x % tiles;
     const int before = p.plan[expert].x, units = p.plan[expert].y;
@@ -699,19 +726,30 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
     const long long unitStride = static_cast<long long>(tiles) * p.tileRows * BN;
     const float* from = p.partial + before * unitStride + static_cast<long long>(tile) * p.tileRows * BN;
     const int row0 = tile / p.columnTiles * p.tileRows, column0 = tile % p.columnTiles * BN;
-    for (int i = threadIdx.x; i < 16 * BN; i += 256) {
-        const int r = blockIdx.y * 16 + i / BN, c = i % BN;
+    for (int i = threadIdx.x; i < JOIN_ELEMENTS / 4; i += 256) {
+        const int r = blockIdx.y * ROWS + i / (BN / 4), c = i % (BN / 4) * 4;
         if (row0 + r >= p.sum || column0 + c >= p.columns) continue;
-        float sum = 0.f;
-#pragma unroll 8
-        for (int u = 0; u < units; ++u) sum += from[u * unitStride + r * BN + c];
-        static_cast<T*>(p.out)[(static_cast<long long>(expert) * p.sum + row0 + r) * p.outStride + column0 + c] = Element<T>::from(sum);
+        float4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int u = 0; u < units; ++u) {
+            const float4 v = *reinterpret_cast<const float4*>(from + u * unitStride + r * BN + c);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+        T* out = static_cast<T*>(p.out) + (static_cast<long long>(expert) * p.sum + row0 + r) * p.outStride + column0 + c;
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (p.wideStore) store<T, 4>(out, pack<T, 4>(f));
+        else
+            for (int k = 0; k < 4 && column0 + c + k < p.columns; ++k) out[k] = Element<T>::from(f[k]);
     }
-    if (p.gradBias != nullptr && column0 == 0 && threadIdx.x < 16) {
-        const int channel = row0 + blockIdx.y * 16 + threadIdx.x;
-        if (channel < p.sum) {
+    if (p.gradBias != nullptr && column0 == 0) {
+        for (int r = threadIdx.x; r < ROWS; r += 256) {
+            const int channel = row0 + blockIdx.y * ROWS + r;
+            if (channel >= p.sum || blockIdx.y * ROWS + r >= p.tileRows) break;
             float sum = 0.f;
-#pragma unroll 8
+#pragma unroll 4
             for (int u = 0; u < units; ++u) sum += p.partialBias[static_cast<long long>(before + u) * p.sum + channel];
             static_cast<T*>(p.gradBias)[static_cast<long long>(expert) * p.sum + channel] = Element<T>::from(sum);
         }
@@ -1126,7 +1164,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         e = a.gradBias != nullptr ? launchShape<T, WEIGHTS, true>(s.shape, mapY, mapX, p, a.numSMs, stream)
                                   : launchShape<T, WEIGHTS, false>(s.shape, mapY, mapX, p, a.numSMs, stream);
         if (e == cudaSuccess && a.rows > s.chunk) {
-            const dim3 grid(a.experts * s.rowTiles * s.columnTiles, s.tileRows / 16);
+            const dim3 grid(a.experts * s.rowTiles * s.columnTiles, s.tileRows * s.shape.width / JOIN_ELEMENTS);
             if (s.shape.width == 64) expert_join_kernel<T, 64><<<grid, 256, 0, stream>>>(p);
             else if (s.shape.width == 128) expert_join_kernel<T, 128><<<grid, 256, 0, stream>>>(p);
             else expert_join_kernel<T, 256><<<grid, 256, 0, stream>>>(p);
