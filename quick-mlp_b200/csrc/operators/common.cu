@@ -19,6 +19,7 @@ cudaError_t allowShared(const void* kernel, int bytes)
     std::lock_guard<std::mutex> lock(mutex);
     if (allowed.count({device, kernel}) != 0) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess) allowed.insert({device, kernel});
     return e;
 }

@@ -26,30 +26,30 @@ __device__ __forceinline__ long long tokenAt(const EmbeddingArgs& a, long long t
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-constexpr int LOOKUPS = 4;   // accesses in flight per thread
+// A thread takes one access' worth of LOOKUPS rows, `pass` rows apart, so that it divides once; 256 / accesses of a row rows per pass (rows of more than
+// 256 accesses: blockIdx.y counts their parts).
+constexpr int LOOKUPS = 4;
 template <class T, int VEC>
-__global__ void __launch_bounds__(256) embedding_forward_kernel(const __grid_constant__ EmbeddingArgs a, long long total, int perRow)
+__global__ void __launch_bounds__(256) embedding_forward_kernel(const __grid_constant__ EmbeddingArgs a, int perRow, int pass)
 {
     const T* table = static_cast<const T*>(a.table.data);
     T* y = static_cast<T*>(a.y.data);
-    const long long first = blockIdx.x * (256ll * LOOKUPS) + threadIdx.x;
+    const int rowInPass = pass == 1 ? 0 : static_cast<int>(threadIdx.x) / perRow, access = blockIdx.y * 256 + (pass == 1 ? threadIdx.x : threadIdx.x - rowInPass * perRow);
+    if (rowInPass >= pass || access >= perRow) return;
+    const int c = access * VEC;
+    const long long first = static_cast<long long>(blockIdx.x) * (pass * LOOKUPS) + rowInPass;
+    long long token[LOOKUPS];
     Pack<T, VEC> v[LOOKUPS];
-    long long at[LOOKUPS];
+#pragma unroll
+    for (int k = 0; k < LOOKUPS; ++k) token[k] = first + k * pass < a.tokens ? tokenAt(a, first + k * pass) : -1;
 #pragma unroll
     for (int k = 0; k < LOOKUPS; ++k) {
-        const long long i = first + k * 256;
-        at[k] = -1;
         v[k] = {};
-        if (i >= total) continue;
-        const long long t = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(perRow) : i / perRow;
-        const int c = static_cast<int>(i - t * perRow) * VEC;
-        at[k] = t * a.y.stride + c;
-        const long long r = tokenAt(a, t);
-        if (r >= 0 && r < a.rows) v[k] = load<T, VEC>(table + r * a.table.stride + c);
+        if (token[k] >= 0 && token[k] < a.rows) v[k] = load<T, VEC>(table + token[k] * a.table.stride + c);
     }
 #pragma unroll
     for (int k = 0; k < LOOKUPS; ++k) {
-        if (at[k] < 0) continue;
+        if (first + k * pass >= a.tokens) break;
         if (a.scale != 1.f) {
             float f[VEC];
             unpack<T, VEC>(v[k], f);
@@ -57,116 +57,175 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const __grid_con
             for (int i = 0; i < VEC; ++i) f[i] *= a.scale;
             v[k] = pack<T, VEC>(f);
         }
-        store<T, VEC>(y + at[k], v[k]);
+        store<T, VEC>(y + (first + k * pass) * a.y.stride + c, v[k]);
     }
 }
 
 // ---- sort -------------------------------------------------------------------------------------------------------------
-constexpr int SORT_ITEMS = 8, SORT_TILE = SORT_ITEMS * PARTITION_THREADS;
-
+// Tiles of 1024 tokens (256 threads) while they leave SMs without one, of 4096 (512 threads) above: the counters of a tile's digits are cleared and
+// added up once per tile. A million tokens, 1024 digits, tiles of 2048 (256 threads): move 29 us; of 4096: MOVE8 us.
+// A tile's items go through shared memory into the order of their digits, so that what is written to memory lies side by side.
 struct SortArgs {
-    const int *keysIn, *slotsIn;   // null in the first pass: tokens, and their own numbers
-    int *keysOut, *slotsOut;
-    int *counts, *totals;
+    const int2* in;                // key and slot; null in the first pass: the tokens, and their own numbers
+    int2* out;
+    int *counts, *before, *totals;
+    uint8_t* present;              // rows of the table that have a token, set in the first of several passes; null: totals say so
     int items, blocks, shift, digits;
 };
-__device__ __forceinline__ int sortKey(const EmbeddingArgs& a, const SortArgs& s, int i)
+__device__ __forceinline__ int2 sortItem(const EmbeddingArgs& a, const SortArgs& s, int i)
 {
-    if (s.keysIn != nullptr) return s.keysIn[i];
+    if (s.in != nullptr) return s.in[i];
     const long long r = tokenAt(a, i);
-    return static_cast<int>(r >= 0 && r < a.rows ? r : a.rows);
+    return make_int2(static_cast<int>(r >= 0 && r < a.rows ? r : a.rows), i);
 }
-__global__ void __launch_bounds__(PARTITION_THREADS) sort_count_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ SortArgs s)
+template <int ITEMS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) sort_count_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ SortArgs s)
 {
     __shared__ int count[PARTITION_MAX_DIGITS];
-    for (int i = threadIdx.x; i < s.digits; i += PARTITION_THREADS) count[i] = 0;
-    __syncthreads();
-    const int first = blockIdx.x * SORT_TILE;
+    for (int i = threadIdx.x; i < s.digits; i += WARPS * 32) count[i] = 0;
+    const int first = blockIdx.x * (ITEMS * WARPS * 32);
+    int key[ITEMS];
 #pragma unroll
-    for (int k = 0; k < SORT_ITEMS; ++k) {
-        const int i = first + k * PARTITION_THREADS + threadIdx.x;
-        if (i < s.items) atomicAdd(&count[(sortKey(a, s, i) >> s.shift) & (s.digits - 1)], 1);
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = first + k * WARPS * 32 + threadIdx.x;
+        key[k] = i < s.items ? sortItem(a, s, i).x : -1;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < s.digits; i += PARTITION_THREADS) s.counts[static_cast<long long>(i) * s.blocks + blockIdx.x] = count[i];
-}
-__global__ void __launch_bounds__(PARTITION_THREADS) sort_move_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ SortArgs s)
-{
-    extern __shared__ int dynamic[];
-    int *start = dynamic, *counts = dynamic + s.digits;   // digits, warps x digits
-    __shared__ int warpSums[PARTITION_WARPS];
-    for (int i = threadIdx.x; i < s.digits; i += PARTITION_THREADS) start[i] = s.totals[i];
-    __syncthreads();
-    blockExclusive(start, s.digits, warpSums);
-    const int first = blockIdx.x * SORT_TILE;
-    int digit[SORT_ITEMS], rank[SORT_ITEMS], key[SORT_ITEMS], at = 0;
-    tileRanks<SORT_ITEMS>([&](int i) {
-        const int k = first + i < s.items ? sortKey(a, s, first + i) : -1;
-        key[at++] = k;
-        return k < 0 ? -1 : (k >> s.shift) & (s.digits - 1);
-    }, s.digits, counts, digit, rank);
-    for (int d = threadIdx.x; d < s.digits; d += PARTITION_THREADS)
-        warpOffsets(counts, s.digits, d, start[d] + s.counts[static_cast<long long>(d) * s.blocks + blockIdx.x]);
-    __syncthreads();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool mark = s.in == nullptr && s.present != nullptr;
 #pragma unroll
-    for (int k = 0; k < SORT_ITEMS; ++k) {
-        if (digit[k] < 0) continue;
-        const int i = first + (warp * SORT_ITEMS + k) * 32 + lane, to = counts[warp * s.digits + digit[k]] + rank[k];
-        s.keysOut[to] = key[k];
-        s.slotsOut[to] = s.slotsIn != nullptr ? s.slotsIn[i] : i;
+    for (int k = 0; k < ITEMS; ++k) {
+        if (key[k] >= 0) atomicAdd(&count[(key[k] >> s.shift) & (s.digits - 1)], 1);
+        if (mark) {   // once per warp: a hot row's stores would wait for one another
+            const unsigned same = __match_any_sync(0xffffffffu, key[k]);
+            if ((threadIdx.x & 31) == __ffs(same) - 1 && key[k] >= 0 && key[k] < a.rows) s.present[key[k]] = 1;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < s.digits; i += WARPS * 32) s.counts[static_cast<long long>(i) * s.blocks + blockIdx.x] = count[i];
+}
+template <int ITEMS, int WARPS>
+constexpr int moveBytes(int digits) { return ITEMS * WARPS * 32 * 8 + 2 * digits * 4 + WARPS * digits * 2; }
+template <int ITEMS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1024 / (WARPS * 32)) sort_move_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ SortArgs s)
+{
+    constexpr int THREADS = WARPS * 32, TILE = ITEMS * THREADS;
+    extern __shared__ __align__(16) int2 sorted[];                           // TILE
+    int *start = reinterpret_cast<int*>(sorted + TILE), *local = start + s.digits;   // digits: where the tile's items go, in memory and in the tile
+    uint16_t* counts = reinterpret_cast<uint16_t*>(local + s.digits);        // warps x digits
+    __shared__ int warpSums[WARPS];
+    for (int i = threadIdx.x; i < s.digits; i += THREADS) start[i] = s.totals[i];
+    __syncthreads();
+    blockExclusive<WARPS>(start, s.digits, warpSums);
+    const int first = blockIdx.x * TILE;
+    for (int d = threadIdx.x; d < s.digits; d += THREADS) start[d] += s.before[static_cast<long long>(blockIdx.x) * s.digits + d];
+    int digit[ITEMS], rank[ITEMS];
+    tileRanks<ITEMS, WARPS>([&](int i) { return first + i < s.items ? (sortItem(a, s, first + i).x >> s.shift) & (s.digits - 1) : -1; }, s.digits, counts, digit, rank);
+    for (int d = threadIdx.x; d < s.digits; d += THREADS) local[d] = warpOffsets<WARPS>(counts, s.digits, d);
+    __syncthreads();
+    blockExclusive<WARPS>(local, s.digits, warpSums);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)   // (the items once more: they would cost the registers of a second block)
+        if (digit[k] >= 0) sorted[local[digit[k]] + counts[warp * s.digits + digit[k]] + rank[k]] = sortItem(a, s, first + (warp * ITEMS + k) * 32 + lane);
+    __syncthreads();
+    const int here = min(TILE, s.items - first);
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = k * THREADS + threadIdx.x;
+        if (i >= here) break;
+        const int2 v = sorted[i];
+        const int d = (v.x >> s.shift) & (s.digits - 1);
+        s.out[start[d] + i - local[d]] = v;
     }
 }
 
 // ---- sums over runs of equal tokens -------------------------------------------------------------------------------------
 struct RunArgs {
-    const int *keys, *slots;
-    int items, chunk, chunks;
+    const int2* sorted;            // key, slot
+    const uint8_t* present;        // rows with a token, or null:
+    const int* totals;             // tokens of a row
+    int items, chunk, chunks, runBlocks;
     float* partial;      // chunks x 2 x channels: the run a chunk begins with (if it began before), the run it ends with (if it goes on)
 };
-constexpr int RUN_UNROLL = 4;
+constexpr int RUN_STEP = 8;    // rows in flight per group; chunks are multiples of it
+constexpr int FILL_ROWS = 8;   // rows of the table a group looks at
 
+// Blocks of the first kind add up runs, a chunk per group of G lanes; the others write the zeros of the rows without a token meanwhile.
 template <class T, int VEC, int G>
-__global__ void __launch_bounds__(256) embedding_runs_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ RunArgs r)
+__global__ void __launch_bounds__(256, 3) embedding_runs_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ RunArgs r)
 {
     constexpr int GROUPS = 256 / G;
-    const int chunk = blockIdx.x * GROUPS + threadIdx.x / G;
     const int c = (blockIdx.y * G + threadIdx.x % G) * VEC;
-    if (chunk >= r.chunks || c >= a.channels) return;
-    const T* dy = static_cast<const T*>(a.gradY.data);
+    if (c >= a.channels) return;
     T* out = static_cast<T*>(a.gradTable.data);
+    if (blockIdx.x >= static_cast<unsigned>(r.runBlocks)) {
+        const long long first = (static_cast<long long>(blockIdx.x - r.runBlocks) * FILL_ROWS) * GROUPS + threadIdx.x / G;
+#pragma unroll
+        for (int k = 0; k < FILL_ROWS; ++k) {
+            const long long row = first + k * GROUPS;
+            if (row < a.rows && (r.present != nullptr ? r.present[row] == 0 : r.totals[row] == 0)) store<T, VEC>(out + row * a.gradTable.stride + c, Pack<T, VEC>{});
+        }
+        return;
+    }
+    const int chunk = blockIdx.x * GROUPS + threadIdx.x / G;
+    if (chunk >= r.chunks) return;
+    const T* dy = static_cast<const T*>(a.gradY.data);
     const int begin = chunk * r.chunk, end = min(r.items, begin + r.chunk);
     const int none = static_cast<int>(a.rows);   // key of the tokens outside the table
-    int current = r.keys[begin];
-    bool entered = begin > 0 && r.keys[begin - 1] == current;   // the current run began in an earlier chunk
+    int current = r.sorted[begin].x;
+    bool entered = begin > 0 && r.sorted[begin - 1].x == current;   // the current run began in an earlier chunk
     float sum[VEC] = {};
     auto flush = [&](bool leaves) {
-        if (current < none) {
-            if (!entered && !leaves) {
-                float f[VEC];
+        if (!entered && !leaves) {
+            float f[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) f[i] = sum[i] * a.scale;
-                store<T, VEC>(out + static_cast<long long>(current) * a.gradTable.stride + c, pack<T, VEC>(f));
-            } else {
-                float* p = r.partial + (static_cast<long long>(chunk) * 2 + (entered ? 0 : 1)) * a.channels + c;
+            for (int i = 0; i < VEC; ++i) f[i] = sum[i] * a.scale;
+            store<T, VEC>(out + static_cast<long long>(current) * a.gradTable.stride + c, pack<T, VEC>(f));
+        } else {
+            float* p = r.partial + (static_cast<long long>(chunk) * 2 + (entered ? 0 : 1)) * a.channels + c;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) p[i] = sum[i];
-            }
+            for (int i = 0; i < VEC; ++i) p[i] = sum[i];
         }
     };
-    for (int i = begin; i < end; i += RUN_UNROLL) {
-        int key[RUN_UNROLL];
-        Pack<T, VEC> v[RUN_UNROLL];
+    // the list holds whole steps (behind the last item: whatever, not used), 16-byte aligned
+    int4 next[RUN_STEP / 2];
+    auto fetch = [&](int i) {
 #pragma unroll
-        for (int k = 0; k < RUN_UNROLL; ++k) {
-            key[k] = i + k < end ? r.keys[i + k] : none;
-            if (key[k] < none) v[k] = load<T, VEC>(dy + static_cast<long long>(r.slots[i + k]) * a.gradY.stride + c);
+        for (int h = 0; h < RUN_STEP / 2; ++h) next[h] = *reinterpret_cast<const int4*>(r.sorted + i + 2 * h);
+    };
+    fetch(begin);
+    for (int i = begin; i < end; i += RUN_STEP) {
+        int key[RUN_STEP], slot[RUN_STEP];
+#pragma unroll
+        for (int h = 0; h < RUN_STEP / 2; ++h) {
+            key[2 * h] = next[h].x;
+            slot[2 * h] = next[h].y;
+            key[2 * h + 1] = next[h].z;
+            slot[2 * h + 1] = next[h].w;
+        }
+        if (i + RUN_STEP < end) fetch(i + RUN_STEP);
+        Pack<T, VEC> v[RUN_STEP];
+#pragma unroll
+        for (int k = 0; k < RUN_STEP; ++k) {
+            if (i + k >= end) key[k] = none;
+            v[k] = {};
+            if (key[k] < none) v[k] = load<T, VEC>(dy + static_cast<long long>(slot[k]) * a.gradY.stride + c);
+        }
+        if (key[0] == current && key[RUN_STEP - 1] == current && current < none) {   // one run
+#pragma unroll
+            for (int k = 0; k < RUN_STEP; ++k) {
+                float f[VEC];
+                unpack<T, VEC>(v[k], f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum[j] += f[j];
+            }
+            continue;
         }
 #pragma unroll
-        for (int k = 0; k < RUN_UNROLL; ++k) {
+        for (int k = 0; k < RUN_STEP; ++k) {
             if (i + k >= end) break;
             if (key[k] != current) {
-                flush(false);
+                if (current < none) flush(false);
                 current = key[k];
                 entered = false;
 #pragma unroll
@@ -179,43 +238,85 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(const __grid_consta
             for (int j = 0; j < VEC; ++j) sum[j] += f[j];
         }
     }
-    flush(end < r.items && r.keys[end] == current);
+    if (current < none) flush(end < r.items && r.sorted[end].x == current);
 }
 
-// A block per chunk: if a run begins in it and goes on behind it, the sums of its parts, in order: each of the block's 8 warps
-// adds up consecutive parts, then the warps' sums follow one another.
-template <class T>
-__global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ RunArgs r)
+// Joins the runs that cross chunks. A block looks at JOIN_CHUNKS chunks, a warp each; for every run that begins in one of them and goes on behind
+// it, its parts are added up: by G lanes side by side along the columns where they are few, else by 512 / G such shares of
+// consecutive parts, then the shares in order.
+constexpr int JOIN_CHUNKS = 8, JOIN_FEW = 16;
+template <class T, int G>
+__global__ void __launch_bounds__(512) embedding_join_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ RunArgs r)
 {
-    __shared__ float shared[8][32];
-    const int chunk = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int end = (chunk + 1) * r.chunk;
-    if (end >= r.items) return;
-    const int key = r.keys[end];
-    const int begin = chunk * r.chunk;
-    if (key >= static_cast<int>(a.rows) || r.keys[end - 1] != key || (r.keys[begin] == key && begin > 0 && r.keys[begin - 1] == key)) return;
-    // chunks whose first key is still `key`: the run enters them
-    int low = chunk + 1, high = r.chunks;   // the run enters `low`, not `high`
-    while (low + 1 < high) {
-        const int mid = (low + high) / 2;
-        if (r.keys[mid * r.chunk] == key) low = mid;
-        else high = mid;
+    constexpr int SHARES = 512 / G;
+    __shared__ int keyOf[JOIN_CHUNKS], partsOf[JOIN_CHUNKS];
+    __shared__ float shared[512];
+    if (threadIdx.x < JOIN_CHUNKS * 32) {   // a warp per chunk
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int chunk = blockIdx.x * JOIN_CHUNKS + warp, begin = chunk * r.chunk, end = begin + r.chunk;
+        int parts = 0, key = 0;
+        if (chunk < r.chunks && end < r.items) {
+            key = r.sorted[end].x;
+            const int last = r.sorted[end - 1].x, first = r.sorted[begin].x, before = begin > 0 ? r.sorted[begin - 1].x : -1;
+            if (key < static_cast<int>(a.rows) && last == key && !(first == key && before == key)) {
+                // the tail of `chunk`, and the heads of the chunks whose first item still has the key: 32 looked at in a step, the steps 32 times
+                // as long for as long as all have it
+                int known = chunk + 1;   // has it
+                for (int stride = 1;;) {
+                    const long long probe = known + static_cast<long long>(lane + 1) * stride;
+                    const unsigned have = __ballot_sync(0xffffffffu, probe < r.chunks && r.sorted[probe * r.chunk].x == key);
+                    known += __popc(have) * stride;
+                    if (have == 0xffffffffu) {
+                        if (stride <= 1024) stride *= 32;
+                    } else if (stride == 1) {
+                        break;
+                    } else {
+                        stride /= 32;
+                    }
+                }
+                parts = known + 1 - chunk;
+            }
+        }
+        if (lane == 0) {
+            keyOf[warp] = key;
+            partsOf[warp] = parts;
+        }
     }
-    const int parts = low + 1 - chunk;      // the tail of `chunk`, the heads of chunk + 1 .. low
-    const int share = (parts + 7) / 8, from = warp * share, to = min(parts, from + share);
-    const int c = blockIdx.y * 32 + lane;
-    float sum = 0.f;
-    if (c < a.channels) {
-#pragma unroll 8
-        for (int p = from; p < to; ++p) sum += r.partial[(static_cast<long long>(chunk + p) * 2 + (p == 0 ? 1 : 0)) * a.channels + c];
-    }
-    shared[warp][lane] = sum;
     __syncthreads();
-    if (warp == 0 && c < a.channels) {
-        sum = 0.f;
+    const int share = threadIdx.x / G, c = blockIdx.y * G + threadIdx.x % G;
+    const long long pair = 2ll * a.channels;
+    const float* from = r.partial + static_cast<long long>(blockIdx.x) * JOIN_CHUNKS * pair + c;
+    auto write = [&](int k, float sum) {
+        static_cast<T*>(a.gradTable.data)[static_cast<long long>(keyOf[k]) * a.gradTable.stride + c] = Element<T>::from(sum * a.scale);
+    };
+    // runs of few parts: a share each
+    for (int k = share; k < JOIN_CHUNKS; k += SHARES) {
+        const int parts = partsOf[k];
+        if (parts == 0 || parts > JOIN_FEW || c >= a.channels) continue;
+        float v[JOIN_FEW], sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) sum += shared[w][lane];
-        static_cast<T*>(a.gradTable.data)[static_cast<long long>(key) * a.gradTable.stride + c] = Element<T>::from(sum * a.scale);
+        for (int p = 0; p < JOIN_FEW; ++p) v[p] = p < parts ? from[(k + p) * pair + (p == 0 ? a.channels : 0)] : 0.f;
+#pragma unroll
+        for (int p = 0; p < JOIN_FEW; ++p) sum += v[p];
+        write(k, sum);
+    }
+    for (int k = 0; k < JOIN_CHUNKS; ++k) {
+        const int parts = partsOf[k];
+        if (parts <= JOIN_FEW) continue;
+        const int each = (parts + SHARES - 1) / SHARES, first = share * each, last = min(parts, first + each);
+        float sum = 0.f;
+        if (c < a.channels) {
+#pragma unroll 8
+            for (int p = first; p < last; ++p) sum += from[(k + p) * pair + (p == 0 ? a.channels : 0)];
+        }
+        shared[threadIdx.x] = sum;
+        __syncthreads();
+        if (share == 0 && c < a.channels) {
+            const int used = (parts + each - 1) / each;
+            for (int s = 1; s < used; ++s) sum += shared[s * G + threadIdx.x];
+            write(k, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -224,7 +325,8 @@ size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 struct SortPlan {
     int passes, bits, digits, blocks, chunk, chunks;
-    size_t keys, counts, totals, partial, bytes;   // bytes of one array of keys, offsets of the rest
+    bool large;
+    size_t list, counts, before, totals, present, partial, bytes;   // bytes of one list of keys and slots, offsets of the rest
     SortPlan(long long tokens, long long rows, int channels, int type, int numSMs)
     {
         int keyBits = 1;
@@ -232,16 +334,21 @@ struct SortPlan {
         passes = (keyBits + 9) / 10;
         bits = (keyBits + passes - 1) / passes;
         digits = 1 << bits;
-        blocks = static_cast<int>((tokens + SORT_TILE - 1) / SORT_TILE);
-        // chunks of 16 occurrences and more: enough of them that every SM has 32 warps' worth, one group of lanes each
-        const long long lanes = std::max<long long>(1, (channels + 16 / typeBytes(type) - 1) / (16 / typeBytes(type)));
-        const long long groups = std::max<long long>(1, static_cast<long long>(numSMs) * 1024 / lanes);
+        large = tokens > numSMs * 2048ll;
+        const int tile = large ? 4096 : 1024;
+        blocks = static_cast<int>((tokens + tile - 1) / tile);
+        // chunks: 1024 threads' worth of groups per SM, 8 rows in flight each
+        const int wide = 16 / typeBytes(type);
+        const long long lanes = std::max<long long>(1, (channels + wide - 1) / wide), groups = std::max<long long>(1, numSMs * 1024ll / lanes);
         chunk = static_cast<int>(std::min<long long>(256, std::max<long long>(16, (tokens + groups - 1) / groups)));
+        chunk = (chunk + RUN_STEP - 1) / RUN_STEP * RUN_STEP;
         chunks = static_cast<int>((tokens + chunk - 1) / chunk);
-        keys = align256(static_cast<size_t>(tokens) * 4);
-        counts = 4 * keys;
-        totals = counts + align256(static_cast<size_t>(digits) * blocks * 4);
-        partial = totals + align256(digits * 4);
+        list = align256((static_cast<size_t>(tokens) + RUN_STEP) * sizeof(int2));
+        counts = (passes > 1 ? 2 : 1) * list;
+        before = counts + align256(static_cast<size_t>(digits) * blocks * 4);
+        totals = before + align256(static_cast<size_t>(digits) * blocks * 4);
+        present = totals + align256(digits * 4);
+        partial = present + (passes > 1 ? align256(static_cast<size_t>(rows)) : 0);
         bytes = partial + align256(static_cast<size_t>(chunks) * 2 * channels * 4);
     }
 };
@@ -255,20 +362,38 @@ cudaError_t byType(int type, F&& f)
     default: return f(__nv_bfloat16());
     }
 }
+template <class F>
+cudaError_t byLanes(int vectors, F&& f)
+{
+    if (vectors <= 1) return f(std::integral_constant<int, 1>());
+    if (vectors <= 4) return f(std::integral_constant<int, 4>());
+    if (vectors <= 8) return f(std::integral_constant<int, 8>());
+    if (vectors <= 16) return f(std::integral_constant<int, 16>());
+    return f(std::integral_constant<int, 32>());
+}
 template <class T, int VEC>
-cudaError_t launchRuns(const EmbeddingArgs& a, const RunArgs& r, cudaStream_t stream)
+cudaError_t launchRuns(const EmbeddingArgs& a, RunArgs r, cudaStream_t stream)
 {
     const int vectors = (a.channels + VEC - 1) / VEC;
-    auto go = [&](auto g) {
-        constexpr int G = decltype(g)::value;
-        embedding_runs_kernel<T, VEC, G><<<dim3((r.chunks + 256 / G - 1) / (256 / G), (vectors + G - 1) / G), 256, 0, stream>>>(a, r);
+    return byLanes(vectors, [&](auto g) {
+        constexpr int G = decltype(g)::value, GROUPS = 256 / G;
+        r.runBlocks = (r.chunks + GROUPS - 1) / GROUPS;
+        const long long fill = (a.rows + GROUPS * FILL_ROWS - 1) / (GROUPS * FILL_ROWS);
+        embedding_runs_kernel<T, VEC, G><<<dim3(static_cast<unsigned>(r.runBlocks + fill), (vectors + G - 1) / G), 256, 0, stream>>>(a, r);
         return cudaGetLastError();
-    };
-    if (vectors <= 1) return go(std::integral_constant<int, 1>());
-    if (vectors <= 4) return go(std::integral_constant<int, 4>());
-    if (vectors <= 8) return go(std::integral_constant<int, 8>());
-    if (vectors <= 16) return go(std::integral_constant<int, 16>());
-    return go(std::integral_constant<int, 32>());
+    });
+}
+template <int ITEMS, int WARPS>
+cudaError_t launchSort(const EmbeddingArgs& a, const SortArgs& s, cudaStream_t stream)
+{
+    sort_count_kernel<ITEMS, WARPS><<<s.blocks, WARPS * 32, 0, stream>>>(a, s);
+    partition_scan_kernel<<<(s.digits + PARTITION_WARPS - 1) / PARTITION_WARPS, PARTITION_THREADS, 0, stream>>>(s.counts, s.before, s.totals, s.digits, s.blocks);
+    if (moveBytes<ITEMS, WARPS>(PARTITION_MAX_DIGITS) > 48 * 1024) {
+        const cudaError_t e = allowShared(reinterpret_cast<const void*>(sort_move_kernel<ITEMS, WARPS>), moveBytes<ITEMS, WARPS>(PARTITION_MAX_DIGITS));
+        if (e != cudaSuccess) return e;
+    }
+    sort_move_kernel<ITEMS, WARPS><<<s.blocks, WARPS * 32, moveBytes<ITEMS, WARPS>(s.digits), stream>>>(a, s);
+    return cudaGetLastError();
 }
 
 } // namespace
@@ -284,50 +409,50 @@ cudaError_t launchEmbeddingForward(const EmbeddingArgs& a, cudaStream_t stream)
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
         const bool vec = wide(a.table, a.type, a.channels) && wide(a.y, a.type, a.channels);
-        const int perRow = vec ? a.channels / WIDE<T> : a.channels;
-        const long long total = a.tokens * perRow, blocks = (total + 256 * LOOKUPS - 1) / (256 * LOOKUPS);
-        if (vec) embedding_forward_kernel<T, WIDE<T>><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, total, perRow);
-        else embedding_forward_kernel<T, 1><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, total, perRow);
+        const int perRow = vec ? a.channels / WIDE<T> : a.channels, pass = perRow > 128 ? 1 : 256 / perRow;
+        const dim3 grid(static_cast<unsigned>((a.tokens + pass * LOOKUPS - 1) / (pass * LOOKUPS)), pass == 1 ? (perRow + 255) / 256 : 1);
+        if (vec) embedding_forward_kernel<T, WIDE<T>><<<grid, 256, 0, stream>>>(a, perRow, pass);
+        else embedding_forward_kernel<T, 1><<<grid, 256, 0, stream>>>(a, perRow, pass);
         return cudaGetLastError();
     });
 }
 
 cudaError_t launchEmbeddingAdjoint(const EmbeddingArgs& a, cudaStream_t stream)
 {
-    cudaError_t e = cudaSuccess;
-    if (a.rows > 0)
-        e = cudaMemset2DAsync(a.gradTable.data, static_cast<size_t>(a.gradTable.stride) * typeBytes(a.type), 0,
-                              static_cast<size_t>(a.channels) * typeBytes(a.type), static_cast<size_t>(a.rows), stream);
-    if (e != cudaSuccess || a.tokens == 0 || a.rows == 0) return e;
+    if (a.rows == 0) return cudaSuccess;
+    if (a.tokens == 0)
+        return cudaMemset2DAsync(a.gradTable.data, static_cast<size_t>(a.gradTable.stride) * typeBytes(a.type), 0, static_cast<size_t>(a.channels) * typeBytes(a.type),
+                                 static_cast<size_t>(a.rows), stream);
     const SortPlan p(a.tokens, a.rows, a.channels, a.type, a.numSMs);
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
-    int* keys[2] = {reinterpret_cast<int*>(base), reinterpret_cast<int*>(base + p.keys)};
-    int* slots[2] = {reinterpret_cast<int*>(base + 2 * p.keys), reinterpret_cast<int*>(base + 3 * p.keys)};
+    int2* lists[2] = {reinterpret_cast<int2*>(base), reinterpret_cast<int2*>(base + p.list)};
     SortArgs s{};
     s.counts = reinterpret_cast<int*>(base + p.counts);
+    s.before = reinterpret_cast<int*>(base + p.before);
     s.totals = reinterpret_cast<int*>(base + p.totals);
+    s.present = p.passes > 1 ? base + p.present : nullptr;
     s.items = static_cast<int>(a.tokens);
     s.blocks = p.blocks;
     s.digits = p.digits;
-    for (int k = 0; k < p.passes; ++k) {
-        s.keysIn = k > 0 ? keys[(k + 1) & 1] : nullptr;
-        s.slotsIn = k > 0 ? slots[(k + 1) & 1] : nullptr;
-        s.keysOut = keys[k & 1];
-        s.slotsOut = slots[k & 1];
+    cudaError_t e = p.passes > 1 ? cudaMemsetAsync(s.present, 0, static_cast<size_t>(a.rows), stream) : cudaSuccess;
+    for (int k = 0; k < p.passes && e == cudaSuccess; ++k) {
+        s.in = k > 0 ? lists[(k + 1) & 1] : nullptr;
+        s.out = lists[k & 1];
         s.shift = k * p.bits;
-        sort_count_kernel<<<p.blocks, PARTITION_THREADS, 0, stream>>>(a, s);
-        partition_scan_kernel<<<(p.digits + PARTITION_WARPS - 1) / PARTITION_WARPS, PARTITION_THREADS, 0, stream>>>(s.counts, s.totals, p.digits, p.blocks);
-        sort_move_kernel<<<p.blocks, PARTITION_THREADS, (PARTITION_WARPS + 1) * p.digits * sizeof(int), stream>>>(a, s);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        e = p.large ? launchSort<8, 16>(a, s, stream) : launchSort<4, 8>(a, s, stream);
     }
-    RunArgs r{s.keysOut, s.slotsOut, s.items, p.chunk, p.chunks, reinterpret_cast<float*>(base + p.partial)};
+    if (e != cudaSuccess) return e;
+    RunArgs r{s.out, s.present, s.totals, s.items, p.chunk, p.chunks, 0, reinterpret_cast<float*>(base + p.partial)};
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
         const bool vec = wide(a.gradTable, a.type, a.channels) && wide(a.gradY, a.type, a.channels);
         const cudaError_t status = vec ? launchRuns<T, WIDE<T>>(a, r, stream) : launchRuns<T, 1>(a, r, stream);
         if (status != cudaSuccess || p.chunks < 2) return status;
-        embedding_join_kernel<T><<<dim3(p.chunks - 1, (a.channels + 31) / 32), 256, 0, stream>>>(a, r);
-        return cudaGetLastError();
+        return byLanes(a.channels, [&](auto g) {
+            constexpr int G = decltype(g)::value;
+            embedding_join_kernel<T, G><<<dim3((p.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS, (a.channels + G - 1) / G), 512, 0, stream>>>(a, r);
+            return cudaGetLastError();
+        });
     });
 }
 

@@ -14,51 +14,73 @@ namespace ops {
 constexpr int PARTITION_THREADS = 256, PARTITION_WARPS = PARTITION_THREADS / 32;
 constexpr int PARTITION_MAX_DIGITS = 1024;
 
-// Ranks of one tile: items `item(i)` -> digit (or -1: no item) for i in [0, ITEMS * 256), in order; warp w holds the items
-// [w * ITEMS * 32, (w + 1) * ITEMS * 32). `counts` (warps x digits ints in shared memory) is left with the number of items of
-// a digit in the warps before, `rank` with an item's rank within its warp. All threads of the block call it.
-template <int ITEMS, class F>
-__device__ __forceinline__ void tileRanks(F&& item, int digits, int* counts, int (&digit)[ITEMS], int (&rank)[ITEMS])
+// lanes whose digit is this lane's (-1: no item), by a vote per bit
+__device__ __forceinline__ unsigned sameDigit(int d, int bits)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int i = threadIdx.x; i < PARTITION_WARPS * digits; i += PARTITION_THREADS) counts[i] = 0;
-    __syncthreads();
-    int* mine = counts + warp * digits;
+    unsigned same = __ballot_sync(0xffffffffu, d >= 0);
+    if (d < 0) same = ~same;
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int d = item((warp * ITEMS + k) * 32 + lane);
-        const unsigned same = __match_any_sync(0xffffffffu, d);
-        const int before = d >= 0 ? mine[d] : 0;
-        __syncwarp();
-        digit[k] = d;
-        rank[k] = before + __popc(same & ((1u << lane) - 1));
-        if (d >= 0 && lane == 31 - __clz(same)) mine[d] = before + __popc(same);
-        __syncwarp();
+    for (int b = 0; b < 10; ++b) {
+        if (b >= bits) break;
+        const unsigned set = __ballot_sync(0xffffffffu, (d >> b) & 1);
+        same &= (d >> b) & 1 ? set : ~set;
     }
-    __syncthreads();
-}
-// counts (warps x digits) -> items of the digit in the warps before; returns the block's count of digit `d`
-__device__ __forceinline__ int warpOffsets(int* counts, int digits, int d, int start)
-{
-    int sum = start;
-#pragma unroll
-    for (int w = 0; w < PARTITION_WARPS; ++w) {
-        const int c = counts[w * digits + d];
-        counts[w * digits + d] = sum;
-        sum += c;
-    }
-    return sum - start;
+    return same;
 }
 
-// exclusive sums of up to 1024 ints by one block of 256 threads: values in `v` (shared, n ints) are replaced; `warpSums`: 8 ints.
-// Returns the total to every thread.
-__device__ __forceinline__ int blockExclusive(int* v, int n, int* warpSums)
+// Ranks of one tile: items `item(i)` -> digit (or -1: no item) for i in [0, ITEMS * 32 * WARPS), in order; warp w holds the items
+// [w * ITEMS * 32, (w + 1) * ITEMS * 32). `counts` (WARPS x digits, 16 bits each, in shared memory) is left with the number of items of a digit in
+// each warp, `rank` with an item's rank within its warp. All threads of the block call it; it ends in a barrier.
+template <int ITEMS, int WARPS, class F>
+__device__ __forceinline__ void tileRanks(F&& item, int digits, uint16_t* counts, int (&digit)[ITEMS], int (&rank)[ITEMS])
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int own[4], sum = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = threadIdx.x * 4 + i;
+    for (int k = 0; k < ITEMS; ++k) digit[k] = item((warp * ITEMS + k) * 32 + lane);   // (all on their way before the first is used)
+    for (int i = threadIdx.x; i < (WARPS * digits + 1) / 2; i += WARPS * 32) reinterpret_cast<uint32_t*>(counts)[i] = 0;
+    __syncthreads();
+    uint16_t* mine = counts + warp * digits;
+    const int bits = 32 - __clz(digits - 1);
+    unsigned same[ITEMS];   // (votes of all items first: they do not wait for one another's counters)
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) same[k] = sameDigit(digit[k], bits);
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int d = digit[k];
+        const int before = d >= 0 ? mine[d] : 0;
+        __syncwarp();
+        rank[k] = before + __popc(same[k] & ((1u << lane) - 1));
+        if (d >= 0 && lane == 31 - __clz(same[k])) mine[d] = static_cast<uint16_t>(before + __popc(same[k]));
+        __syncwarp();
+    }
+    __syncthreads();
+}
+// counts (WARPS x digits) of digit `d` -> items of the digit in the warps before; returns the block's count of it
+template <int WARPS>
+__device__ __forceinline__ int warpOffsets(uint16_t* counts, int digits, int d)
+{
+    int c[WARPS], sum = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) c[w] = counts[w * digits + d];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        counts[w * digits + d] = static_cast<uint16_t>(sum);
+        sum += c[w];
+    }
+    return sum;
+}
+
+// exclusive sums of up to 1024 ints by one block of at least 256 threads: values in `v` (shared, n ints) are replaced; `warpSums`: an int per warp.
+// Returns the total to every thread.
+template <int WARPS = PARTITION_WARPS>
+__device__ __forceinline__ int blockExclusive(int* v, int n, int* warpSums)
+{
+    constexpr int EACH = 1024 / (WARPS * 32);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int own[EACH], sum = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int k = threadIdx.x * EACH + i;
         own[i] = k < n ? v[k] : 0;
         sum += own[i];
     }
@@ -72,13 +94,13 @@ __device__ __forceinline__ int blockExclusive(int* v, int n, int* warpSums)
     __syncthreads();
     int before = inclusive - sum, total = 0;
 #pragma unroll
-    for (int w = 0; w < PARTITION_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         if (w < warp) before += warpSums[w];
         total += warpSums[w];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = threadIdx.x * 4 + i;
+    for (int i = 0; i < EACH; ++i) {
+        const int k = threadIdx.x * EACH + i;
         if (k < n) v[k] = before;
         before += own[i];
     }
@@ -86,12 +108,14 @@ __device__ __forceinline__ int blockExclusive(int* v, int n, int* warpSums)
     return total;
 }
 
-// counts[digit * blocks + block] -> exclusive sums over the blocks; totals[digit]. One warp per digit.
-static __global__ void __launch_bounds__(PARTITION_THREADS) partition_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int digits, int blocks)
+// counts[digit * blocks + block] -> exclusive sums over the blocks, before[block * digits + digit]; totals[digit]. One warp per digit. (Either side reads what
+// it needs side by side: a block of the move that gathered a column of 1024 digits took 5000 clocks for it.)
+static __global__ void __launch_bounds__(PARTITION_THREADS)
+    partition_scan_kernel(const int* __restrict__ counts, int* __restrict__ before, int* __restrict__ totals, int digits, int blocks)
 {
     const int d = blockIdx.x * PARTITION_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (d >= digits) return;
-    int* row = counts + static_cast<long long>(d) * blocks;
+    const int* row = counts + static_cast<long long>(d) * blocks;
     int carry = 0;
     for (int b0 = 0; b0 < blocks; b0 += 128) {
         int v[4];
@@ -105,7 +129,7 @@ static __global__ void __launch_bounds__(PARTITION_THREADS) partition_scan_kerne
                 const int up = __shfl_up_sync(0xffffffffu, inclusive, o);
                 if (lane >= o) inclusive += up;
             }
-            if (b0 + i * 32 + lane < blocks) row[b0 + i * 32 + lane] = carry + inclusive - v[i];
+            if (b0 + i * 32 + lane < blocks) before[static_cast<long long>(b0 + i * 32 + lane) * digits + d] = carry + inclusive - v[i];
             carry += __shfl_sync(0xffffffffu, inclusive, 31);
         }
     }

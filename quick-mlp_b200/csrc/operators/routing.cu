@@ -66,11 +66,11 @@ constexpr int TILE_ITEMS = 4, TILE_SLOTS = TILE_ITEMS * PARTITION_THREADS;   // 
 // Ranks the slots of a tile and writes order and position. `expertOf(i)`: expert of the tile's i-th slot, -1: none.
 // `start`: where the tile's slots of an expert begin (shared memory), `last`: experts.
 template <class F>
-__device__ __forceinline__ void placeSlots(const RouteArgs& a, F&& expertOf, long long firstSlot, int slots, const int* start, int* counts)
+__device__ __forceinline__ void placeSlots(const RouteArgs& a, F&& expertOf, long long firstSlot, int slots, const int* start, uint16_t* counts)
 {
     int digit[TILE_ITEMS], rank[TILE_ITEMS];
-    tileRanks<TILE_ITEMS>([&](int i) { return i < slots ? expertOf(i) : -1; }, a.experts, counts, digit, rank);
-    for (int d = threadIdx.x; d < a.experts; d += PARTITION_THREADS) warpOffsets(counts, a.experts, d, start[d]);
+    tileRanks<TILE_ITEMS, PARTITION_WARPS>([&](int i) { return i < slots ? expertOf(i) : -1; }, a.experts, counts, digit, rank);
+    for (int d = threadIdx.x; d < a.experts; d += PARTITION_THREADS) warpOffsets<PARTITION_WARPS>(counts, a.experts, d);
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -80,7 +80,7 @@ __device__ __forceinline__ void placeSlots(const RouteArgs& a, F&& expertOf, lon
         const long long slot = firstSlot + i;
         int to = -1;
         if (digit[k] >= 0) {
-            to = counts[warp * a.experts + digit[k]] + rank[k];
+            to = start[digit[k]] + counts[warp * a.experts + digit[k]] + rank[k];
             a.order[to] = static_cast<int>(slot);
         }
         a.position[slot] = to;
@@ -89,13 +89,14 @@ __device__ __forceinline__ void placeSlots(const RouteArgs& a, F&& expertOf, lon
 
 struct RoutePlan {
     int tokensPerTile, tiles;
-    size_t counts, bytes;
+    size_t counts, before, bytes;
     RoutePlan(long long tokens, int experts, int chosen)
     {
         tokensPerTile = std::max(1, TILE_SLOTS / chosen);
         tiles = static_cast<int>((tokens + tokensPerTile - 1) / tokensPerTile);
         counts = (static_cast<size_t>(experts) * 4 + 255) / 256 * 256;
-        bytes = counts + static_cast<size_t>(experts) * tiles * 4;
+        before = counts + (static_cast<size_t>(experts) * tiles * 4 + 255) / 256 * 256;
+        bytes = before + static_cast<size_t>(experts) * tiles * 4;
     }
 };
 
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant
     __syncthreads();
     if constexpr (ALONE) {
         __shared__ int warpSums[PARTITION_WARPS];
-        int* counts = shCount + a.experts;   // warps x experts
+        uint16_t* counts = reinterpret_cast<uint16_t*>(shCount + a.experts);   // warps x experts
         const int total = blockExclusive(shCount, a.experts, warpSums);
         for (int e = threadIdx.x; e < a.experts; e += 256) a.offsets[e] = shCount[e];
         if (threadIdx.x == 0) a.offsets[a.experts] = total;
@@ -184,11 +185,12 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant
     }
 }
 
-__global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, const int* __restrict__ tileCounts,
-                                                                        const int* __restrict__ totals, int tiles)
+__global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, const int* __restrict__ tileBefore,
+                                                                        const int* __restrict__ totals)
 {
     extern __shared__ int dynamic[];
-    int *start = dynamic, *counts = dynamic + a.experts;
+    int* start = dynamic;
+    uint16_t* counts = reinterpret_cast<uint16_t*>(dynamic + a.experts);
     __shared__ int warpSums[PARTITION_WARPS];
     for (int e = threadIdx.x; e < a.experts; e += PARTITION_THREADS) start[e] = totals[e];
     __syncthreads();
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __
     for (long long i = total + static_cast<long long>(blockIdx.x) * PARTITION_THREADS + threadIdx.x; i < all; i += static_cast<long long>(gridDim.x) * PARTITION_THREADS)
         a.order[i] = -1;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += PARTITION_THREADS) start[e] += tileCounts[static_cast<long long>(e) * tiles + blockIdx.x];
+    for (int e = threadIdx.x; e < a.experts; e += PARTITION_THREADS) start[e] += tileBefore[static_cast<long long>(blockIdx.x) * a.experts + e];
     __syncthreads();
     placeSlots(a, [&](int i) { return a.expert[firstSlot + i]; }, firstSlot, slots, start, counts);
 }
@@ -419,6 +421,7 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
     const bool alone = p.tiles == 1, vec = wide(a.logits, a.type, a.experts);
     int* totals = static_cast<int*>(a.scratch);
     int* counts = reinterpret_cast<int*>(static_cast<unsigned char*>(a.scratch) + p.counts);
+    int* before = reinterpret_cast<int*>(static_cast<unsigned char*>(a.scratch) + p.before);
     cudaError_t e = byType(a.type, [&](auto t) {
         using T = decltype(t);
         return byExperts(a.experts, [&](auto l, auto per) {
@@ -433,8 +436,8 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
         });
     });
     if (e != cudaSuccess || alone) return e;
-    partition_scan_kernel<<<(a.experts + PARTITION_WARPS - 1) / PARTITION_WARPS, PARTITION_THREADS, 0, stream>>>(counts, totals, a.experts, p.tiles);
-    route_place_kernel<<<p.tiles, PARTITION_THREADS, (1 + PARTITION_WARPS) * a.experts * sizeof(int), stream>>>(a, p.tokensPerTile, counts, totals, p.tiles);
+    partition_scan_kernel<<<(a.experts + PARTITION_WARPS - 1) / PARTITION_WARPS, PARTITION_THREADS, 0, stream>>>(counts, before, totals, a.experts, p.tiles);
+    route_place_kernel<<<p.tiles, PARTITION_THREADS, (1 + PARTITION_WARPS) * a.experts * sizeof(int), stream>>>(a, p.tokensPerTile, before, totals);
     return cudaGetLastError();
 }
 

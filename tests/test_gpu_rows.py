@@ -128,7 +128,7 @@ def embedding_case(qmlp, tokens, table, scale, grad):
 
 @pytest.mark.parametrize("dtype", FLOATS, ids=IDS.get)
 @pytest.mark.parametrize("tokens,rows,channels", [(1, 1, 1), (1, 1000, 64), (7, 3, 8), (100, 1, 33), (2048, 17, 32), (2049, 1023, 4), (5000, 1024, 16),
-                                                  (3001, 1025, 100), (70000, 300, 24), (20000, 40000, 7), (300, 100000, 256), (4097, 50, 1030)])
+                                                  (3001, 1025, 100), (70000, 300, 24), (20000, 40000, 7), (300, 100000, 256), (4097, 50, 1030), (310001, 700, 8), (320000, 3000, 5)])
 def test_embedding(qmlp, tokens, rows, channels, dtype):
     t = ints(30, (tokens,), -2, rows + 2)       # a few outside the table
     embedding_case(qmlp, t, rand(31, (rows, channels), dtype), 1.0 if channels % 2 else channels ** 0.5, rand(32, (tokens, channels), dtype))
