@@ -111,6 +111,7 @@ kernel::ExchangeArgs exchange(const qmlp_routing_t* r, const qmlp_tensor_t* feat
     a.order = r->order;
     a.position = r->positions;
     a.weights = r->weights;
+    a.numSMs = Library::instance().smCount();
     return a;
 }
 void checkSlots(const qmlp_tensor_t* t, const qmlp_routing_t* r, const qmlp_tensor_t* features, const char* name, bool written)

@@ -94,6 +94,19 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
     return d;
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// an access' elements in pairs (an odd one with a zero)
+template <int VEC> constexpr int PAIRS = (VEC + 1) / 2;
+template <class T, int VEC>
+__device__ __forceinline__ void unpackPairs(const Pack<T, VEC>& p, float2 (&f)[PAIRS<VEC>])
+{
+    if constexpr (VEC == 1) f[0] = make_float2(Element<T>::to(p.v[0]), 0.f);
+    else unpack<T, VEC>(p, *reinterpret_cast<float (*)[VEC]>(&f[0]));
+}
+template <class T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> packPairs(const float2 (&f)[PAIRS<VEC>])
+{
+    return pack<T, VEC>(*reinterpret_cast<const float (*)[VEC]>(&f[0]));
+}
 
 // 16-byte accesses go through uint4, so that they stay one instruction
 template <class T, int VEC>

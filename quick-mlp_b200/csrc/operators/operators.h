@@ -78,7 +78,7 @@ cudaError_t launchRouteAdjoint(const RouteArgs& a, cudaStream_t stream);
 
 struct ExchangeArgs {
     long long tokens;
-    int chosen, channels, type;
+    int chosen, channels, type, numSMs;
     Rows x, rows;              // (tokens, channels), (tokens * chosen, channels)
     const int *order, *position;
     const float* weights;      // (tokens, chosen)

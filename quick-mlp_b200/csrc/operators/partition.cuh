@@ -108,32 +108,46 @@ __device__ __forceinline__ int blockExclusive(int* v, int n, int* warpSums)
     return total;
 }
 
-// counts[digit * blocks + block] -> exclusive sums over the blocks, before[block * digits + digit]; totals[digit]. One warp per digit. (Either side reads what
-// it needs side by side: a block of the move that gathered a column of 1024 digits took 5000 clocks for it.)
+// counts[digit * blocks + block] -> exclusive sums over the blocks, before[block * digits + digit]; totals[digit]. One thread block per digit. (Either side reads
+// what it needs side by side.)
 static __global__ void __launch_bounds__(PARTITION_THREADS)
     partition_scan_kernel(const int* __restrict__ counts, int* __restrict__ before, int* __restrict__ totals, int digits, int blocks)
 {
-    const int d = blockIdx.x * PARTITION_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (d >= digits) return;
+    __shared__ int warpSums[PARTITION_WARPS];
+    const int d = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int* row = counts + static_cast<long long>(d) * blocks;
     int carry = 0;
-    for (int b0 = 0; b0 < blocks; b0 += 128) {
-        int v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = b0 + i * 32 + lane < blocks ? row[b0 + i * 32 + lane] : 0;
+    for (int b0 = 0; b0 < blocks; b0 += 4 * PARTITION_THREADS) {
+        int v[4], sum = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            int inclusive = v[i];
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int up = __shfl_up_sync(0xffffffffu, inclusive, o);
-                if (lane >= o) inclusive += up;
-            }
-            if (b0 + i * 32 + lane < blocks) before[static_cast<long long>(b0 + i * 32 + lane) * digits + d] = carry + inclusive - v[i];
-            carry += __shfl_sync(0xffffffffu, inclusive, 31);
+            const int b = b0 + static_cast<int>(threadIdx.x) * 4 + i;
+            v[i] = b < blocks ? row[b] : 0;
+            sum += v[i];
         }
+        int inclusive = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, inclusive, o);
+            if (lane >= o) inclusive += up;
+        }
+        if (lane == 31) warpSums[warp] = inclusive;
+        __syncthreads();
+        int at = carry + inclusive - sum;
+#pragma unroll
+        for (int w = 0; w < PARTITION_WARPS; ++w) {
+            if (w < warp) at += warpSums[w];
+            carry += warpSums[w];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = b0 + static_cast<int>(threadIdx.x) * 4 + i;
+            if (b < blocks) before[static_cast<long long>(b) * digits + d] = at;
+            at += v[i];
+        }
+        __syncthreads();
     }
-    if (lane == 0) totals[d] = carry;
+    if (threadIdx.x == 0) totals[d] = carry;
 }
 
 } // namespace ops

@@ -7,8 +7,7 @@
 //   adjoint over the chosen: dz_j = w_j (g_j - sum_i g_i w_i);  over all: dz_i = p_i (g of the slot that chose i, or 0, - sum_j g_j w_j)
 //
 // A row belongs to LANES lanes of 8 logits each (one for 8 experts, a warp for 256; 32 logits each above that). Every round takes
-// the maximum over the lanes of one 64-bit key, the order-preserving form of the logit above the complement of its index, so the
-// tie goes to the lowest index without a second reduction.
+// the maximum over the lanes of one key that holds the logit and its expert.
 #include "partition.cuh"
 
 #include <algorithm>
@@ -19,63 +18,91 @@ namespace {
 
 using namespace ops;
 
-// order-preserving: larger floats give larger integers, NaN the largest of all, -inf 0 (never chosen)
-__device__ __forceinline__ unsigned orderedKey(float f)
-{
-    if (f != f) return 0xffffffffu;
-    const unsigned u = __float_as_uint(f + 0.f);   // (-0 becomes +0: the two are equal)
-    const unsigned key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return key == 0x007fffffu ? 0u : key;
-}
-__device__ __forceinline__ float orderedValue(unsigned key)
-{
-    if (key == 0xffffffffu) return __uint_as_float(0x7fc00000u);
-    if (key == 0u) return __uint_as_float(0xff800000u);
-    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
-}
-template <int LANES>
-__device__ __forceinline__ unsigned long long groupMax(unsigned long long v)
+// Keys of logits: larger logits give larger keys, NaN the largest of all, -inf gives 0 (never chosen); below the logit's bits the complement of the
+// expert's number, so that the largest key is the first of equal logits. 32 bits hold a 16-bit logit and its expert, floats take 64.
+template <class T> struct Key;
+template <> struct Key<float> {
+    using Type = unsigned long long;
+    static __device__ __forceinline__ Type of(float f, int expert)
+    {
+        const unsigned u = __float_as_uint(f + 0.f);   // (-0 becomes +0: the two are equal)
+        const unsigned key = f != f ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+        return key == 0x007fffffu ? 0ull : static_cast<Type>(key) << 32 | ~static_cast<unsigned>(expert);
+    }
+    static __device__ __forceinline__ float value(Type k)
+    {
+        const unsigned key = static_cast<unsigned>(k >> 32);
+        return __uint_as_float(key == 0xffffffffu ? 0x7fc00000u : (key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+    }
+    static __device__ __forceinline__ int expert(Type k) { return static_cast<int>(~static_cast<unsigned>(k)); }
+};
+template <class T, unsigned INF>
+struct ShortKey {
+    using Type = unsigned;
+    static __device__ __forceinline__ Type of(T f, int expert)
+    {
+        const unsigned u = *reinterpret_cast<const unsigned short*>(&f), magnitude = u & 0x7fffu;
+        unsigned key = u > 0x8000u ? ~u & 0xffffu : magnitude | 0x8000u;   // (-0 becomes +0: the two are equal)
+        if (magnitude > INF) key = 0xffffu;
+        return u == (0x8000u | INF) ? 0u : key << 16 | (0xffffu - expert);
+    }
+    static __device__ __forceinline__ float value(Type k)
+    {
+        const unsigned key = k >> 16;
+        const unsigned short u = static_cast<unsigned short>(key == 0xffffu ? 0x7fffu : (key & 0x8000u) ? key & 0x7fffu : ~key);
+        return Element<T>::to(*reinterpret_cast<const T*>(&u));
+    }
+    static __device__ __forceinline__ int expert(Type k) { return static_cast<int>(0xffffu - (k & 0xffffu)); }
+};
+template <> struct Key<__half> : ShortKey<__half, 0x7c00u> {};
+template <> struct Key<__nv_bfloat16> : ShortKey<__nv_bfloat16, 0x7f80u> {};
+
+template <int LANES, class K>
+__device__ __forceinline__ K groupMax(K v)
 {
 #pragma unroll
     for (int o = LANES / 2; o > 0; o /= 2) {
-        const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
+        const K w = __shfl_xor_sync(0xffffffffu, v, o);
         v = w > v ? w : v;
     }
     return v;
 }
 
-// the PER logits of lane `lane` of a row, -inf behind the last expert
+template <class T> __device__ __forceinline__ T minusInfinity() { return Element<T>::from(__uint_as_float(0xff800000u)); }
+// the PER logits of lane `lane` of a row, as they lie in memory; -inf behind the last expert
 template <class T, int PER, bool VECTOR>
-__device__ __forceinline__ void loadLogits(const T* row, int lane, int experts, float (&z)[PER])
+__device__ __forceinline__ void loadLogits(const T* row, int lane, int experts, T (&z)[PER])
 {
     constexpr int W = VECTOR ? WIDE<T> : 1;
 #pragma unroll
     for (int i = 0; i < PER; i += W) {
         const int c = lane * PER + i;
-        float f[W];
+        Pack<T, W> p;
 #pragma unroll
-        for (int k = 0; k < W; ++k) f[k] = __uint_as_float(0xff800000u);
-        if (c < experts) unpack<T, W>(load<T, W>(row + c), f);
+        for (int k = 0; k < W; ++k) p.v[k] = minusInfinity<T>();
+        if (c < experts) p = load<T, W>(row + c);
 #pragma unroll
-        for (int k = 0; k < W; ++k) z[i + k] = f[k];
+        for (int k = 0; k < W; ++k) z[i + k] = p.v[k];
     }
 }
 
-constexpr int TILE_ITEMS = 4, TILE_SLOTS = TILE_ITEMS * PARTITION_THREADS;   // slots per block, at most
+// slots per block, at most: a block that is alone takes 1024, else 512, so that the rows of a tile are few passes of a block
+constexpr int ALONE_ITEMS = 4, TILE_ITEMS = 2;
+constexpr int ALONE_SLOTS = ALONE_ITEMS * PARTITION_THREADS, TILE_SLOTS = TILE_ITEMS * PARTITION_THREADS;
 
 // Ranks the slots of a tile and writes order and position. `expertOf(i)`: expert of the tile's i-th slot, -1: none.
 // `start`: where the tile's slots of an expert begin (shared memory), `last`: experts.
-template <class F>
+template <int ITEMS, class F>
 __device__ __forceinline__ void placeSlots(const RouteArgs& a, F&& expertOf, long long firstSlot, int slots, const int* start, uint16_t* counts)
 {
-    int digit[TILE_ITEMS], rank[TILE_ITEMS];
-    tileRanks<TILE_ITEMS, PARTITION_WARPS>([&](int i) { return i < slots ? expertOf(i) : -1; }, a.experts, counts, digit, rank);
+    int digit[ITEMS], rank[ITEMS];
+    tileRanks<ITEMS, PARTITION_WARPS>([&](int i) { return i < slots ? expertOf(i) : -1; }, a.experts, counts, digit, rank);
     for (int d = threadIdx.x; d < a.experts; d += PARTITION_THREADS) warpOffsets<PARTITION_WARPS>(counts, a.experts, d);
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int k = 0; k < TILE_ITEMS; ++k) {
-        const int i = (warp * TILE_ITEMS + k) * 32 + lane;
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = (warp * ITEMS + k) * 32 + lane;
         if (i >= slots) continue;
         const long long slot = firstSlot + i;
         int to = -1;
@@ -92,7 +119,7 @@ struct RoutePlan {
     size_t counts, before, bytes;
     RoutePlan(long long tokens, int experts, int chosen)
     {
-        tokensPerTile = std::max(1, TILE_SLOTS / chosen);
+        tokensPerTile = std::max(1, (tokens * chosen <= ALONE_SLOTS ? ALONE_SLOTS : TILE_SLOTS) / chosen);
         tiles = static_cast<int>((tokens + tokensPerTile - 1) / tokensPerTile);
         counts = (static_cast<size_t>(experts) * 4 + 255) / 256 * 256;
         before = counts + (static_cast<size_t>(experts) * tiles * 4 + 255) / 256 * 256;
@@ -101,42 +128,44 @@ struct RoutePlan {
 };
 
 // One tile of rows per block: choose, weigh, count the chosen experts. With ALONE there is one tile, and the block places its
-// slots itself.
+// slots itself. 262147 rows of 64 half logits, 2 chosen: 33 us (with 64-bit keys, tiles of 1024 slots and no row fetched ahead 60 us).
 template <class T, int LANES, int PER, bool VECTOR, bool ALONE>
 __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, int* __restrict__ tileCounts, int tiles)
 {
+    using K = Key<T>;
+    constexpr int SLOTS = ALONE ? ALONE_SLOTS : TILE_SLOTS;
     extern __shared__ int dynamic[];
-    float* shWeight = reinterpret_cast<float*>(dynamic);        // TILE_SLOTS
-    int* shExpert = dynamic + TILE_SLOTS;                       // TILE_SLOTS
-    int* shCount = shExpert + TILE_SLOTS;                       // experts
+    float* shWeight = reinterpret_cast<float*>(dynamic);        // SLOTS: exp(logit - largest)
+    int* shExpert = dynamic + SLOTS;                            // SLOTS
+    float* shTotal = reinterpret_cast<float*>(dynamic + 2 * SLOTS);   // SLOTS: of a row
+    int* shCount = dynamic + 3 * SLOTS;                         // experts
     const int lane = threadIdx.x % LANES;
     const long long first = static_cast<long long>(blockIdx.x) * tokensPerTile;
     const int tokens = static_cast<int>(min(static_cast<long long>(tokensPerTile), a.tokens - first));
+    const T* logits = static_cast<const T*>(a.logits.data) + first * a.logits.stride;
+    T next[PER];   // the row after is on its way while one is worked on
+    int t = threadIdx.x / LANES;
+    loadLogits<T, PER, VECTOR>(logits + (t < tokens ? t : 0) * a.logits.stride, lane, a.experts, next);
     for (int i = threadIdx.x; i < a.experts; i += 256) shCount[i] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < tokens; t0 += 256 / LANES) {
-        const int t = t0 + threadIdx.x / LANES;
+    for (int t0 = 0; t0 < tokens; t0 += 256 / LANES, t += 256 / LANES) {
         const bool active = t < tokens;
+        typename K::Type key[PER], best = 0;
         float z[PER];
-        loadLogits<T, PER, VECTOR>(static_cast<const T*>(a.logits.data) + (first + (active ? t : 0)) * a.logits.stride, lane, a.experts, z);
-        unsigned key[PER];
-        unsigned long long best = 0;
-        auto localBest = [&]() {
-            best = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const unsigned long long k = (static_cast<unsigned long long>(key[i]) << 32) | (~static_cast<unsigned>(lane * PER + i));
-                if (key[i] != 0 && k > best) best = k;
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < PER; ++i) key[i] = orderedKey(z[i]);
-        localBest();
+        for (int i = 0; i < PER; ++i) {
+            key[i] = K::of(next[i], lane * PER + i);
+            z[i] = Element<T>::to(next[i]);
+            best = key[i] > best ? key[i] : best;
+        }
+        if (t0 + 256 / LANES < tokens) {
+            const int after = t + 256 / LANES;
+            loadLogits<T, PER, VECTOR>(logits + (after < tokens ? after : 0) * a.logits.stride, lane, a.experts, next);
+        }
         float top = 0.f, total = 0.f;
         for (int j = 0; j < a.chosen; ++j) {
-            const unsigned long long m = groupMax<LANES>(best);
-            const int expert = m == 0 ? -1 : static_cast<int>(~static_cast<unsigned>(m));
-            const float value = orderedValue(static_cast<unsigned>(m >> 32));
+            const typename K::Type m = groupMax<LANES>(best);
+            const float value = K::value(m);
             if (j == 0) {
                 top = m == 0 ? 0.f : value;
                 if (!a.normalize) {
@@ -148,29 +177,27 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant
             }
             const float share = m == 0 ? 0.f : expf(value - top);
             if (a.normalize) total += share;
-            if (expert >= 0 && expert / PER == lane) {
+            best = 0;
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (expert % PER == i) key[i] = 0;
-                localBest();
+            for (int i = 0; i < PER; ++i) {
+                if (key[i] == m) key[i] = 0;
+                best = key[i] > best ? key[i] : best;
             }
             if (active && lane == 0) {
+                const int expert = m == 0 ? -1 : K::expert(m);
                 shWeight[t * a.chosen + j] = share;
                 shExpert[t * a.chosen + j] = expert;
                 if (expert >= 0) atomicAdd(&shCount[expert], 1);
             }
         }
-        __syncwarp();
-        if (active) {   // the lanes of the row share the division of its slots
-            for (int j = lane; j < a.chosen; j += LANES) {
-                const int i = t * a.chosen + j;
-                const float w = shExpert[i] < 0 ? 0.f : shWeight[i] / total;
-                a.weights[first * a.chosen + i] = w;
-                a.expert[first * a.chosen + i] = shExpert[i];
-            }
-        }
+        if (active && lane == 0) shTotal[t] = total;
     }
     __syncthreads();
+    for (int i = threadIdx.x; i < tokens * a.chosen; i += 256) {
+        const int expert = shExpert[i];
+        a.weights[first * a.chosen + i] = expert < 0 ? 0.f : shWeight[i] / shTotal[i / a.chosen];
+        a.expert[first * a.chosen + i] = expert;
+    }
     if constexpr (ALONE) {
         __shared__ int warpSums[PARTITION_WARPS];
         uint16_t* counts = reinterpret_cast<uint16_t*>(shCount + a.experts);   // warps x experts
@@ -179,7 +206,7 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant
         if (threadIdx.x == 0) a.offsets[a.experts] = total;
         const int slots = tokens * a.chosen;
         for (int i = total + threadIdx.x; i < slots; i += 256) a.order[i] = -1;
-        placeSlots(a, [&](int i) { return shExpert[i]; }, 0, slots, shCount, counts);
+        placeSlots<ALONE_ITEMS>(a, [&](int i) { return shExpert[i]; }, 0, slots, shCount, counts);
     } else {
         for (int e = threadIdx.x; e < a.experts; e += 256) tileCounts[static_cast<long long>(e) * tiles + blockIdx.x] = shCount[e];
     }
@@ -207,7 +234,7 @@ __global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __
     __syncthreads();
     for (int e = threadIdx.x; e < a.experts; e += PARTITION_THREADS) start[e] += tileBefore[static_cast<long long>(blockIdx.x) * a.experts + e];
     __syncthreads();
-    placeSlots(a, [&](int i) { return a.expert[firstSlot + i]; }, firstSlot, slots, start, counts);
+    placeSlots<TILE_ITEMS>(a, [&](int i) { return a.expert[firstSlot + i]; }, firstSlot, slots, start, counts);
 }
 
 template <class T, int LANES, int PER, bool VECTOR>
@@ -227,16 +254,22 @@ __global__ void __launch_bounds__(256) route_adjoint_kernel(const __grid_constan
 #pragma unroll
     for (int i = 0; i < PER; ++i) d[i] = 0.f;
     if (!a.normalize) {
-        float z[PER];
-        loadLogits<T, PER, VECTOR>(static_cast<const T*>(a.logits.data) + row * a.logits.stride, lane, a.experts, z);
-        unsigned long long best = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) best = max(best, static_cast<unsigned long long>(orderedKey(z[i])));
-        const float top = orderedValue(static_cast<unsigned>(groupMax<LANES>(best)));
-        float s = 0.f;
+        using K = Key<T>;
+        T raw[PER];
+        loadLogits<T, PER, VECTOR>(static_cast<const T*>(a.logits.data) + row * a.logits.stride, lane, a.experts, raw);
+        typename K::Type best = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            z[i] = z[i] == __uint_as_float(0xff800000u) ? 0.f : expf(z[i] - top);
+            const typename K::Type key = K::of(raw[i], lane * PER + i);
+            best = key > best ? key : best;
+        }
+        best = groupMax<LANES>(best);
+        const float top = K::value(best);
+        float s = 0.f, z[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            z[i] = Element<T>::to(raw[i]);
+            z[i] = best == 0 || z[i] == __uint_as_float(0xff800000u) ? 0.f : expf(z[i] - top);
             s += z[i];
         }
         const float inverse = 1.f / groupSum<LANES>(s);
@@ -267,117 +300,190 @@ __global__ void __launch_bounds__(256) route_adjoint_kernel(const __grid_constan
 }
 
 // ---- movement of feature rows --------------------------------------------------------------------------------------------
-// rows[r] = x[order[r] / chosen], zeros behind the last expert's rows. One access per thread and step.
+// As in the embedding: a thread takes one access' worth of several rows, `pass` rows apart, so that it divides once; rows of more than 256 accesses are
+// cut over blockIdx.y.
+struct Place {
+    int row, c;   // row within a block's first pass, element within the row
+    bool inside;
+    __device__ __forceinline__ Place(int perRow, int pass, int vec)
+    {
+        row = pass == 1 ? 0 : static_cast<int>(threadIdx.x) / perRow;
+        const int access = pass == 1 ? blockIdx.y * 256 + threadIdx.x : threadIdx.x - row * perRow;
+        inside = row < pass && access < perRow;
+        c = access * vec;
+    }
+};
+
+// rows[r] = x[order[r] / chosen], zeros behind the last expert's rows. 262144 rows of 256 half: 38 us, 5.4 TB/s (blocks that walk on: 41 us).
 constexpr int MOVES = 4;
 template <class T, int VEC>
-__global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ ExchangeArgs a, long long total, int perRow)
+__global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ ExchangeArgs a, int perRow, int pass)
 {
+    const Place at(perRow, pass, VEC);
+    if (!at.inside) return;
     const T* x = static_cast<const T*>(a.x.data);
     T* rows = static_cast<T*>(a.rows.data);
-    const long long first = blockIdx.x * (256ll * MOVES) + threadIdx.x;
+    const long long first = static_cast<long long>(blockIdx.x) * (pass * MOVES) + at.row, slots = a.tokens * a.chosen;
+    int token[MOVES];
     Pack<T, VEC> v[MOVES];
-    long long at[MOVES];
 #pragma unroll
     for (int k = 0; k < MOVES; ++k) {
-        const long long i = first + k * 256;
-        at[k] = -1;
+        const int slot = first + k * pass < slots ? a.order[first + k * pass] : -1;
+        token[k] = slot < 0 ? -1 : slot / a.chosen;
+    }
+#pragma unroll
+    for (int k = 0; k < MOVES; ++k) {
         v[k] = {};
-        if (i >= total) continue;
-        const long long r = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(perRow) : i / perRow;
-        const int c = static_cast<int>(i - r * perRow) * VEC, slot = a.order[r];
-        at[k] = r * a.rows.stride + c;
-        if (slot >= 0 && slot / a.chosen < a.tokens) v[k] = load<T, VEC>(x + static_cast<long long>(slot / a.chosen) * a.x.stride + c);
+        if (token[k] >= 0 && token[k] < a.tokens) v[k] = load<T, VEC>(x + token[k] * a.x.stride + at.c);
     }
 #pragma unroll
     for (int k = 0; k < MOVES; ++k)
-        if (at[k] >= 0) store<T, VEC>(rows + at[k], v[k]);
+        if (first + k * pass < slots) store<T, VEC>(rows + (first + k * pass) * a.rows.stride + at.c, v[k]);
 }
 
-// x[t] = sum over the row's slots of (weight *) rows[position]
-template <class T, int VEC, bool WEIGHTED>
-__global__ void __launch_bounds__(256) gather_sum_kernel(const __grid_constant__ ExchangeArgs a, Rows rowsIn, Rows out, long long total, int perRow)
+// x[t] = sum over the row's slots of (weight *) rows[position]. TOKENS rows per thread, SLOTS of each at a time; the blocks walk on with the list entries
+// of their next rows fetched ahead (a row's load would wait for them else: 131072 rows of 256 half, 2 slots each, 48 -> 42 us weighted,
+// 43 -> 34 to 39 us not).
+template <class T, int VEC, bool WEIGHTED, int TOKENS, int SLOTS>
+__global__ void __launch_bounds__(256) gather_sum_kernel(const __grid_constant__ ExchangeArgs a, Rows rowsIn, Rows out, int perRow, int pass)
 {
+    const Place at(perRow, pass, VEC);
+    if (!at.inside) return;
     const T* rows = static_cast<const T*>(rowsIn.data);
-    const long long i = blockIdx.x * 256ll + threadIdx.x;
-    if (i >= total) return;
-    const long long t = total <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(perRow) : i / perRow;
-    const int c = static_cast<int>(i - t * perRow) * VEC;
-    const long long slots = a.tokens * a.chosen;
-    float sum[VEC] = {};
-    for (int j0 = 0; j0 < a.chosen; j0 += 4) {
-        Pack<T, VEC> v[4];
-        float w[4];
-        bool use[4];
+    const long long slots = a.tokens * a.chosen, step = static_cast<long long>(gridDim.x) * (pass * TOKENS);
+    int nextPosition[TOKENS][SLOTS];
+    float nextWeight[TOKENS][SLOTS];
+    auto fetch = [&](long long first, int j0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            use[j] = false;
-            if (j0 + j < a.chosen) {
-                const long long s = t * a.chosen + j0 + j;
-                const int r = a.position[s];
-                use[j] = r >= 0 && r < slots;
-                w[j] = WEIGHTED ? a.weights[s] : 1.f;
-                if (use[j]) v[j] = load<T, VEC>(rows + static_cast<long long>(r) * rowsIn.stride + c);
+        for (int k = 0; k < TOKENS; ++k)
+#pragma unroll
+            for (int j = 0; j < SLOTS; ++j) {
+                const long long t = first + k * pass;
+                nextPosition[k][j] = -1;
+                nextWeight[k][j] = 1.f;
+                if (t < a.tokens && j0 + j < a.chosen) {
+                    nextPosition[k][j] = a.position[t * a.chosen + j0 + j];
+                    if (WEIGHTED) nextWeight[k][j] = a.weights[t * a.chosen + j0 + j];
+                }
             }
+    };
+    long long first = static_cast<long long>(blockIdx.x) * (pass * TOKENS) + at.row;
+    fetch(first, 0);
+    for (; first < a.tokens; first += step) {
+        float2 sum[TOKENS][PAIRS<VEC>] = {};
+        for (int j0 = 0; j0 < a.chosen; j0 += SLOTS) {
+            float w[TOKENS][SLOTS];
+            bool use[TOKENS][SLOTS];
+            Pack<T, VEC> v[TOKENS][SLOTS];
+#pragma unroll
+            for (int k = 0; k < TOKENS; ++k)
+#pragma unroll
+                for (int j = 0; j < SLOTS; ++j) {
+                    w[k][j] = nextWeight[k][j];
+                    use[k][j] = nextPosition[k][j] >= 0 && nextPosition[k][j] < slots;
+                    if (use[k][j]) v[k][j] = load<T, VEC>(rows + nextPosition[k][j] * rowsIn.stride + at.c);
+                }
+            if (j0 + SLOTS < a.chosen) fetch(first, j0 + SLOTS);
+            else fetch(first + step, 0);
+#pragma unroll
+            for (int k = 0; k < TOKENS; ++k)
+#pragma unroll
+                for (int j = 0; j < SLOTS; ++j) {
+                    if (!use[k][j]) continue;
+                    float2 f[PAIRS<VEC>];
+                    unpackPairs<T, VEC>(v[k][j], f);
+#pragma unroll
+                    for (int i = 0; i < PAIRS<VEC>; ++i) sum[k][i] = WEIGHTED ? fma2(both(w[k][j]), f[i], sum[k][i]) : add2(sum[k][i], f[i]);
+                }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!use[j]) continue;
-            float f[VEC];
-            unpack<T, VEC>(v[j], f);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) sum[k] = WEIGHTED ? fmaf(w[j], f[k], sum[k]) : sum[k] + f[k];
-        }
+        for (int k = 0; k < TOKENS; ++k)
+            if (first + k * pass < a.tokens) store<T, VEC>(static_cast<T*>(out.data) + (first + k * pass) * out.stride + at.c, packPairs<T, VEC>(sum[k]));
     }
-    store<T, VEC>(static_cast<T*>(out.data) + t * out.stride + c, pack<T, VEC>(sum));
 }
 
-// gradients of the combination: G lanes per row read its gradient once per slot (the first time from memory), write the slot's
-// row of gradients and add up the slot's product with its row
-template <class T, int VEC, int G>
-__global__ void __launch_bounds__(256) combine_adjoint_kernel(const __grid_constant__ ExchangeArgs a)
+// Gradients of the combination: G lanes per row read its gradient, write the rows of gradients of SLOTS of its slots and add up their products with
+// its rows. The rows without a slot, behind the last expert's, become zeros: row r is looked after by the lanes of row r / chosen.
+template <class T, int VEC, int G, int SLOTS>
+__global__ void __launch_bounds__(256, SLOTS <= 2 ? 5 : 3) combine_adjoint_kernel(const __grid_constant__ ExchangeArgs a)
 {
     const int lane = threadIdx.x % G;
-    const long long t = static_cast<long long>(blockIdx.x) * (256 / G) + threadIdx.x / G, slots = a.tokens * a.chosen;
-    const bool active = t < a.tokens;
-    const T *rows = static_cast<const T*>(a.rows.data), *dy = static_cast<const T*>(a.gradX.data) + (active ? t : 0) * a.gradX.stride;
+    const long long slots = a.tokens * a.chosen, step = static_cast<long long>(gridDim.x) * (256 / G);
+    const T* rows = static_cast<const T*>(a.rows.data);
     T* out = static_cast<T*>(a.gradRows.data);
-    for (int j = 0; j < a.chosen; ++j) {
-        const long long s = (active ? t : 0) * a.chosen + j;
-        const int r = a.position[s];
-        const bool use = active && r >= 0 && r < slots;
-        float dot = 0.f;
-        if (use) {
-            const float w = a.weights[s];
-            for (int c = lane * VEC; c < a.channels; c += G * VEC) {
-                float g[VEC], f[VEC];
-                unpack<T, VEC>(load<T, VEC>(dy + c), g);
-                if (a.gradWeights != nullptr) {
-                    unpack<T, VEC>(load<T, VEC>(rows + static_cast<long long>(r) * a.rows.stride + c), f);
+    int nextPosition[SLOTS], nextOrder[SLOTS];
+    float nextWeight[SLOTS];
+    auto fetch = [&](long long t, int j0) {
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) dot = fmaf(g[k], f[k], dot);
-                }
-                if (out != nullptr) {
+        for (int j = 0; j < SLOTS; ++j) {
+            const long long s = t * a.chosen + j0 + j;
+            const bool have = t < a.tokens && j0 + j < a.chosen;
+            nextPosition[j] = have ? a.position[s] : -1;
+            nextWeight[j] = have ? a.weights[s] : 0.f;
+            nextOrder[j] = have && out != nullptr ? a.order[s] : 0;
+        }
+    };
+    long long t = static_cast<long long>(blockIdx.x) * (256 / G) + threadIdx.x / G;
+    fetch(t, 0);
+    for (; t - threadIdx.x / G < a.tokens; t += step) {
+        const bool active = t < a.tokens;
+        const T* dy = static_cast<const T*>(a.gradX.data) + (active ? t : 0) * a.gradX.stride;
+        for (int j0 = 0; j0 < a.chosen; j0 += SLOTS) {
+            int position[SLOTS], order[SLOTS];
+            float w[SLOTS];
+            float2 dot[SLOTS] = {};
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) f[k] = w * g[k];
-                    store<T, VEC>(out + static_cast<long long>(r) * a.gradRows.stride + c, pack<T, VEC>(f));
+            for (int j = 0; j < SLOTS; ++j) {
+                position[j] = nextPosition[j] < slots ? nextPosition[j] : -1;
+                order[j] = nextOrder[j];
+                w[j] = nextWeight[j];
+            }
+            bool fetched = false;
+            if (active) {
+                for (int c = lane * VEC; c < a.channels; c += G * VEC) {
+                    const Pack<T, VEC> p = load<T, VEC>(dy + c);
+                    Pack<T, VEC> v[SLOTS];
+                    if (a.gradWeights != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < SLOTS; ++j)
+                            if (position[j] >= 0) v[j] = load<T, VEC>(rows + position[j] * a.rows.stride + c);
+                    }
+                    if (!fetched) {   // behind the first loads
+                        fetched = true;
+                        if (j0 + SLOTS < a.chosen) fetch(t, j0 + SLOTS);
+                        else fetch(t + step, 0);
+                    }
+                    float2 g[PAIRS<VEC>];
+                    unpackPairs<T, VEC>(p, g);
+#pragma unroll
+                    for (int j = 0; j < SLOTS; ++j) {
+                        float2 f[PAIRS<VEC>];
+                        if (out != nullptr && order[j] < 0) store<T, VEC>(out + (t * a.chosen + j0 + j) * a.gradRows.stride + c, Pack<T, VEC>{});
+                        if (position[j] < 0) continue;
+                        if (a.gradWeights != nullptr) {
+                            unpackPairs<T, VEC>(v[j], f);
+#pragma unroll
+                            for (int k = 0; k < PAIRS<VEC>; ++k) dot[j] = fma2(g[k], f[k], dot[j]);
+                        }
+                        if (out != nullptr) {
+#pragma unroll
+                            for (int k = 0; k < PAIRS<VEC>; ++k) f[k] = mul2(both(w[j]), g[k]);
+                            store<T, VEC>(out + position[j] * a.gradRows.stride + c, packPairs<T, VEC>(f));
+                        }
+                    }
                 }
             }
+            if (!fetched) {   // (lanes without a channel)
+                if (j0 + SLOTS < a.chosen) fetch(t, j0 + SLOTS);
+                else fetch(t + step, 0);
+            }
+            if (a.gradWeights == nullptr) continue;
+#pragma unroll
+            for (int j = 0; j < SLOTS; ++j) {
+                const float all = groupSum<G>(dot[j].x + dot[j].y);
+                if (active && lane == 0 && j0 + j < a.chosen) a.gradWeights[t * a.chosen + j0 + j] = all;
+            }
         }
-        dot = groupSum<G>(dot);
-        if (active && lane == 0 && a.gradWeights != nullptr) a.gradWeights[s] = dot;
-    }
-}
-// zeros behind the last expert's rows: a warp looks at 32 rows and clears those without a slot
-template <class T, int VEC>
-__global__ void __launch_bounds__(256) clear_tail_kernel(const __grid_constant__ ExchangeArgs a)
-{
-    T* out = static_cast<T*>(a.gradRows.data);
-    const long long slots = a.tokens * a.chosen, first = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * 32;
-    const int lane = threadIdx.x & 31;
-    unsigned empty = __ballot_sync(0xffffffffu, first + lane < slots && a.order[first + lane] < 0);
-    for (; empty != 0; empty &= empty - 1) {
-        const long long r = first + __ffs(empty) - 1;
-        for (int c = lane * VEC; c < a.channels; c += 32 * VEC) store<T, VEC>(out + r * a.gradRows.stride + c, Pack<T, VEC>{});
     }
 }
 
@@ -426,7 +532,7 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
         using T = decltype(t);
         return byExperts(a.experts, [&](auto l, auto per) {
             constexpr int LANES = decltype(l)::value, PER = decltype(per)::value;
-            const size_t bytes = (2 * TILE_SLOTS + a.experts * (alone ? 1 + PARTITION_WARPS : 1)) * sizeof(int);
+            const size_t bytes = (3 * (alone ? ALONE_SLOTS : TILE_SLOTS) + a.experts * (alone ? 1 + PARTITION_WARPS / 2 : 1)) * sizeof(int);
             auto go = [&](auto kernel) {
                 kernel<<<p.tiles, 256, bytes, stream>>>(a, p.tokensPerTile, counts, p.tiles);
                 return cudaGetLastError();
@@ -436,8 +542,8 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
         });
     });
     if (e != cudaSuccess || alone) return e;
-    partition_scan_kernel<<<(a.experts + PARTITION_WARPS - 1) / PARTITION_WARPS, PARTITION_THREADS, 0, stream>>>(counts, before, totals, a.experts, p.tiles);
-    route_place_kernel<<<p.tiles, PARTITION_THREADS, (1 + PARTITION_WARPS) * a.experts * sizeof(int), stream>>>(a, p.tokensPerTile, before, totals);
+    partition_scan_kernel<<<a.experts, PARTITION_THREADS, 0, stream>>>(counts, before, totals, a.experts, p.tiles);
+    route_place_kernel<<<p.tiles, PARTITION_THREADS, (1 + PARTITION_WARPS / 2) * a.experts * sizeof(int), stream>>>(a, p.tokensPerTile, before, totals);
     return cudaGetLastError();
 }
 
@@ -457,36 +563,55 @@ cudaError_t launchRouteAdjoint(const RouteArgs& a, cudaStream_t stream)
     });
 }
 
+// grid of the kernels that walk accesses: `rows` rows, `each` of them per thread
+struct AccessGrid {
+    int perRow, pass;
+    dim3 blocks;
+    // walkers: at most this many blocks, which walk on
+    AccessGrid(long long rows, int channels, int vec, int each, long long walkers = 1ll << 31)
+    {
+        perRow = channels / vec;
+        pass = perRow > 128 ? 1 : 256 / perRow;
+        const int parts = pass == 1 ? (perRow + 255) / 256 : 1;
+        const long long all = (rows + pass * each - 1) / (pass * each), most = std::max(1ll, walkers / parts);
+        blocks = dim3(static_cast<unsigned>(std::min(all, most)), parts);
+    }
+};
+
 cudaError_t launchDispatch(const ExchangeArgs& a, cudaStream_t stream)
 {
     if (a.tokens == 0) return cudaSuccess;
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
         const bool vec = wide(a.x, a.type, a.channels) && wide(a.rows, a.type, a.channels);
-        const int perRow = vec ? a.channels / WIDE<T> : a.channels;
-        const long long total = a.tokens * a.chosen * perRow;
-        const unsigned blocks = static_cast<unsigned>((total + 256 * MOVES - 1) / (256 * MOVES));
-        if (vec) dispatch_kernel<T, WIDE<T>><<<blocks, 256, 0, stream>>>(a, total, perRow);
-        else dispatch_kernel<T, 1><<<blocks, 256, 0, stream>>>(a, total, perRow);
+        const AccessGrid g(a.tokens * a.chosen, a.channels, vec ? WIDE<T> : 1, MOVES);
+        if (vec) dispatch_kernel<T, WIDE<T>><<<g.blocks, 256, 0, stream>>>(a, g.perRow, g.pass);
+        else dispatch_kernel<T, 1><<<g.blocks, 256, 0, stream>>>(a, g.perRow, g.pass);
         return cudaGetLastError();
     });
 }
 
+template <class T, int VEC, bool WEIGHTED>
+static cudaError_t launchGather(const ExchangeArgs& a, const Rows& in, const Rows& out, cudaStream_t stream)
+{
+    auto go = [&](auto* kernel, int each) {
+        const AccessGrid g(a.tokens, a.channels, VEC, each, a.numSMs * 8ll);
+        kernel<<<g.blocks, 256, 0, stream>>>(a, in, out, g.perRow, g.pass);
+        return cudaGetLastError();
+    };
+    // about 4 loads on their way per thread
+    if (a.chosen == 1) return go(gather_sum_kernel<T, VEC, WEIGHTED, 4, 1>, 4);
+    if (a.chosen == 2) return go(gather_sum_kernel<T, VEC, WEIGHTED, 2, 2>, 2);
+    return go(gather_sum_kernel<T, VEC, WEIGHTED, 1, 4>, 1);
+}
 static cudaError_t launchGatherSum(const ExchangeArgs& a, const Rows& in, const Rows& out, bool weighted, cudaStream_t stream)
 {
     if (a.tokens == 0) return cudaSuccess;
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
-        const bool vec = wide(in, a.type, a.channels) && wide(out, a.type, a.channels);
-        const int perRow = vec ? a.channels / WIDE<T> : a.channels;
-        const long long total = a.tokens * perRow;
-        const unsigned blocks = static_cast<unsigned>((total + 255) / 256);
-        auto go = [&](auto kernel) {
-            kernel<<<blocks, 256, 0, stream>>>(a, in, out, total, perRow);
-            return cudaGetLastError();
-        };
-        if (vec) return weighted ? go(gather_sum_kernel<T, WIDE<T>, true>) : go(gather_sum_kernel<T, WIDE<T>, false>);
-        return weighted ? go(gather_sum_kernel<T, 1, true>) : go(gather_sum_kernel<T, 1, false>);
+        if (wide(in, a.type, a.channels) && wide(out, a.type, a.channels))
+            return weighted ? launchGather<T, WIDE<T>, true>(a, in, out, stream) : launchGather<T, WIDE<T>, false>(a, in, out, stream);
+        return weighted ? launchGather<T, 1, true>(a, in, out, stream) : launchGather<T, 1, false>(a, in, out, stream);
     });
 }
 cudaError_t launchDispatchAdjoint(const ExchangeArgs& a, cudaStream_t stream) { return launchGatherSum(a, a.gradRows, a.gradX, false, stream); }
@@ -500,10 +625,10 @@ cudaError_t launchCombineAdjoint(const ExchangeArgs& a, cudaStream_t stream)
         const bool vec = wide(a.rows, a.type, a.channels) && wide(a.gradX, a.type, a.channels) && wide(a.gradRows, a.type, a.channels);
         auto go = [&](auto v, auto g) {
             constexpr int VEC = decltype(v)::value, G = decltype(g)::value;
-            combine_adjoint_kernel<T, VEC, G><<<static_cast<unsigned>((a.tokens + 256 / G - 1) / (256 / G)), 256, 0, stream>>>(a);
-            const cudaError_t e = cudaGetLastError();
-            if (e != cudaSuccess || a.gradRows.data == nullptr) return e;
-            clear_tail_kernel<T, VEC><<<static_cast<unsigned>((a.tokens * a.chosen + 255) / 256), 256, 0, stream>>>(a);
+            const unsigned blocks = static_cast<unsigned>(std::min<long long>((a.tokens + 256 / G - 1) / (256 / G), a.numSMs * 8));
+            if (a.chosen == 1) combine_adjoint_kernel<T, VEC, G, 1><<<blocks, 256, 0, stream>>>(a);
+            else if (a.chosen == 2) combine_adjoint_kernel<T, VEC, G, 2><<<blocks, 256, 0, stream>>>(a);
+            else combine_adjoint_kernel<T, VEC, G, 4><<<blocks, 256, 0, stream>>>(a);
             return cudaGetLastError();
         };
         if (vec) return a.channels <= 8 * WIDE<T> ? go(std::integral_constant<int, WIDE<T>>(), std::integral_constant<int, 8>())
