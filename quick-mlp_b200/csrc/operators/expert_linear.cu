@@ -367,8 +367,40 @@ __device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, volatile in
     return ok;
 }
 
+// barrier over the four warps that sum, with the conjunction of their answers
+__device__ __forceinline__ bool sumWarpsAgree(bool answer)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(answer)) : "memory");
+    return r != 0;
+}
+
 // operand format in the instruction descriptor
 template <class T> constexpr uint32_t FORMAT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+
+// A warp writes 32 rows x 32 columns of fp32 (a row per lane) from column c0 on to the rows of `out` (which has `columns` columns and `rows` rows from
+// the first lane's on), through 2 KB of shared memory: rows of 64 bytes, their 16-byte chunks exchanged so that neither side meets a bank twice.
+template <class T>
+__device__ __forceinline__ void storeTile(const float (&v)[32], unsigned char* mine, T* out, long long stride, int rows, int c0, int columns, bool wideStore)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        store<T, 8>(reinterpret_cast<T*>(mine + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)), pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[i * 8])));
+    __syncwarp();
+    if (wideStore) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2), chunk = lane & 3, column = c0 + chunk * 8;
+            if (r < rows && column < columns) store<T, 8>(out + r * stride + column, load<T, 8>(reinterpret_cast<const T*>(mine + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4))));
+        }
+    } else {
+        const int column = c0 + lane;
+        for (int r = 0; r < 32 && r < rows; ++r)
+            if (column < columns) out[r * stride + column] = *reinterpret_cast<const T*>(mine + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+    }
+    __syncwarp();
+}
 
 // boxes of 64 that `n` elements fill, 0 to `most`
 __device__ __forceinline__ int boxes(int n, int most) { return max(0, min(most, (n + 63) / 64)); }
@@ -597,29 +629,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                             }
                         }
                     }
-                    // rows of 64 bytes, their 16-byte chunks exchanged so that neither side meets a bank twice
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float f[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) f[k] = v[h][i * 8 + k];
-                        store<T, 8>(reinterpret_cast<T*>(mine + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)), pack<T, 8>(f));
-                    }
-                    __syncwarp();
-                    if (p.wideStore) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int r = i * 8 + (lane >> 2), chunk = lane & 3, column = t.column + c0 + chunk * 8;
-                            if (r < rowsLeft && column < p.columns)
-                                store<T, 8>(out + (firstRow + r) * p.outStride + column, load<T, 8>(reinterpret_cast<const T*>(mine + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4))));
-                        }
-                    } else {
-                        const int column = t.column + c0 + lane;
-                        for (int r = 0; r < 32 && r < rowsLeft; ++r)
-                            if (column < p.columns)
-                                out[(firstRow + r) * p.outStride + column] = *reinterpret_cast<const T*>(mine + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-                    }
-                    __syncwarp();
+                    storeTile<T>(v[h], mine, out + firstRow * p.outStride + t.column, p.outStride, rowsLeft, c0, p.columns - t.column, p.wideStore);
                 }
             }
             if (steps > 0) {
@@ -658,7 +668,8 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
             const int tileRow = t.row + rank * BM;
             float2 sum[4] = {};
             for (int k = 0; k < steps; ++k) {
-                if (!await(landed + stage * 8, phases >> stage & 1, failed)) { ok = false; break; }
+                // (the four warps leave together: none may wait for another below)
+                if (!sumWarpsAgree(await(landed + stage * 8, phases >> stage & 1, failed))) { ok = false; break; }
                 phases ^= 1u << stage;
                 const int left = t.end - t.begin - k * BK;
                 const unsigned char* box = base + stage * L::STAGE + (chunk >> 3) * BOX;
@@ -710,6 +721,404 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     }
     if constexpr (CTAS > 1) clusterSync();   // nothing reaches the other block any more
     if (warp == 1) tmemFree<CTAS>(tmem, L::TMEM);
+}
+
+// ---- both gradients of a narrow layer in one pass --------------------------------------------------------------------------------
+// Up to 128 channels in and out, the two gradients are bound by memory, and both read dy: here a tile of 128 rows of dy and x is fetched once, and
+// four operands are read from it: dy K-major and the expert's matrix for the input gradient, dy and x along their rows for the weight
+// gradient, whose accumulator stays in tensor memory for as long as the block's rows belong to one expert. Blocks take consecutive tiles, an equal
+// share each. An expert whose tiles lie in several blocks leaves partial sums, at most two per block (the run a block begins with, if it began
+// before; the run it ends with, if it goes on), which a second kernel adds up in order.
+// Four warps add up dy's columns (the bias gradient) and write the weight gradients. 512 experts, 1000003 rows, 64 -> 64 half: 72 us and 5 us for
+// the sums (apart: 49 us for the input gradient, 64 and 7 us for the others).
+template <int NB, int KB>   // boxes of 64 channels out, channels in
+struct NarrowLayout {
+    static constexpr int TILE = 128 * 128;                    // 128 rows x 64 elements
+    static constexpr int STAGE = (NB + KB) * TILE, MATRIX = NB * KB * BOX;
+    static constexpr int STAGES = (NB + KB) == 2 ? 5 : (NB + KB) == 3 ? 3 : 2;
+    static constexpr int COLUMNS = KB * 64, TMEM = 4 * COLUMNS;   // two accumulators of either gradient
+    static constexpr int OUT = EPILOGUE_WARPS * 32 * 64;
+    // barriers: full, empty, landed (8 each); matrix full, empty; input gradient full, empty; weight gradient full, empty (2 each); drain; flag, tensor memory
+    static constexpr int FULL = 0, EMPTY = 64, LANDED = 128, W_FULL = 192, W_EMPTY = 208, DX_FULL = 224, DX_EMPTY = 240, DW_FULL = 256, DW_EMPTY = 272, DRAIN = 288,
+                         FAILED = 296, BASE = 300, BARS = 320;
+    static constexpr int bytes(int experts) { return 1024 + STAGES * STAGE + 2 * MATRIX + OUT + BARS + listInts(experts) * 4; }
+    static_assert(bytes(EXPERTS_MAX) + 512 <= 227 * 1024, "shared memory");
+};
+
+// the tiles of a block, one after the other
+struct NarrowTile {
+    int expert, begin, end;   // its rows
+    bool first, last;         // of the expert's tiles in this block
+    bool entered, leaves;     // the expert's tiles began in an earlier block, go on in a later one
+};
+struct NarrowWalk {
+    const int *bounds, *before;
+    int tile, firstTile, end, expert = 0;
+    __device__ __forceinline__ NarrowWalk(const int* rows, const int* units, int experts) : bounds(rows), before(units)
+    {
+        const long long total = before[experts];
+        firstTile = tile = static_cast<int>(total * blockIdx.x / gridDim.x);
+        end = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x);
+    }
+    __device__ __forceinline__ bool next(NarrowTile& t, int experts)
+    {
+        if (tile >= end) return false;
+        const int lane = threadIdx.x & 31;
+        for (;;) {   // first expert whose tiles reach behind `tile`
+            const int e = expert + 1 + lane;
+            const unsigned passed = __ballot_sync(0xffffffffu, e <= experts && before[e] <= tile);
+            expert += __popc(passed);
+            if (passed != 0xffffffffu) break;
+        }
+        const int from = before[expert], to = before[expert + 1];
+        t.expert = expert;
+        t.begin = bounds[expert] + (tile - from) * BM;
+        t.end = min(bounds[expert + 1], t.begin + BM);
+        t.first = tile == from || tile == firstTile;
+        t.last = tile == to - 1 || tile == end - 1;
+        t.entered = from < firstTile;
+        t.leaves = to > end;
+        ++tile;
+        return true;
+    }
+};
+
+template <class T, int NB, int KB, bool SUMS>
+__global__ void __launch_bounds__(blockThreads(true), 1)
+    expert_narrow_adjoint_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW,
+                                 const __grid_constant__ ProductArgs p, T* __restrict__ gradX, long long gradXStride, bool wideX)
+{
+    // p.columns: channels in, p.sum: channels out, p.out: weight gradient
+    using L = NarrowLayout<NB, KB>;
+    extern __shared__ unsigned char dynamic[];
+    const uint32_t raw = smemAddress(dynamic), ring = (raw + 1023u) & ~1023u;
+    unsigned char* base = dynamic + (ring - raw);
+    const uint32_t matrices = ring + L::STAGES * L::STAGE;
+    unsigned char* outStage = base + L::STAGES * L::STAGE + 2 * L::MATRIX;
+    unsigned char* control = outStage + L::OUT;
+    const uint32_t bars = smemAddress(control);
+    volatile int* failed = reinterpret_cast<volatile int*>(control + L::FAILED);
+    uint32_t* tmemBase = reinterpret_cast<uint32_t*>(control + L::BASE);
+    int *bounds = reinterpret_cast<int*>(control + L::BARS), *before = bounds + listStride(p.experts);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    constexpr int THREADS = blockThreads(true);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) {
+            barrierInit(bars + L::FULL + s * 8, 1);
+            barrierInit(bars + L::EMPTY + s * 8, SUMS ? SUM_WARPS : 1);
+            barrierInit(bars + L::LANDED + s * 8, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            barrierInit(bars + L::W_FULL + i * 8, 1);
+            barrierInit(bars + L::W_EMPTY + i * 8, 1);
+            barrierInit(bars + L::DX_FULL + i * 8, 1);
+            barrierInit(bars + L::DX_EMPTY + i * 8, 4);
+            barrierInit(bars + L::DW_FULL + i * 8, 1);
+            barrierInit(bars + L::DW_EMPTY + i * 8, 4);
+        }
+        barrierInit(bars + L::DRAIN, 1);
+        *failed = 0;
+        barrierInitDone();
+    }
+    if (warp == 1) tmemAlloc<1>(smemAddress(tmemBase), L::TMEM);
+    planExperts<INPUT>(p, bounds, before, nullptr, THREADS);
+    fenceBefore();
+    __syncthreads();
+    fenceAfter();
+    const uint32_t tmem = *tmemBase, tmemW = tmem + 2 * L::COLUMNS;
+    if (blockIdx.x == 0)   // for the kernel that joins the partial sums
+        for (int e = threadIdx.x; e <= p.experts; e += THREADS) reinterpret_cast<int*>(p.plan)[e] = before[e];
+    NarrowWalk walk(bounds, before, p.experts);
+    NarrowTile t;
+
+    if (warp == 0) {
+        // ---- operands -------------------------------------------------------------------------------------------------
+        const uint32_t lead = electOne();
+        uint32_t stage = 0, phase = 0, matrix = 0, matrixPhase = 0;
+        int issued = 0;
+        bool ok = true;
+        while (ok && walk.next(t, p.experts)) {
+            if (__all_sync(0xffffffffu, t.first)) {
+                if (!await(bars + L::W_EMPTY + matrix * 8, matrixPhase ^ 1, failed)) break;
+                const uint32_t bar = bars + L::W_FULL + matrix * 8;
+                if (lead) barrierExpect(bar, L::MATRIX);
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) tmaLoad3<1>(lead, matrices + matrix * L::MATRIX + (k * NB + n) * BOX, &mapW, k * 64, n * 64, t.expert, bar);
+                if (++matrix == 2) { matrix = 0; matrixPhase ^= 1; }
+            }
+            if (!await(bars + L::EMPTY + stage * 8, phase ^ 1, failed)) { ok = false; break; }
+            const uint32_t at = ring + stage * L::STAGE, bar = bars + L::FULL + stage * 8;
+            const int halves = boxes(t.end - t.begin, 2);   // of 64 rows
+            if (lead) barrierExpect(bar, halves * (NB + KB) * BOX);
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) tmaLoad2<1>(lead && h < halves, at + n * L::TILE + h * BOX, &mapY, n * 64, t.begin + h * 64, bar);
+#pragma unroll
+                for (int k = 0; k < KB; ++k) tmaLoad2<1>(lead && h < halves, at + (NB + k) * L::TILE + h * BOX, &mapX, k * 64, t.begin + h * 64, bar);
+            }
+            ++issued;
+            if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (*failed != 0) {   // copies in flight land before the block's shared memory is given back
+            for (int i = 0; i < min(issued, L::STAGES); ++i) {
+                if (stage == 0) { stage = L::STAGES; phase ^= 1; }
+                --stage;
+                barrierWait(bars + L::FULL + stage * 8, phase);
+            }
+            for (int i = 0; i < 2; ++i) {
+                if (matrix == 0) { matrix = 2; matrixPhase ^= 1; }
+                --matrix;
+                barrierWait(bars + L::W_FULL + matrix * 8, matrixPhase);
+            }
+        }
+    } else if (warp == 1) {
+        // ---- products -------------------------------------------------------------------------------------------------
+        constexpr uint32_t shape = (1u << 4) | (FORMAT<T> << 7) | (FORMAT<T> << 10) | (1u << 16) | (static_cast<uint32_t>(L::COLUMNS >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
+        constexpr uint32_t inputShape = shape, weightShape = shape | 1u << 15;   // the matrix, x along their rows; dy too in the weight gradient
+        const uint32_t lead = electOne();
+        uint32_t stage = 0, phase = 0, matrix = 1, matrixPhases = 0, dx = 0, dxPhase = 0, dwPhases = 0;   // `matrix`: also the weight gradient's accumulator
+        bool ok = true;
+        while (ok && walk.next(t, p.experts)) {
+            if (__all_sync(0xffffffffu, t.first)) {
+                matrix ^= 1;
+                if (!await(bars + L::W_FULL + matrix * 8, matrixPhases >> matrix & 1, failed)) break;
+                if (!await(bars + L::DW_EMPTY + matrix * 8, (dwPhases >> matrix & 1) ^ 1, failed)) break;
+                matrixPhases ^= 1u << matrix;
+                dwPhases ^= 1u << matrix;
+            }
+            if (!await(bars + L::FULL + stage * 8, phase, failed)) break;
+            if (!await(bars + L::DX_EMPTY + dx * 8, dxPhase ^ 1, failed)) break;
+            fenceAfter();
+            const uint32_t y = ring + stage * L::STAGE, x = y + NB * L::TILE;
+            const int rows = t.end - t.begin, parts = (rows + 15) / 16;
+            if (__all_sync(0xffffffffu, rows < parts * 16)) {   // the rows behind belong to another expert
+                const int clear = parts * 16 - rows;
+                for (int i = lane; i < clear * (NB + KB) * 8; i += 32) {
+                    const int tile = i / (clear * 8), r = rows + i / 8 % clear, chunk = i % 8;
+                    *reinterpret_cast<uint4*>(base + stage * L::STAGE + tile * L::TILE + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fenceProxyAsync();
+                __syncwarp();
+            }
+            // input gradient: sum over the channels out
+            const uint64_t w = operandDescriptor(matrices + matrix * L::MATRIX, NB * BOX);
+#pragma unroll
+            for (int n = 0; n < NB * 4; ++n)
+                mma<1>(lead && n * 16 < p.sum, tmem + dx * L::COLUMNS, operandDescriptor(y + n / 4 * L::TILE, 16) + (n % 4) * (32 >> 4), w + n * (2048 >> 4), inputShape, n > 0);
+            mmaCommit<1>(lead, bars + L::DX_FULL + dx * 8);
+            // weight gradient: sum over the rows
+            const uint64_t a = operandDescriptor(y, L::TILE), b = operandDescriptor(x, L::TILE);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                mma<1>(lead && r < parts, tmemW + matrix * L::COLUMNS, a + r * (2048 >> 4), b + r * (2048 >> 4), weightShape, r > 0 || !t.first);
+            mmaCommit<1>(lead, bars + (SUMS ? L::LANDED : L::EMPTY) + stage * 8);
+            mmaCommit<1>(lead && t.last, bars + L::DW_FULL + matrix * 8);
+            mmaCommit<1>(lead && t.last, bars + L::W_EMPTY + matrix * 8);
+            if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
+            if (++dx == 2) { dx = 0; dxPhase ^= 1; }
+        }
+    } else if (warp < 2 + EPILOGUE_WARPS) {
+        // ---- input gradient: two groups of four warps, one per accumulator ------------------------------------------------------
+        const int group = (warp - 2) / 4, quarter = warp & 3;
+        unsigned char* mine = outStage + (warp - 2) * 32 * 64;
+        uint32_t phase = 0;
+        int turn = 1;
+        while (walk.next(t, p.experts)) {
+            turn ^= 1;
+            if (turn != group) continue;
+            if (!await(bars + L::DX_FULL + group * 8, phase, failed)) break;
+            phase ^= 1;
+            fenceAfter();
+            const uint32_t from = tmem + group * L::COLUMNS + (static_cast<uint32_t>(quarter * 32) << 16);
+            const int rowsLeft = t.end - t.begin - quarter * 32;
+            T* out = gradX + static_cast<long long>(t.begin + quarter * 32) * gradXStride;
+#pragma unroll
+            for (int pair = 0; pair < KB; ++pair) {
+                if (pair * 64 >= p.columns || rowsLeft <= 0) break;
+                float v[2][32];
+                tmemLoad32(from + pair * 64, v[0]);
+                tmemLoad32(from + pair * 64 + 32, v[1]);
+                tmemWait(v[0], v[1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (pair * 64 + h * 32 < p.columns) storeTile<T>(v[h], mine, out, gradXStride, rowsLeft, pair * 64 + h * 32, p.columns, wideX);
+            }
+            fenceBefore();
+            __syncwarp();
+            if (lane == 0) barrierArrive(bars + L::DX_EMPTY + group * 8);
+        }
+        // rows before the first and behind the last expert belong to nobody
+        const int first = bounds[0], last = bounds[p.experts];
+        const long long threads = static_cast<long long>(gridDim.x) * EPILOGUE_WARPS, me = static_cast<long long>(blockIdx.x) * EPILOGUE_WARPS + (warp - 2);
+        for (long long r = me; r < first + (p.rows - last); r += threads) {
+            T* row = gradX + (r < first ? r : last + (r - first)) * gradXStride;
+            for (int c = lane; c < p.columns; c += 32) row[c] = Element<T>::from(0.f);
+        }
+    } else {
+        // ---- weight and bias gradients -----------------------------------------------------------------------------------------
+        const int thread = threadIdx.x - (2 + EPILOGUE_WARPS) * 32, quarter = warp & 3;
+        constexpr int CHUNKS = NB * 8, SHARES = 128 / CHUNKS;   // 16-byte chunks of a row of dy; threads that share one (8 or 16 neighbouring lanes)
+        const int chunk = thread / SHARES, share = thread % SHARES;
+        T *gradW = static_cast<T*>(p.out), *gradB = static_cast<T*>(p.gradBias);
+        // experts without rows
+        for (int e = blockIdx.x; e < p.experts; e += gridDim.x) {
+            if (bounds[e + 1] > bounds[e]) continue;
+            for (long long i = thread; i < static_cast<long long>(p.sum) * p.columns; i += 128) gradW[static_cast<long long>(e) * p.sum * p.columns + i] = Element<T>::from(0.f);
+            if (SUMS)
+                for (int i = thread; i < p.sum; i += 128) gradB[static_cast<long long>(e) * p.sum + i] = Element<T>::from(0.f);
+        }
+        uint32_t stage = 0, phase = 0, acc = 1, accPhases = 0;
+        float2 sum[4] = {};
+        bool ok = true;
+        while (ok && walk.next(t, p.experts)) {
+            if (t.first) acc ^= 1;
+            const int rows = t.end - t.begin;
+            if constexpr (SUMS) {
+                if (!await(bars + L::LANDED + stage * 8, phase, failed)) break;
+                const unsigned char* tile = base + stage * L::STAGE + (chunk >> 3) * L::TILE;
+#pragma unroll
+                for (int i0 = 0; i0 < 128 / SHARES; i0 += 8) {
+                    Pack<T, 8> v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = (i0 + i) * SHARES + share;
+                        v[i] = load<T, 8>(reinterpret_cast<const T*>(tile + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)));
+                        if (r >= rows) v[i] = {};   // rows of another expert
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[j] = add2(sum[j], toPair(&v[i].v[2 * j]));
+                }
+                __syncwarp();
+                if (lane == 0) barrierArrive(bars + L::EMPTY + stage * 8);
+                if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (!t.last) continue;
+            // the block's last tile of this expert
+            const bool whole = !t.entered && !t.leaves;
+            const long long slot = static_cast<long long>(blockIdx.x) * 2 + (t.entered ? 0 : 1);
+            if constexpr (SUMS) {
+                float mine = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float all = groupSum<SHARES>(j % 2 == 0 ? sum[j / 2].x : sum[j / 2].y);
+                    mine = share == j ? all : mine;
+                }
+                const int channel = chunk * 8 + share;
+                if (share < 8 && channel < p.sum) {
+                    if (whole) gradB[static_cast<long long>(t.expert) * p.sum + channel] = Element<T>::from(mine);
+                    else p.partialBias[slot * 128 + channel] = mine;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = make_float2(0.f, 0.f);
+            }
+            if (!await(bars + L::DW_FULL + acc * 8, accPhases >> acc & 1, failed)) break;
+            accPhases ^= 1u << acc;
+            fenceAfter();
+            const uint32_t from = tmemW + acc * L::COLUMNS + (static_cast<uint32_t>(quarter * 32) << 16);
+            const int n = quarter * 32 + lane;   // this lane's channel out
+#pragma unroll
+            for (int pair = 0; pair < KB; ++pair) {
+                float v[2][32];
+                tmemLoad32(from + pair * 64, v[0]);
+                tmemLoad32(from + pair * 64 + 32, v[1]);
+                tmemWait(v[0], v[1]);
+                if (n >= p.sum) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c0 = pair * 64 + h * 32;
+                    if (!whole) {
+                        float* to = p.partial + (slot * 128 + n) * L::COLUMNS + c0;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(v[h][i], v[h][i + 1], v[h][i + 2], v[h][i + 3]);
+                    } else {
+                        T* to = gradW + (static_cast<long long>(t.expert) * p.sum + n) * p.columns + c0;
+                        if (p.wideStore) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8)
+                                if (c0 + i < p.columns) store<T, 8>(to + i, pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[h][i])));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (c0 + i < p.columns) to[i] = Element<T>::from(v[h][i]);
+                        }
+                    }
+                }
+            }
+            fenceBefore();
+            __syncwarp();
+            if (lane == 0) barrierArrive(bars + L::DW_EMPTY + acc * 8);
+        }
+    }
+    fenceBefore();
+    __syncthreads();
+    fenceAfter();
+    if (*failed != 0 && warp == 1) {
+        mmaCommit<1>(electOne(), bars + L::DRAIN);   // (elects the lane that issued the products)
+        if (lane == 0) {
+            barrierWait(bars + L::DRAIN, 0);
+            atomicOr(p.status, 1);
+        }
+        __syncwarp();
+    }
+    if (warp == 1) tmemFree<1>(tmem, L::TMEM);
+}
+
+// Joins the partial sums of an expert whose tiles lie in several blocks of the kernel above: thread block b looks after the expert that begins in that
+// kernel's block b and goes on behind it, if there is one. `blocks`: blocks of that kernel.
+template <class T>
+__global__ void __launch_bounds__(256) expert_narrow_join_kernel(const __grid_constant__ ProductArgs p, int blocks, int columns)
+{
+    const int* before = reinterpret_cast<const int*>(p.plan);
+    const long long total = before[p.experts];
+    const int block = blockIdx.x;
+    const int begin = static_cast<int>(total * block / blocks), end = static_cast<int>(total * (block + 1) / blocks);
+    if (begin == end || end >= total) return;
+    __shared__ int found;
+    for (int e = threadIdx.x; e < p.experts; e += 256)   // the expert of tile `end`
+        if (before[e] <= end && before[e + 1] > end) found = e;
+    __syncthreads();
+    const int expert = found;
+    if (before[expert] >= end || before[expert] < begin) return;
+    // block of its last tile: the first whose end, total * (b + 1) / blocks, reaches before[expert + 1]
+    const int last = static_cast<int>((static_cast<long long>(before[expert + 1]) * blocks + total - 1) / total) - 1;
+    const int more = last - block;
+    // blocks without a tile (fewer tiles than blocks) have left nothing
+    auto wrote = [&](int b) { return total >= blocks || total * (block + b + 1) / blocks > total * (block + b) / blocks; };
+    const int i0 = (blockIdx.y * 256 + threadIdx.x) * 4, n = i0 / columns, c = i0 - n * columns;   // 4 of 128 x columns sums
+    if (n < p.sum && c < p.columns) {
+        const float* from = p.partial + (static_cast<long long>(block) * 2 * 128 + n) * columns + c;
+        float4 sum = *reinterpret_cast<const float4*>(from + 128ll * columns);   // the run that block ends with
+#pragma unroll 4
+        for (int b = 1; b <= more; ++b) {                                        // the run the later ones begin with
+            if (!wrote(b)) continue;
+            const float4 v = *reinterpret_cast<const float4*>(from + b * 2 * 128ll * columns);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        T* out = static_cast<T*>(p.out) + (static_cast<long long>(expert) * p.sum + n) * p.columns + c;
+        if (p.wideStore) store<T, 4>(out, pack<T, 4>(f));
+        else
+            for (int k = 0; k < 4 && c + k < p.columns; ++k) out[k] = Element<T>::from(f[k]);
+    }
+    if (p.gradBias != nullptr && blockIdx.y == 0 && threadIdx.x < p.sum) {
+        const float* from = p.partialBias + static_cast<long long>(block) * 2 * 128 + threadIdx.x;
+        float sum = from[128];
+#pragma unroll 4
+        for (int b = 1; b <= more; ++b)
+            if (wrote(b)) sum += from[b * 2 * 128];
+        static_cast<T*>(p.gradBias)[static_cast<long long>(expert) * p.sum + threadIdx.x] = Element<T>::from(sum);
+    }
 }
 
 // Adds up the partial sums of the weight gradients (and, behind the tiles, of the bias gradients) of experts with more than one item. blockIdx.x: tile
@@ -975,6 +1384,7 @@ int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
 // scratch: [x | weight | dy in a form the TMA reads, where needed | partial sums of the weight and bias gradients | their plan]
 struct Scratch {
     size_t x, weight, gradY, partial, partialBias, plan, bytes;
+    bool narrow;   // both gradients in one pass
     int chunk, rowTiles, columnTiles, tileRows;
     Shape shape;
     Scratch(const ExpertArgs& a, bool adjoint)
@@ -997,6 +1407,14 @@ struct Scratch {
         columnTiles = (a.channelsIn + shape.width - 1) / shape.width;
         const int tiles = rowTiles * columnTiles;
         chunk = weightChunk(a, tiles, tileRows * shape.width, a.numSMs / shape.ctas);
+        narrow = weights && a.gradX.data != nullptr && a.channelsIn <= 128 && a.channelsOut <= 128;
+        if (narrow) {
+            const size_t slots = static_cast<size_t>(a.numSMs) * 2 * 128;
+            partial = take(true, slots * (a.channelsIn <= 64 ? 64 : 128) * 4);
+            partialBias = take(true, slots * 4);
+            plan = take(true, (static_cast<size_t>(a.experts) + 1) * 4);
+            return;
+        }
         const size_t items = a.rows > chunk ? a.experts + rows / chunk : 0;
         partial = take(weights, items * tiles * tileRows * shape.width * 4);
         partialBias = take(weights, items * a.channelsOut * 4);
@@ -1106,6 +1524,22 @@ cudaError_t forward(const ExpertArgs& a, cudaStream_t stream)
     return launchShape<T, FORWARD>(shape, mapX, mapW, p, a.numSMs, stream);
 }
 
+template <class T, int NB, int KB>
+cudaError_t launchNarrow(const CUtensorMap& y, const CUtensorMap& x, const CUtensorMap& w, const ProductArgs& p, const ExpertArgs& a, cudaStream_t stream)
+{
+    auto go = [&](auto* kernel) {
+        const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), NarrowLayout<NB, KB>::bytes(EXPERTS_MAX));
+        if (e != cudaSuccess) return e;
+        kernel<<<a.numSMs, blockThreads(true), NarrowLayout<NB, KB>::bytes(a.experts), stream>>>(y, x, w, p, static_cast<T*>(a.gradX.data), a.gradX.stride,
+                                                                                                 wideOut(a.gradX.data, a.gradX.stride, a.channelsIn));
+        return cudaGetLastError();
+    };
+    cudaError_t e = a.gradBias != nullptr ? go(expert_narrow_adjoint_kernel<T, NB, KB, true>) : go(expert_narrow_adjoint_kernel<T, NB, KB, false>);
+    if (e != cudaSuccess) return e;
+    expert_narrow_join_kernel<T><<<dim3(a.numSMs, (a.channelsOut * KB * 64 + 1023) / 1024), 256, 0, stream>>>(p, a.numSMs, KB * 64);
+    return cudaGetLastError();
+}
+
 template <class T>
 cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
 {
@@ -1128,6 +1562,25 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
     CUtensorMap mapX, mapW, mapY;
     if (e == cudaSuccess) e = readable<T>(dy, dyStride, a.rows, a.channelsOut, base + s.gradY, a.numSMs, stream);
     if (e == cudaSuccess) e = encodeMap(mapY, a.type, dy, 0, a.rows, a.channelsOut, dyStride);
+    if (e == cudaSuccess && s.narrow) {
+        e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, a.numSMs, stream);
+        if (e == cudaSuccess) e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, a.numSMs, stream);
+        if (e == cudaSuccess) e = encodeMap(mapW, a.type, w, a.experts, a.channelsOut, a.channelsIn, wStride);
+        if (e == cudaSuccess) e = encodeMap(mapX, a.type, x, 0, a.rows, a.channelsIn, xStride);
+        if (e != cudaSuccess) return e;
+        ProductArgs p = common(a);
+        p.columns = a.channelsIn;
+        p.sum = a.channelsOut;
+        p.tileRows = BM;
+        p.out = a.gradWeight;
+        p.gradBias = a.gradBias;
+        p.partial = reinterpret_cast<float*>(base + s.partial);
+        p.partialBias = reinterpret_cast<float*>(base + s.partialBias);
+        p.plan = reinterpret_cast<int2*>(base + s.plan);
+        p.wideStore = wideOut(a.gradWeight, a.channelsIn, a.channelsIn);
+        if (a.channelsOut <= 64) return a.channelsIn <= 64 ? launchNarrow<T, 1, 1>(mapY, mapX, mapW, p, a, stream) : launchNarrow<T, 1, 2>(mapY, mapX, mapW, p, a, stream);
+        return a.channelsIn <= 64 ? launchNarrow<T, 2, 1>(mapY, mapX, mapW, p, a, stream) : launchNarrow<T, 2, 2>(mapY, mapX, mapW, p, a, stream);
+    }
     if (e == cudaSuccess && a.gradX.data != nullptr) {
         e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, a.numSMs, stream);
         if (e == cudaSuccess) e = encodeMap(mapW, a.type, w, a.experts, a.channelsOut, a.channelsIn, wStride);

@@ -296,7 +296,7 @@ def experts_case(qmlp, x, weight, offsets, bias, grad):
 SHAPES = [  # counts of rows, channels in, channels out
     ([1], 8, 8), ([1, 0, 1], 64, 64), ([5, 0, 3, 0], 16, 24), ([128], 64, 64), ([127, 1, 129, 256], 64, 128), ([130, 0, 0, 70, 64], 128, 64),
     ([300, 5], 200, 136), ([64, 64], 72, 264), ([33] * 40, 64, 64), ([1000, 1], 256, 256), ([513, 2000], 64, 64), ([3000], 32, 48), ([700, 20], 520, 300),
-    ([2, 1, 3], 13, 5), ([200, 17], 77, 65), ([1500, 0, 300], 264, 320), ([600, 1029], 144, 392), ([700, 513], 200, 130), ([90], 1, 1), ([10, 140], 31, 257), ([40, 0, 30], 130, 7),
+    ([2, 1, 3], 13, 5), ([200, 17], 77, 65), ([1500, 0, 300], 264, 320), ([600, 1029], 144, 392), ([700, 513], 200, 130), ([90], 1, 1), ([20000, 0, 3, 5000], 64, 64), ([128] * 300, 128, 128), ([40000], 80, 64), ([9000, 1, 0, 11000], 64, 96), ([10, 140], 31, 257), ([40, 0, 30], 130, 7),
 ]
 
 
@@ -477,6 +477,18 @@ def test_modules(qmlp):
         opt.step()
         losses.append(loss.item())
     assert losses[-1] < 0.2 * losses[0], losses
+
+
+def test_example():
+    """the example's model, from coordinates to colour: its error falls"""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "images_by_experts.py")
+    spec = importlib.util.spec_from_file_location("images_by_experts", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    losses = module.fit(images=4, points=8192, steps=80, report=None)
+    assert losses[-1] < 0.25 * losses[0], losses[::10]
 
 
 def test_refusals(qmlp):
