@@ -153,6 +153,31 @@ __device__ __forceinline__ float groupSum(float v)
     return v;
 }
 
+// ---- launches that overlap -----------------------------------------------------------------------------------------------
+// Every kernel of the operators is launched so that its launch overlaps the kernel before it (programmatic stream serialisation), and begins with
+// chained(), which waits until all kernels before it are complete and their writes visible; what goes in front of the call touches no
+// global memory. The gradient of an embedding of a million tokens, five kernels: 111 -> 97 us, of 65536 tokens over 50000 rows, nine: 131 -> 109 us.
+// (Kernels that let the next one start while their own last blocks run were slower, 119 and 113 us: its blocks then crowd on the SMs that are free first.)
+__device__ __forceinline__ void chained() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... P, class... A>
+cudaError_t launchChained(void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, int cluster, const A&... arguments)
+{
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<P>(arguments)...);
+}
+
 // ---- mbarriers and bulk copies ---------------------------------------------------------------------------------------
 constexpr uint32_t WAIT_LIMIT = 1u << 22;   // polls of an mbarrier before a kernel gives up
 

@@ -32,6 +32,7 @@ constexpr int LOOKUPS = 4;
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(const __grid_constant__ EmbeddingArgs a, int perRow, int pass)
 {
+    chained();
     const T* table = static_cast<const T*>(a.table.data);
     T* y = static_cast<T*>(a.y.data);
     const int rowInPass = pass == 1 ? 0 : static_cast<int>(threadIdx.x) / perRow, access = blockIdx.y * 256 + (pass == 1 ? threadIdx.x : threadIdx.x - rowInPass * perRow);
@@ -81,6 +82,7 @@ __device__ __forceinline__ int2 sortItem(const EmbeddingArgs& a, const SortArgs&
 template <int ITEMS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) sort_count_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ SortArgs s)
 {
+    chained();
     __shared__ int count[PARTITION_MAX_DIGITS];
     for (int i = threadIdx.x; i < s.digits; i += WARPS * 32) count[i] = 0;
     const int first = blockIdx.x * (ITEMS * WARPS * 32);
@@ -108,6 +110,7 @@ constexpr int moveBytes(int digits) { return ITEMS * WARPS * 32 * 8 + 2 * digits
 template <int ITEMS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1024 / (WARPS * 32)) sort_move_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ SortArgs s)
 {
+    chained();
     constexpr int THREADS = WARPS * 32, TILE = ITEMS * THREADS;
     extern __shared__ __align__(16) int2 sorted[];                           // TILE
     int *start = reinterpret_cast<int*>(sorted + TILE), *local = start + s.digits;   // digits: where the tile's items go, in memory and in the tile
@@ -154,6 +157,7 @@ constexpr int FILL_ROWS = 8;   // rows of the table a group looks at
 template <class T, int VEC, int G>
 __global__ void __launch_bounds__(256, 3) embedding_runs_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ RunArgs r)
 {
+    chained();
     constexpr int GROUPS = 256 / G;
     const int c = (blockIdx.y * G + threadIdx.x % G) * VEC;
     if (c >= a.channels) return;
@@ -248,6 +252,7 @@ constexpr int JOIN_CHUNKS = 8, JOIN_FEW = 16;
 template <class T, int G>
 __global__ void __launch_bounds__(512) embedding_join_kernel(const __grid_constant__ EmbeddingArgs a, const __grid_constant__ RunArgs r)
 {
+    chained();
     constexpr int SHARES = 512 / G;
     __shared__ int keyOf[JOIN_CHUNKS], partsOf[JOIN_CHUNKS];
     __shared__ float shared[512];
@@ -379,20 +384,20 @@ cudaError_t launchRuns(const EmbeddingArgs& a, RunArgs r, cudaStream_t stream)
         constexpr int G = decltype(g)::value, GROUPS = 256 / G;
         r.runBlocks = (r.chunks + GROUPS - 1) / GROUPS;
         const long long fill = (a.rows + GROUPS * FILL_ROWS - 1) / (GROUPS * FILL_ROWS);
-        embedding_runs_kernel<T, VEC, G><<<dim3(static_cast<unsigned>(r.runBlocks + fill), (vectors + G - 1) / G), 256, 0, stream>>>(a, r);
+        launchChained(embedding_runs_kernel<T, VEC, G>, dim3(static_cast<unsigned>(r.runBlocks + fill), (vectors + G - 1) / G), 256, 0, stream, 1, a, r);
         return cudaGetLastError();
     });
 }
 template <int ITEMS, int WARPS>
 cudaError_t launchSort(const EmbeddingArgs& a, const SortArgs& s, cudaStream_t stream)
 {
-    sort_count_kernel<ITEMS, WARPS><<<s.blocks, WARPS * 32, 0, stream>>>(a, s);
-    partition_scan_kernel<<<s.digits, PARTITION_THREADS, 0, stream>>>(s.counts, s.before, s.totals, s.digits, s.blocks);
+    launchChained(sort_count_kernel<ITEMS, WARPS>, s.blocks, WARPS * 32, 0, stream, 1, a, s);
+    launchChained(partition_scan_kernel, s.digits, PARTITION_THREADS, 0, stream, 1, s.counts, s.before, s.totals, s.digits, s.blocks);
     if (moveBytes<ITEMS, WARPS>(PARTITION_MAX_DIGITS) > 48 * 1024) {
         const cudaError_t e = allowShared(reinterpret_cast<const void*>(sort_move_kernel<ITEMS, WARPS>), moveBytes<ITEMS, WARPS>(PARTITION_MAX_DIGITS));
         if (e != cudaSuccess) return e;
     }
-    sort_move_kernel<ITEMS, WARPS><<<s.blocks, WARPS * 32, moveBytes<ITEMS, WARPS>(s.digits), stream>>>(a, s);
+    launchChained(sort_move_kernel<ITEMS, WARPS>, s.blocks, WARPS * 32, moveBytes<ITEMS, WARPS>(s.digits), stream, 1, a, s);
     return cudaGetLastError();
 }
 
@@ -411,8 +416,8 @@ cudaError_t launchEmbeddingForward(const EmbeddingArgs& a, cudaStream_t stream)
         const bool vec = wide(a.table, a.type, a.channels) && wide(a.y, a.type, a.channels);
         const int perRow = vec ? a.channels / WIDE<T> : a.channels, pass = perRow > 128 ? 1 : 256 / perRow;
         const dim3 grid(static_cast<unsigned>((a.tokens + pass * LOOKUPS - 1) / (pass * LOOKUPS)), pass == 1 ? (perRow + 255) / 256 : 1);
-        if (vec) embedding_forward_kernel<T, WIDE<T>><<<grid, 256, 0, stream>>>(a, perRow, pass);
-        else embedding_forward_kernel<T, 1><<<grid, 256, 0, stream>>>(a, perRow, pass);
+        if (vec) launchChained(embedding_forward_kernel<T, WIDE<T>>, grid, 256, 0, stream, 1, a, perRow, pass);
+        else launchChained(embedding_forward_kernel<T, 1>, grid, 256, 0, stream, 1, a, perRow, pass);
         return cudaGetLastError();
     });
 }
@@ -450,7 +455,7 @@ cudaError_t launchEmbeddingAdjoint(const EmbeddingArgs& a, cudaStream_t stream)
         if (status != cudaSuccess || p.chunks < 2) return status;
         return byLanes(a.channels, [&](auto g) {
             constexpr int G = decltype(g)::value;
-            embedding_join_kernel<T, G><<<dim3((p.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS, (a.channels + G - 1) / G), 512, 0, stream>>>(a, r);
+            launchChained(embedding_join_kernel<T, G>, dim3((p.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS, (a.channels + G - 1) / G), 512, 0, stream, 1, a, r);
             return cudaGetLastError();
         });
     });

@@ -439,6 +439,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         barrierInitDone();
     }
     if (warp == 1) tmemAlloc<CTAS>(smemAddress(tmemBase), L::TMEM);
+    chained();
     planExperts<MODE>(p, bounds, before, order, blockThreads(SUMS));
     fenceBefore();
     __syncthreads();
@@ -822,6 +823,7 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
         barrierInitDone();
     }
     if (warp == 1) tmemAlloc<1>(smemAddress(tmemBase), L::TMEM);
+    chained();
     planExperts<INPUT>(p, bounds, before, nullptr, THREADS);
     fenceBefore();
     __syncthreads();
@@ -1076,6 +1078,7 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
 template <class T>
 __global__ void __launch_bounds__(256) expert_narrow_join_kernel(const __grid_constant__ ProductArgs p, int blocks, int columns)
 {
+    chained();
     const int* before = reinterpret_cast<const int*>(p.plan);
     const long long total = before[p.experts];
     const int block = blockIdx.x;
@@ -1127,6 +1130,7 @@ constexpr int JOIN_ELEMENTS = 8192;
 template <class T, int BN>
 __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant__ ProductArgs p)
 {
+    chained();
     constexpr int ROWS = JOIN_ELEMENTS / BN;
     const int tiles = p.rowTiles * p.columnTiles;
     const int expert = blockIdx.x / tiles, tile = blockIdx.x % tiles;
@@ -1173,6 +1177,7 @@ constexpr int FEW_ROWS = 4, FEW_OUT = 4, FEW_WARPS = 4;
 template <class T, int VEC>
 __global__ void __launch_bounds__(FEW_WARPS * 32) expert_few_rows_kernel(const __grid_constant__ ExpertArgs a)
 {
+    chained();
     extern __shared__ __align__(16) float rowsIn[];   // FEW_ROWS x channels in, rounded up to whole accesses of a warp
     __shared__ int found[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
@@ -1266,6 +1271,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) expert_few_rows_kernel(const _
 template <class T>
 __global__ void __launch_bounds__(256) expert_bias_kernel(const __grid_constant__ ProductArgs p, const T* __restrict__ dy, long long stride, T* __restrict__ out)
 {
+    chained();
     __shared__ float shared[8][32];
     __shared__ int reached[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.y * 32 + lane;
@@ -1297,6 +1303,7 @@ __global__ void __launch_bounds__(256) expert_bias_kernel(const __grid_constant_
 template <class T>
 __global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ in, long long stride, T* __restrict__ out, long long rows, int columns, int padded)
 {
+    chained();
     const long long total = rows * padded;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * 256) {
         const long long r = i / padded;
@@ -1428,7 +1435,7 @@ cudaError_t readable(const void*& data, long long& stride, long long rows, int c
     if (direct(data, stride, columns)) return cudaSuccess;
     const int padded = pad8(columns);
     const long long blocks = std::min<long long>((rows * padded + 255) / 256, numSMs * 16ll);
-    pad_rows_kernel<T><<<static_cast<unsigned>(std::max(1ll, blocks)), 256, 0, stream>>>(static_cast<const T*>(data), stride, static_cast<T*>(scratch), rows, columns, padded);
+    launchChained(pad_rows_kernel<T>, static_cast<unsigned>(std::max(1ll, blocks)), 256, 0, stream, 1, static_cast<const T*>(data), stride, static_cast<T*>(scratch), rows, columns, padded);
     data = scratch;
     stride = padded;
     return cudaGetLastError();
@@ -1440,18 +1447,7 @@ cudaError_t launchProduct(const CUtensorMap& a, const CUtensorMap& b, const Prod
     auto* kernel = expert_product_kernel<T, MODE, BN, CTAS, SUMS>;
     const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), Layout<BN, CTAS>::bytes(EXPERTS_MAX));
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(numSMs / CTAS * CTAS);
-    config.blockDim = dim3(blockThreads(SUMS));
-    config.dynamicSmemBytes = Layout<BN, CTAS>::bytes(p.experts);
-    config.stream = stream;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = CTAS;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = CTAS > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&config, kernel, a, b, p);
+    return launchChained(kernel, numSMs / CTAS * CTAS, blockThreads(SUMS), Layout<BN, CTAS>::bytes(p.experts), stream, CTAS, a, b, p);
 }
 template <class T, int MODE, bool SUMS = false>
 cudaError_t launchShape(const Shape& shape, const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, int numSMs, cudaStream_t stream)
@@ -1491,7 +1487,7 @@ cudaError_t forwardFewRows(const ExpertArgs& a, cudaStream_t stream)
             const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), 200 * 1024);
             if (e != cudaSuccess) return e;
         }
-        kernel<<<grid, FEW_WARPS * 32, bytes, stream>>>(a);
+        launchChained(kernel, grid, FEW_WARPS * 32, bytes, stream, 1, a);
         return cudaGetLastError();
     };
     return vec ? go(expert_few_rows_kernel<T, 8>, 8) : go(expert_few_rows_kernel<T, 1>, 1);
@@ -1530,13 +1526,12 @@ cudaError_t launchNarrow(const CUtensorMap& y, const CUtensorMap& x, const CUten
     auto go = [&](auto* kernel) {
         const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), NarrowLayout<NB, KB>::bytes(EXPERTS_MAX));
         if (e != cudaSuccess) return e;
-        kernel<<<a.numSMs, blockThreads(true), NarrowLayout<NB, KB>::bytes(a.experts), stream>>>(y, x, w, p, static_cast<T*>(a.gradX.data), a.gradX.stride,
-                                                                                                 wideOut(a.gradX.data, a.gradX.stride, a.channelsIn));
+        launchChained(kernel, a.numSMs, blockThreads(true), NarrowLayout<NB, KB>::bytes(a.experts), stream, 1, y, x, w, p, static_cast<T*>(a.gradX.data), a.gradX.stride, wideOut(a.gradX.data, a.gradX.stride, a.channelsIn));
         return cudaGetLastError();
     };
     cudaError_t e = a.gradBias != nullptr ? go(expert_narrow_adjoint_kernel<T, NB, KB, true>) : go(expert_narrow_adjoint_kernel<T, NB, KB, false>);
     if (e != cudaSuccess) return e;
-    expert_narrow_join_kernel<T><<<dim3(a.numSMs, (a.channelsOut * KB * 64 + 1023) / 1024), 256, 0, stream>>>(p, a.numSMs, KB * 64);
+    launchChained(expert_narrow_join_kernel<T>, dim3(a.numSMs, (a.channelsOut * KB * 64 + 1023) / 1024), 256, 0, stream, 1, p, a.numSMs, KB * 64);
     return cudaGetLastError();
 }
 
@@ -1549,7 +1544,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
     if (a.gradBias != nullptr && (a.gradWeight == nullptr || a.rows == 0)) {
         ProductArgs p = common(a);
         p.columns = a.channelsOut;
-        expert_bias_kernel<T><<<dim3(a.experts, (a.channelsOut + 31) / 32), 256, 0, stream>>>(p, static_cast<const T*>(a.gradY.data), a.gradY.stride, static_cast<T*>(a.gradBias));
+        launchChained(expert_bias_kernel<T>, dim3(a.experts, (a.channelsOut + 31) / 32), 256, 0, stream, 1, p, static_cast<const T*>(a.gradY.data), a.gradY.stride, static_cast<T*>(a.gradBias));
         e = cudaGetLastError();
     }
     if (a.rows == 0) {
@@ -1618,9 +1613,9 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
                                   : launchShape<T, WEIGHTS, false>(s.shape, mapY, mapX, p, a.numSMs, stream);
         if (e == cudaSuccess && a.rows > s.chunk) {
             const dim3 grid(a.experts * s.rowTiles * s.columnTiles, s.tileRows * s.shape.width / JOIN_ELEMENTS);
-            if (s.shape.width == 64) expert_join_kernel<T, 64><<<grid, 256, 0, stream>>>(p);
-            else if (s.shape.width == 128) expert_join_kernel<T, 128><<<grid, 256, 0, stream>>>(p);
-            else expert_join_kernel<T, 256><<<grid, 256, 0, stream>>>(p);
+            if (s.shape.width == 64) launchChained(expert_join_kernel<T, 64>, grid, 256, 0, stream, 1, p);
+            else if (s.shape.width == 128) launchChained(expert_join_kernel<T, 128>, grid, 256, 0, stream, 1, p);
+            else launchChained(expert_join_kernel<T, 256>, grid, 256, 0, stream, 1, p);
             e = cudaGetLastError();
         }
     }

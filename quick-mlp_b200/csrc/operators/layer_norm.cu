@@ -251,6 +251,7 @@ __host__ __device__ constexpr int forwardPerSM(int g) { return g <= 32 ? 3 : g <
 template <class T, int VEC, int G, int EPT, bool RINGED>
 __global__ void __launch_bounds__(threadsFor(G), forwardPerSM(G)) layer_norm_forward_kernel(const __grid_constant__ LayerNormArgs a)
 {
+    chained();
     constexpr int GROUPS = threadsFor(G) / G;
     extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ __align__(8) float shared[2 * 64];
@@ -319,6 +320,7 @@ struct Piece {
 template <class T, int VEC, int G, int EPT, bool RINGED>
 __global__ void __launch_bounds__(threadsFor(G), perSM(G)) layer_norm_adjoint_kernel(const __grid_constant__ LayerNormArgs a)
 {
+    chained();
     constexpr int THREADS = threadsFor(G), GROUPS = THREADS / G, NV = EPT / VEC;
     constexpr bool TWICE = G == 1024;
     extern __shared__ __align__(128) unsigned char dynamic[];
@@ -475,6 +477,7 @@ __global__ void __launch_bounds__(threadsFor(G), perSM(G)) layer_norm_adjoint_ke
 __global__ void __launch_bounds__(512) layer_norm_parameters_kernel(const float* __restrict__ partial, int blocks, int channels, void* gradWeight, int weightType,
                                                                     void* gradBias, int biasType)
 {
+    chained();
     __shared__ float shared[16][33];
     const int k = blockIdx.x * 32 + threadIdx.x;   // of 2 x channels
     float sum = 0.f;
@@ -502,6 +505,7 @@ __device__ __forceinline__ void blockSum(float (&v)[N], float* shared, int& half
 template <class T>
 __global__ void __launch_bounds__(1024) layer_norm_wide_forward_kernel(const __grid_constant__ LayerNormArgs a)
 {
+    chained();
     __shared__ float shared[2 * 32];
     int half = 0;
     const float invC = 1.f / static_cast<float>(a.channels);
@@ -531,6 +535,7 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_forward_kernel(const __g
 template <class T>
 __global__ void __launch_bounds__(1024) layer_norm_wide_adjoint_kernel(const __grid_constant__ LayerNormArgs a)
 {
+    chained();
     __shared__ float shared[2 * 32 * 2];
     int half = 0;
     const float invC = 1.f / static_cast<float>(a.channels);
@@ -556,6 +561,7 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_adjoint_kernel(const __g
 template <class T>
 __global__ void __launch_bounds__(256) layer_norm_wide_partial_kernel(const __grid_constant__ LayerNormArgs a)
 {
+    chained();
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.channels) return;
     float dw = 0.f, db = 0.f;
@@ -624,7 +630,7 @@ cudaError_t launchRinged(K kernel, LayerNormArgs a, int matrices, unsigned block
     const int bytes = 128 + a.ringStages * slot;
     const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), SHARED);
     if (e != cudaSuccess) return e;
-    kernel<<<blocks, threads, bytes, stream>>>(a);
+    launchChained(kernel, blocks, threads, bytes, stream, 1, a);
     return cudaGetLastError();
 }
 
@@ -638,7 +644,7 @@ cudaError_t launchLayerNormForward(const LayerNormArgs& a, cudaStream_t stream)
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
         if (a.channels > WIDEST) {
-            layer_norm_wide_forward_kernel<T><<<blocksFor(a.rows, 1, a.numSMs, 2), 1024, 0, stream>>>(a);
+            launchChained(layer_norm_wide_forward_kernel<T>, blocksFor(a.rows, 1, a.numSMs, 2), 1024, 0, stream, 1, a);
             return cudaGetLastError();
         }
         const bool vec = wide(a.x, a.type, a.channels) && wide(a.y, a.type, a.channels);
@@ -648,8 +654,8 @@ cudaError_t launchLayerNormForward(const LayerNormArgs& a, cudaStream_t stream)
                 if (vec) return launchRinged(layer_norm_forward_kernel<T, WIDE<T>, G, EPT, true>, a, 1, blocksFor(a.rows, 1, a.numSMs, forwardPerSM(G)), G, forwardPerSM(G), stream);
             }
             const unsigned blocks = blocksFor(a.rows, groupsOf(G), a.numSMs, 2 * forwardPerSM(G));
-            if (vec && G <= 32) layer_norm_forward_kernel<T, WIDE<T>, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
-            else layer_norm_forward_kernel<T, 1, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
+            if (vec && G <= 32) launchChained(layer_norm_forward_kernel<T, WIDE<T>, G, EPT, false>, blocks, threadsFor(G), 0, stream, 1, a);
+            else launchChained(layer_norm_forward_kernel<T, 1, G, EPT, false>, blocks, threadsFor(G), 0, stream, 1, a);
             return cudaGetLastError();
         });
     });
@@ -666,11 +672,11 @@ cudaError_t launchLayerNormAdjoint(const LayerNormArgs& a, cudaStream_t stream)
             using T = decltype(t);
             if (a.channels > WIDEST) {
                 if (a.gradX.data != nullptr) {
-                    layer_norm_wide_adjoint_kernel<T><<<blocksFor(a.rows, 1, a.numSMs, 2), 1024, 0, stream>>>(a);
+                    launchChained(layer_norm_wide_adjoint_kernel<T>, blocksFor(a.rows, 1, a.numSMs, 2), 1024, 0, stream, 1, a);
                     const cudaError_t s = cudaGetLastError();
                     if (s != cudaSuccess) return s;
                 }
-                if (parameters) layer_norm_wide_partial_kernel<T><<<dim3((a.channels + 255) / 256, blocks), 256, 0, stream>>>(a);
+                if (parameters) launchChained(layer_norm_wide_partial_kernel<T>, dim3((a.channels + 255) / 256, blocks), 256, 0, stream, 1, a);
                 return cudaGetLastError();
             }
             const bool vec = wide(a.x, a.type, a.channels) && wide(a.gradY, a.type, a.channels) && wide(a.gradX, a.type, a.channels);
@@ -679,15 +685,14 @@ cudaError_t launchLayerNormAdjoint(const LayerNormArgs& a, cudaStream_t stream)
                 if constexpr (G > 32) {
                     if (vec) return launchRinged(layer_norm_adjoint_kernel<T, WIDE<T>, G, EPT, true>, a, 2, blocks, G, perSM(G), stream);
                 }
-                if (vec && G <= 32) layer_norm_adjoint_kernel<T, WIDE<T>, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
-                else layer_norm_adjoint_kernel<T, 1, G, EPT, false><<<blocks, threadsFor(G), 0, stream>>>(a);
+                if (vec && G <= 32) launchChained(layer_norm_adjoint_kernel<T, WIDE<T>, G, EPT, false>, blocks, threadsFor(G), 0, stream, 1, a);
+                else launchChained(layer_norm_adjoint_kernel<T, 1, G, EPT, false>, blocks, threadsFor(G), 0, stream, 1, a);
                 return cudaGetLastError();
             });
         });
     }
     if (e != cudaSuccess || !parameters) return e;
-    layer_norm_parameters_kernel<<<(2 * a.channels + 31) / 32, dim3(32, 16), 0, stream>>>(a.partial, static_cast<int>(blocks), a.channels, a.gradWeight,
-                                                                                         a.gradWeightType, a.gradBias, a.gradBiasType);
+    launchChained(layer_norm_parameters_kernel, (2 * a.channels + 31) / 32, dim3(32, 16), 0, stream, 1, a.partial, static_cast<int>(blocks), a.channels, a.gradWeight, a.gradWeightType, a.gradBias, a.gradBiasType);
     return cudaGetLastError();
 }
 

@@ -113,6 +113,7 @@ __device__ __forceinline__ int blockExclusive(int* v, int n, int* warpSums)
 static __global__ void __launch_bounds__(PARTITION_THREADS)
     partition_scan_kernel(const int* __restrict__ counts, int* __restrict__ before, int* __restrict__ totals, int digits, int blocks)
 {
+    chained();
     __shared__ int warpSums[PARTITION_WARPS];
     const int d = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int* row = counts + static_cast<long long>(d) * blocks;

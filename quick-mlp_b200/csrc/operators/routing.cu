@@ -132,6 +132,7 @@ struct RoutePlan {
 template <class T, int LANES, int PER, bool VECTOR, bool ALONE>
 __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, int* __restrict__ tileCounts, int tiles)
 {
+    chained();
     using K = Key<T>;
     constexpr int SLOTS = ALONE ? ALONE_SLOTS : TILE_SLOTS;
     extern __shared__ int dynamic[];
@@ -215,6 +216,7 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant
 __global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, const int* __restrict__ tileBefore,
                                                                         const int* __restrict__ totals)
 {
+    chained();
     extern __shared__ int dynamic[];
     int* start = dynamic;
     uint16_t* counts = reinterpret_cast<uint16_t*>(dynamic + a.experts);
@@ -240,6 +242,7 @@ __global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __
 template <class T, int LANES, int PER, bool VECTOR>
 __global__ void __launch_bounds__(256) route_adjoint_kernel(const __grid_constant__ RouteArgs a)
 {
+    chained();
     const int lane = threadIdx.x % LANES;
     const long long t = static_cast<long long>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     const bool active = t < a.tokens;
@@ -319,6 +322,7 @@ constexpr int MOVES = 4;
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ ExchangeArgs a, int perRow, int pass)
 {
+    chained();
     const Place at(perRow, pass, VEC);
     if (!at.inside) return;
     const T* x = static_cast<const T*>(a.x.data);
@@ -347,6 +351,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ E
 template <class T, int VEC, bool WEIGHTED, int TOKENS, int SLOTS>
 __global__ void __launch_bounds__(256) gather_sum_kernel(const __grid_constant__ ExchangeArgs a, Rows rowsIn, Rows out, int perRow, int pass)
 {
+    chained();
     const Place at(perRow, pass, VEC);
     if (!at.inside) return;
     const T* rows = static_cast<const T*>(rowsIn.data);
@@ -407,6 +412,7 @@ __global__ void __launch_bounds__(256) gather_sum_kernel(const __grid_constant__
 template <class T, int VEC, int G, int SLOTS>
 __global__ void __launch_bounds__(256, SLOTS <= 2 ? 5 : 3) combine_adjoint_kernel(const __grid_constant__ ExchangeArgs a)
 {
+    chained();
     const int lane = threadIdx.x % G;
     const long long slots = a.tokens * a.chosen, step = static_cast<long long>(gridDim.x) * (256 / G);
     const T* rows = static_cast<const T*>(a.rows.data);
@@ -534,7 +540,7 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
             constexpr int LANES = decltype(l)::value, PER = decltype(per)::value;
             const size_t bytes = (3 * (alone ? ALONE_SLOTS : TILE_SLOTS) + a.experts * (alone ? 1 + PARTITION_WARPS / 2 : 1)) * sizeof(int);
             auto go = [&](auto kernel) {
-                kernel<<<p.tiles, 256, bytes, stream>>>(a, p.tokensPerTile, counts, p.tiles);
+                launchChained(kernel, p.tiles, 256, bytes, stream, 1, a, p.tokensPerTile, counts, p.tiles);
                 return cudaGetLastError();
             };
             if (vec) return alone ? go(route_choose_kernel<T, LANES, PER, true, true>) : go(route_choose_kernel<T, LANES, PER, true, false>);
@@ -542,8 +548,8 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
         });
     });
     if (e != cudaSuccess || alone) return e;
-    partition_scan_kernel<<<a.experts, PARTITION_THREADS, 0, stream>>>(counts, before, totals, a.experts, p.tiles);
-    route_place_kernel<<<p.tiles, PARTITION_THREADS, (1 + PARTITION_WARPS / 2) * a.experts * sizeof(int), stream>>>(a, p.tokensPerTile, before, totals);
+    launchChained(partition_scan_kernel, a.experts, PARTITION_THREADS, 0, stream, 1, counts, before, totals, a.experts, p.tiles);
+    launchChained(route_place_kernel, p.tiles, PARTITION_THREADS, (1 + PARTITION_WARPS / 2) * a.experts * sizeof(int), stream, 1, a, p.tokensPerTile, before, totals);
     return cudaGetLastError();
 }
 
@@ -556,8 +562,8 @@ cudaError_t launchRouteAdjoint(const RouteArgs& a, cudaStream_t stream)
         return byExperts(a.experts, [&](auto l, auto per) {
             constexpr int LANES = decltype(l)::value, PER = decltype(per)::value;
             const unsigned blocks = static_cast<unsigned>((a.tokens + 256 / LANES - 1) / (256 / LANES));
-            if (vec) route_adjoint_kernel<T, LANES, PER, true><<<blocks, 256, 0, stream>>>(a);
-            else route_adjoint_kernel<T, LANES, PER, false><<<blocks, 256, 0, stream>>>(a);
+            if (vec) launchChained(route_adjoint_kernel<T, LANES, PER, true>, blocks, 256, 0, stream, 1, a);
+            else launchChained(route_adjoint_kernel<T, LANES, PER, false>, blocks, 256, 0, stream, 1, a);
             return cudaGetLastError();
         });
     });
@@ -585,8 +591,8 @@ cudaError_t launchDispatch(const ExchangeArgs& a, cudaStream_t stream)
         using T = decltype(t);
         const bool vec = wide(a.x, a.type, a.channels) && wide(a.rows, a.type, a.channels);
         const AccessGrid g(a.tokens * a.chosen, a.channels, vec ? WIDE<T> : 1, MOVES);
-        if (vec) dispatch_kernel<T, WIDE<T>><<<g.blocks, 256, 0, stream>>>(a, g.perRow, g.pass);
-        else dispatch_kernel<T, 1><<<g.blocks, 256, 0, stream>>>(a, g.perRow, g.pass);
+        if (vec) launchChained(dispatch_kernel<T, WIDE<T>>, g.blocks, 256, 0, stream, 1, a, g.perRow, g.pass);
+        else launchChained(dispatch_kernel<T, 1>, g.blocks, 256, 0, stream, 1, a, g.perRow, g.pass);
         return cudaGetLastError();
     });
 }
@@ -596,7 +602,7 @@ static cudaError_t launchGather(const ExchangeArgs& a, const Rows& in, const Row
 {
     auto go = [&](auto* kernel, int each) {
         const AccessGrid g(a.tokens, a.channels, VEC, each, a.numSMs * 8ll);
-        kernel<<<g.blocks, 256, 0, stream>>>(a, in, out, g.perRow, g.pass);
+        launchChained(kernel, g.blocks, 256, 0, stream, 1, a, in, out, g.perRow, g.pass);
         return cudaGetLastError();
     };
     // about 4 loads on their way per thread
@@ -626,9 +632,9 @@ cudaError_t launchCombineAdjoint(const ExchangeArgs& a, cudaStream_t stream)
         auto go = [&](auto v, auto g) {
             constexpr int VEC = decltype(v)::value, G = decltype(g)::value;
             const unsigned blocks = static_cast<unsigned>(std::min<long long>((a.tokens + 256 / G - 1) / (256 / G), a.numSMs * 8));
-            if (a.chosen == 1) combine_adjoint_kernel<T, VEC, G, 1><<<blocks, 256, 0, stream>>>(a);
-            else if (a.chosen == 2) combine_adjoint_kernel<T, VEC, G, 2><<<blocks, 256, 0, stream>>>(a);
-            else combine_adjoint_kernel<T, VEC, G, 4><<<blocks, 256, 0, stream>>>(a);
+            if (a.chosen == 1) launchChained(combine_adjoint_kernel<T, VEC, G, 1>, blocks, 256, 0, stream, 1, a);
+            else if (a.chosen == 2) launchChained(combine_adjoint_kernel<T, VEC, G, 2>, blocks, 256, 0, stream, 1, a);
+            else launchChained(combine_adjoint_kernel<T, VEC, G, 4>, blocks, 256, 0, stream, 1, a);
             return cudaGetLastError();
         };
         if (vec) return a.channels <= 8 * WIDE<T> ? go(std::integral_constant<int, WIDE<T>>(), std::integral_constant<int, 8>())
