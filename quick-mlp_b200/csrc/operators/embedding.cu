@@ -342,9 +342,9 @@ struct SortPlan {
         large = tokens > numSMs * 2048ll;
         const int tile = large ? 4096 : 1024;
         blocks = static_cast<int>((tokens + tile - 1) / tile);
-        // chunks: 1024 threads' worth of groups per SM, 8 rows in flight each
+        // chunks: 512 threads' worth of groups per SM, 8 rows in flight each (1024: sums 34 us and joins 10 us for a million rows of 32 floats, against 30 and 6)
         const int wide = 16 / typeBytes(type);
-        const long long lanes = std::max<long long>(1, (channels + wide - 1) / wide), groups = std::max<long long>(1, numSMs * 1024ll / lanes);
+        const long long lanes = std::max<long long>(1, (channels + wide - 1) / wide), groups = std::max<long long>(1, numSMs * 512ll / lanes);
         chunk = static_cast<int>(std::min<long long>(256, std::max<long long>(16, (tokens + groups - 1) / groups)));
         chunk = (chunk + RUN_STEP - 1) / RUN_STEP * RUN_STEP;
         chunks = static_cast<int>((tokens + chunk - 1) / chunk);

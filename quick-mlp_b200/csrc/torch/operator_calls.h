@@ -156,8 +156,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> routeForward(const Tensor& lo
     // one allocation for the four integer arrays
     const int64_t slots = n * chosen;
     Tensor weights = emptyFloat({n, chosen}, z), ints = emptyInt({3 * slots + e + 1}, z);
-    Tensor experts = ints.narrow(0, 0, slots).view({n, chosen}), positions = ints.narrow(0, slots, slots).view({n, chosen});
-    Tensor order = ints.narrow(0, 2 * slots, slots), offsets = ints.narrow(0, 3 * slots, e + 1);
+    Tensor experts = ints.as_strided({n, chosen}, {chosen, 1}, 0), positions = ints.as_strided({n, chosen}, {chosen, 1}, slots);
+    Tensor order = ints.as_strided({slots}, {1}, 2 * slots), offsets = ints.as_strided({e + 1}, {1}, 3 * slots);
     qmlp_routing_t r{n, static_cast<int32_t>(e), static_cast<int32_t>(chosen), static_cast<float*>(weights.data_ptr()), static_cast<int*>(experts.data_ptr()),
                      static_cast<int*>(order.data_ptr()), static_cast<int*>(positions.data_ptr()), static_cast<int*>(offsets.data_ptr())};
     size_t bytes = 0;
