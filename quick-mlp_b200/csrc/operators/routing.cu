@@ -89,6 +89,7 @@ __device__ __forceinline__ void loadLogits(const T* row, int lane, int experts, 
 // slots per block, at most: a block that is alone takes 1024, else 512, so that the rows of a tile are few passes of a block
 constexpr int ALONE_ITEMS = 4, TILE_ITEMS = 2;
 constexpr int ALONE_SLOTS = ALONE_ITEMS * PARTITION_THREADS, TILE_SLOTS = TILE_ITEMS * PARTITION_THREADS;
+constexpr int TILE_BLOCKS = 148;   // tiles wanted at least
 
 // Ranks the slots of a tile and writes order and position. `expertOf(i)`: expert of the tile's i-th slot, -1: none.
 // `start`: where the tile's slots of an expert begin (shared memory), `last`: experts.
@@ -119,7 +120,10 @@ struct RoutePlan {
     size_t counts, before, bytes;
     RoutePlan(long long tokens, int experts, int chosen)
     {
-        tokensPerTile = std::max(1, (tokens * chosen <= ALONE_SLOTS ? ALONE_SLOTS : TILE_SLOTS) / chosen);
+        // small batches in tiles of 32 rows and more, so that every SM has one: 2048 rows in 4 tiles of 512 took 12.6 us
+        const int most = std::max(1, TILE_SLOTS / chosen);
+        const long long even = (tokens + TILE_BLOCKS - 1) / TILE_BLOCKS;
+        tokensPerTile = tokens * chosen <= ALONE_SLOTS ? ALONE_SLOTS / chosen : static_cast<int>(std::min<long long>(most, (even + 31) / 32 * 32));
         tiles = static_cast<int>((tokens + tokensPerTile - 1) / tokensPerTile);
         counts = (static_cast<size_t>(experts) * 4 + 255) / 256 * 256;
         before = counts + (static_cast<size_t>(experts) * tiles * 4 + 255) / 256 * 256;
@@ -213,6 +217,201 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const __grid_constant
     }
 }
 
+// ---- a row per thread --------------------------------------------------------------------------------------------------------
+// Groups of lanes spend most of their instructions on one another (92 per row of 64 experts). Where there are rows enough, a thread keeps a row's
+// largest keys in registers, in order, and looks at every logit once; a warp moves its 32 rows through shared memory, 128 bytes of each at a time,
+// so that memory is read and written in whole lines (16-byte pieces of a row are exchanged by the row's number against bank conflicts).
+// 262147 rows of 64 half logits, 2 chosen: 22 us, adjoint 10 us (groups of 8 lanes: 33 and 19 us).
+constexpr int ROWS_CHOSEN = 8, ROWS_EXPERTS = 256;   // most of either
+template <class T>
+struct RowStage {
+    static constexpr int W = WIDE<T>, COLUMNS = 128 / static_cast<int>(sizeof(T));
+    unsigned char* mine;   // 32 rows x 128 bytes of this warp
+    int lane;
+    __device__ __forceinline__ explicit RowStage(unsigned char* memory) : mine(memory + (threadIdx.x >> 5) * 32 * 128), lane(threadIdx.x & 31) {}
+    // columns [c0, c0 + COLUMNS) of the rows [0, rows) of `matrix`; -inf behind either
+    __device__ __forceinline__ void fetch(const T* matrix, long long stride, long long rows, int c0, int columns)
+    {
+        const int c = c0 + (lane & 7) * W;
+        Pack<T, W> v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[i].v[k] = minusInfinity<T>();
+            if (r < rows && c < columns) v[i] = load<T, W>(matrix + r * stride + c);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            store<T, W>(reinterpret_cast<T*>(mine + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), v[i]);
+        }
+        __syncwarp();
+    }
+    // piece q of this lane's row
+    __device__ __forceinline__ T* piece(int q) const { return reinterpret_cast<T*>(mine + lane * 128 + ((q ^ (lane & 7)) << 4)); }
+    __device__ __forceinline__ void put(T* matrix, long long stride, long long rows, int c0, int columns)
+    {
+        __syncwarp();
+        const int c = c0 + (lane & 7) * W;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (r < rows && c < columns) store<T, W>(matrix + r * stride + c, load<T, W>(reinterpret_cast<const T*>(mine + r * 128 + (((lane & 7) ^ (r & 7)) << 4))));
+        }
+        __syncwarp();
+    }
+};
+
+template <class T, int CHOSEN>
+__global__ void __launch_bounds__(256) route_rows_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, int* __restrict__ tileCounts, int tiles)
+{
+    chained();
+    using K = Key<T>;
+    using Stage = RowStage<T>;
+    extern __shared__ __align__(128) unsigned char rowMemory[];   // 8 warps x 32 rows x 128 bytes
+    __shared__ int count[ROWS_EXPERTS];
+    Stage stage(rowMemory);
+    const long long first = static_cast<long long>(blockIdx.x) * tokensPerTile;
+    const int tokens = static_cast<int>(min(static_cast<long long>(tokensPerTile), a.tokens - first));
+    for (int i = threadIdx.x; i < a.experts; i += 256) count[i] = 0;
+    __syncthreads();
+    for (int t0 = static_cast<int>(threadIdx.x & ~31u); t0 < tokens; t0 += 256) {   // this warp's 32 rows
+        const T* logits = static_cast<const T*>(a.logits.data) + (first + t0) * a.logits.stride;
+        typename K::Type best[CHOSEN] = {};
+        for (int c0 = 0; c0 < a.experts; c0 += Stage::COLUMNS) {
+            stage.fetch(logits, a.logits.stride, tokens - t0, c0, a.experts);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const Pack<T, Stage::W> v = load<T, Stage::W>(stage.piece(q));
+#pragma unroll
+                for (int i = 0; i < Stage::W; ++i) {
+                    typename K::Type key = K::of(v.v[i], c0 + q * Stage::W + i);
+#pragma unroll
+                    for (int j = 0; j < CHOSEN; ++j) {   // into its place among the largest
+                        const bool larger = key > best[j];
+                        const typename K::Type high = larger ? key : best[j];
+                        key = larger ? best[j] : key;
+                        best[j] = high;
+                    }
+                }
+            }
+        }
+        const float top = best[0] == 0 ? 0.f : K::value(best[0]);
+        float total = 0.f, share[CHOSEN];
+#pragma unroll
+        for (int j = 0; j < CHOSEN; ++j) {
+            share[j] = j < a.chosen && best[j] != 0 ? expf(K::value(best[j]) - top) : 0.f;
+            total += share[j];
+        }
+        if (!a.normalize) {
+            total = 0.f;
+            for (int c0 = 0; c0 < a.experts; c0 += Stage::COLUMNS) {
+                if (a.experts > Stage::COLUMNS) stage.fetch(logits, a.logits.stride, tokens - t0, c0, a.experts);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    float f[Stage::W];
+                    unpack<T, Stage::W>(load<T, Stage::W>(stage.piece(q)), f);
+#pragma unroll
+                    for (int i = 0; i < Stage::W; ++i) total += best[0] == 0 || f[i] == __uint_as_float(0xff800000u) ? 0.f : expf(f[i] - top);
+                }
+            }
+        }
+        const int t = t0 + (threadIdx.x & 31);
+        if (t < tokens) {
+#pragma unroll
+            for (int j = 0; j < CHOSEN; ++j) {
+                if (j >= a.chosen) break;
+                const int expert = best[j] == 0 ? -1 : K::expert(best[j]);
+                a.weights[(first + t) * a.chosen + j] = expert < 0 ? 0.f : share[j] / total;
+                a.expert[(first + t) * a.chosen + j] = expert;
+                if (expert >= 0) atomicAdd(&count[expert], 1);
+            }
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.experts; e += 256) tileCounts[static_cast<long long>(e) * tiles + blockIdx.x] = count[e];
+}
+
+template <class T, int CHOSEN>
+__global__ void __launch_bounds__(256) route_rows_adjoint_kernel(const __grid_constant__ RouteArgs a)
+{
+    chained();
+    using Stage = RowStage<T>;
+    extern __shared__ __align__(128) unsigned char rowMemory[];
+    Stage stage(rowMemory);
+    const long long t0 = static_cast<long long>(blockIdx.x) * 256 + (threadIdx.x & ~31u), t = t0 + (threadIdx.x & 31);
+    if (t0 >= a.tokens) return;
+    const T* logits = static_cast<const T*>(a.logits.data) + t0 * a.logits.stride;
+    T* out = static_cast<T*>(a.gradLogits.data) + t0 * a.gradLogits.stride;
+    int expert[CHOSEN];
+    float weight[CHOSEN], grad[CHOSEN], mean = 0.f;
+#pragma unroll
+    for (int j = 0; j < CHOSEN; ++j) {
+        const bool have = t < a.tokens && j < a.chosen;
+        expert[j] = have ? a.expert[t * a.chosen + j] : -1;
+        weight[j] = have ? a.weights[t * a.chosen + j] : 0.f;
+        grad[j] = have ? a.gradWeights[t * a.chosen + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < CHOSEN; ++j)
+        if (expert[j] >= 0) mean = fmaf(grad[j], weight[j], mean);
+    constexpr float NONE = -INFINITY;
+    float top = NONE, total = 0.f;
+    bool nan = false;
+    if (!a.normalize) {
+        for (int c0 = 0; c0 < a.experts; c0 += Stage::COLUMNS) {   // largest logit and sum of the exponentials, a piece of the row at a time
+            stage.fetch(logits, a.logits.stride, a.tokens - t0, c0, a.experts);
+            float high = top;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                float f[Stage::W];
+                unpack<T, Stage::W>(load<T, Stage::W>(stage.piece(q)), f);
+#pragma unroll
+                for (int i = 0; i < Stage::W; ++i) {
+                    high = fmaxf(high, f[i]);
+                    nan = nan || f[i] != f[i];
+                }
+            }
+            if (high == NONE) continue;
+            total *= top == NONE ? 0.f : expf(top - high);
+            top = high;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                float f[Stage::W];
+                unpack<T, Stage::W>(load<T, Stage::W>(stage.piece(q)), f);
+#pragma unroll
+                for (int i = 0; i < Stage::W; ++i) total += f[i] == NONE ? 0.f : expf(f[i] - top);
+            }
+        }
+        if (nan) total = __uint_as_float(0x7fc00000u);
+    }
+    const float inverse = 1.f / total;
+    for (int c0 = 0; c0 < a.experts; c0 += Stage::COLUMNS) {
+        if (a.normalize) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) store<T, Stage::W>(stage.piece(q), Pack<T, Stage::W>{});
+        } else {
+            if (a.experts > Stage::COLUMNS) stage.fetch(logits, a.logits.stride, a.tokens - t0, c0, a.experts);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                float f[Stage::W];
+                unpack<T, Stage::W>(load<T, Stage::W>(stage.piece(q)), f);
+#pragma unroll
+                for (int i = 0; i < Stage::W; ++i) f[i] = f[i] == NONE ? 0.f : -(expf(f[i] - top) * inverse) * mean;
+                store<T, Stage::W>(stage.piece(q), pack<T, Stage::W>(f));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < CHOSEN; ++j) {
+            const int c = expert[j] - c0;
+            if (expert[j] >= 0 && c >= 0 && c < Stage::COLUMNS) stage.piece(c / Stage::W)[c % Stage::W] = Element<T>::from(weight[j] * (grad[j] - mean));
+        }
+        stage.put(out, a.gradLogits.stride, a.tokens - t0, c0, a.experts);
+    }
+}
+
 __global__ void __launch_bounds__(PARTITION_THREADS) route_place_kernel(const __grid_constant__ RouteArgs a, int tokensPerTile, const int* __restrict__ tileBefore,
                                                                         const int* __restrict__ totals)
 {
@@ -277,7 +476,7 @@ __global__ void __launch_bounds__(256) route_adjoint_kernel(const __grid_constan
         }
         const float inverse = 1.f / groupSum<LANES>(s);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) d[i] = z[i] == 0.f ? 0.f : -(z[i] * inverse) * mean;
+        for (int i = 0; i < PER; ++i) d[i] = Element<T>::to(raw[i]) == __uint_as_float(0xff800000u) ? 0.f : -(z[i] * inverse) * mean;
     }
     for (int j = 0; j < a.chosen; ++j) {
         const long long i = row * a.chosen + j;
@@ -519,6 +718,20 @@ cudaError_t byExperts(int experts, F&& f)
 
 } // namespace
 
+// A thread per row. Measured against groups of lanes, us: choice of 2 of 64 experts for 131072 rows of half 18 / 24, of 8 of 64 49 / 38 (the keys' order costs
+// more than the groups' rounds), of 2 of 8 15 / 5 (groups of one lane), of 2 of 64 floats 31 / 31; adjoint, the mean of either kind of weights, 2
+// of 64 13 / 16, 8 of 256 48 / 75, 2 of 8 9 / 4; for 8192 rows 2 of 64 6 / 3.
+static bool chooseByThread(const RouteArgs& a) { return a.type != TYPE_FLOAT && a.tokens >= 16384 && a.experts >= 32 && a.experts <= ROWS_EXPERTS && a.chosen <= 2; }
+static bool adjointByThread(const RouteArgs& a) { return a.tokens >= 65536 && a.experts >= 32 && a.experts <= ROWS_EXPERTS && a.chosen <= ROWS_CHOSEN; }
+template <class F>
+static cudaError_t byChosen(int chosen, F&& f)
+{
+    if (chosen == 1) return f(std::integral_constant<int, 1>());
+    if (chosen == 2) return f(std::integral_constant<int, 2>());
+    if (chosen <= 4) return f(std::integral_constant<int, 4>());
+    return f(std::integral_constant<int, 8>());
+}
+
 size_t routeBytes(long long tokens, int experts, int chosen)
 {
     if (tokens == 0) return 0;
@@ -536,6 +749,13 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
     int* before = reinterpret_cast<int*>(static_cast<unsigned char*>(a.scratch) + p.before);
     cudaError_t e = byType(a.type, [&](auto t) {
         using T = decltype(t);
+        if constexpr (sizeof(T) == 2) {
+            if (!alone && vec && chooseByThread(a)) {
+                if (a.chosen == 1) launchChained(route_rows_kernel<T, 1>, p.tiles, 256, 32 * 1024, stream, 1, a, p.tokensPerTile, counts, p.tiles);
+                else launchChained(route_rows_kernel<T, 2>, p.tiles, 256, 32 * 1024, stream, 1, a, p.tokensPerTile, counts, p.tiles);
+                return cudaGetLastError();
+            }
+        }
         return byExperts(a.experts, [&](auto l, auto per) {
             constexpr int LANES = decltype(l)::value, PER = decltype(per)::value;
             const size_t bytes = (3 * (alone ? ALONE_SLOTS : TILE_SLOTS) + a.experts * (alone ? 1 + PARTITION_WARPS / 2 : 1)) * sizeof(int);
@@ -559,6 +779,11 @@ cudaError_t launchRouteAdjoint(const RouteArgs& a, cudaStream_t stream)
     const bool vec = wide(a.logits, a.type, a.experts) && wide(a.gradLogits, a.type, a.experts);
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
+        if (vec && adjointByThread(a))
+            return byChosen(a.chosen, [&](auto n) {
+                launchChained(route_rows_adjoint_kernel<T, decltype(n)::value>, static_cast<unsigned>((a.tokens + 255) / 256), 256, 32 * 1024, stream, 1, a);
+                return cudaGetLastError();
+            });
         return byExperts(a.experts, [&](auto l, auto per) {
             constexpr int LANES = decltype(l)::value, PER = decltype(per)::value;
             const unsigned blocks = static_cast<unsigned>((a.tokens + 256 / LANES - 1) / (256 / LANES));

@@ -198,6 +198,37 @@ def test_route(qmlp, rows, experts, k, normalize, dtype):
     route_case(qmlp, z, k, normalize)
 
 
+@pytest.mark.parametrize("dtype", FLOATS, ids=IDS.get)
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("rows,experts,k", [(20000, 64, 2), (16385, 8, 1), (17001, 256, 8), (16384, 40, 3), (16500, 136, 5), (66000, 64, 2), (65536, 256, 8), (65601, 40, 1),
+                                            (16400, 32, 2), (3000, 64, 2)])
+def test_route_many_rows(qmlp, rows, experts, k, normalize, dtype):
+    """the kernels for many rows choose and weigh as those for few do, row by row, and order the slots as a sort does"""
+    z = rand(59, (rows, experts), dtype, 1.5)
+    z[ints(60, (rows, experts), 0, 8) == 0] = -INF
+    z[1], z[2], z[3, : experts // 2], z[4, 0], z[5, 1] = -INF, torch.finfo(dtype).min, z[3, 0], float("nan"), INF
+    leaf = z.clone().requires_grad_()
+    r = qmlp.route(leaf, k, normalize)
+    grad = rand(61, (rows, k))
+    dz, = torch.autograd.grad(r.weights, [leaf], grad)
+    for first in range(0, rows, 7000):
+        part = z[first:first + 7000].clone().requires_grad_()
+        few = qmlp.route(part, k, normalize)
+        rows_of = slice(first, first + 7000)
+        assert torch.equal(r.experts[rows_of], few.experts)
+        assert torch.allclose(r.weights[rows_of].detach(), few.weights.detach(), rtol=(experts + 16) * 2.0 ** -22, atol=0, equal_nan=True)
+        d, = torch.autograd.grad(few.weights, [part], grad[rows_of])
+        fine = torch.isfinite(few.weights).all(1)
+        w, s = ref.route_gradient(part.detach()[fine], few.experts[fine], few.weights.detach()[fine], grad[rows_of][fine], normalize)
+        ref.check(dz[rows_of][fine], w, s, "logits' gradient")
+        assert torch.equal(torch.isnan(dz[rows_of]), torch.isnan(d))
+    flat = torch.where(r.experts < 0, experts, r.experts).reshape(-1)
+    order = torch.argsort(flat, stable=True).int()
+    used = int((flat < experts).sum())
+    assert torch.equal(r.order[:used], order[:used]) and (r.order[used:] == -1).all()
+    assert torch.equal(r.offsets, torch.nn.functional.pad(torch.bincount(flat, minlength=experts + 1)[:experts].cumsum(0), (1, 0)).int())
+
+
 def test_route_values(qmlp):
     """equal zeros of both signs, infinity, NaN: the largest first, NaN before all, weights as a softmax says"""
     z = rand(53, (6, 12))
