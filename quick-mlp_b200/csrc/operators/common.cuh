@@ -1,5 +1,7 @@
 // What the kernels of the operators share: element types, 16-byte accesses, reductions over a group of threads.
 #pragma once
+#include <initializer_list>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,7 +30,7 @@ template <> struct Element<__nv_bfloat16> {
 // elements of a 16-byte access
 template <class T> constexpr int WIDE = 16 / static_cast<int>(sizeof(T));
 
-// VEC consecutive elements as they lie in memory; VEC is 1 or WIDE<T>
+// VEC consecutive elements as they lie in memory; VEC is 1, 2 or WIDE<T>
 template <class T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
     T v[VEC];
@@ -218,6 +220,21 @@ inline bool wide(const Rows& r, int type, int channels)
 {
     const int n = 16 / typeBytes(type);
     return r.data == nullptr || ((reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.stride % n == 0 && channels % n == 0);
+}
+
+// The access that all of `matrices` allow, as f(integral_constant of elements): 16 bytes, else pairs of elements, else single ones. 672856 tokens of a table of
+// 50 bfloat16: forward 37 us in pairs and 70 us one by one, the gradient's sums 36 and 59 us.
+template <class T, class F>
+cudaError_t byAccess(std::initializer_list<const Rows*> matrices, int type, int channels, F&& f)
+{
+    bool all = true, pairs = channels % 2 == 0;
+    for (const Rows* r : matrices) {
+        all = all && wide(*r, type, channels);
+        pairs = pairs && (r->data == nullptr || ((reinterpret_cast<uintptr_t>(r->data) % (2 * sizeof(T))) == 0 && r->stride % 2 == 0));
+    }
+    if (all) return f(std::integral_constant<int, WIDE<T>>());
+    if (pairs) return f(std::integral_constant<int, 2>());
+    return f(std::integral_constant<int, 1>());
 }
 
 // lets a kernel use up to `bytes` of dynamic shared memory on the current device; asked for once per kernel and device

@@ -33,23 +33,24 @@ template <class T, int VEC>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(const __grid_constant__ EmbeddingArgs a, int perRow, int pass)
 {
     chained();
+    constexpr int N = LOOKUPS;
     const T* table = static_cast<const T*>(a.table.data);
     T* y = static_cast<T*>(a.y.data);
     const int rowInPass = pass == 1 ? 0 : static_cast<int>(threadIdx.x) / perRow, access = blockIdx.y * 256 + (pass == 1 ? threadIdx.x : threadIdx.x - rowInPass * perRow);
     if (rowInPass >= pass || access >= perRow) return;
     const int c = access * VEC;
-    const long long first = static_cast<long long>(blockIdx.x) * (pass * LOOKUPS) + rowInPass;
-    long long token[LOOKUPS];
-    Pack<T, VEC> v[LOOKUPS];
+    const long long first = static_cast<long long>(blockIdx.x) * (pass * N) + rowInPass;
+    long long token[N];
+    Pack<T, VEC> v[N];
 #pragma unroll
-    for (int k = 0; k < LOOKUPS; ++k) token[k] = first + k * pass < a.tokens ? tokenAt(a, first + k * pass) : -1;
+    for (int k = 0; k < N; ++k) token[k] = first + k * pass < a.tokens ? tokenAt(a, first + k * pass) : -1;
 #pragma unroll
-    for (int k = 0; k < LOOKUPS; ++k) {
+    for (int k = 0; k < N; ++k) {
         v[k] = {};
         if (token[k] >= 0 && token[k] < a.rows) v[k] = load<T, VEC>(table + token[k] * a.table.stride + c);
     }
 #pragma unroll
-    for (int k = 0; k < LOOKUPS; ++k) {
+    for (int k = 0; k < N; ++k) {
         if (first + k * pass >= a.tokens) break;
         if (a.scale != 1.f) {
             float f[VEC];
@@ -70,7 +71,7 @@ struct SortArgs {
     const int2* in;                // key and slot; null in the first pass: the tokens, and their own numbers
     int2* out;
     int *counts, *before, *totals;
-    uint8_t* present;              // rows of the table that have a token, set in the first of several passes; null: totals say so
+    uint8_t* present;              // rows of the table that have a token, set in the last of several passes; null: another pass, or totals say so
     int items, blocks, shift, digits;
 };
 __device__ __forceinline__ int2 sortItem(const EmbeddingArgs& a, const SortArgs& s, int i)
@@ -93,15 +94,9 @@ __global__ void __launch_bounds__(WARPS * 32) sort_count_kernel(const __grid_con
         key[k] = i < s.items ? sortItem(a, s, i).x : -1;
     }
     __syncthreads();
-    const bool mark = s.in == nullptr && s.present != nullptr;
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
+    for (int k = 0; k < ITEMS; ++k)
         if (key[k] >= 0) atomicAdd(&count[(key[k] >> s.shift) & (s.digits - 1)], 1);
-        if (mark) {   // once per warp: a hot row's stores would wait for one another
-            const unsigned same = __match_any_sync(0xffffffffu, key[k]);
-            if ((threadIdx.x & 31) == __ffs(same) - 1 && key[k] >= 0 && key[k] < a.rows) s.present[key[k]] = 1;
-        }
-    }
     __syncthreads();
     for (int i = threadIdx.x; i < s.digits; i += WARPS * 32) s.counts[static_cast<long long>(i) * s.blocks + blockIdx.x] = count[i];
 }
@@ -139,6 +134,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1024 / (WARPS * 32)) sort_move_ker
         const int2 v = sorted[i];
         const int d = (v.x >> s.shift) & (s.digits - 1);
         s.out[start[d] + i - local[d]] = v;
+        // (sorted by now within the tile: once per row and tile. By the count of the first digit, per warp, a table of 1985 rows cost 97 us, not 15:
+        // stores to the same few lines wait for one another)
+        if (s.present != nullptr && v.x < a.rows && (i == 0 || sorted[i - 1].x != v.x)) s.present[v.x] = 1;
     }
 }
 
@@ -413,12 +411,13 @@ cudaError_t launchEmbeddingForward(const EmbeddingArgs& a, cudaStream_t stream)
     if (a.tokens == 0) return cudaSuccess;
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
-        const bool vec = wide(a.table, a.type, a.channels) && wide(a.y, a.type, a.channels);
-        const int perRow = vec ? a.channels / WIDE<T> : a.channels, pass = perRow > 128 ? 1 : 256 / perRow;
-        const dim3 grid(static_cast<unsigned>((a.tokens + pass * LOOKUPS - 1) / (pass * LOOKUPS)), pass == 1 ? (perRow + 255) / 256 : 1);
-        if (vec) launchChained(embedding_forward_kernel<T, WIDE<T>>, grid, 256, 0, stream, 1, a, perRow, pass);
-        else launchChained(embedding_forward_kernel<T, 1>, grid, 256, 0, stream, 1, a, perRow, pass);
-        return cudaGetLastError();
+        return byAccess<T>({&a.table, &a.y}, a.type, a.channels, [&](auto v) {
+            constexpr int VEC = decltype(v)::value, N = LOOKUPS;
+            const int perRow = a.channels / VEC, pass = perRow > 128 ? 1 : 256 / perRow;
+            const dim3 grid(static_cast<unsigned>((a.tokens + pass * N - 1) / (pass * N)), pass == 1 ? (perRow + 255) / 256 : 1);
+            launchChained(embedding_forward_kernel<T, VEC>, grid, 256, 0, stream, 1, a, perRow, pass);
+            return cudaGetLastError();
+        });
     });
 }
 
@@ -435,23 +434,23 @@ cudaError_t launchEmbeddingAdjoint(const EmbeddingArgs& a, cudaStream_t stream)
     s.counts = reinterpret_cast<int*>(base + p.counts);
     s.before = reinterpret_cast<int*>(base + p.before);
     s.totals = reinterpret_cast<int*>(base + p.totals);
-    s.present = p.passes > 1 ? base + p.present : nullptr;
+    uint8_t* present = p.passes > 1 ? base + p.present : nullptr;
     s.items = static_cast<int>(a.tokens);
     s.blocks = p.blocks;
     s.digits = p.digits;
-    cudaError_t e = p.passes > 1 ? cudaMemsetAsync(s.present, 0, static_cast<size_t>(a.rows), stream) : cudaSuccess;
+    cudaError_t e = p.passes > 1 ? cudaMemsetAsync(present, 0, static_cast<size_t>(a.rows), stream) : cudaSuccess;
     for (int k = 0; k < p.passes && e == cudaSuccess; ++k) {
         s.in = k > 0 ? lists[(k + 1) & 1] : nullptr;
         s.out = lists[k & 1];
         s.shift = k * p.bits;
+        s.present = k == p.passes - 1 ? present : nullptr;
         e = p.large ? launchSort<8, 16>(a, s, stream) : launchSort<4, 8>(a, s, stream);
     }
     if (e != cudaSuccess) return e;
-    RunArgs r{s.out, s.present, s.totals, s.items, p.chunk, p.chunks, 0, reinterpret_cast<float*>(base + p.partial)};
+    RunArgs r{s.out, present, s.totals, s.items, p.chunk, p.chunks, 0, reinterpret_cast<float*>(base + p.partial)};
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
-        const bool vec = wide(a.gradTable, a.type, a.channels) && wide(a.gradY, a.type, a.channels);
-        const cudaError_t status = vec ? launchRuns<T, WIDE<T>>(a, r, stream) : launchRuns<T, 1>(a, r, stream);
+        const cudaError_t status = byAccess<T>({&a.gradTable, &a.gradY}, a.type, a.channels, [&](auto v) { return launchRuns<T, decltype(v)::value>(a, r, stream); });
         if (status != cudaSuccess || p.chunks < 2) return status;
         return byLanes(a.channels, [&](auto g) {
             constexpr int G = decltype(g)::value;

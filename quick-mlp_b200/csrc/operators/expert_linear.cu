@@ -218,7 +218,7 @@ __device__ __forceinline__ int clampOffset(const ProductArgs& p, int e)
 template <int MODE>
 __device__ __forceinline__ int unitsOf(const ProductArgs& p, int rows)
 {
-    return MODE == WEIGHTS ? max(1, (rows + p.chunk - 1) / p.chunk) : (rows + p.tileRows - 1) / p.tileRows;
+    return MODE == WEIGHTS ? (rows + p.chunk - 1) / p.chunk : (rows + p.tileRows - 1) / p.tileRows;
 }
 // The experts' runs and units of work, for all threads of a block: bounds[e] = first row of expert e, bounds[experts] the end of the last one;
 // before[i] = units of the experts in front of the i-th in `order`. The weight product takes the longest runs first (up to SORTED_MAX
@@ -402,6 +402,17 @@ __device__ __forceinline__ void storeTile(const float (&v)[32], unsigned char* m
     __syncwarp();
 }
 
+// `n` zeros, by a warp
+constexpr int ZERO_PIECE = 4096;
+template <class T>
+__device__ __forceinline__ void zeroRun(T* at, int n)
+{
+    const int lane = threadIdx.x & 31, head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15) / 2), wide = (n - head) / 8, tail = head + wide * 8;
+    if (lane < head) at[lane] = Element<T>::from(0.f);
+    for (int i = lane; i < wide; i += 32) store<T, 8>(at + head + i * 8, Pack<T, 8>{});
+    if (tail + lane < n) at[tail + lane] = Element<T>::from(0.f);
+}
+
 // boxes of 64 that `n` elements fill, 0 to `most`
 __device__ __forceinline__ int boxes(int n, int most) { return max(0, min(most, (n + 63) / 64)); }
 
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         while (ok && walk.next(t)) {
             const int steps = walk.steps(t);
             acc ^= 1;                   // the tiles' numbers alternate between the accumulators
-            if (__all_sync(0xffffffffu, steps == 0)) continue;   // an expert without rows: the epilogue writes zeros
+            if (__all_sync(0xffffffffu, steps == 0)) continue;   // no tile for this block in the last round
             if (!await(accEmpty + acc * 8, (accPhases >> acc & 1) ^ 1, failed)) break;
             accPhases ^= 1u << acc;
             fenceAfter();
@@ -566,9 +577,21 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         const uint32_t released = CTAS == 1 ? accEmpty + group * 8 : inBlock(accEmpty + group * 8, 0);
         T* out = static_cast<T*>(p.out);
         uint32_t accPhase = 0;
+        if constexpr (MODE == WEIGHTS) {
+            // the gradients of experts without rows, while the first products run (as tiles without products: 431 experts of 66 -> 760, 19 rows, 40 us;
+            // so 22 us)
+            const long long matrix = static_cast<long long>(p.sum) * p.columns;
+            const int pieces = static_cast<int>((matrix + ZERO_PIECE - 1) / ZERO_PIECE), warps = gridDim.x * EPILOGUE_WARPS;
+            for (long long i = blockIdx.x * EPILOGUE_WARPS + (warp - 2); i < static_cast<long long>(p.experts) * pieces; i += warps) {
+                const int e = static_cast<int>(i / pieces), piece = static_cast<int>(i - static_cast<long long>(e) * pieces);
+                if (bounds[e + 1] > bounds[e]) continue;
+                const long long first = static_cast<long long>(piece) * ZERO_PIECE;
+                zeroRun<T>(out + e * matrix + first, static_cast<int>(min(static_cast<long long>(ZERO_PIECE), matrix - first)));
+                if (SUMS && piece == 0) zeroRun<T>(static_cast<T*>(p.gradBias) + static_cast<long long>(e) * p.sum, p.sum);
+            }
+        }
         walk = Walk<MODE, BN, CTAS>(p, bounds, before, order, group, EPILOGUE_GROUPS);
         while (walk.next(t)) {
-            const int steps = walk.steps(t);
             if (t.expert < 0) break;
             const int tileRow = t.row + rank * BM;
             float bias[BN / 32];   // of column c * 32 + lane
@@ -577,11 +600,9 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
 #pragma unroll
                 for (int i = 0; i < BN / 32; ++i) bias[i] = p.bias != nullptr && t.column + i * 32 + lane < p.columns ? Element<T>::to(row[i * 32 + lane]) : 0.f;
             }
-            if (steps > 0) {
-                if (!await(accFull + group * 8, accPhase, failed)) break;
-                accPhase ^= 1;
-                fenceAfter();
-            }
+            if (!await(accFull + group * 8, accPhase, failed)) break;
+            accPhase ^= 1;
+            fenceAfter();
             const uint32_t from = tmem + group * BN + (static_cast<uint32_t>(quarter * 32) << 16);
             // rows of D in memory: expert by expert, channels out (weights); the tile's own rows (else)
             const int rowsLeft = (MODE == WEIGHTS ? p.sum : t.end) - tileRow - quarter * 32;
@@ -597,14 +618,9 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
             for (int pair = 0; pair < BN / 64; ++pair) {
                 if (t.column + pair * 64 >= p.columns || rowsLeft <= 0) break;
                 float v[2][32];
-                if (steps > 0) {
-                    tmemLoad32(from + pair * 64, v[0]);
-                    tmemLoad32(from + pair * 64 + 32, v[1]);
-                    tmemWait(v[0], v[1]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0.f;
-                }
+                tmemLoad32(from + pair * 64, v[0]);
+                tmemLoad32(from + pair * 64 + 32, v[1]);
+                tmemWait(v[0], v[1]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int c0 = pair * 64 + h * 32;
@@ -633,13 +649,11 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                     storeTile<T>(v[h], mine, out + firstRow * p.outStride + t.column, p.outStride, rowsLeft, c0, p.columns - t.column, p.wideStore);
                 }
             }
-            if (steps > 0) {
-                fenceBefore();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CTAS == 1) barrierArrive(released);
-                    else clusterArriveBarrier(released);
-                }
+            fenceBefore();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CTAS == 1) barrierArrive(released);
+                else clusterArriveBarrier(released);
             }
         }
         if constexpr (MODE != WEIGHTS) {
@@ -1090,23 +1104,29 @@ __global__ void __launch_bounds__(256) expert_narrow_join_kernel(const __grid_co
     __syncthreads();
     const int expert = found;
     if (before[expert] >= end || before[expert] < begin) return;
-    // block of its last tile: the first whose end, total * (b + 1) / blocks, reaches before[expert + 1]
-    const int last = static_cast<int>((static_cast<long long>(before[expert + 1]) * blocks + total - 1) / total) - 1;
-    const int more = last - block;
-    // blocks without a tile (fewer tiles than blocks) have left nothing
-    auto wrote = [&](int b) { return total >= blocks || total * (block + b + 1) / blocks > total * (block + b) / blocks; };
+    // Later blocks with a part of it: with tiles for all blocks every one up to that of its last tile, the first whose end, total * (b + 1) / blocks, reaches
+    // before[expert + 1]; with fewer tiles the one block of each tile. (16 parts read at a time; one expert of 298 rows, 24 -> 64, where a loop over
+    // all blocks divided for each, 38 us, so 5 us.)
+    const bool full = total >= blocks;
+    const int behind = before[expert + 1];
+    const int more = full ? static_cast<int>((static_cast<long long>(behind) * blocks + total - 1) / total) - 1 - block : behind - end;
+    auto blockOf = [&](int part) { return full ? block + 1 + part : ((end + part + 1) * blocks + static_cast<int>(total) - 1) / static_cast<int>(total) - 1; };
     const int i0 = (blockIdx.y * 256 + threadIdx.x) * 4, n = i0 / columns, c = i0 - n * columns;   // 4 of 128 x columns sums
     if (n < p.sum && c < p.columns) {
-        const float* from = p.partial + (static_cast<long long>(block) * 2 * 128 + n) * columns + c;
-        float4 sum = *reinterpret_cast<const float4*>(from + 128ll * columns);   // the run that block ends with
-#pragma unroll 4
-        for (int b = 1; b <= more; ++b) {                                        // the run the later ones begin with
-            if (!wrote(b)) continue;
-            const float4 v = *reinterpret_cast<const float4*>(from + b * 2 * 128ll * columns);
-            sum.x += v.x;
-            sum.y += v.y;
-            sum.z += v.z;
-            sum.w += v.w;
+        const float* from = p.partial + static_cast<long long>(n) * columns + c;
+        float4 sum = *reinterpret_cast<const float4*>(from + (static_cast<long long>(block) * 2 + 1) * 128 * columns);   // the run that block ends with
+        for (int part = 0; part < more; part += 16) {                                                                    // the run the later ones begin with
+            float4 v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                v[k] = part + k < more ? *reinterpret_cast<const float4*>(from + static_cast<long long>(blockOf(part + k)) * 2 * 128 * columns) : float4{};
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                sum.x += v[k].x;
+                sum.y += v[k].y;
+                sum.z += v[k].z;
+                sum.w += v[k].w;
+            }
         }
         const float f[4] = {sum.x, sum.y, sum.z, sum.w};
         T* out = static_cast<T*>(p.out) + (static_cast<long long>(expert) * p.sum + n) * p.columns + c;
@@ -1115,11 +1135,10 @@ __global__ void __launch_bounds__(256) expert_narrow_join_kernel(const __grid_co
             for (int k = 0; k < 4 && c + k < p.columns; ++k) out[k] = Element<T>::from(f[k]);
     }
     if (p.gradBias != nullptr && blockIdx.y == 0 && threadIdx.x < p.sum) {
-        const float* from = p.partialBias + static_cast<long long>(block) * 2 * 128 + threadIdx.x;
-        float sum = from[128];
-#pragma unroll 4
-        for (int b = 1; b <= more; ++b)
-            if (wrote(b)) sum += from[b * 2 * 128];
+        const float* from = p.partialBias + threadIdx.x;
+        float sum = from[(block * 2 + 1) * 128];
+#pragma unroll 8
+        for (int part = 0; part < more; ++part) sum += from[blockOf(part) * 2 * 128];
         static_cast<T*>(p.gradBias)[static_cast<long long>(expert) * p.sum + threadIdx.x] = Element<T>::from(sum);
     }
 }
@@ -1135,7 +1154,7 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
     const int tiles = p.rowTiles * p.columnTiles;
     const int expert = blockIdx.x / tiles, tile = blockIdx.x % tiles;
     const int before = p.plan[expert].x, units = p.plan[expert].y;
-    if (units == 1) return;
+    if (units < 2) return;
     const long long unitStride = static_cast<long long>(tiles) * p.tileRows * BN;
     const float* from = p.partial + before * unitStride + static_cast<long long>(tile) * p.tileRows * BN;
     const int row0 = tile / p.columnTiles * p.tileRows, column0 = tile % p.columnTiles * BN;
@@ -1299,17 +1318,44 @@ __global__ void __launch_bounds__(256) expert_bias_kernel(const __grid_constant_
 }
 
 // ---- copies of operands the TMA cannot read --------------------------------------------------------------------------------
-// rows of `columns` elements -> rows of `padded` (a multiple of 8) elements, zeros behind
-template <class T>
-__global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ in, long long stride, T* __restrict__ out, long long rows, int columns, int padded)
+// rows of `columns` elements -> rows of `padded` (a multiple of 8) elements, zeros behind. A thread puts 8 elements together from reads of WORD elements
+// (2 where the rows begin on 4 bytes), for PAD_ROWS rows, `pass` rows apart. With `offsets`, rows of an expert without rows of x, which no product reads, are
+// left out. 36838 rows of 690 bfloat16: 27 us (element by element, which divides for each, 60 us).
+constexpr int PAD_ROWS = 4;
+template <class T, int WORD>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ in, long long stride, T* __restrict__ out, long long rows, int columns, int pieces, int pass,
+                                                       const int* __restrict__ offsets, int perExpert)
 {
     chained();
-    const long long total = rows * padded;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * 256) {
-        const long long r = i / padded;
-        const int c = static_cast<int>(i - r * padded);
-        out[i] = c < columns ? in[r * stride + c] : Element<T>::from(0.f);
+    const int rowInPass = pass == 1 ? 0 : static_cast<int>(threadIdx.x) / pieces, piece = blockIdx.y * 256 + (pass == 1 ? threadIdx.x : threadIdx.x - rowInPass * pieces);
+    if (rowInPass >= pass || piece >= pieces) return;
+    const int c = piece * 8;
+    const long long first = static_cast<long long>(blockIdx.x) * (pass * PAD_ROWS) + rowInPass;
+    bool copy[PAD_ROWS];
+    Pack<T, 8> v[PAD_ROWS];
+#pragma unroll
+    for (int k = 0; k < PAD_ROWS; ++k) {
+        const long long r = first + k * pass;
+        copy[k] = r < rows;
+        if (copy[k] && offsets != nullptr) {
+            const int e = static_cast<int>(r / perExpert);
+            copy[k] = offsets[e + 1] > offsets[e];
+        }
     }
+#pragma unroll
+    for (int k = 0; k < PAD_ROWS; ++k) {
+        const T* from = in + (first + k * pass) * stride + c;
+#pragma unroll
+        for (int i = 0; i < 8; i += WORD) {
+            Pack<T, WORD> w = {};
+            if (copy[k] && c + i < columns) w = load<T, WORD>(from + i);
+#pragma unroll
+            for (int j = 0; j < WORD; ++j) v[k].v[i + j] = w.v[j];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < PAD_ROWS; ++k)
+        if (copy[k]) store<T, 8>(out + ((first + k * pass) * pieces + piece) * 8, v[k]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -1429,15 +1475,18 @@ struct Scratch {
     }
 };
 
+// `offsets`: of experts with `perExpert` rows of the matrix each, or null
 template <class T>
-cudaError_t readable(const void*& data, long long& stride, long long rows, int columns, void* scratch, int numSMs, cudaStream_t stream)
+cudaError_t readable(const void*& data, long long& stride, long long rows, int columns, void* scratch, cudaStream_t stream, const int* offsets = nullptr, int perExpert = 1)
 {
     if (direct(data, stride, columns)) return cudaSuccess;
-    const int padded = pad8(columns);
-    const long long blocks = std::min<long long>((rows * padded + 255) / 256, numSMs * 16ll);
-    launchChained(pad_rows_kernel<T>, static_cast<unsigned>(std::max(1ll, blocks)), 256, 0, stream, 1, static_cast<const T*>(data), stride, static_cast<T*>(scratch), rows, columns, padded);
+    const int pieces = pad8(columns) / 8, pass = pieces > 128 ? 1 : 256 / pieces;
+    const dim3 grid(static_cast<unsigned>((rows + pass * PAD_ROWS - 1) / (pass * PAD_ROWS)), pass == 1 ? (pieces + 255) / 256 : 1);
+    const bool pairs = columns % 2 == 0 && stride % 2 == 0 && reinterpret_cast<uintptr_t>(data) % 4 == 0;
+    launchChained(pairs ? pad_rows_kernel<T, 2> : pad_rows_kernel<T, 1>, grid, 256, 0, stream, 1, static_cast<const T*>(data), stride, static_cast<T*>(scratch), rows, columns, pieces,
+                  pass, offsets, perExpert);
     data = scratch;
-    stride = padded;
+    stride = pieces * 8;
     return cudaGetLastError();
 }
 
@@ -1501,8 +1550,8 @@ cudaError_t forward(const ExpertArgs& a, cudaStream_t stream)
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
     const void *x = a.x.data, *w = a.weight;
     long long xStride = a.x.stride, wStride = a.channelsIn;
-    cudaError_t e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, a.numSMs, stream);
-    if (e == cudaSuccess) e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, a.numSMs, stream);
+    cudaError_t e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, stream);
+    if (e == cudaSuccess) e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, stream, a.offsets, a.channelsOut);
     CUtensorMap mapX, mapW;
     if (e == cudaSuccess) e = encodeMap(mapX, a.type, x, 0, a.rows, a.channelsIn, xStride);
     if (e == cudaSuccess) e = encodeMap(mapW, a.type, w, a.experts, a.channelsOut, a.channelsIn, wStride);
@@ -1555,11 +1604,11 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
     const void *x = a.x.data, *w = a.weight, *dy = a.gradY.data;
     long long xStride = a.x.stride, wStride = a.channelsIn, dyStride = a.gradY.stride;
     CUtensorMap mapX, mapW, mapY;
-    if (e == cudaSuccess) e = readable<T>(dy, dyStride, a.rows, a.channelsOut, base + s.gradY, a.numSMs, stream);
+    if (e == cudaSuccess) e = readable<T>(dy, dyStride, a.rows, a.channelsOut, base + s.gradY, stream);
     if (e == cudaSuccess) e = encodeMap(mapY, a.type, dy, 0, a.rows, a.channelsOut, dyStride);
     if (e == cudaSuccess && s.narrow) {
-        e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, a.numSMs, stream);
-        if (e == cudaSuccess) e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, a.numSMs, stream);
+        e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, stream, a.offsets, a.channelsOut);
+        if (e == cudaSuccess) e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, stream);
         if (e == cudaSuccess) e = encodeMap(mapW, a.type, w, a.experts, a.channelsOut, a.channelsIn, wStride);
         if (e == cudaSuccess) e = encodeMap(mapX, a.type, x, 0, a.rows, a.channelsIn, xStride);
         if (e != cudaSuccess) return e;
@@ -1577,7 +1626,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         return a.channelsIn <= 64 ? launchNarrow<T, 2, 1>(mapY, mapX, mapW, p, a, stream) : launchNarrow<T, 2, 2>(mapY, mapX, mapW, p, a, stream);
     }
     if (e == cudaSuccess && a.gradX.data != nullptr) {
-        e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, a.numSMs, stream);
+        e = readable<T>(w, wStride, static_cast<long long>(a.experts) * a.channelsOut, a.channelsIn, base + s.weight, stream, a.offsets, a.channelsOut);
         if (e == cudaSuccess) e = encodeMap(mapW, a.type, w, a.experts, a.channelsOut, a.channelsIn, wStride);
         if (e != cudaSuccess) return e;
         ProductArgs p = common(a);
@@ -1592,7 +1641,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         e = launchShape<T, INPUT>(shape, mapY, mapW, p, a.numSMs, stream);
     }
     if (e == cudaSuccess && a.gradWeight != nullptr) {
-        e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, a.numSMs, stream);
+        e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, stream);
         if (e == cudaSuccess) e = encodeMap(mapX, a.type, x, 0, a.rows, a.channelsIn, xStride);
         if (e != cudaSuccess) return e;
         ProductArgs p = common(a);

@@ -290,9 +290,8 @@ __global__ void __launch_bounds__(256) route_rows_kernel(const __grid_constant__
                     typename K::Type key = K::of(v.v[i], c0 + q * Stage::W + i);
 #pragma unroll
                     for (int j = 0; j < CHOSEN; ++j) {   // into its place among the largest
-                        const bool larger = key > best[j];
-                        const typename K::Type high = larger ? key : best[j];
-                        key = larger ? best[j] : key;
+                        const typename K::Type high = max(key, best[j]);
+                        key = min(key, best[j]);
                         best[j] = high;
                     }
                 }
@@ -522,25 +521,26 @@ template <class T, int VEC>
 __global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ ExchangeArgs a, int perRow, int pass)
 {
     chained();
+    constexpr int N = MOVES;
     const Place at(perRow, pass, VEC);
     if (!at.inside) return;
     const T* x = static_cast<const T*>(a.x.data);
     T* rows = static_cast<T*>(a.rows.data);
-    const long long first = static_cast<long long>(blockIdx.x) * (pass * MOVES) + at.row, slots = a.tokens * a.chosen;
-    int token[MOVES];
-    Pack<T, VEC> v[MOVES];
+    const long long first = static_cast<long long>(blockIdx.x) * (pass * N) + at.row, slots = a.tokens * a.chosen;
+    int token[N];
+    Pack<T, VEC> v[N];
 #pragma unroll
-    for (int k = 0; k < MOVES; ++k) {
+    for (int k = 0; k < N; ++k) {
         const int slot = first + k * pass < slots ? a.order[first + k * pass] : -1;
         token[k] = slot < 0 ? -1 : slot / a.chosen;
     }
 #pragma unroll
-    for (int k = 0; k < MOVES; ++k) {
+    for (int k = 0; k < N; ++k) {
         v[k] = {};
         if (token[k] >= 0 && token[k] < a.tokens) v[k] = load<T, VEC>(x + token[k] * a.x.stride + at.c);
     }
 #pragma unroll
-    for (int k = 0; k < MOVES; ++k)
+    for (int k = 0; k < N; ++k)
         if (first + k * pass < slots) store<T, VEC>(rows + (first + k * pass) * a.rows.stride + at.c, v[k]);
 }
 
@@ -718,10 +718,14 @@ cudaError_t byExperts(int experts, F&& f)
 
 } // namespace
 
-// A thread per row. Measured against groups of lanes, us: choice of 2 of 64 experts for 131072 rows of half 18 / 24, of 8 of 64 49 / 38 (the keys' order costs
-// more than the groups' rounds), of 2 of 8 15 / 5 (groups of one lane), of 2 of 64 floats 31 / 31; adjoint, the mean of either kind of weights, 2
-// of 64 13 / 16, 8 of 256 48 / 75, 2 of 8 9 / 4; for 8192 rows 2 of 64 6 / 3.
-static bool chooseByThread(const RouteArgs& a) { return a.type != TYPE_FLOAT && a.tokens >= 16384 && a.experts >= 32 && a.experts <= ROWS_EXPERTS && a.chosen <= 2; }
+// A thread per row. Measured against groups of lanes, us: choice of 2 of 64 experts for 131072 rows of half 18 / 24, of 4 of 64 24 / 27, of 4 of 256 87 / 104,
+// of 8 of 64 49 / 38 (the keys' order costs more than the groups' rounds), of 2 of 8 15 / 5 (groups of one lane); of 1 and 2 of 64 floats, whose keys have 64
+// bits, 26 / 28 and 31 / 31, of 4 55 / 39. Adjoint, the mean of either kind of weights, 2 of 64 13 / 16, 8 of 256 48 / 75, 2 of 8 9 / 4; for 8192 rows 2 of 64
+// 6 / 3.
+static bool chooseByThread(const RouteArgs& a)
+{
+    return a.tokens >= 16384 && a.experts >= 32 && a.experts <= ROWS_EXPERTS && a.chosen <= (a.type == TYPE_FLOAT ? 2 : 4);
+}
 static bool adjointByThread(const RouteArgs& a) { return a.tokens >= 65536 && a.experts >= 32 && a.experts <= ROWS_EXPERTS && a.chosen <= ROWS_CHOSEN; }
 template <class F>
 static cudaError_t byChosen(int chosen, F&& f)
@@ -749,12 +753,16 @@ cudaError_t launchRouteForward(const RouteArgs& a, cudaStream_t stream)
     int* before = reinterpret_cast<int*>(static_cast<unsigned char*>(a.scratch) + p.before);
     cudaError_t e = byType(a.type, [&](auto t) {
         using T = decltype(t);
-        if constexpr (sizeof(T) == 2) {
-            if (!alone && vec && chooseByThread(a)) {
-                if (a.chosen == 1) launchChained(route_rows_kernel<T, 1>, p.tiles, 256, 32 * 1024, stream, 1, a, p.tokensPerTile, counts, p.tiles);
-                else launchChained(route_rows_kernel<T, 2>, p.tiles, 256, 32 * 1024, stream, 1, a, p.tokensPerTile, counts, p.tiles);
+        if (!alone && vec && chooseByThread(a)) {
+            auto go = [&](auto* kernel) {
+                launchChained(kernel, p.tiles, 256, 32 * 1024, stream, 1, a, p.tokensPerTile, counts, p.tiles);
                 return cudaGetLastError();
+            };
+            if (a.chosen == 1) return go(route_rows_kernel<T, 1>);
+            if constexpr (sizeof(T) == 2) {
+                if (a.chosen > 2) return go(route_rows_kernel<T, 4>);
             }
+            return go(route_rows_kernel<T, 2>);
         }
         return byExperts(a.experts, [&](auto l, auto per) {
             constexpr int LANES = decltype(l)::value, PER = decltype(per)::value;
@@ -814,11 +822,12 @@ cudaError_t launchDispatch(const ExchangeArgs& a, cudaStream_t stream)
     if (a.tokens == 0) return cudaSuccess;
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
-        const bool vec = wide(a.x, a.type, a.channels) && wide(a.rows, a.type, a.channels);
-        const AccessGrid g(a.tokens * a.chosen, a.channels, vec ? WIDE<T> : 1, MOVES);
-        if (vec) launchChained(dispatch_kernel<T, WIDE<T>>, g.blocks, 256, 0, stream, 1, a, g.perRow, g.pass);
-        else launchChained(dispatch_kernel<T, 1>, g.blocks, 256, 0, stream, 1, a, g.perRow, g.pass);
-        return cudaGetLastError();
+        return byAccess<T>({&a.x, &a.rows}, a.type, a.channels, [&](auto v) {
+            constexpr int VEC = decltype(v)::value;
+            const AccessGrid g(a.tokens * a.chosen, a.channels, VEC, MOVES);
+            launchChained(dispatch_kernel<T, VEC>, g.blocks, 256, 0, stream, 1, a, g.perRow, g.pass);
+            return cudaGetLastError();
+        });
     });
 }
 
@@ -831,6 +840,7 @@ static cudaError_t launchGather(const ExchangeArgs& a, const Rows& in, const Row
         return cudaGetLastError();
     };
     // about 4 loads on their way per thread
+    
     if (a.chosen == 1) return go(gather_sum_kernel<T, VEC, WEIGHTED, 4, 1>, 4);
     if (a.chosen == 2) return go(gather_sum_kernel<T, VEC, WEIGHTED, 2, 2>, 2);
     return go(gather_sum_kernel<T, VEC, WEIGHTED, 1, 4>, 1);
@@ -840,9 +850,10 @@ static cudaError_t launchGatherSum(const ExchangeArgs& a, const Rows& in, const 
     if (a.tokens == 0) return cudaSuccess;
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
-        if (wide(in, a.type, a.channels) && wide(out, a.type, a.channels))
-            return weighted ? launchGather<T, WIDE<T>, true>(a, in, out, stream) : launchGather<T, WIDE<T>, false>(a, in, out, stream);
-        return weighted ? launchGather<T, 1, true>(a, in, out, stream) : launchGather<T, 1, false>(a, in, out, stream);
+        return byAccess<T>({&in, &out}, a.type, a.channels, [&](auto v) {
+            constexpr int VEC = decltype(v)::value;
+            return weighted ? launchGather<T, VEC, true>(a, in, out, stream) : launchGather<T, VEC, false>(a, in, out, stream);
+        });
     });
 }
 cudaError_t launchDispatchAdjoint(const ExchangeArgs& a, cudaStream_t stream) { return launchGatherSum(a, a.gradRows, a.gradX, false, stream); }
@@ -853,7 +864,6 @@ cudaError_t launchCombineAdjoint(const ExchangeArgs& a, cudaStream_t stream)
     if (a.tokens == 0) return cudaSuccess;
     return byType(a.type, [&](auto t) {
         using T = decltype(t);
-        const bool vec = wide(a.rows, a.type, a.channels) && wide(a.gradX, a.type, a.channels) && wide(a.gradRows, a.type, a.channels);
         auto go = [&](auto v, auto g) {
             constexpr int VEC = decltype(v)::value, G = decltype(g)::value;
             const unsigned blocks = static_cast<unsigned>(std::min<long long>((a.tokens + 256 / G - 1) / (256 / G), a.numSMs * 8));
@@ -862,9 +872,9 @@ cudaError_t launchCombineAdjoint(const ExchangeArgs& a, cudaStream_t stream)
             else launchChained(combine_adjoint_kernel<T, VEC, G, 4>, blocks, 256, 0, stream, 1, a);
             return cudaGetLastError();
         };
-        if (vec) return a.channels <= 8 * WIDE<T> ? go(std::integral_constant<int, WIDE<T>>(), std::integral_constant<int, 8>())
-                                                  : go(std::integral_constant<int, WIDE<T>>(), std::integral_constant<int, 32>());
-        return a.channels <= 8 ? go(std::integral_constant<int, 1>(), std::integral_constant<int, 8>()) : go(std::integral_constant<int, 1>(), std::integral_constant<int, 32>());
+        return byAccess<T>({&a.rows, &a.gradX, &a.gradRows}, a.type, a.channels, [&](auto v) {
+            return a.channels <= 8 * decltype(v)::value ? go(v, std::integral_constant<int, 8>()) : go(v, std::integral_constant<int, 32>());
+        });
     });
 }
 

@@ -160,6 +160,18 @@ def test_embedding_layouts(qmlp):
     embedding_case(qmlp, huge, table, 1.0, rand(43, (5, 70), torch.float16))
 
 
+@pytest.mark.parametrize("dtype", FLOATS, ids=IDS.get)
+@pytest.mark.parametrize("channels", [2, 50, 49])
+def test_embedding_narrow_rows(qmlp, channels, dtype):
+    """rows that allow accesses of two elements or one; tables whose tokens are sorted in one pass and in two"""
+    for tokens, rows in ((3000, 700), (6000, 2000), (300, 40000)):
+        t = ints(48, (tokens,), -2, rows + 2)
+        embedding_case(qmlp, t, rand(49, (rows, channels), dtype), 0.5, rand(53, (tokens, channels), dtype))
+    wider = rand(54, (700, channels + 3), dtype)
+    for first in (1, 2):
+        embedding_case(qmlp, ints(55, (500,), 0, 700), wider[:, first:first + channels], 1.0, rand(56, (500, channels), dtype))
+
+
 def test_embedding_difference(qmlp):
     """linear in the table: the difference of two outputs is the output of the difference, and pairs with the gradient"""
     tokens, table, d, g = ints(44, (500,), 0, 40), rand(45, (40, 12)), rand(46, (40, 12)), rand(47, (500, 12))
@@ -269,7 +281,8 @@ def test_route_difference(qmlp):
 
 
 @pytest.mark.parametrize("dtype", FLOATS, ids=IDS.get)
-@pytest.mark.parametrize("rows,experts,k,channels", [(1, 4, 2, 8), (100, 3, 1, 1), (333, 8, 3, 17), (257, 64, 2, 256), (50, 16, 5, 1000), (40, 8, 8, 2049)])
+@pytest.mark.parametrize("rows,experts,k,channels", [(1, 4, 2, 8), (100, 3, 1, 1), (333, 8, 3, 17), (257, 64, 2, 256), (50, 16, 5, 1000), (40, 8, 8, 2049),
+                                                     (120, 5, 2, 50), (90, 4, 1, 6), (70, 9, 3, 270)])
 def test_exchange(qmlp, rows, experts, k, channels, dtype):
     z = rand(60, (rows, experts))
     z[ints(61, (rows, experts), 0, 3) == 0] = -INF       # slots without an expert
@@ -347,6 +360,21 @@ def test_expert_linear_ragged(qmlp, experts):
     rows = sum(counts)
     experts_case(qmlp, rand(111, (rows, 40), torch.float16), rand(112, (experts, 24, 40), torch.float16, 0.2), offsets_of(counts),
                  rand(113, (experts, 24), torch.float16), rand(114, (rows, 24), torch.float16))
+
+
+@pytest.mark.parametrize("n_in,n_out,bias", [(66, 264, True), (530, 12, False), (31, 200, True), (256, 136, True)])
+def test_expert_linear_mostly_empty(qmlp, n_in, n_out, bias):
+    """few rows among many experts: gradients of the others are zeros, whatever lay there, and their matrices are not read"""
+    experts, dtype = 150, torch.float16
+    counts = [0] * experts
+    counts[0], counts[70], counts[71], counts[149] = 2, 130, 1, 3
+    x, w, g = rand(111, (136, n_in), dtype), rand(112, (experts, n_out, n_in), dtype, n_in ** -0.5), rand(113, (136, n_out), dtype)
+    b = rand(114, (experts, n_out), dtype) if bias else None
+    experts_case(qmlp, x, w, offsets_of(counts), b, g)
+    empty = torch.tensor([c == 0 for c in counts], device="cuda")
+    leaves = [t.requires_grad_() for t in (x, torch.where(empty[:, None, None], float("nan"), w))]
+    dx, dw = torch.autograd.grad(qmlp.expert_linear(*leaves, offsets_of(counts)), leaves, g)
+    assert dx.isfinite().all() and dw.isfinite().all() and not dw[empty].any()
 
 
 def test_expert_linear_many(qmlp):
