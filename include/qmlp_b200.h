@@ -112,7 +112,7 @@ QMLP_API int qmlp_device_status(int* status);
 QMLP_API int qmlp_set_tuning(const char* key, int value);
 /* Per-kernel device timing: while enabled, every kernel the library launches is bracketed by a CUDA event pair on its
  * stream; qmlp_read_kernel_timing waits for the recorded launches, sums them per kernel (ids: the library's kernel
- * numbers, 100 = Adam, 101 = half-copy refresh) into the caller's arrays, forgets them and returns the number of
+ * numbers, 100 = Adam, 101 = half-copy refresh, 110 to 121 = the operators on feature rows, one record per call) into the caller's arrays, forgets them and returns the number of
  * distinct kernels. No counterpart in the reference (its only timing aid is the wall-clock script
  * tests_py/qmlp_tests/profile_network.py:168-188). */
 QMLP_API int qmlp_set_kernel_timing(int enabled);
