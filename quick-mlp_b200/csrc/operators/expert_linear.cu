@@ -21,7 +21,7 @@
 // sizes never travel to the host. 16 experts, 131072 rows, 1024 -> 1024 bfloat16: 200, 196 and 205 us for the three products, 3 us more
 // with the bias gradient (1.34 to 1.40 PFLOP/s; a library product of one matrix of that size 198 us, at clocks that the power limit holds
 // down; 128 x 256 tiles of single blocks 254, 239 and 346 us: their operands ask for more bytes a clock than shared memory has).
-// 512 experts, 1000003 rows, 64 -> 64 half: 49, 49 and 56 us, bound by memory (40 us each at the copy rate).
+// 512 experts, 1000003 rows, 64 -> 64 half: forward 52 us, bound by memory (40 us at the copy rate).
 // Waits are bounded: on a timeout the block drains, gives its tensor memory back and sets the library's status word.
 #include "common.cuh"
 
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
 // gradient, whose accumulator stays in tensor memory for as long as the block's rows belong to one expert. Blocks take consecutive tiles, an equal
 // share each. An expert whose tiles lie in several blocks leaves partial sums, at most two per block (the run a block begins with, if it began
 // before; the run it ends with, if it goes on), which a second kernel adds up in order.
-// Four warps add up dy's columns (the bias gradient) and write the weight gradients. 512 experts, 1000003 rows, 64 -> 64 half: 72 us and 5 us for
+// Four warps add up dy's columns (the bias gradient) and write the weight gradients. 512 experts, 1000003 rows, 64 -> 64 half: 73 us and 7 us for
 // the sums (apart: 49 us for the input gradient, 64 and 7 us for the others).
 template <int NB, int KB>   // boxes of 64 channels out, channels in
 struct NarrowLayout {
@@ -1105,7 +1105,7 @@ __global__ void __launch_bounds__(256) expert_narrow_join_kernel(const __grid_co
     const int expert = found;
     if (before[expert] >= end || before[expert] < begin) return;
     // Later blocks with a part of it: with tiles for all blocks every one up to that of its last tile, the first whose end, total * (b + 1) / blocks, reaches
-    // before[expert + 1]; with fewer tiles the one block of each tile. (16 parts read at a time; one expert of 298 rows, 24 -> 64, where a loop over
+    // before[expert + 1]; with fewer tiles the one block of each tile. (2 or 16 parts read at a time; one expert of 298 rows, 24 -> 64, where a loop over
     // all blocks divided for each, 38 us, so 5 us.)
     const bool full = total >= blocks;
     const int behind = before[expert + 1];
@@ -1115,19 +1115,24 @@ __global__ void __launch_bounds__(256) expert_narrow_join_kernel(const __grid_co
     if (n < p.sum && c < p.columns) {
         const float* from = p.partial + static_cast<long long>(n) * columns + c;
         float4 sum = *reinterpret_cast<const float4*>(from + (static_cast<long long>(block) * 2 + 1) * 128 * columns);   // the run that block ends with
-        for (int part = 0; part < more; part += 16) {                                                                    // the run the later ones begin with
-            float4 v[16];
+        int part = 0;                                                                                                    // the runs the later ones begin with
+        auto add = [&](auto count) {
+            constexpr int N = decltype(count)::value;
+            float4 v[N];
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
+            for (int k = 0; k < N; ++k)
                 v[k] = part + k < more ? *reinterpret_cast<const float4*>(from + static_cast<long long>(blockOf(part + k)) * 2 * 128 * columns) : float4{};
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
+            for (int k = 0; k < N; ++k) {
                 sum.x += v[k].x;
                 sum.y += v[k].y;
                 sum.z += v[k].z;
                 sum.w += v[k].w;
             }
-        }
+            part += N;
+        };
+        while (more - part >= 8) add(std::integral_constant<int, 16>());
+        while (part < more) add(std::integral_constant<int, 2>());
         const float f[4] = {sum.x, sum.y, sum.z, sum.w};
         T* out = static_cast<T*>(p.out) + (static_cast<long long>(expert) * p.sum + n) * p.columns + c;
         if (p.wideStore) store<T, 4>(out, pack<T, 4>(f));
