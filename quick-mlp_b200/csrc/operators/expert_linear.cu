@@ -630,6 +630,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(partial + c0 + i) = make_float4(v[h][i], v[h][i + 1], v[h][i + 2], v[h][i + 3]);
                         }
+                        __syncwarp();   // (the next load of tensor memory is the whole warp's)
                         continue;
                     }
                     if constexpr (MODE == FORWARD) {
@@ -703,6 +704,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) sum[j] = add2(sum[j], toPair(&v[i].v[2 * j]));
+                __syncwarp();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (thread == 0) barrierArrive(empty + stage * 8);
                 if (++stage == L::STAGES) stage = 0;
@@ -1046,27 +1048,29 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
                 tmemLoad32(from + pair * 64, v[0]);
                 tmemLoad32(from + pair * 64 + 32, v[1]);
                 tmemWait(v[0], v[1]);
-                if (n >= p.sum) continue;
+                if (n < p.sum) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c0 = pair * 64 + h * 32;
-                    if (!whole) {
-                        float* to = p.partial + (slot * 128 + n) * L::COLUMNS + c0;
+                    for (int h = 0; h < 2; ++h) {
+                        const int c0 = pair * 64 + h * 32;
+                        if (!whole) {
+                            float* to = p.partial + (slot * 128 + n) * L::COLUMNS + c0;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(v[h][i], v[h][i + 1], v[h][i + 2], v[h][i + 3]);
-                    } else {
-                        T* to = gradW + (static_cast<long long>(t.expert) * p.sum + n) * p.columns + c0;
-                        if (p.wideStore) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 8)
-                                if (c0 + i < p.columns) store<T, 8>(to + i, pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[h][i])));
+                            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(v[h][i], v[h][i + 1], v[h][i + 2], v[h][i + 3]);
                         } else {
+                            T* to = gradW + (static_cast<long long>(t.expert) * p.sum + n) * p.columns + c0;
+                            if (p.wideStore) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (c0 + i < p.columns) to[i] = Element<T>::from(v[h][i]);
+                                for (int i = 0; i < 32; i += 8)
+                                    if (c0 + i < p.columns) store<T, 8>(to + i, pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[h][i])));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (c0 + i < p.columns) to[i] = Element<T>::from(v[h][i]);
+                            }
                         }
                     }
                 }
+                __syncwarp();   // (the next load of tensor memory is the whole warp's)
             }
             fenceBefore();
             __syncwarp();
