@@ -86,11 +86,18 @@ std::tuple<Tensor, Tensor> layerNormForward(const Tensor& input, const OptTensor
     check(api.layer_norm_forward(&vx, &vw, &vb, static_cast<float>(epsilon), &vy, static_cast<float*>(stats.data_ptr()), currentStream()));
     return {y, stats};
 }
+// what the forward pass left: means and reciprocal deviations of the rows
+void checkStats(const Tensor& stats, const c10::SymInt& rows)
+{
+    if (stats.scalar_type() != torch::kFloat32 || stats.dim() != 2 || stats.sym_size(0) != 2 || stats.sym_size(1) != rows || !stats.is_contiguous())
+        raiseError("stats must be a contiguous float32 tensor (2, rows)");
+}
 std::tuple<Tensor, Tensor, Tensor> layerNormAdjoint(const Tensor& input, const Tensor& adjOutput, const OptTensor& weight, const OptTensor& bias, const Tensor& stats,
                                                     bool wantInput, bool wantWeight, bool wantBias)
 {
     const OnDevice on(input, adjOutput, weight, bias, stats);
     const Tensor x = asRows(input), g = asRows(adjOutput), w = contiguousOf(weight);
+    checkStats(stats, x.size(0));
     const bool haveWeight = wantWeight && w.defined(), haveBias = wantBias && bias.has_value() && bias->defined();
     Tensor dx = wantInput ? emptyLike(input) : Tensor(), dw = haveWeight ? emptyLike(w) : Tensor(), db = haveBias ? emptyLike(*bias) : Tensor();
     size_t bytes = 0;
@@ -535,9 +542,10 @@ std::tuple<Tensor, Tensor> layerNormForwardMeta(const Tensor& input, const OptTe
 {
     return {emptyOf(input, input.sym_sizes()), emptyOf(input, {2, rowsIn(input)}, torch::kFloat32)};
 }
-std::tuple<Tensor, Tensor, Tensor> layerNormAdjointMeta(const Tensor& input, const Tensor&, const OptTensor& weight, const OptTensor& bias, const Tensor&, bool wantInput,
+std::tuple<Tensor, Tensor, Tensor> layerNormAdjointMeta(const Tensor& input, const Tensor&, const OptTensor& weight, const OptTensor& bias, const Tensor& stats, bool wantInput,
                                                         bool wantWeight, bool wantBias)
 {
+    checkStats(stats, rowsIn(input));
     return {wantInput ? emptyOf(input, input.sym_sizes()) : nothing(input), wantWeight && weight.has_value() ? at::empty_like(*weight) : nothing(input),
             wantBias && bias.has_value() ? at::empty_like(*bias) : nothing(input)};
 }
