@@ -31,6 +31,7 @@ qmlp_tensor_t viewOf(const Tensor& t)
     qmlp_tensor_t v{};
     if (!t.defined()) return v;
     if (!t.is_cuda()) raiseError("tensor must live on a CUDA device");
+    if (t.dim() < 1 || t.dim() > 2) raiseError("only 1-D and 2-D tensors are supported");
     v.precision = precisionOf(t);
     v.data = t.data_ptr();
     v.ndim = static_cast<int>(t.dim());
@@ -68,6 +69,13 @@ struct ScratchMemory {
     }
     void* data() const { return bytes > 0 ? memory.data_ptr() : nullptr; }
 };
+// a parameter of a layer, if there is one: its dimensions, the last of them `channels` (no dimension would read as no parameter)
+void checkParameter(const OptTensor& t, int64_t dim, const c10::SymInt& channels, const char* name)
+{
+    if (!t.has_value() || !t->defined()) return;
+    if (t->dim() != dim) raiseError(std::string(name) + " has the wrong dimension, expected " + std::to_string(dim) + " but got " + std::to_string(t->dim()));
+    if (t->sym_size(-1) != channels) raiseError(std::string(name) + " has the wrong number of channels");
+}
 Tensor contiguousOf(const OptTensor& t) { return t.has_value() && t->defined() ? t->contiguous() : Tensor(); }
 Tensor emptyLike(const Tensor& t) { return at::empty(t.sizes(), t.options().memory_format(c10::MemoryFormat::Contiguous)); }
 Tensor emptyFloat(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, floatLike(like)); }
@@ -78,7 +86,10 @@ Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }   
 std::tuple<Tensor, Tensor> layerNormForward(const Tensor& input, const OptTensor& weight, const OptTensor& bias, double epsilon)
 {
     const OnDevice on(input, weight, bias);
-    const Tensor x = asRows(input), w = contiguousOf(weight), b = contiguousOf(bias);
+    const Tensor x = asRows(input);
+    checkParameter(weight, 1, x.size(1), "weight");
+    checkParameter(bias, 1, x.size(1), "bias");
+    const Tensor w = contiguousOf(weight), b = contiguousOf(bias);
     Tensor y = emptyLike(input), stats = emptyFloat({2, x.size(0)}, x);
     const Tensor rows = y.dim() == 2 ? y : y.view(x.sizes());
     const qmlp_tensor_t vx = viewOf(x), vw = viewOf(w), vb = viewOf(b);
@@ -97,6 +108,8 @@ std::tuple<Tensor, Tensor, Tensor> layerNormAdjoint(const Tensor& input, const T
 {
     const OnDevice on(input, adjOutput, weight, bias, stats);
     const Tensor x = asRows(input), g = asRows(adjOutput), w = contiguousOf(weight);
+    checkParameter(weight, 1, x.size(1), "weight");
+    checkParameter(bias, 1, x.size(1), "bias");
     checkStats(stats, x.size(0));
     const bool haveWeight = wantWeight && w.defined(), haveBias = wantBias && bias.has_value() && bias->defined();
     Tensor dx = wantInput ? emptyLike(input) : Tensor(), dw = haveWeight ? emptyLike(w) : Tensor(), db = haveBias ? emptyLike(*bias) : Tensor();
@@ -269,7 +282,9 @@ int* offsetsOf(const Tensor& offsets, const Tensor& weight)
 Tensor expertLinearForward(const Tensor& input, const Tensor& weight, const Tensor& offsets, const OptTensor& bias)
 {
     const OnDevice on(input, weight, offsets, bias);
-    const Tensor x = asRows(input), w = matricesOf(weight), b = contiguousOf(bias);
+    const Tensor x = asRows(input), w = matricesOf(weight);
+    checkParameter(bias, 2, weight.size(1), "bias");
+    const Tensor b = contiguousOf(bias);
     const int experts = static_cast<int>(weight.size(0));
     Tensor y = at::empty({x.size(0), weight.size(1)}, x.options().memory_format(c10::MemoryFormat::Contiguous));
     const qmlp_tensor_t vx = viewOf(x), vw = viewOf(w), vb = viewOf(b);
@@ -538,13 +553,17 @@ Tensor emptyOf(const Tensor& like, c10::SymIntArrayRef sizes) { return at::empty
 Tensor emptyOf(const Tensor& like, c10::SymIntArrayRef sizes, c10::ScalarType type) { return at::empty_symint(sizes, like.options().dtype(type)); }
 c10::SymInt rowsIn(const Tensor& t) { return t.sym_numel() / t.sym_size(-1); }
 
-std::tuple<Tensor, Tensor> layerNormForwardMeta(const Tensor& input, const OptTensor&, const OptTensor&, double)
+std::tuple<Tensor, Tensor> layerNormForwardMeta(const Tensor& input, const OptTensor& weight, const OptTensor& bias, double)
 {
+    checkParameter(weight, 1, input.sym_size(-1), "weight");
+    checkParameter(bias, 1, input.sym_size(-1), "bias");
     return {emptyOf(input, input.sym_sizes()), emptyOf(input, {2, rowsIn(input)}, torch::kFloat32)};
 }
 std::tuple<Tensor, Tensor, Tensor> layerNormAdjointMeta(const Tensor& input, const Tensor&, const OptTensor& weight, const OptTensor& bias, const Tensor& stats, bool wantInput,
                                                         bool wantWeight, bool wantBias)
 {
+    checkParameter(weight, 1, input.sym_size(-1), "weight");
+    checkParameter(bias, 1, input.sym_size(-1), "bias");
     checkStats(stats, rowsIn(input));
     return {wantInput ? emptyOf(input, input.sym_sizes()) : nothing(input), wantWeight && weight.has_value() ? at::empty_like(*weight) : nothing(input),
             wantBias && bias.has_value() ? at::empty_like(*bias) : nothing(input)};
@@ -570,7 +589,12 @@ std::tuple<Tensor, Tensor> combineAdjointMeta(const Tensor& rows, const Tensor&,
 {
     return {wantRows ? emptyOf(rows, rows.sym_sizes()) : nothing(rows), wantWeights ? emptyOf(weights, weights.sym_sizes()) : nothing(weights)};
 }
-Tensor expertLinearForwardMeta(const Tensor& input, const Tensor& weight, const Tensor&, const OptTensor&) { return emptyOf(input, {rowsIn(input), weight.sym_size(1)}); }
+Tensor expertLinearForwardMeta(const Tensor& input, const Tensor& weight, const Tensor&, const OptTensor& bias)
+{
+    if (weight.dim() != 3) raiseError("weight must be (experts, channels out, channels in)");
+    checkParameter(bias, 2, weight.sym_size(1), "bias");
+    return emptyOf(input, {rowsIn(input), weight.sym_size(1)});
+}
 std::tuple<Tensor, Tensor, Tensor> expertLinearAdjointMeta(const Tensor& input, const Tensor&, const Tensor& weight, const Tensor&, bool wantInput, bool wantWeight,
                                                            bool wantBias)
 {

@@ -22,3 +22,20 @@ def test_layer_norm_stats(error):
     for stats in (meta(2, 29), meta(60), meta(30, 2), meta(2, 30, dtype=torch.float16), meta(30, 2).t(), meta(2, 0)):
         with pytest.raises(error, match="stats"):
             adjoint(x, x, None, None, stats, True, False, False)
+
+
+def test_parameters_of_other_dimensions(error):
+    """a weight or bias of more dimensions than a view holds, or of none (which is not "no parameter"), or of another width"""
+    import qmlp
+    x, h = meta(4, 8), meta(4, 8, dtype=torch.float16)
+    for wrong in (meta(1, 1, 8), meta(1, 8), meta(1, 1, 1, 1, 1, 8), meta(), meta(7)):
+        for weight, bias in ((wrong, None), (None, wrong), (meta(8), wrong)):
+            with pytest.raises(error, match="wrong dimension|number of channels"):
+                qmlp.layer_norm(x, weight, bias)
+            with pytest.raises(error, match="wrong dimension|number of channels"):
+                torch.ops.qmlp_b200.layer_norm_adjoint(x, x, weight, bias, meta(2, 4), True, True, True)
+    matrices, offsets = meta(3, 5, 8, dtype=torch.float16), meta(4, dtype=torch.int32)
+    assert qmlp.expert_linear(h, matrices, offsets, meta(3, 5, dtype=torch.float16)).shape == (4, 5)
+    for wrong in (meta(), meta(5), meta(1, 3, 5), meta(3, 6)):
+        with pytest.raises(error, match="bias"):
+            qmlp.expert_linear(h, matrices, offsets, wrong.half())
