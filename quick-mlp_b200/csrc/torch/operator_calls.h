@@ -551,20 +551,27 @@ std::tuple<Tensor, Tensor, Tensor> expertLinearAdjointAutograd(const Tensor& inp
 // ---- shapes (meta tensors) ---------------------------------------------------------------------------------------------------
 Tensor emptyOf(const Tensor& like, c10::SymIntArrayRef sizes) { return at::empty_symint(sizes, like.options().memory_format(c10::MemoryFormat::Contiguous)); }
 Tensor emptyOf(const Tensor& like, c10::SymIntArrayRef sizes, c10::ScalarType type) { return at::empty_symint(sizes, like.options().dtype(type)); }
-c10::SymInt rowsIn(const Tensor& t) { return t.sym_numel() / t.sym_size(-1); }
+c10::SymInt rowsIn(const Tensor& t)
+{
+    if (t.dim() < 1) raiseError("a tensor of at least one dimension is needed");
+    if (t.sym_size(-1) == 0) raiseError("a tensor of at least one channel is needed");   // (a division by zero ends the process)
+    return t.sym_numel() / t.sym_size(-1);
+}
 
 std::tuple<Tensor, Tensor> layerNormForwardMeta(const Tensor& input, const OptTensor& weight, const OptTensor& bias, double)
 {
+    const c10::SymInt rows = rowsIn(input);
     checkParameter(weight, 1, input.sym_size(-1), "weight");
     checkParameter(bias, 1, input.sym_size(-1), "bias");
-    return {emptyOf(input, input.sym_sizes()), emptyOf(input, {2, rowsIn(input)}, torch::kFloat32)};
+    return {emptyOf(input, input.sym_sizes()), emptyOf(input, {2, rows}, torch::kFloat32)};
 }
 std::tuple<Tensor, Tensor, Tensor> layerNormAdjointMeta(const Tensor& input, const Tensor&, const OptTensor& weight, const OptTensor& bias, const Tensor& stats, bool wantInput,
                                                         bool wantWeight, bool wantBias)
 {
+    const c10::SymInt rows = rowsIn(input);
     checkParameter(weight, 1, input.sym_size(-1), "weight");
     checkParameter(bias, 1, input.sym_size(-1), "bias");
-    checkStats(stats, rowsIn(input));
+    checkStats(stats, rows);
     return {wantInput ? emptyOf(input, input.sym_sizes()) : nothing(input), wantWeight && weight.has_value() ? at::empty_like(*weight) : nothing(input),
             wantBias && bias.has_value() ? at::empty_like(*bias) : nothing(input)};
 }

@@ -39,3 +39,31 @@ def test_parameters_of_other_dimensions(error):
     for wrong in (meta(), meta(5), meta(1, 3, 5), meta(3, 6)):
         with pytest.raises(error, match="bias"):
             qmlp.expert_linear(h, matrices, offsets, wrong.half())
+
+
+def test_no_channels(error):
+    """rows without a channel, and a tensor without a dimension, are an error and no division by zero (in a process of its own)"""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, qmlp
+from qmlp._capi import QmlpError
+ops = torch.ops.qmlp_b200
+x, s = torch.empty((5, 0), device="meta"), torch.empty((), device="meta")
+h, w = x.half(), torch.empty((2, 3, 0), dtype=torch.float16, device="meta")
+o = torch.empty(3, dtype=torch.int32, device="meta")
+calls = [lambda: qmlp.layer_norm(x), lambda: qmlp.layer_norm(s), lambda: ops.layer_norm_adjoint(x, x, None, None, torch.empty((2, 5), device="meta"), True, False, False),
+         lambda: qmlp.expert_linear(h, w, o), lambda: ops.expert_linear_adjoint(h, torch.empty((5, 3), device="meta").half(), w, o, True, True, False)]
+for call in calls:
+    try:
+        call()
+    except QmlpError as e:
+        assert "at least one" in str(e), e
+    else:
+        raise AssertionError("not refused")
+print("fine")
+"""
+    package = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "quick-mlp_b200")
+    done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": package}, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "fine" in done.stdout, (done.returncode, done.stderr[-2000:])
