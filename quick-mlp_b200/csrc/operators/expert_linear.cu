@@ -1541,7 +1541,7 @@ cudaError_t forwardFewRows(const ExpertArgs& a, cudaStream_t stream)
     const bool vec = (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0 && a.channelsIn % 8 == 0;
     auto go = [&](auto* kernel, int width) {
         const int bytes = FEW_ROWS * ((a.channelsIn + 32 * width - 1) / (32 * width) * (32 * width)) * 4;
-        if (bytes > 48 * 1024) {
+        if (bytes > 47 * 1024) {   // (48 KB without asking, which the kernel's static shared memory counts towards)
             const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), 200 * 1024);
             if (e != cudaSuccess) return e;
         }

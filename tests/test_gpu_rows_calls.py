@@ -47,3 +47,28 @@ def test_parameters_of_other_dimensions(qmlp, error):
     for wrong in (b[0, 0], b[0], b[None], b[:, :4], b[:2]):
         with pytest.raises(error):
             qmlp.expert_linear(h, matrices, offsets, wrong)
+
+
+def test_expert_linear_few_rows_wide(qmlp):
+    """few rows of every width around the shared memory that a block has without asking, in ascending order and a process of its own: a wider
+    call before would have asked for it"""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, qmlp
+torch.manual_seed(0)
+for dtype in (torch.float16, torch.bfloat16):
+    for n_in in (2816, 2824, 2880, 2944, 3041, 3056, 3064, 3071, 3080, 3328):
+        for rows in (1, 5):
+            x, w = (torch.randint(-2, 3, s, device="cuda").to(dtype) for s in ((rows, n_in), (3, 24, n_in)))
+            for first in (0, 1):     # 16-byte and single accesses
+                w = torch.randint(-2, 3, (3 * 24 * n_in + 1,), device="cuda").to(dtype)[first:first + 3 * 24 * n_in].view(3, 24, n_in)
+                y = qmlp.expert_linear(x, w, torch.tensor([0, 1, 1, rows], dtype=torch.int32, device="cuda"))
+                exact = torch.cat([x[:1].double() @ w[0].double().T, x[1:].double() @ w[2].double().T])
+                assert torch.equal(y, exact.to(dtype)), (n_in, rows, first)
+print("fine")
+"""
+    package = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "quick-mlp_b200")
+    done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": package}, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
