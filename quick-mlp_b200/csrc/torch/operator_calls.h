@@ -264,7 +264,7 @@ std::tuple<Tensor, Tensor> combineAdjoint(const Tensor& rows, const Tensor& adjO
     const qmlp_tensor_t vy = viewOf(y), vg = viewOf(g);
     qmlp_tensor_t vd = viewOf(dy);
     check(api.combine_adjoint(&vy, &vg, &r, &vd, wantWeights ? static_cast<float*>(dw.data_ptr()) : nullptr, currentStream()));
-    return {wantRows ? dy : nothing(rows), wantWeights ? dw : nothing(weights)};
+    return {wantRows ? dy.view(rows.sizes()) : nothing(rows), wantWeights ? dw : nothing(weights)};
 }
 
 // ---- products grouped by expert ----------------------------------------------------------------------------------------------

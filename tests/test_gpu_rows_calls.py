@@ -72,3 +72,27 @@ print("fine")
     package = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "quick-mlp_b200")
     done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": package}, capture_output=True, text=True, timeout=600)
     assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float", "bfloat16"])
+def test_leading_dimensions(qmlp, dtype):
+    """rows of more than two dimensions, (experts, capacity, channels) say: every operator's gradient has the shape of what it is a gradient of, and is the
+    flat call's"""
+    r = qmlp.route(rand(10, (30, 6)), 2)
+    w = r.weights.clone().requires_grad_()
+    y, x, g, gx = rand(11, (6, 10, 16), dtype), rand(12, (5, 6, 16), dtype), rand(13, (30, 16), dtype), rand(14, (60, 16), dtype)
+    got, want = [], []
+    for shape, out in ((lambda t: t, got), (lambda t: t.reshape(-1, 16), want)):
+        rows, inputs = shape(y).clone().requires_grad_(), shape(x).clone().requires_grad_()
+        back, sent = qmlp.combine(rows, r._replace(weights=w)), qmlp.dispatch(inputs, r)
+        grads = torch.autograd.grad([back, sent], [rows, w, inputs], [g, gx])
+        assert grads[0].shape == rows.shape and grads[2].shape == inputs.shape
+        out += [back.detach(), sent.detach(), *(t.reshape(-1, t.shape[-1]) for t in grads)]
+        only, = torch.autograd.grad(qmlp.combine(rows, r), [rows], g)
+        assert only.shape == rows.shape and torch.equal(only, grads[0])
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+    if dtype != torch.float32:
+        h, weight, offsets = rand(15, (4, 15, 16), dtype).requires_grad_(), rand(16, (6, 24, 16), dtype).requires_grad_(), r.offsets
+        dh, dw = torch.autograd.grad(qmlp.expert_linear(h, weight, offsets), [h, weight], rand(17, (60, 24), dtype))
+        assert dh.shape == h.shape and dw.shape == weight.shape
