@@ -337,6 +337,14 @@ variable_list once(const char* op, variable_list results, std::vector<Tensor> so
     if (!torch::GradMode::is_enabled() || wanted.empty()) return results;
     return OnceFunction::apply(std::string(op), results, at::TensorList(wanted));
 }
+// The operators have no forward-mode formula. A dual tensor, which torch.func.jvp makes too, is refused: below autograd its tangent would be lost.
+bool hasTangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool hasTangent(const OptTensor& t) { return t.has_value() && hasTangent(*t); }
+template <class... T>
+void refuseTangents(const char* op, const T&... tensors)
+{
+    if ((hasTangent(tensors) || ...)) raiseError(std::string("qmlp_b200::") + op + " has no forward-mode derivative");
+}
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
@@ -360,6 +368,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
 };
 std::tuple<Tensor, Tensor> layerNormForwardAutograd(const Tensor& input, const OptTensor& weight, const OptTensor& bias, double epsilon)
 {
+    refuseTangents("layer_norm_forward", input, weight, bias);
     if (wantsNode(input, weight, bias)) {
         auto r = LayerNormFunction::apply(input, weight, bias, epsilon);
         return {r[0], r[1]};
@@ -370,6 +379,7 @@ std::tuple<Tensor, Tensor> layerNormForwardAutograd(const Tensor& input, const O
 std::tuple<Tensor, Tensor, Tensor> layerNormAdjointAutograd(const Tensor& input, const Tensor& adjOutput, const OptTensor& weight, const OptTensor& bias,
                                                             const Tensor& stats, bool wantInput, bool wantWeight, bool wantBias)
 {
+    refuseTangents("layer_norm_adjoint", input, adjOutput, weight, bias);
     variable_list r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -397,12 +407,14 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
 };
 Tensor embeddingForwardAutograd(const Tensor& tokens, const Tensor& table, double scale)
 {
+    refuseTangents("embedding_forward", table);
     if (wantsNode(table)) return EmbeddingFunction::apply(tokens, table, scale);
     at::AutoDispatchBelowADInplaceOrView below;
     return QMLP_CALL("embedding_forward", embeddingForward).call(tokens, table, scale);
 }
 Tensor embeddingAdjointAutograd(const Tensor& tokens, const Tensor& adjOutput, int64_t rows, double scale)
 {
+    refuseTangents("embedding_adjoint", adjOutput);
     variable_list r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -432,6 +444,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
 };
 RouteResult routeForwardAutograd(const Tensor& logits, int64_t chosen, bool normalize)
 {
+    refuseTangents("route_forward", logits);
     if (wantsNode(logits)) {
         auto r = RouteFunction::apply(logits, chosen, normalize);
         return {r[0], r[1], r[2], r[3], r[4]};
@@ -441,6 +454,7 @@ RouteResult routeForwardAutograd(const Tensor& logits, int64_t chosen, bool norm
 }
 Tensor routeAdjointAutograd(const Tensor& logits, bool normalize, const Tensor& weights, const Tensor& experts, const Tensor& adjWeights)
 {
+    refuseTangents("route_adjoint", logits, weights, adjWeights);
     variable_list r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -465,12 +479,14 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
 };
 Tensor dispatchForwardAutograd(const Tensor& input, const Tensor& order, const Tensor& positions)
 {
+    refuseTangents("dispatch_forward", input);
     if (wantsNode(input)) return DispatchFunction::apply(input, order, positions);
     at::AutoDispatchBelowADInplaceOrView below;
     return QMLP_CALL("dispatch_forward", dispatchForward).call(input, order, positions);
 }
 Tensor dispatchAdjointAutograd(const Tensor& adjRows, const Tensor& positions)
 {
+    refuseTangents("dispatch_adjoint", adjRows);
     variable_list r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -496,6 +512,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
 };
 Tensor combineForwardAutograd(const Tensor& rows, const Tensor& weights, const Tensor& order, const Tensor& positions)
 {
+    refuseTangents("combine_forward", rows, weights);
     if (wantsNode(rows, weights)) return CombineFunction::apply(rows, weights, order, positions);
     at::AutoDispatchBelowADInplaceOrView below;
     return QMLP_CALL("combine_forward", combineForward).call(rows, weights, order, positions);
@@ -503,6 +520,7 @@ Tensor combineForwardAutograd(const Tensor& rows, const Tensor& weights, const T
 std::tuple<Tensor, Tensor> combineAdjointAutograd(const Tensor& rows, const Tensor& adjOutput, const Tensor& weights, const Tensor& order, const Tensor& positions,
                                                   bool wantRows, bool wantWeights)
 {
+    refuseTangents("combine_adjoint", rows, adjOutput, weights);
     variable_list r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -531,6 +549,7 @@ struct ExpertLinearFunction : torch::autograd::Function<ExpertLinearFunction> {
 };
 Tensor expertLinearForwardAutograd(const Tensor& input, const Tensor& weight, const Tensor& offsets, const OptTensor& bias)
 {
+    refuseTangents("expert_linear_forward", input, weight, bias);
     if (wantsNode(input, weight, bias)) return ExpertLinearFunction::apply(input, weight, offsets, bias);
     at::AutoDispatchBelowADInplaceOrView below;
     return QMLP_CALL("expert_linear_forward", expertLinearForward).call(input, weight, offsets, bias);
@@ -538,6 +557,7 @@ Tensor expertLinearForwardAutograd(const Tensor& input, const Tensor& weight, co
 std::tuple<Tensor, Tensor, Tensor> expertLinearAdjointAutograd(const Tensor& input, const Tensor& adjOutput, const Tensor& weight, const Tensor& offsets, bool wantInput,
                                                                bool wantWeight, bool wantBias)
 {
+    refuseTangents("expert_linear_adjoint", input, adjOutput, weight);
     variable_list r;
     {
         at::AutoDispatchBelowADInplaceOrView below;

@@ -67,3 +67,39 @@ print("fine")
     package = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "quick-mlp_b200")
     done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": package}, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "fine" in done.stdout, (done.returncode, done.stderr[-2000:])
+
+
+def test_forward_mode(error):
+    """The operators have no forward-mode formula: a tangent is refused, whether or not a gradient is asked for, and never dropped."""
+    import torch.autograd.forward_ad as fwad
+    import qmlp
+    half = torch.float16
+    tokens, ints = meta(5, dtype=torch.int64), meta(12, dtype=torch.int32)
+    positions, offsets = meta(6, 2, dtype=torch.int32), meta(4, dtype=torch.int32)
+    r = qmlp.Routing(meta(6, 2), positions, ints, positions, offsets)
+    ops = torch.ops.qmlp_b200
+    calls = [   # a call of its differentiable arguments, and these
+        (lambda x, w, b: qmlp.layer_norm(x, w, b), [meta(6, 8), meta(8), meta(8)]),
+        (lambda t: qmlp.embedding(tokens, t), [meta(9, 8)]),
+        (lambda z: qmlp.route(z, 2).weights, [meta(6, 3)]),
+        (lambda x: qmlp.dispatch(x, r), [meta(6, 8)]),
+        (lambda y, w: qmlp.combine(y, r._replace(weights=w)), [meta(12, 8), meta(6, 2)]),
+        (lambda x, w, b: qmlp.expert_linear(x, w, offsets, b), [meta(12, 8, dtype=half), meta(3, 4, 8, dtype=half), meta(3, 4, dtype=half)]),
+        (lambda x, g: ops.layer_norm_adjoint(x, g, None, None, meta(2, 6), True, False, False)[0], [meta(6, 8), meta(6, 8)]),
+        (lambda g: ops.embedding_adjoint(tokens, g, 9, 1.0), [meta(5, 8)]),
+        (lambda z, w, g: ops.route_adjoint(z, True, w, positions, g), [meta(6, 3), meta(6, 2), meta(6, 2)]),
+        (lambda g: ops.dispatch_adjoint(g, positions), [meta(12, 8)]),
+        (lambda y, g, w: ops.combine_adjoint(y, g, w, ints, positions, True, True)[0], [meta(12, 8), meta(6, 8), meta(6, 2)]),
+        (lambda x, g, w: ops.expert_linear_adjoint(x, g, w, offsets, True, True, True)[0], [meta(12, 8, dtype=half), meta(12, 4, dtype=half), meta(3, 4, 8, dtype=half)]),
+    ]
+    for n, (call, args) in enumerate(calls):
+        call(*args)
+        for i, a in enumerate(args):
+            for leaf in (a, a.clone().requires_grad_()):
+                with fwad.dual_level(), pytest.raises(error, match="forward-mode"):
+                    call(*args[:i], fwad.make_dual(leaf, torch.empty_like(a)), *args[i + 1:])
+                    print("not refused:", n, i)
+            with fwad.dual_level(), torch.no_grad(), pytest.raises(error, match="forward-mode"):
+                call(*args[:i], fwad.make_dual(a, torch.empty_like(a)), *args[i + 1:])
+        with pytest.raises(error, match="forward-mode"):
+            torch.func.jvp(call, tuple(args), tuple(torch.empty_like(a) for a in args))
