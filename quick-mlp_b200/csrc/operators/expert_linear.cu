@@ -201,11 +201,11 @@ struct ProductArgs {
     void* out;
     long long outStride;          // elements between rows of D in memory
     const void* bias;             // forward: (experts, columns) or null
-    int2* plan;                   // weights: first item and items of an expert, written for the join; null where no expert can have two
-    float* partial;               // weights: items x tiles x 128 x BN sums of experts with more than one item
+    int2* plan;                   // weights: first slot and items of an expert, written for the join; null where no expert can have two
+    float* partial;               // weights: slots x tiles x tileRows x BN sums; the items of experts with more than one have a slot each
     int* status;
     void* gradBias;               // weights: (experts, channels out) or null
-    float* partialBias;           // weights: items x tiles of rows x tileRows sums of experts with more than one item
+    float* partialBias;           // weights: slots x channels out sums
     bool wideStore;               // rows of D can be written 16 bytes at a time
 };
 
@@ -292,10 +292,10 @@ __device__ __forceinline__ void planExperts(const ProductArgs& p, int* bounds, i
     // (the caller's barrier follows)
 }
 
-// One tile of D: its expert (-1: no tile), the unit it belongs to, the expert's units, the run of rows it reads (forward, input: its own rows)
+// One tile of D: its expert (-1: no tile), the slot of its partial sums if the expert has several units, the expert's units, the run of rows it reads (forward, input: its own rows)
 // and where it lies.
 struct Tile {
-    int expert, item, units, begin, end, row, column;
+    int expert, slot, units, begin, end, row, column;
 };
 // Walks the tiles of a block or pair of blocks: one of every round, from alternating ends, so that with the longest first the shares come out
 // even; rounds `round`, `round` + `stride`, ... All threads of a warp call next() together: 32 experts are looked at in one step.
@@ -304,7 +304,7 @@ struct Walk {
     const ProductArgs* args;
     const int *bounds, *before, *order;   // planExperts
     long long total;
-    int perUnit, round, stride, at = 0;   // at: place in `order` (the expert itself without one)
+    int perUnit, round, stride, at = 0, singles = 0;   // at: place in `order` (the expert itself without one); singles: experts of one unit in front of it
     __device__ __forceinline__ Walk(const ProductArgs& p, const int* rows, const int* units, const int* list, int first, int step)
         : args(&p), bounds(rows), before(units), order(MODE == WEIGHTS ? list : nullptr), round(first), stride(step)
     {
@@ -327,13 +327,15 @@ struct Walk {
         const int lane = threadIdx.x & 31;
         for (;;) {   // first expert whose units reach behind `unit`
             const int i = at + 1 + lane;
-            const unsigned passed = __ballot_sync(0xffffffffu, i <= p.experts && before[i] <= unit);
+            const bool behind = i <= p.experts && before[i] <= unit;
+            const unsigned passed = __ballot_sync(0xffffffffu, behind);
+            if constexpr (MODE == WEIGHTS) singles += __popc(__ballot_sync(0xffffffffu, behind && before[i] - before[i - 1] == 1));
             at += __popc(passed);
             if (passed != 0xffffffffu) break;
         }
         t.expert = order != nullptr ? order[at] : at;
         const int first = bounds[t.expert], last = bounds[t.expert + 1];
-        t.item = unit;
+        t.slot = unit - singles;
         t.units = before[at + 1] - before[at];
         const int part = unit - before[at];
         if constexpr (MODE == WEIGHTS) {
@@ -457,8 +459,6 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     if constexpr (CTAS > 1) clusterSync();   // the other block's barriers are set
     fenceAfter();
     const uint32_t tmem = *tmemBase;
-    if (MODE == WEIGHTS && p.plan != nullptr && blockIdx.x == 0)   // for the kernel that joins the partial sums
-        for (int i = threadIdx.x; i < p.experts; i += blockThreads(SUMS)) p.plan[order != nullptr ? order[i] : i] = make_int2(before[i], before[i + 1] - before[i]);
     Walk<MODE, BN, CTAS> walk(p, bounds, before, order, 0, 1);
     Tile t;
 
@@ -577,6 +577,15 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
         const uint32_t released = CTAS == 1 ? accEmpty + group * 8 : inBlock(accEmpty + group * 8, 0);
         T* out = static_cast<T*>(p.out);
         uint32_t accPhase = 0;
+        if (MODE == WEIGHTS && p.plan != nullptr && blockIdx.x == 0 && warp == 2) {   // for the kernel that joins the partial sums
+            int singles = 0;
+            for (int i = lane; i - lane < p.experts; i += 32) {
+                const int units = i < p.experts ? before[i + 1] - before[i] : 0;
+                const unsigned single = __ballot_sync(0xffffffffu, units == 1);
+                if (i < p.experts) p.plan[order != nullptr ? order[i] : i] = make_int2(before[i] - singles - __popc(single & ((1u << lane) - 1)), units);
+                singles += __popc(single);
+            }
+        }
         if constexpr (MODE == WEIGHTS) {
             // the gradients of experts without rows, while the first products run (as tiles without products: 431 experts of 66 -> 760, 19 rows, 40 us;
             // so 22 us)
@@ -610,8 +619,8 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
             const bool split = MODE == WEIGHTS && t.units > 1;
             float* partial = nullptr;
             if constexpr (MODE == WEIGHTS) {
-                const long long item = t.item, tileAt = static_cast<long long>(t.row / (BM * CTAS)) * p.columnTiles + t.column / BN;
-                partial = p.partial + ((item * p.rowTiles * p.columnTiles + tileAt) * (BM * CTAS) + rank * BM + quarter * 32 + lane) * BN;
+                const long long slot = t.slot, tileAt = static_cast<long long>(t.row / (BM * CTAS)) * p.columnTiles + t.column / BN;
+                partial = p.partial + ((slot * p.rowTiles * p.columnTiles + tileAt) * (BM * CTAS) + rank * BM + quarter * 32 + lane) * BN;
             }
             // 64 columns of the accumulator at a time, 32 through shared memory
 #pragma unroll
@@ -718,7 +727,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                 }
                 const int channel = tileRow + chunk * 8 + first;
                 if (channel < p.sum) {
-                    if (t.units > 1) p.partialBias[static_cast<long long>(t.item) * p.sum + channel] = mine;
+                    if (t.units > 1) p.partialBias[static_cast<long long>(t.slot) * p.sum + channel] = mine;
                     else static_cast<T*>(p.gradBias)[static_cast<long long>(t.expert) * p.sum + channel] = Element<T>::from(mine);
                 }
             }
@@ -1162,10 +1171,10 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
     constexpr int ROWS = JOIN_ELEMENTS / BN;
     const int tiles = p.rowTiles * p.columnTiles;
     const int expert = blockIdx.x / tiles, tile = blockIdx.x % tiles;
-    const int before = p.plan[expert].x, units = p.plan[expert].y;
+    const int slot = p.plan[expert].x, units = p.plan[expert].y;
     if (units < 2) return;
     const long long unitStride = static_cast<long long>(tiles) * p.tileRows * BN;
-    const float* from = p.partial + before * unitStride + static_cast<long long>(tile) * p.tileRows * BN;
+    const float* from = p.partial + slot * unitStride + static_cast<long long>(tile) * p.tileRows * BN;
     const int row0 = tile / p.columnTiles * p.tileRows, column0 = tile % p.columnTiles * BN;
     for (int i = threadIdx.x; i < JOIN_ELEMENTS / 4; i += 256) {
         const int r = blockIdx.y * ROWS + i / (BN / 4), c = i % (BN / 4) * 4;
@@ -1191,7 +1200,7 @@ __global__ void __launch_bounds__(256) expert_join_kernel(const __grid_constant_
             if (channel >= p.sum || blockIdx.y * ROWS + r >= p.tileRows) break;
             float sum = 0.f;
 #pragma unroll 4
-            for (int u = 0; u < units; ++u) sum += p.partialBias[static_cast<long long>(before + u) * p.sum + channel];
+            for (int u = 0; u < units; ++u) sum += p.partialBias[static_cast<long long>(slot + u) * p.sum + channel];
             static_cast<T*>(p.gradBias)[static_cast<long long>(expert) * p.sum + channel] = Element<T>::from(sum);
         }
     }
@@ -1425,7 +1434,11 @@ Shape weightShape(const ExpertArgs& a) { return shapeOf(a.channelsOut > 128 ? 51
 // Rows per item of the weight gradient. Cutting an expert's rows fills the blocks where its tiles alone do not, at the price of a write and
 // a read of an fp32 tile per item. The estimate below weighs the two for runs of average length: a step of 64 rows takes about 0.3 us
 // (256 x 256 tiles at the tensor core's rate, narrow ones at the memory's), partial sums move at about 5 TB/s. 64 experts of 4096 rows of
-// 256 x 256: whole runs 49 us, cut into 320 items 74 us and 44 us for their sums. An expert with more than twice the average is cut in any case.
+// 256 x 256: whole runs 49 us, cut into 320 items 74 us and 44 us for their sums. An expert with more than twice the average is cut in any case, or with
+// more than a quarter of a block's share of all steps where that is later: every item that may be cut wants an fp32 tile of scratch, and with the shares
+// in mind their number goes with the blocks (8 tiles of a block and no more, 150 MB), not with the experts. 65536 rows are cut in any case: tensor
+// memory cuts its sums off instead of rounding them, and a sum of one sign comes out too small, by 1.0e-4 of itself over 16384 rows and 3.9e-4, less than
+// half a unit of half's last place, over 65536.
 int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
 {
     const double run = static_cast<double>(a.rows) / a.experts;
@@ -1439,8 +1452,8 @@ int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
             pieces = k;
         }
     }
-    const double rows = pieces == 1 ? 2 * run : run / pieces;
-    return static_cast<int>(std::min<double>(std::max<double>(std::ceil(rows / BK) * BK, 512), 1 << 30));
+    const double rows = pieces == 1 ? run * std::max(2.0, static_cast<double>(a.experts) * tiles / blocks / 4) : run / pieces;
+    return static_cast<int>(std::min<double>(std::max<double>(std::ceil(rows / BK) * BK, 512), 1 << 16));
 }
 
 // scratch: [x | weight | dy in a form the TMA reads, where needed | partial sums of the weight and bias gradients | their plan]
@@ -1477,10 +1490,11 @@ struct Scratch {
             plan = take(true, (static_cast<size_t>(a.experts) + 1) * 4);
             return;
         }
-        const size_t items = a.rows > chunk ? a.experts + rows / chunk : 0;
-        partial = take(weights, items * tiles * tileRows * shape.width * 4);
-        partialBias = take(weights, items * a.channelsOut * 4);
-        plan = take(weights && items > 0, static_cast<size_t>(a.experts) * sizeof(int2));
+        // slots: items of the runs that are cut, which have at least chunk + 1 rows each
+        const size_t cut = std::min<size_t>(a.experts, rows / (static_cast<size_t>(chunk) + 1)), slots = cut > 0 ? rows / chunk + cut : 0;
+        partial = take(weights, slots * tiles * tileRows * shape.width * 4);
+        partialBias = take(weights, slots * a.channelsOut * 4);
+        plan = take(weights && slots > 0, static_cast<size_t>(a.experts) * sizeof(int2));
     }
 };
 

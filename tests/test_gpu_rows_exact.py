@@ -45,3 +45,34 @@ def experts_exact(qmlp, counts, n_in, n_out, dtype, wanted=("x", "weight", "bias
 def test_expert_linear_lanes(qmlp, counts, n_in, n_out, dtype):
     """channels out that leave a warp of the gradients' epilogues with some of its lanes, before and between reads of tensor memory; runs that are cut"""
     experts_exact(qmlp, counts, n_in, n_out, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=IDS.get)
+@pytest.mark.parametrize("experts", [60, 700])
+def test_expert_linear_slots(qmlp, experts, dtype):
+    """cut runs between whole and empty ones, in order of length (up to 512 experts) and not: each finds the partial sums that are its own"""
+    counts = [0] * experts
+    for i, n in enumerate((3, 1700, 0, 1, 2100, 5, 40, 0, 5000, 512, 513, 511, 2100, 64, 1025)):
+        counts[i * 4 + i % 3] = n
+    counts[-1] = 3000
+    experts_exact(qmlp, counts, 200, 136, dtype)
+    experts_exact(qmlp, counts, 136, 40, dtype, ("weight",))
+
+
+def test_expert_linear_scratch(qmlp):
+    """the scratch of a weight gradient follows the runs that can be cut: no copy of all matrices"""
+    import ctypes as C
+    from qmlp import _capi
+    lib = _capi.lib()
+
+    def matrix(rows, channels):
+        t = _capi.Tensor(data=1 << 20, precision=_capi.QMLP_HALF, ndim=2)     # (the pointers are not followed)
+        t.sizes[0], t.sizes[1], t.strides[0], t.strides[1] = rows, channels, channels, 1
+        return C.byref(t)
+
+    for rows, experts, n_in, n_out in ((131072, 512, 1024, 1024), (131072, 256, 2048, 2048), (600, 256, 1024, 4096), (131072, 512, 1024, 4096), (1 << 20, 2048, 512, 512),
+                                       (2000, 2048, 1024, 1024)):
+        size = C.c_size_t()
+        assert lib.qmlp_expert_linear_adjoint_memory(matrix(rows, n_in), matrix(rows, n_out), matrix(experts * n_out, n_in), experts, _capi.GRADIENTS_INPUT | _capi.GRADIENTS_NETWORK_WEIGHTS,
+                                                     C.byref(size)) == 0
+        assert size.value < 2 * experts * n_in * n_out / 4, (experts, size.value)
