@@ -214,11 +214,17 @@ __device__ __forceinline__ int clampOffset(const ProductArgs& p, int e)
 {
     return static_cast<int>(max(0ll, min(p.rows, static_cast<long long>(p.offsets[e]))));
 }
+// pieces of at most `piece` rows that `rows` rows fill, and the end of one that begins at `begin` (a sum of rows and a piece can pass 31 bits)
+__host__ __device__ constexpr int piecesOf(int rows, int piece) { return rows > 0 ? (rows - 1) / piece + 1 : 0; }
+__host__ __device__ constexpr int pieceEnd(int begin, int piece, int last) { return last - begin > piece ? begin + piece : last; }
+constexpr int MOST_ROWS = 0x7fffffff - 4095;   // what the entry points let pass
+static_assert(piecesOf(MOST_ROWS, 1 << 16) == 1 << 15 && piecesOf(MOST_ROWS, 1 << 30) == 2 && piecesOf(1, 128) == 1 && piecesOf(128, 128) == 1 && piecesOf(0, 128) == 0, "");
+static_assert(pieceEnd(MOST_ROWS - 10, 1 << 16, MOST_ROWS) == MOST_ROWS && pieceEnd(5, 128, 300) == 133 && pieceEnd(172, 128, 300) == 300 && pieceEnd(173, 128, 300) == 300, "");
 // units of work along `rows` rows of an expert
 template <int MODE>
 __device__ __forceinline__ int unitsOf(const ProductArgs& p, int rows)
 {
-    return MODE == WEIGHTS ? (rows + p.chunk - 1) / p.chunk : (rows + p.tileRows - 1) / p.tileRows;
+    return piecesOf(rows, MODE == WEIGHTS ? p.chunk : p.tileRows);
 }
 // The experts' runs and units of work, for all threads of a block: bounds[e] = first row of expert e, bounds[experts] the end of the last one;
 // before[i] = units of the experts in front of the i-th in `order`. The weight product takes the longest runs first (up to SORTED_MAX
@@ -341,12 +347,12 @@ struct Walk {
         if constexpr (MODE == WEIGHTS) {
             const int row = within / p.columnTiles;
             t.begin = first + part * p.chunk;
-            t.end = min(last, t.begin + p.chunk);
+            t.end = pieceEnd(t.begin, p.chunk, last);
             t.row = row * (BM * CTAS);
             t.column = (within - row * p.columnTiles) * BN;
         } else {
             t.begin = first + part * (BM * CTAS);
-            t.end = min(last, t.begin + BM * CTAS);
+            t.end = pieceEnd(t.begin, BM * CTAS, last);
             t.row = t.begin;
             t.column = within * BN;
         }
@@ -799,7 +805,7 @@ struct NarrowWalk {
         const int from = before[expert], to = before[expert + 1];
         t.expert = expert;
         t.begin = bounds[expert] + (tile - from) * BM;
-        t.end = min(bounds[expert + 1], t.begin + BM);
+        t.end = pieceEnd(t.begin, BM, bounds[expert + 1]);
         t.first = tile == from || tile == firstTile;
         t.last = tile == to - 1 || tile == end - 1;
         t.entered = from < firstTile;
