@@ -375,6 +375,21 @@ __device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, volatile in
     return ok;
 }
 
+// Where the warp that issues copies has stopped. When a warp of the block has given up, whichever it was, the copies that are still on their way
+// land (or are waited for to the limit) before the block's shared memory is given back.
+struct InFlight {
+    uint32_t stage = 0, phase = 0, tailPhase = 0, tail = 0;
+    int count = 0;
+    __device__ __forceinline__ void land(uint32_t full, uint32_t stages)
+    {
+        for (; count > 0; --count) {
+            if (stage == 0) { stage = stages; phase ^= 1; }
+            --stage;
+            barrierWait(full + stage * 8, phase);
+        }
+    }
+};
+
 // barrier over the four warps that sum, with the conjunction of their answers
 __device__ __forceinline__ bool sumWarpsAgree(bool answer)
 {
@@ -467,6 +482,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     const uint32_t tmem = *tmemBase;
     Walk<MODE, BN, CTAS> walk(p, bounds, before, order, 0, 1);
     Tile t;
+    InFlight copies;   // of warp 0
 
     if (warp == 0) {
         // ---- operands -------------------------------------------------------------------------------------------------
@@ -510,7 +526,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                 }
                 if constexpr (MODE == WEIGHTS && CTAS > 1) {
                     if (tail > 0) {
-                        if (!await(bar, tailPhase, failed)) { ok = false; break; }
+                        if (!await(bar, tailPhase, failed)) { copies.tail = 1; ok = false; break; }
                         tailPhase ^= 1;
                         for (int i = lane; i < tail * (L::STAGE / BOX) * 8; i += 32) {
                             const int box = i / (tail * 8), r = left + i / 8 % tail, chunk = i % 8;
@@ -526,14 +542,10 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                 if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
             }
         }
-        if (!ok && rank == 0) {   // copies in flight land before the blocks' shared memory is given back
-            const int outstanding = static_cast<int>(min(issued, static_cast<long long>(L::STAGES)));
-            for (int i = 0; i < outstanding; ++i) {
-                if (stage == 0) { stage = L::STAGES; phase ^= 1; }
-                --stage;
-                barrierWait(full + stage * 8, phase);
-            }
-        }
+        copies.stage = stage;
+        copies.phase = phase;
+        copies.tailPhase = tailPhase;
+        copies.count = rank == 0 ? static_cast<int>(min(issued, static_cast<long long>(L::STAGES))) : 0;   // (the other block's arrive here too)
     } else if (warp == 1) {
         // ---- products -------------------------------------------------------------------------------------------------
         constexpr uint32_t instruction = (1u << 4) | (FORMAT<T> << 7) | (FORMAT<T> << 10) | (MODE == WEIGHTS ? 1u << 15 : 0u) | (MODE != FORWARD ? 1u << 16 : 0u) |
@@ -742,6 +754,11 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
     fenceBefore();
     __syncthreads();
     fenceAfter();
+    if (*failed != 0 && warp == 0) {
+        copies.land(full, L::STAGES);
+        if (copies.tail) barrierWait(bars + L::TAIL, copies.tailPhase);
+        __syncwarp();
+    }
     if (*failed != 0 && warp == 1 && rank == 0) {
         // products that were issued end before the tensor memory is given back
         mmaCommit<CTAS>(electOne(), bars + L::DRAIN);   // (elects the lane that issued the products)
@@ -864,12 +881,13 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
         for (int e = threadIdx.x; e <= p.experts; e += THREADS) reinterpret_cast<int*>(p.plan)[e] = before[e];
     NarrowWalk walk(bounds, before, p.experts);
     NarrowTile t;
+    InFlight copies, matricesIn;   // of warp 0
 
     if (warp == 0) {
         // ---- operands -------------------------------------------------------------------------------------------------
         const uint32_t lead = electOne();
         uint32_t stage = 0, phase = 0, matrix = 0, matrixPhase = 0;
-        int issued = 0;
+        int issued = 0, matricesIssued = 0;
         bool ok = true;
         while (ok && walk.next(t, p.experts)) {
             if (__all_sync(0xffffffffu, t.first)) {
@@ -881,6 +899,7 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
                     for (int n = 0; n < NB; ++n) tmaLoad3<1>(lead, matrices + matrix * L::MATRIX + (k * NB + n) * BOX, &mapW, k * 64, n * 64, t.expert, bar);
+                ++matricesIssued;
                 if (++matrix == 2) { matrix = 0; matrixPhase ^= 1; }
             }
             if (!await(bars + L::EMPTY + stage * 8, phase ^ 1, failed)) { ok = false; break; }
@@ -898,18 +917,12 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
             ++issued;
             if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
         }
-        if (*failed != 0) {   // copies in flight land before the block's shared memory is given back
-            for (int i = 0; i < min(issued, L::STAGES); ++i) {
-                if (stage == 0) { stage = L::STAGES; phase ^= 1; }
-                --stage;
-                barrierWait(bars + L::FULL + stage * 8, phase);
-            }
-            for (int i = 0; i < 2; ++i) {
-                if (matrix == 0) { matrix = 2; matrixPhase ^= 1; }
-                --matrix;
-                barrierWait(bars + L::W_FULL + matrix * 8, matrixPhase);
-            }
-        }
+        copies.stage = stage;
+        copies.phase = phase;
+        copies.count = min(issued, L::STAGES);
+        matricesIn.stage = matrix;
+        matricesIn.phase = matrixPhase;
+        matricesIn.count = min(matricesIssued, 2);
     } else if (warp == 1) {
         // ---- products -------------------------------------------------------------------------------------------------
         constexpr uint32_t shape = (1u << 4) | (FORMAT<T> << 7) | (FORMAT<T> << 10) | (1u << 16) | (static_cast<uint32_t>(L::COLUMNS >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
@@ -1095,6 +1108,10 @@ __global__ void __launch_bounds__(blockThreads(true), 1)
     fenceBefore();
     __syncthreads();
     fenceAfter();
+    if (*failed != 0 && warp == 0) {
+        copies.land(bars + L::FULL, L::STAGES);
+        matricesIn.land(bars + L::W_FULL, 2);
+    }
     if (*failed != 0 && warp == 1) {
         mmaCommit<1>(electOne(), bars + L::DRAIN);   // (elects the lane that issued the products)
         if (lane == 0) {
