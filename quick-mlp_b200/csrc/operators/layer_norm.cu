@@ -207,6 +207,10 @@ struct Parameters {
 
 // Rows on their way to a block of one row: bulk copies ahead of the row that is worked on, into a ring of `stages` slots in
 // shared memory. What is in flight then does not depend on what the threads are doing, nor on their registers.
+// A thread that gives up a wait waits no more. The one that issues the copies then issues no more either, and before the block ends those that were
+// under way land, or are waited for to the limit once more. (Place and phase of that moment lie in shared memory: registers, or a flag that
+// is looked at before every copy, cost the adjoint 4 to 9 %.) The rows are wrong then, and the status says so.
+constexpr int RING_MAX = 8;
 struct Ring {
     uint32_t slots, bars, slotBytes, rowBytes;
     int stages, stage = 0, phase = 0;
@@ -229,10 +233,21 @@ struct Ring {
         if (second != nullptr) bulkLoad(slots + at * slotBytes + rowBytes, second, rowBytes, bars + at * 8);
     }
     // offset of the slot whose row is there now
-    __device__ __forceinline__ uint32_t await()
+    __device__ __forceinline__ uint32_t await(unsigned char* memory)
     {
-        ok = barrierWait(bars + stage * 8, phase) && ok;
+        if (ok && !barrierWait(bars + stage * 8, phase)) {
+            ok = false;
+            if (threadIdx.x == 0) *reinterpret_cast<int*>(memory + RING_MAX * 8) = stage * 2 + phase;
+        }
         return 128 + stage * slotBytes;
+    }
+    // after a wait was given up
+    __device__ __forceinline__ void land(unsigned char* memory, int* status) const
+    {
+        atomicOr(status, 1);
+        if (threadIdx.x != 0) return;
+        const int at = *reinterpret_cast<const int*>(memory + RING_MAX * 8);
+        for (int i = 0; i < stages; ++i) barrierWait(bars + i * 8, (i < (at >> 1) ? 1 : 0) ^ (at & 1));
     }
     __device__ __forceinline__ void advance()
     {
@@ -242,7 +257,6 @@ struct Ring {
         }
     }
 };
-constexpr int RING_MAX = 8;
 
 // blocks per SM that the registers have to allow
 __host__ __device__ constexpr int perSM(int g) { return g <= 32 ? 2 : g <= 256 ? 512 / g : 1; }
@@ -271,11 +285,11 @@ __global__ void __launch_bounds__(threadsFor(G), forwardPerSM(G)) layer_norm_for
     for (; row - group < a.rows; row += step) {
         const bool active = row < a.rows;
         float2 v[EPT / 2], f[EPT / 2];
-        fetchRow<T, VEC, G, EPT>(RINGED ? reinterpret_cast<const T*>(dynamic + ring.await()) : x + row * a.x.stride, lane, a.channels, active, v);
+        fetchRow<T, VEC, G, EPT>(RINGED ? reinterpret_cast<const T*>(dynamic + ring.await(dynamic)) : x + row * a.x.stride, lane, a.channels, active, v);
         float mean, variance;
         moments(lane, a.channels, v, mean, variance);
         if constexpr (RINGED) {   // (behind the barrier of the sums: the slot has been read)
-            if (threadIdx.x == 0 && row + a.ringStages * step < a.rows) ring.issue(ring.stage, x + (row + a.ringStages * step) * a.x.stride, nullptr);
+            if (threadIdx.x == 0 && ring.ok && row + a.ringStages * step < a.rows) ring.issue(ring.stage, x + (row + a.ringStages * step) * a.x.stride, nullptr);
             ring.advance();
         }
         const float rstd = rsqrtf(variance + a.epsilon);
@@ -292,7 +306,7 @@ __global__ void __launch_bounds__(threadsFor(G), forwardPerSM(G)) layer_norm_for
         for (int i = 0; i < EPT / 2; ++i) v[i] = add2(v[i], f[i]);
         storeRow<T, VEC, G, EPT>(y + row * a.y.stride, lane, a.channels, v);
     }
-    if (RINGED && !ring.ok) atomicOr(a.status, 1);
+    if (RINGED && !ring.ok) ring.land(dynamic, a.status);
 }
 
 // VEC elements of a row in the adjoint, from the packed x and dy: u = (x - mean) / deviation, d = dy, g = dy w
@@ -352,7 +366,7 @@ __global__ void __launch_bounds__(threadsFor(G), perSM(G)) layer_norm_adjoint_ke
         fetchStats(row + step);
         const T *rowX = x + row * a.x.stride, *rowY = dy + row * a.gradY.stride;
         if constexpr (RINGED) {
-            const unsigned char* slot = dynamic + ring.await();
+            const unsigned char* slot = dynamic + ring.await(dynamic);
             rowX = reinterpret_cast<const T*>(slot);
             rowY = reinterpret_cast<const T*>(slot + ring.rowBytes);
         }
@@ -400,7 +414,7 @@ __global__ void __launch_bounds__(threadsFor(G), perSM(G)) layer_norm_adjoint_ke
         else if (RINGED) __syncthreads();
         auto release = [&] {   // behind a barrier: the slot has been read
             const long long after = row + a.ringStages * step;
-            if (threadIdx.x == 0 && after < a.rows) ring.issue(ring.stage, x + after * a.x.stride, dy + after * a.gradY.stride);
+            if (threadIdx.x == 0 && ring.ok && after < a.rows) ring.issue(ring.stage, x + after * a.x.stride, dy + after * a.gradY.stride);
             ring.advance();
         };
         if constexpr (RINGED && !TWICE) release();
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(threadsFor(G), perSM(G)) layer_norm_adjoint_ke
             release();
         }
     }
-    if (RINGED && !ring.ok) atomicOr(a.status, 1);
+    if (RINGED && !ring.ok) ring.land(dynamic, a.status);
     if (a.partial == nullptr) return;
     float* out = a.partial + static_cast<long long>(blockIdx.x) * 2 * a.channels;
     if constexpr (GROUPS == 1) {
