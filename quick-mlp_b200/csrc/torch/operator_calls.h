@@ -78,8 +78,9 @@ void checkParameter(const OptTensor& t, int64_t dim, const c10::SymInt& channels
 }
 Tensor contiguousOf(const OptTensor& t) { return t.has_value() && t->defined() ? t->contiguous() : Tensor(); }
 Tensor emptyLike(const Tensor& t) { return at::empty(t.sizes(), t.options().memory_format(c10::MemoryFormat::Contiguous)); }
-Tensor emptyFloat(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, floatLike(like)); }
-Tensor emptyInt(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, at::TensorOptions().dtype(torch::kInt32).device(like.device())); }
+// (below the dispatcher, which takes as long as the allocation itself: the sizes are checked, the device is a CUDA device)
+Tensor emptyFloat(at::IntArrayRef sizes, const Tensor& like) { return at::detail::empty_cuda(sizes, torch::kFloat32, like.device(), std::nullopt); }
+Tensor emptyInt(at::IntArrayRef sizes, const Tensor& like) { return at::detail::empty_cuda(sizes, torch::kInt32, like.device(), std::nullopt); }
 Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }   // in the place of a gradient that is not asked for
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------------
@@ -173,11 +174,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> routeForward(const Tensor& lo
     const Tensor z = asRows(logits);
     const int64_t n = z.size(0), e = z.size(1);
     if (chosen < 1 || chosen > 32 || chosen > e || e > 1024) raiseError("a row chooses 1 to 32 of its experts, of which there are at most 1024");
-    // one allocation for the four integer arrays
-    const int64_t slots = n * chosen;
-    Tensor weights = emptyFloat({n, chosen}, z), ints = emptyInt({3 * slots + e + 1}, z);
-    Tensor experts = ints.as_strided({n, chosen}, {chosen, 1}, 0), positions = ints.as_strided({n, chosen}, {chosen, 1}, slots);
-    Tensor order = ints.as_strided({slots}, {1}, 2 * slots), offsets = ints.as_strided({e + 1}, {1}, 3 * slots);
+    // (the schema promises results that share nothing: views of one allocation would do away with three of five)
+    Tensor weights = emptyFloat({n, chosen}, z), experts = emptyInt({n, chosen}, z), positions = emptyInt({n, chosen}, z), order = emptyInt({n * chosen}, z),
+           offsets = emptyInt({e + 1}, z);
     qmlp_routing_t r{n, static_cast<int32_t>(e), static_cast<int32_t>(chosen), static_cast<float*>(weights.data_ptr()), static_cast<int*>(experts.data_ptr()),
                      static_cast<int*>(order.data_ptr()), static_cast<int*>(positions.data_ptr()), static_cast<int*>(offsets.data_ptr())};
     size_t bytes = 0;

@@ -96,3 +96,15 @@ def test_leading_dimensions(qmlp, dtype):
         h, weight, offsets = rand(15, (4, 15, 16), dtype).requires_grad_(), rand(16, (6, 24, 16), dtype).requires_grad_(), r.offsets
         dh, dw = torch.autograd.grad(qmlp.expert_linear(h, weight, offsets), [h, weight], rand(17, (60, 24), dtype))
         assert dh.shape == h.shape and dw.shape == weight.shape
+
+
+@pytest.mark.parametrize("rows", [1, 37, 5000])
+def test_route_results_apart(qmlp, rows):
+    """the results of the router share no memory: one that is written leaves the others, one that is kept keeps nothing else"""
+    r = qmlp.route(rand(20, (rows, 12)), 3)
+    assert len({t.untyped_storage().data_ptr() for t in r}) == 5 and all(t.storage_offset() == 0 and t.untyped_storage().nbytes() == t.numel() * 4 for t in r)
+    kept = [t.clone() for t in r]
+    for i, t in enumerate(r):
+        t.fill_(-7)
+        for other in range(i + 1, 5):
+            assert torch.equal(r[other], kept[other])
