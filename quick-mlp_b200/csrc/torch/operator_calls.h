@@ -60,12 +60,15 @@ struct OnDevice {
         if (t.has_value()) same(first, *t);
     }
 };
+// memory on the device of `like`, a CUDA tensor (below the dispatcher, which takes as long as the allocation itself)
+Tensor emptyOn(at::IntArrayRef sizes, c10::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
+Tensor emptyAs(at::IntArrayRef sizes, const Tensor& like) { return emptyOn(sizes, like.scalar_type(), like); }
 struct ScratchMemory {
     Tensor memory;
     size_t bytes;
     ScratchMemory(size_t n, const Tensor& like) : bytes(n)
     {
-        if (n > 0) memory = at::empty({static_cast<int64_t>(n)}, at::TensorOptions().dtype(torch::kUInt8).device(like.device()));
+        if (n > 0) memory = emptyOn({static_cast<int64_t>(n)}, torch::kUInt8, like);
     }
     void* data() const { return bytes > 0 ? memory.data_ptr() : nullptr; }
 };
@@ -77,10 +80,9 @@ void checkParameter(const OptTensor& t, int64_t dim, const c10::SymInt& channels
     if (t->sym_size(-1) != channels) raiseError(std::string(name) + " has the wrong number of channels");
 }
 Tensor contiguousOf(const OptTensor& t) { return t.has_value() && t->defined() ? t->contiguous() : Tensor(); }
-Tensor emptyLike(const Tensor& t) { return at::empty(t.sizes(), t.options().memory_format(c10::MemoryFormat::Contiguous)); }
-// (below the dispatcher, which takes as long as the allocation itself: the sizes are checked, the device is a CUDA device)
-Tensor emptyFloat(at::IntArrayRef sizes, const Tensor& like) { return at::detail::empty_cuda(sizes, torch::kFloat32, like.device(), std::nullopt); }
-Tensor emptyInt(at::IntArrayRef sizes, const Tensor& like) { return at::detail::empty_cuda(sizes, torch::kInt32, like.device(), std::nullopt); }
+Tensor emptyLike(const Tensor& t) { return emptyAs(t.sizes(), t); }
+Tensor emptyFloat(at::IntArrayRef sizes, const Tensor& like) { return emptyOn(sizes, torch::kFloat32, like); }
+Tensor emptyInt(at::IntArrayRef sizes, const Tensor& like) { return emptyOn(sizes, torch::kInt32, like); }
 Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }   // in the place of a gradient that is not asked for
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------------
@@ -136,7 +138,7 @@ Tensor embeddingForward(const Tensor& tokens, const Tensor& table, double scale)
     const OnDevice on(table, tokens);
     if (table.dim() != 2) raiseError("table must be a matrix of rows and channels");
     const Tensor t = flatTokens(tokens), rows = asRows(table);
-    Tensor y = at::empty(rowShape(tokens, table.size(1)), table.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor y = emptyAs(rowShape(tokens, table.size(1)), table);
     const qmlp_tensor_t vt = viewOf(t), vr = viewOf(rows);
     qmlp_tensor_t vy = viewOf(y.dim() == 2 ? y : y.view({t.size(0), table.size(1)}));
     check(api.embedding_forward(&vt, &vr, static_cast<float>(scale), &vy, currentStream()));
@@ -146,7 +148,7 @@ Tensor embeddingAdjoint(const Tensor& tokens, const Tensor& adjOutput, int64_t r
 {
     const OnDevice on(adjOutput, tokens);
     const Tensor t = flatTokens(tokens), g = asRows(adjOutput);
-    Tensor table = at::empty({rows, g.size(1)}, g.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor table = emptyAs({rows, g.size(1)}, g);
     size_t bytes = 0;
     check(api.embedding_adjoint_memory(t.size(0), rows, static_cast<int>(g.size(1)), precisionOf(g), &bytes));
     const ScratchMemory tmp(bytes, g);
@@ -223,7 +225,7 @@ Tensor dispatchForward(const Tensor& input, const Tensor& order, const Tensor& p
     const OnDevice on(input, order, positions);
     const Tensor x = asRows(input);
     const qmlp_routing_t r = routingOf(order, positions, std::nullopt);
-    Tensor rows = at::empty({order.size(0), x.size(1)}, x.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor rows = emptyAs({order.size(0), x.size(1)}, x);
     const qmlp_tensor_t vx = viewOf(x);
     qmlp_tensor_t vr = viewOf(rows);
     check(api.dispatch_forward(&vx, &r, &vr, currentStream()));
@@ -234,7 +236,7 @@ Tensor dispatchAdjoint(const Tensor& adjRows, const Tensor& positions)
     const OnDevice on(adjRows, positions);
     const Tensor g = asRows(adjRows);
     const qmlp_routing_t r = routingOf(Tensor(), positions, std::nullopt);
-    Tensor dx = at::empty({positions.size(0), g.size(1)}, g.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor dx = emptyAs({positions.size(0), g.size(1)}, g);
     const qmlp_tensor_t vg = viewOf(g);
     qmlp_tensor_t vd = viewOf(dx);
     check(api.dispatch_adjoint(&vg, &r, &vd, currentStream()));
@@ -247,7 +249,7 @@ Tensor combineForward(const Tensor& rows, const Tensor& weights, const Tensor& o
     const Tensor y = asRows(rows);
     const Tensor w = weights.contiguous();
     const qmlp_routing_t r = routingOf(order, positions, w);
-    Tensor out = at::empty({positions.size(0), y.size(1)}, y.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor out = emptyAs({positions.size(0), y.size(1)}, y);
     const qmlp_tensor_t vy = viewOf(y);
     qmlp_tensor_t vo = viewOf(out);
     check(api.combine_forward(&vy, &r, &vo, currentStream()));
@@ -285,7 +287,7 @@ Tensor expertLinearForward(const Tensor& input, const Tensor& weight, const Tens
     checkParameter(bias, 2, weight.size(1), "bias");
     const Tensor b = contiguousOf(bias);
     const int experts = static_cast<int>(weight.size(0));
-    Tensor y = at::empty({x.size(0), weight.size(1)}, x.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor y = emptyAs({x.size(0), weight.size(1)}, x);
     const qmlp_tensor_t vx = viewOf(x), vw = viewOf(w), vb = viewOf(b);
     qmlp_tensor_t vy = viewOf(y);
     size_t bytes = 0;
@@ -300,8 +302,8 @@ std::tuple<Tensor, Tensor, Tensor> expertLinearAdjoint(const Tensor& input, cons
     const OnDevice on(input, adjOutput, weight, offsets);
     const Tensor x = asRows(input), g = asRows(adjOutput), w = matricesOf(weight);
     const int experts = static_cast<int>(weight.size(0));
-    Tensor dx = wantInput ? emptyLike(x) : Tensor(), dw = wantWeight ? at::empty(weight.sizes(), w.options()) : Tensor();
-    Tensor db = wantBias ? at::empty({weight.size(0), weight.size(1)}, w.options()) : Tensor();
+    Tensor dx = wantInput ? emptyLike(x) : Tensor(), dw = wantWeight ? emptyAs(weight.sizes(), w) : Tensor();
+    Tensor db = wantBias ? emptyAs({weight.size(0), weight.size(1)}, w) : Tensor();
     const qmlp_tensor_t vx = viewOf(x), vg = viewOf(g), vw = viewOf(w);
     qmlp_tensor_t vdx = viewOf(dx), vdw = viewOf(wantWeight ? dw.view(w.sizes()) : dw), vdb = viewOf(db);
     size_t bytes = 0;

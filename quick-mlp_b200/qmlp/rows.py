@@ -4,13 +4,24 @@ latent codes, routing of rows to experts, matrix products grouped by expert.
 The reference leaves these to PyTorch. Here they are kernels of the library behind registered operators
 (torch.ops.qmlp_b200.layer_norm_forward, ... in qmlp/ops.py), differentiable once. Features are float32, float16 or
 bfloat16 tensors (..., channels); sums are float32, results have the features' type. Results are the same every run.
+
+The functions call the native call path, which goes through the dispatcher without the interpreter's detour. While torch.compile traces, which
+cannot look into it, they call the registered operators themselves.
 """
 from typing import NamedTuple, Optional
 
 import torch
+from torch.compiler import assume_constant_result, is_compiling
 
 from . import _capi
 from . import ops  # noqa: F401  (registers torch.ops.qmlp_b200.*)
+
+
+@assume_constant_result
+def _loaded():
+    """loads the kernels behind the registered operators, while torch.compile traces"""
+    _capi.calls()
+    return True
 
 
 class Routing(NamedTuple):
@@ -24,12 +35,16 @@ class Routing(NamedTuple):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension. weight, bias: float32 or x's type."""
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.layer_norm_forward(x, weight, bias, eps)[0]
     return _capi.calls().layer_norm(x, weight, bias, eps)
 
 
 def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * table[tokens] for int32 or int64 tokens of any shape. A token outside the table (-1, say) is masked: its row
     is zeros and it contributes to no gradient. The table's gradient sums the sorted tokens' rows in float32, in their order."""
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.embedding_forward(tokens, table, scale)
     return _capi.calls().embedding(tokens, table, scale)
 
 
@@ -37,16 +52,22 @@ def route(logits: torch.Tensor, k: int, normalize: bool = True) -> Routing:
     """The k (at most 32) experts with the largest logits of every row of (rows, experts <= 1024), ties to the lowest index.
     Weights are a softmax over the chosen experts (normalize) or over all of the row. An expert with logit -inf is never
     chosen: a row with fewer than k others has slots without an expert."""
+    if is_compiling() and _loaded():
+        return Routing(*torch.ops.qmlp_b200.route_forward(logits, k, normalize))
     return Routing(*_capi.calls().route(logits, k, normalize))
 
 
 def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Feature rows (rows, channels) -> (rows * k, channels) in the experts' order; zeros behind the last expert's rows."""
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.dispatch_forward(x, routing.order, routing.positions)
     return _capi.calls().dispatch(x, routing.order, routing.positions)
 
 
 def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Rows in the experts' order -> (rows, channels): the weighted sum of each row's slots."""
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.combine_forward(rows, routing.weights, routing.order, routing.positions)
     return _capi.calls().combine(rows, routing.weights, routing.order, routing.positions)
 
 
@@ -55,6 +76,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
 
     x: (rows, channels in), weight: (experts <= 2048, channels out, channels in), bias: (experts, channels out), all float16 or
     all bfloat16; offsets: (experts + 1) ascending int32 on the device (Routing.offsets)."""
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.expert_linear_forward(x, weight, offsets, bias)
     return _capi.calls().expert_linear(x, weight, offsets, bias)
 
 

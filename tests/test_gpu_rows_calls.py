@@ -108,3 +108,21 @@ def test_route_results_apart(qmlp, rows):
         t.fill_(-7)
         for other in range(i + 1, 5):
             assert torch.equal(r[other], kept[other])
+
+
+def test_compiled(qmlp):
+    """traced by torch.compile, the operators give what they give without: results and gradients"""
+    def model(tokens, table, w, b, router, weight, bias):
+        x = qmlp.layer_norm(qmlp.embedding(tokens, table, 2.0), w, b)
+        r = qmlp.route(x.float() @ router, 2)
+        return qmlp.combine(qmlp.expert_linear(qmlp.dispatch(x, r), weight, r.offsets, bias), r)
+    half = torch.float16
+    tokens = torch.arange(300, device="cuda") % 41
+    leaves = [t.requires_grad_() for t in (rand(30, (40, 16), half), rand(31, (16,)), rand(32, (16,)), rand(33, (16, 6)), rand(34, (6, 24, 16), half), rand(35, (6, 24), half))]
+    grad = rand(36, (300, 24), half)
+    results = []
+    for call in (model, torch.compile(model, fullgraph=True, backend="aot_eager")):
+        y = call(tokens, *leaves)
+        results.append([y.detach(), *torch.autograd.grad(y, leaves, grad)])
+    for a, e in zip(*results):
+        assert torch.equal(a, e)

@@ -103,3 +103,48 @@ def test_forward_mode(error):
                 call(*args[:i], fwad.make_dual(a, torch.empty_like(a)), *args[i + 1:])
         with pytest.raises(error, match="forward-mode"):
             torch.func.jvp(call, tuple(args), tuple(torch.empty_like(a) for a in args))
+
+
+def test_functions_are_traceable():
+    """torch.compile takes the functions and FusedExperts' layer whole, with their gradients: the registered operators stand in the graph"""
+    import qmlp
+    half = torch.float16
+    seen = []
+
+    def backend(graph, inputs):
+        seen.extend(str(n.target) for n in graph.graph.nodes if n.op == "call_function")
+        return graph.forward
+
+    def model(tokens, table, w, b, router, weight, bias):
+        x = qmlp.layer_norm(qmlp.embedding(tokens, table, 2.0), w, b)
+        r = qmlp.route(x @ router, 2)
+        return qmlp.combine(qmlp.expert_linear(qmlp.dispatch(x.half(), r), weight, r.offsets, bias), r)
+    args = [meta(30, dtype=torch.int64), meta(9, 16), meta(16), meta(16), meta(16, 6), meta(6, 8, 16, dtype=half), meta(6, 8, dtype=half)]
+    leaves = [a.requires_grad_() if a.is_floating_point() else a for a in args]
+    torch._dynamo.reset()
+    y = torch.compile(model, fullgraph=True, backend=backend)(*leaves)
+    assert y.shape == (30, 8) and y.dtype == half
+    for name in ("layer_norm", "embedding", "route", "dispatch", "combine", "expert_linear"):
+        assert any(f"qmlp_b200.{name}_forward" in t for t in seen), (name, seen)
+    y = torch.compile(model, fullgraph=True, backend="aot_eager")(*leaves)
+    grads = torch.autograd.grad(y, leaves[1:], torch.empty_like(y))
+    assert [(g.shape, g.dtype) for g in grads] == [(t.shape, t.dtype) for t in leaves[1:]]
+    layer = qmlp.FusedExperts(16, 32, 8, experts=4, dtype=torch.bfloat16, device="meta")
+    assert torch.compile(layer, fullgraph=True, backend="aot_eager")(meta(5, 3, 16)).shape == (5, 3, 8)
+    torch._dynamo.reset()
+
+
+def test_first_call_is_traced():
+    """torch.compile before anything has loaded the native call path (in a process of its own)"""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, qmlp
+f = torch.compile(lambda x: qmlp.layer_norm(x) * 2, fullgraph=True, backend="aot_eager")
+assert f(torch.empty((4, 8), device="meta", requires_grad=True)).shape == (4, 8)
+print("fine")
+"""
+    package = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "quick-mlp_b200")
+    done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": package}, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "fine" in done.stdout, (done.returncode, done.stderr[-2000:])
