@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const __grid_con
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         if (first + k * pass >= a.tokens) break;
-        if (a.scale != 1.f) {
+        if (a.scale != 1.f && token[k] >= 0 && token[k] < a.rows) {   // (zeros stay zeros, whatever the scale)
             float f[VEC];
             unpack<T, VEC>(v[k], f);
 #pragma unroll

@@ -126,3 +126,16 @@ def test_compiled(qmlp):
         results.append([y.detach(), *torch.autograd.grad(y, leaves, grad)])
     for a, e in zip(*results):
         assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -2.0])
+def test_embedding_masked_rows(qmlp, scale):
+    """masked tokens give rows of zeros and no gradient, whatever the scale"""
+    table = rand(40, (20, 24), torch.float16).requires_grad_()
+    tokens = torch.tensor([3, -1, 20, 7, 3, 2 ** 40], device="cuda")
+    y = qmlp.embedding(tokens, table, scale)
+    assert not y[[1, 2, 5]].any() and torch.allclose(y[[0, 3, 4]], table[[3, 7, 3]] * scale, rtol=2.0 ** -11, atol=0, equal_nan=True)
+    dt, = torch.autograd.grad(y, table, torch.ones_like(y))
+    hit = torch.zeros(20, dtype=torch.bool, device="cuda")
+    hit[3] = hit[7] = True
+    assert not dt[~hit].any() and (torch.isnan(dt[hit]) | (dt[hit] != 0)).all()
