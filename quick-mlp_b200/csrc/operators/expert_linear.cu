@@ -1564,11 +1564,13 @@ ProductArgs common(const ExpertArgs& a)
 }
 bool wideOut(const void* out, long long stride, int columns) { return (reinterpret_cast<uintptr_t>(out) & 15) == 0 && stride % 8 == 0 && columns % 8 == 0; }
 
-// Rows that the matrix-vector kernel takes. Its time goes with the rows, the tensor kernel's hardly; half, us of the two: 64 experts of 1024 -> 2048,
-// 2 rows 4.1 / 13, 16 rows 17 / 18, 64 rows 59 / 50; 512 experts of 256 -> 256, 64 rows 6.3 / 15; one of 4096 -> 4096, 4 rows 19 / 33, 16 rows 55 / 34.
+// Rows that the matrix-vector kernel takes. Its time goes with the rows, the tensor kernel's hardly; half, us of the two, back to back: 64 experts of
+// 1024 -> 2048, 2 rows 3.6 / 10.6, 16 rows 12.0 / 13.1, 24 rows 21 / 20, 32 rows 31 / 26; 16 experts of 1024 -> 1024, 32 rows 11.8 / 11.7, 64 rows 21 / 11;
+// 512 experts of 256 -> 256, 64 rows 6.0 / 9.1; 128 experts of 512 -> 2048, 16 rows 10.5 / 9.8, 32 rows 22 / 13, 64 rows 39 / 16; one of 4096 -> 4096, 2 rows
+// 11 / 24, 4 rows (which share their reads) 18 / 24.
 bool fewRows(const ExpertArgs& a)
 {
-    return a.rows <= 64 && a.rows * a.channelsIn * a.channelsOut <= 1ll << 26 && FEW_ROWS * (a.channelsIn + 256) * 4 <= 200 * 1024;
+    return a.rows <= 64 && a.rows * a.channelsIn * a.channelsOut <= 1ll << (a.rows <= FEW_ROWS ? 26 : 25) && FEW_ROWS * (a.channelsIn + 256) * 4 <= 200 * 1024;
 }
 
 template <class T>
