@@ -1458,8 +1458,9 @@ Shape weightShape(const ExpertArgs& a) { return shapeOf(a.channelsOut > 128 ? 51
 // a read of an fp32 tile per item. The estimate below weighs the two for runs of average length: a step of 64 rows takes about 0.3 us
 // (256 x 256 tiles at the tensor core's rate, narrow ones at the memory's), partial sums move at about 5 TB/s. 64 experts of 4096 rows of
 // 256 x 256: whole runs 49 us, cut into 320 items 74 us and 44 us for their sums. An expert with more than twice the average is cut in any case, or with
-// more than a quarter of a block's share of all steps where that is later: every item that may be cut wants an fp32 tile of scratch, and with the shares
-// in mind their number goes with the blocks (8 tiles of a block and no more, 150 MB), not with the experts. 65536 rows are cut in any case: tensor
+// more than a sixth of a block's share of all steps where that is later (a quarter cost 64 experts of 1024 x 1024, one with 8 times the rows of the others, 154
+// us for 148): every item that may be cut wants an fp32 tile of scratch, and with the shares in mind their number goes with the blocks (12 tiles of a block and no
+// more, 230 MB), not with the experts. 65536 rows are cut in any case: tensor
 // memory cuts its sums off instead of rounding them, and a sum of one sign comes out too small, by 1.0e-4 of itself over 16384 rows and 3.9e-4, less than
 // half a unit of half's last place, over 65536.
 int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
@@ -1475,7 +1476,7 @@ int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
             pieces = k;
         }
     }
-    const double rows = pieces == 1 ? run * std::max(2.0, static_cast<double>(a.experts) * tiles / blocks / 4) : run / pieces;
+    const double rows = pieces == 1 ? run * std::max(2.0, static_cast<double>(a.experts) * tiles / blocks / 6) : run / pieces;
     return static_cast<int>(std::min<double>(std::max<double>(std::ceil(rows / BK) * BK, 512), 1 << 16));
 }
 
