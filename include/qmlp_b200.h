@@ -331,7 +331,7 @@ QMLP_API int qmlp_trainer_update(qmlp_trainer_t* tr, int64_t step, float grad_sc
 /* ---- operators on feature rows ------------------------------------------------------------------
  * What a user of the reference writes in PyTorch between an encoding and a network, or around several networks (no
  * counterpart in the reference): layer norm, lookup of latent codes, routing of rows to experts, matrix products grouped by
- * expert. Feature matrices are (rows, channels) views of float, half or bfloat16 elements; the elements of a row lie side by
+ * expert, dropout, matrices in 4 bits and products with them. Feature matrices are (rows, channels) views of float, half or bfloat16 elements; the elements of a row lie side by
  * side, rows may be any distance apart (16-byte aligned rows are read and written 16 bytes at a time). Sums and statistics are fp32,
  * results are rounded once. Results are written, not accumulated, and do not change from run to run. Scratch memory is 256-byte
  * aligned, its contents irrelevant; a *_memory function gives its size (0: none is needed, pass NULL). */
@@ -401,6 +401,43 @@ QMLP_API int qmlp_expert_linear_adjoint_memory(const qmlp_tensor_t* input, const
 QMLP_API int qmlp_expert_linear_adjoint(const qmlp_tensor_t* input, const qmlp_tensor_t* adj_output, const qmlp_tensor_t* weight,
                                         const int32_t* offsets, int num_experts, qmlp_tensor_t* adj_input, qmlp_tensor_t* adj_weight,
                                         qmlp_tensor_t* adj_bias, qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes);
+
+/* Dropout: output = residual + input * 65536 / (65536 - T) where an element is kept, residual (0 if NULL or undefined) where it is dropped;
+ * T = round(65536 * probability), so that the expected value is the input's. Element i (in the order of the rows: row * channels + channel) is dropped if
+ * its 16-bit number is below T: half i % 2 (low first) of word i / 2 % 4 of Philox4x32-10 with the key `seed` and the counter (i / 8, offset + *step). step:
+ * an int64 on the device, read when the kernel runs (a captured graph draws other numbers when its program advances it), or NULL. Nothing is kept for
+ * the adjoint: adj_input is this call on adj_output, without a residual (whose adjoint is adj_output itself). output may be the input. */
+QMLP_API int qmlp_dropout(const qmlp_tensor_t* input, const qmlp_tensor_t* residual, double probability, uint64_t seed, uint64_t offset,
+                          const int64_t* step, qmlp_tensor_t* output, qmlp_stream_t stream);
+
+/* `matrices` matrices of (rows, channels) in microscaled 4-bit floating point (MXFP4): blocks of 32 channels of a row share a power of two, elements
+ * are e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign). Device memory of the caller, both arrays 16-byte aligned:
+ * codes: matrices * rows rows of 16 * ceil(channels / 32) bytes, two elements a byte, the first in the low bits, zeros behind the last channel;
+ * scales: tiles of 128 rows x 128 channels, 512 bytes each, (matrices, ceil(rows / 128), ceil(channels / 128)) of them, the rows of a matrix starting a tile: the
+ * exponent + 127 (255: NaN) of row 32 q + i and of the channels from 32 j on of a tile is its byte 16 i + 4 q + j, zero where there is no such block. */
+typedef struct qmlp_mx {
+    int64_t matrices, rows;
+    int32_t channels;
+    uint8_t* codes;
+    uint8_t* scales;
+} qmlp_mx_t;
+/* Bytes of the two arrays. */
+QMLP_API int qmlp_mx_memory(int64_t matrices, int64_t rows, int channels, size_t* code_bytes, size_t* scale_bytes);
+/* input: (matrices * rows, channels). The power of a block is floor(log2(largest magnitude)) - 2 (at least -127), its elements are rounded to the nearest,
+ * ties to the even code, at most 6 in magnitude; a block with an infinity or NaN becomes NaN. */
+QMLP_API int qmlp_mx_quantize(const qmlp_tensor_t* input, qmlp_mx_t* output, qmlp_stream_t stream);
+QMLP_API int qmlp_mx_dequantize(const qmlp_mx_t* input, qmlp_tensor_t* output, qmlp_stream_t stream);
+/* output[r] = weight[e] q(input[r]) + bias[e] for the rows r in [offsets[e], offsets[e + 1]) of expert e (matrix e of weight, its rows the channels out); q: the row
+ * quantised as above. Rows of no expert are zeros. Half or bfloat16 input, output and bias ((matrices, channels out) or undefined, contiguous); offsets: matrices
+ * + 1 ascending int32 on the device (at most 2048 experts), or NULL for one matrix that all rows are multiplied with. Sums are fp32. A kernel that gives up a
+ * bounded wait sets bit 0 of qmlp_device_status. */
+QMLP_API int qmlp_mx_linear_forward_memory(const qmlp_tensor_t* input, const qmlp_mx_t* weight, size_t* bytes);
+QMLP_API int qmlp_mx_linear_forward(const qmlp_tensor_t* input, const qmlp_mx_t* weight, const int32_t* offsets, const qmlp_tensor_t* bias, qmlp_tensor_t* output,
+                                    qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes);
+/* Gradients of what is given (adj_input, adj_bias may be NULL or undefined), the quantisation of the rows taken as the identity. */
+QMLP_API int qmlp_mx_linear_adjoint_memory(const qmlp_tensor_t* adj_output, const qmlp_mx_t* weight, int adjoint_flags, size_t* bytes);
+QMLP_API int qmlp_mx_linear_adjoint(const qmlp_tensor_t* adj_output, const qmlp_mx_t* weight, const int32_t* offsets, qmlp_tensor_t* adj_input, qmlp_tensor_t* adj_bias,
+                                    qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes);
 
 #ifdef __cplusplus
 }

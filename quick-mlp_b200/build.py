@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libqmlp_b200.so")
 SOURCES = ["host.cpp", "jit.cpp", "capi.cpp", "capi_operators.cpp", "generic_kernels.cu", "static_scratch.cu",
-           "operators/common.cu", "operators/layer_norm.cu", "operators/embedding.cu", "operators/routing.cu", "operators/expert_linear.cu"]
+           "operators/common.cu", "operators/layer_norm.cu", "operators/embedding.cu", "operators/routing.cu", "operators/expert_linear.cu",
+           "operators/dropout.cu", "operators/mx.cu", "operators/mx_linear.cu"]
 NVCC = os.environ.get("QMLP_NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

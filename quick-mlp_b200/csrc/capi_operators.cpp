@@ -1,7 +1,9 @@
 // extern "C" entry points of the operators on feature rows: layer norm, embedding lookup, routing to experts, products grouped
-// by expert. No counterpart in the reference: its callers write them in PyTorch around the network.
+// by expert, dropout, 4-bit matrices and their products. No counterpart in the reference: its callers write them in PyTorch around the network.
 #include "entry.hpp"
 #include "operators/operators.h"
+
+#include <cmath>
 
 using namespace qmlp;
 
@@ -11,7 +13,8 @@ namespace {
 enum : int {
     KERNEL_ID_LAYER_NORM_FORWARD = 110, KERNEL_ID_LAYER_NORM_ADJOINT, KERNEL_ID_EMBEDDING_FORWARD, KERNEL_ID_EMBEDDING_ADJOINT, KERNEL_ID_ROUTE_FORWARD,
     KERNEL_ID_ROUTE_ADJOINT, KERNEL_ID_DISPATCH_FORWARD, KERNEL_ID_DISPATCH_ADJOINT, KERNEL_ID_COMBINE_FORWARD, KERNEL_ID_COMBINE_ADJOINT,
-    KERNEL_ID_EXPERT_LINEAR_FORWARD, KERNEL_ID_EXPERT_LINEAR_ADJOINT
+    KERNEL_ID_EXPERT_LINEAR_FORWARD, KERNEL_ID_EXPERT_LINEAR_ADJOINT, KERNEL_ID_DROPOUT, KERNEL_ID_MX_QUANTIZE, KERNEL_ID_MX_DEQUANTIZE, KERNEL_ID_MX_LINEAR_FORWARD,
+    KERNEL_ID_MX_LINEAR_ADJOINT
 };
 constexpr int64_t MAX_CHANNELS = 1 << 20, MAX_ROWS = (1ll << 31) - 4096, MAX_SORTED = 1ll << 30;
 
@@ -160,6 +163,59 @@ void expertGradients(kernel::ExpertArgs& a, const qmlp_tensor_t* adjOutput, cons
     checkSize(adjOutput, 0, input->sizes[0], "adj_output");
     checkSize(adjOutput, 1, a.channelsOut, "adj_output");
     a.gradY = rowsOf(adjOutput);
+}
+
+void checkMx(const qmlp_mx_t* m, const char* name)
+{
+    if (m == nullptr) throw std::runtime_error(std::string(name) + " is undefined");
+    if (m->channels < 1 || m->channels > MAX_CHANNELS)
+        throw std::runtime_error(format("%s must have 1 to %lld channels, got %d", name, static_cast<long long>(MAX_CHANNELS), m->channels));
+    if (m->matrices < 0 || m->rows < 0 || m->matrices > MAX_ROWS || (m->matrices > 0 && m->rows > MAX_ROWS / m->matrices)) throw std::runtime_error(format("%s has too many rows", name));
+    if (m->matrices * kernel::mxTiles(m->rows) > 0x7fffffffll / kernel::mxTiles(m->channels)) throw std::runtime_error(format("%s has too many tiles of scales", name));
+    if (m->matrices == 0 || m->rows == 0) return;
+    if (m->codes == nullptr || m->scales == nullptr) throw std::runtime_error(std::string(name) + " is undefined");
+    if (((reinterpret_cast<uintptr_t>(m->codes) | reinterpret_cast<uintptr_t>(m->scales)) & 15) != 0) throw std::runtime_error(format("the arrays of %s must be 16-byte aligned", name));
+}
+kernel::MxMatrix matrixOf(const qmlp_mx_t* m) { return {m->matrices, m->rows, m->channels, m->codes, m->scales}; }
+void checkMxFeatures(const qmlp_tensor_t* t, const qmlp_mx_t* m, const char* name, bool written)
+{
+    checkFeatures(t, name, written);
+    checkSize(t, 0, m->matrices * m->rows, name);
+    checkSize(t, 1, m->channels, name);
+}
+// products with 4-bit matrices of the rows of `rows`, which have `channels` channels
+kernel::MxLinearArgs mxLinear(const qmlp_tensor_t* rows, const qmlp_mx_t* weight, int64_t channels, const char* name)
+{
+    checkFeatures(rows, name, false);
+    if (rows->precision == QMLP_FLOAT) throw std::runtime_error(format("%s has the wrong data type, expected half or bfloat16", name));
+    checkMx(weight, "weight");
+    if (weight->matrices < 1 || weight->matrices > kernel::EXPERTS_MAX)
+        throw std::runtime_error(format("1 to %d experts are supported, got %lld", kernel::EXPERTS_MAX, static_cast<long long>(weight->matrices)));
+    if (weight->rows < 1 || weight->rows > MAX_CHANNELS)
+        throw std::runtime_error(format("weight must have 1 to %lld channels out, got %lld", static_cast<long long>(MAX_CHANNELS), static_cast<long long>(weight->rows)));
+    checkSize(rows, 1, channels, name);
+    kernel::MxLinearArgs a{};
+    a.rows = rows->sizes[0];
+    // (two tiles of 128 rows per expert may be partly empty)
+    if (a.rows / kernel::MX_TILE + 2 * kernel::EXPERTS_MAX > 0x7fffffffll / kernel::mxTiles(weight->channels))
+        throw std::runtime_error(format("%s has too many rows (%lld) of %d channels", name, static_cast<long long>(a.rows), weight->channels));
+    a.type = rows->precision;
+    a.weight = matrixOf(weight);
+    a.numSMs = Library::instance().smCount();
+    a.status = Library::instance().statusWord();
+    return a;
+}
+void checkMxOffsets(const kernel::MxLinearArgs& a, const int32_t* offsets)
+{
+    if (offsets == nullptr && a.weight.matrices != 1) throw std::runtime_error("offsets is undefined");
+}
+const void* mxBias(const qmlp_tensor_t* bias, const kernel::MxLinearArgs& a, const char* name)
+{
+    kernel::ExpertArgs e{};
+    e.experts = static_cast<int>(a.weight.matrices);
+    e.channelsOut = static_cast<int>(a.weight.rows);
+    e.type = a.type;
+    return expertBias(bias, e, name);
 }
 
 } // namespace
@@ -474,6 +530,123 @@ int qmlp_expert_linear_adjoint(const qmlp_tensor_t* input, const qmlp_tensor_t* 
     checkScratch(tmp_memory, tmp_bytes, kernel::expertBytes(a, true));
     a.scratch = tmp_memory;
     launch(KERNEL_ID_EXPERT_LINEAR_ADJOINT, stream, [&](cudaStream_t s) { return kernel::launchExpertAdjoint(a, s); });
+    QMLP_CATCH
+}
+
+int qmlp_dropout(const qmlp_tensor_t* input, const qmlp_tensor_t* residual, double probability, uint64_t seed, uint64_t offset, const int64_t* step,
+                 qmlp_tensor_t* output, qmlp_stream_t stream)
+{
+    QMLP_TRY
+    checkFeatures(input, "input", false);
+    checkLike(output, input, "output", true);
+    if (!(probability >= 0. && probability <= 1.)) throw std::runtime_error("probability must be between 0 and 1");
+    kernel::DropoutArgs a{};
+    a.rows = input->sizes[0];
+    a.channels = static_cast<int>(input->sizes[1]);
+    a.type = input->precision;
+    a.x = rowsOf(input);
+    if (defined(residual)) {
+        checkLike(residual, input, "residual", false);
+        a.residual = rowsOf(residual);
+    }
+    a.y = rowsOf(output);
+    a.cut = static_cast<unsigned>(std::nearbyint(probability * 65536.));
+    a.seed = seed;
+    a.offset = offset;
+    a.step = reinterpret_cast<const long long*>(step);
+    launch(KERNEL_ID_DROPOUT, stream, [&](cudaStream_t s) { return kernel::launchDropout(a, s); });
+    QMLP_CATCH
+}
+
+int qmlp_mx_memory(int64_t matrices, int64_t rows, int channels, size_t* code_bytes, size_t* scale_bytes)
+{
+    QMLP_TRY
+    checkPointer(code_bytes, "code_bytes");
+    checkPointer(scale_bytes, "scale_bytes");
+    alignas(16) uint8_t nothing[16];
+    const qmlp_mx_t m{matrices, rows, channels, nothing, nothing};
+    checkMx(&m, "matrix");
+    *code_bytes = static_cast<size_t>(matrices * rows) * kernel::mxCodeBytes(channels);
+    *scale_bytes = static_cast<size_t>(matrices) * kernel::mxTiles(rows) * kernel::mxTiles(channels) * kernel::MX_TILE_BYTES;
+    QMLP_CATCH
+}
+int qmlp_mx_quantize(const qmlp_tensor_t* input, qmlp_mx_t* output, qmlp_stream_t stream)
+{
+    QMLP_TRY
+    checkMx(output, "output");
+    checkMxFeatures(input, output, "input", false);
+    launch(KERNEL_ID_MX_QUANTIZE, stream, [&](cudaStream_t s) { return kernel::launchMxQuantize(matrixOf(output), input->precision, rowsOf(input), s); });
+    QMLP_CATCH
+}
+int qmlp_mx_dequantize(const qmlp_mx_t* input, qmlp_tensor_t* output, qmlp_stream_t stream)
+{
+    QMLP_TRY
+    checkMx(input, "input");
+    checkMxFeatures(output, input, "output", true);
+    launch(KERNEL_ID_MX_DEQUANTIZE, stream, [&](cudaStream_t s) { return kernel::launchMxDequantize(matrixOf(input), output->precision, rowsOf(output), s); });
+    QMLP_CATCH
+}
+
+int qmlp_mx_linear_forward_memory(const qmlp_tensor_t* input, const qmlp_mx_t* weight, size_t* bytes)
+{
+    QMLP_TRY
+    checkPointer(bytes, "bytes");
+    checkPointer(weight, "weight");
+    *bytes = kernel::mxLinearBytes(mxLinear(input, weight, weight->channels, "input"));
+    QMLP_CATCH
+}
+int qmlp_mx_linear_forward(const qmlp_tensor_t* input, const qmlp_mx_t* weight, const int32_t* offsets, const qmlp_tensor_t* bias, qmlp_tensor_t* output,
+                           qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes)
+{
+    QMLP_TRY
+    checkPointer(weight, "weight");
+    kernel::MxLinearArgs a = mxLinear(input, weight, weight->channels, "input");
+    checkMxOffsets(a, offsets);
+    a.bias = mxBias(bias, a, "bias");
+    checkFeatures(output, "output", true);
+    checkDtype(output, a.type, "output");
+    checkSize(output, 0, a.rows, "output");
+    checkSize(output, 1, weight->rows, "output");
+    a.offsets = offsets;
+    a.x = rowsOf(input);
+    a.y = rowsOf(output);
+    checkScratch(tmp_memory, tmp_bytes, kernel::mxLinearBytes(a));
+    a.scratch = tmp_memory;
+    launch(KERNEL_ID_MX_LINEAR_FORWARD, stream, [&](cudaStream_t s) { return kernel::launchMxLinear(a, s); });
+    QMLP_CATCH
+}
+int qmlp_mx_linear_adjoint_memory(const qmlp_tensor_t* adj_output, const qmlp_mx_t* weight, int adjoint_flags, size_t* bytes)
+{
+    QMLP_TRY
+    checkPointer(bytes, "bytes");
+    checkPointer(weight, "weight");
+    kernel::MxLinearArgs a = mxLinear(adj_output, weight, weight->rows, "adj_output");
+    a.gradY = rowsOf(adj_output);
+    char wanted = 0;   // (only whether a gradient is wanted enters the size)
+    if (adjoint_flags & QMLP_GRADIENTS_INPUT) a.gradX.data = &wanted;
+    *bytes = kernel::mxLinearAdjointBytes(a);
+    QMLP_CATCH
+}
+int qmlp_mx_linear_adjoint(const qmlp_tensor_t* adj_output, const qmlp_mx_t* weight, const int32_t* offsets, qmlp_tensor_t* adj_input, qmlp_tensor_t* adj_bias,
+                           qmlp_stream_t stream, void* tmp_memory, size_t tmp_bytes)
+{
+    QMLP_TRY
+    checkPointer(weight, "weight");
+    kernel::MxLinearArgs a = mxLinear(adj_output, weight, weight->rows, "adj_output");
+    checkMxOffsets(a, offsets);
+    a.offsets = offsets;
+    a.gradY = rowsOf(adj_output);
+    if (defined(adj_input)) {
+        checkFeatures(adj_input, "adj_input", true);
+        checkDtype(adj_input, a.type, "adj_input");
+        checkSize(adj_input, 0, a.rows, "adj_input");
+        checkSize(adj_input, 1, weight->channels, "adj_input");
+        a.gradX = rowsOf(adj_input);
+    }
+    a.gradBias = const_cast<void*>(mxBias(adj_bias, a, "adj_bias"));
+    checkScratch(tmp_memory, tmp_bytes, kernel::mxLinearAdjointBytes(a));
+    a.scratch = tmp_memory;
+    launch(KERNEL_ID_MX_LINEAR_ADJOINT, stream, [&](cudaStream_t s) { return kernel::launchMxLinearAdjoint(a, s); });
     QMLP_CATCH
 }
 

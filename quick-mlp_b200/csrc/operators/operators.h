@@ -1,4 +1,5 @@
-// Launchers of the operators on feature rows: layer norm, embedding lookup, routing to experts, products grouped by expert.
+// Launchers of the operators on feature rows: layer norm, embedding lookup, routing to experts, products grouped by expert, dropout, 4-bit matrices
+// and their products.
 // The arguments are checked by the entry points (capi_operators.cpp); every launcher returns the status of its launches.
 #pragma once
 #include <cuda_runtime.h>
@@ -109,6 +110,52 @@ struct ExpertArgs {
 size_t expertBytes(const ExpertArgs& a, bool adjoint);
 cudaError_t launchExpertForward(const ExpertArgs& a, cudaStream_t stream);
 cudaError_t launchExpertAdjoint(const ExpertArgs& a, cudaStream_t stream);
+
+// ---- dropout ---------------------------------------------------------------------------------------------------------------
+struct DropoutArgs {
+    long long rows;
+    int channels, type;
+    Rows x, residual, y;       // residual.data may be null
+    unsigned cut;              // of 65536 numbers, those below it drop
+    unsigned long long seed, offset;
+    const long long* step;     // added to the offset, may be null
+};
+cudaError_t launchDropout(const DropoutArgs& a, cudaStream_t stream);
+
+// ---- microscaled 4-bit matrices ----------------------------------------------------------------------------------------------
+// `matrices` matrices of (rows, channels). Codes: rows of mxCodeBytes(channels), two e2m1 elements a byte, the first in the low bits, zeros behind the
+// last channel. Scales: tiles of 128 rows x 128 channels, 512 bytes each, [matrix][row tile][channel tile]; the exponent (+ 127) of row 32 q + i and of
+// the channels from 32 j on lies at byte 16 i + 4 q + j of its tile, where a tensor core's scales come from without a change.
+constexpr int MX_BLOCK = 32, MX_TILE = 128, MX_TILE_BYTES = 512;
+inline int mxBlocks(int channels) { return (channels + MX_BLOCK - 1) / MX_BLOCK; }
+inline int mxCodeBytes(int channels) { return mxBlocks(channels) * (MX_BLOCK / 2); }
+inline int mxTiles(long long n) { return static_cast<int>((n + MX_TILE - 1) / MX_TILE); }
+struct MxMatrix {
+    long long matrices, rows;
+    int channels;
+    unsigned char *codes, *scales;
+};
+cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStream_t stream);
+cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream);
+
+// products of rows with such matrices (weight.matrices experts, weight.rows channels out)
+struct MxLinearArgs {
+    long long rows;
+    int type, numSMs;
+    Rows x, y;
+    MxMatrix weight;
+    const void* bias;          // (experts, channels out), contiguous, may be null
+    const int* offsets;        // experts + 1; null: all rows are the one expert's
+    // adjoint
+    Rows gradY, gradX;         // gradX.data may be null
+    void* gradBias;            // may be null
+    void* scratch;
+    int* status;
+};
+size_t mxLinearBytes(const MxLinearArgs& a);
+size_t mxLinearAdjointBytes(const MxLinearArgs& a);
+cudaError_t launchMxLinear(const MxLinearArgs& a, cudaStream_t stream);
+cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream);
 
 } // namespace kernel
 } // namespace qmlp

@@ -40,7 +40,8 @@ using OptTensor = std::optional<Tensor>;
     X(layer_norm_forward) X(layer_norm_adjoint_memory) X(layer_norm_adjoint) X(embedding_forward) X(embedding_adjoint_memory)  \
     X(embedding_adjoint) X(route_memory) X(route_forward) X(route_adjoint) X(dispatch_forward) X(dispatch_adjoint)         \
     X(combine_forward) X(combine_adjoint) X(expert_linear_forward_memory) X(expert_linear_forward)                         \
-    X(expert_linear_adjoint_memory) X(expert_linear_adjoint)
+    X(expert_linear_adjoint_memory) X(expert_linear_adjoint) X(dropout) X(mx_quantize) X(mx_dequantize)                    \
+    X(mx_linear_forward_memory) X(mx_linear_forward) X(mx_linear_adjoint_memory) X(mx_linear_adjoint)
 
 struct Api {
 #define QMLP_MEMBER(name) decltype(&qmlp_##name) name = nullptr;
@@ -567,4 +568,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("dispatch", wrap_pybind_function_no_gil(dispatchRows));
     m.def("combine", wrap_pybind_function_no_gil(combineRows));
     m.def("expert_linear", wrap_pybind_function_no_gil(expertLinear));
+    m.def("dropout", wrap_pybind_function_no_gil(dropoutRows));
+    m.def("mx_quantize", wrap_pybind_function_no_gil(mxQuantized));
+    m.def("mx_linear", wrap_pybind_function_no_gil(mxLinear));
 }

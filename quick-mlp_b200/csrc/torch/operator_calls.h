@@ -1,5 +1,5 @@
-// The operators on feature rows in PyTorch: torch.ops.qmlp_b200.{layer_norm, embedding, route, dispatch, combine, expert_linear}_forward
-// and _adjoint, with their autograd nodes. Included by calls.cpp (whose helpers it uses); schemas in qmlp/ops.py.
+// The operators on feature rows in PyTorch: torch.ops.qmlp_b200.{layer_norm, embedding, route, dispatch, combine, expert_linear, mx_linear}_forward
+// and _adjoint, dropout_forward (its own adjoint), mx_quantize and mx_dequantize, with their autograd nodes. Included by calls.cpp (whose helpers it uses); schemas in qmlp/ops.py.
 //
 // Every operator takes (..., channels) tensors; the leading dimensions are rows. A tensor whose rows the kernels cannot walk (elements of
 // a row not side by side, leading dimensions that are no single stride) is copied first.
@@ -313,6 +313,145 @@ std::tuple<Tensor, Tensor, Tensor> expertLinearAdjoint(const Tensor& input, cons
     return {wantInput ? dx : nothing(input), wantWeight ? dw : nothing(weight), wantBias ? db : nothing(weight)};
 }
 
+// ---- dropout -----------------------------------------------------------------------------------------------------------------
+void checkDropout(const Tensor& input, const OptTensor& residual, double probability, const OptTensor& step)
+{
+    if (residual.has_value() && residual->defined()) {
+        if (residual->sym_sizes() != input.sym_sizes()) raiseError("residual must have the input's shape");
+        if (residual->scalar_type() != input.scalar_type()) raiseError("residual must have the input's type");
+    }
+    if (!(probability >= 0. && probability <= 1.)) raiseError("probability must be between 0 and 1");
+    if (step.has_value() && step->defined() && (step->scalar_type() != torch::kInt64 || step->sym_numel() != 1)) raiseError("step must be an int64 tensor of one element");
+}
+Tensor dropoutForward(const Tensor& input, const OptTensor& residual, double probability, int64_t seed, int64_t offset, const OptTensor& step)
+{
+    const OnDevice on(input, residual, step);
+    checkDropout(input, residual, probability, step);
+    const Tensor x = asRows(input), r = residual.has_value() && residual->defined() ? asRows(*residual) : Tensor();
+    Tensor y = emptyLike(input);
+    const qmlp_tensor_t vx = viewOf(x), vr = viewOf(r);
+    qmlp_tensor_t vy = viewOf(y.dim() == 2 ? y : y.view(x.sizes()));
+    check(api.dropout(&vx, &vr, probability, static_cast<uint64_t>(seed), static_cast<uint64_t>(offset),
+                      step.has_value() && step->defined() ? static_cast<const int64_t*>(step->data_ptr()) : nullptr, &vy, currentStream()));
+    return y;
+}
+
+// ---- 4-bit matrices --------------------------------------------------------------------------------------------------------------
+template <class Int>
+Int ceilDiv(const Int& n, int64_t d) { return (n + (d - 1)) / d; }
+// (rows, channels) or (matrices, rows, channels): the sizes of codes and scales
+template <class Sizes, class Int = std::decay_t<decltype(std::declval<Sizes>()[0])>>
+std::pair<std::vector<Int>, std::vector<Int>> mxSizes(const Sizes& sizes)
+{
+    const size_t dims = sizes.size();
+    if (dims != 2 && dims != 3) raiseError("a matrix (rows, channels) or matrices (matrices, rows, channels) are needed");
+    std::vector<Int> codes(sizes.begin(), sizes.end()), scales(sizes.begin(), sizes.end());
+    codes[dims - 1] = ceilDiv(sizes[dims - 1], 32) * 16;
+    scales[dims - 2] = ceilDiv(sizes[dims - 2], 128);
+    scales[dims - 1] = ceilDiv(sizes[dims - 1], 128);
+    for (int n : {32, 4, 4}) scales.push_back(Int(n));
+    return {codes, scales};
+}
+// a tensor of bytes as the kernels read it: contiguous, from a 16-byte boundary on
+Tensor readableBytes(const Tensor& t)
+{
+    const Tensor c = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
+}
+void checkMx(const Tensor& codes, const Tensor& scales, int64_t channels)
+{
+    if (codes.scalar_type() != torch::kUInt8 || scales.scalar_type() != torch::kUInt8) raiseError("codes and scales must be uint8 tensors");
+    if (codes.dim() != 2 && codes.dim() != 3) raiseError("codes must be (rows, bytes) or (matrices, rows, bytes)");
+    if (channels < 1) raiseError("a 4-bit matrix of at least one channel is needed");
+    c10::SymDimVector sizes(codes.sym_sizes().begin(), codes.sym_sizes().end());
+    sizes.back() = channels;
+    const auto expected = mxSizes(sizes);
+    if (codes.sym_sizes() != c10::SymIntArrayRef(expected.first)) raiseError("codes must have 16 bytes per 32 of " + std::to_string(channels) + " channels in a row");
+    if (scales.sym_sizes() != c10::SymIntArrayRef(expected.second)) raiseError("scales must be (..., rows / 128, channels / 128, 32, 4, 4), both rounded up");
+}
+struct MxView {
+    Tensor codes, scales;
+    qmlp_mx_t m;
+    MxView(const Tensor& c, const Tensor& s, int64_t channels) : codes(readableBytes(c)), scales(readableBytes(s))
+    {
+        if (channels > (1 << 20)) raiseError("a 4-bit matrix has at most 1048576 channels");
+        m = {codes.dim() == 3 ? codes.size(0) : 1, codes.size(-2), static_cast<int32_t>(channels), static_cast<uint8_t*>(codes.data_ptr()), static_cast<uint8_t*>(scales.data_ptr())};
+    }
+};
+std::tuple<Tensor, Tensor> mxQuantize(const Tensor& input)
+{
+    const OnDevice on(input);
+    const auto sizes = mxSizes(input.sizes());
+    if (input.size(-1) < 1) raiseError("a 4-bit matrix of at least one channel is needed");
+    const Tensor x = asRows(input);
+    const qmlp_tensor_t vx = viewOf(x);
+    Tensor codes = emptyOn(sizes.first, torch::kUInt8, input), scales = emptyOn(sizes.second, torch::kUInt8, input);
+    MxView q(codes, scales, input.size(-1));
+    check(api.mx_quantize(&vx, &q.m, currentStream()));
+    return {codes, scales};
+}
+Tensor mxDequantize(const Tensor& codes, const Tensor& scales, int64_t channels, c10::ScalarType type)
+{
+    const OnDevice on(codes, scales);
+    checkMx(codes, scales, channels);
+    const MxView q(codes, scales, channels);
+    std::vector<int64_t> sizes = codes.sizes().vec();
+    sizes.back() = channels;
+    Tensor y = emptyOn(sizes, type, codes);
+    qmlp_tensor_t vy = viewOf(y.dim() == 2 ? y : y.view({-1, channels}));
+    if (y.numel() == 0) return y;
+    check(api.mx_dequantize(&q.m, &vy, currentStream()));
+    return y;
+}
+// offsets and bias of a product with `codes`, which hold matrices of experts or one matrix
+void checkMxLinear(const Tensor& codes, const OptTensor& offsets, const OptTensor& bias)
+{
+    const bool experts = codes.dim() == 3, given = offsets.has_value() && offsets->defined();
+    if (experts != given) raiseError(experts ? "matrices of several experts need offsets" : "a single matrix takes no offsets");
+    checkParameter(bias, experts ? 2 : 1, codes.sym_size(-2), "bias");
+    if (experts && bias.has_value() && bias->defined() && bias->sym_size(0) != codes.sym_size(0)) raiseError("bias must have a row per expert");
+}
+const int* mxOffsets(const OptTensor& offsets, const Tensor& codes) { return offsets.has_value() && offsets->defined() ? offsetsOf(*offsets, codes) : nullptr; }
+Tensor mxLinearForward(const Tensor& input, const Tensor& codes, const Tensor& scales, const OptTensor& offsets, const OptTensor& bias)
+{
+    const OnDevice on(input, codes, scales, offsets, bias);
+    const Tensor x = asRows(input);
+    checkMx(codes, scales, x.size(1));
+    checkMxLinear(codes, offsets, bias);
+    const MxView q(codes, scales, x.size(1));
+    const Tensor b = bias.has_value() && bias->defined() ? bias->contiguous().view({q.m.matrices, q.m.rows}) : Tensor();
+    std::vector<int64_t> sizes = input.sizes().vec();
+    sizes.back() = q.m.rows;
+    Tensor y = emptyAs(sizes, x);
+    const qmlp_tensor_t vx = viewOf(x), vb = viewOf(b);
+    qmlp_tensor_t vy = viewOf(y.dim() == 2 ? y : y.view({x.size(0), q.m.rows}));
+    size_t bytes = 0;
+    check(api.mx_linear_forward_memory(&vx, &q.m, &bytes));
+    const ScratchMemory tmp(bytes, x);
+    check(api.mx_linear_forward(&vx, &q.m, mxOffsets(offsets, codes), &vb, &vy, currentStream(), tmp.data(), bytes));
+    return y;
+}
+std::tuple<Tensor, Tensor> mxLinearAdjoint(const Tensor& adjOutput, const Tensor& codes, const Tensor& scales, int64_t channels, const OptTensor& offsets, bool wantInput,
+                                           bool wantBias)
+{
+    const OnDevice on(adjOutput, codes, scales, offsets);
+    checkMx(codes, scales, channels);
+    checkMxLinear(codes, offsets, std::nullopt);
+    const Tensor g = asRows(adjOutput);
+    const MxView q(codes, scales, channels);
+    std::vector<int64_t> sizes = adjOutput.sizes().vec(), biasSizes = codes.sizes().vec();
+    sizes.back() = channels;
+    biasSizes.pop_back();
+    Tensor dx = wantInput ? emptyAs(sizes, g) : Tensor(), db = wantBias ? emptyAs(biasSizes, g) : Tensor();
+    const qmlp_tensor_t vg = viewOf(g);
+    qmlp_tensor_t vdx = viewOf(wantInput ? dx.view({g.size(0), channels}) : dx), vdb = viewOf(wantBias ? db.view({q.m.matrices, q.m.rows}) : db);
+    size_t bytes = 0;
+    check(api.mx_linear_adjoint_memory(&vg, &q.m, wantInput ? QMLP_GRADIENTS_INPUT : 0, &bytes));
+    const ScratchMemory tmp(bytes, g);
+    check(api.mx_linear_adjoint(&vg, &q.m, mxOffsets(offsets, codes), &vdx, &vdb, currentStream(), tmp.data(), bytes));
+    return {wantInput ? dx : nothing(adjOutput), wantBias ? db : nothing(adjOutput)};
+}
+
 // ---- autograd --------------------------------------------------------------------------------------------------------------
 template <class F>
 auto operatorHandle(const char* name)
@@ -569,6 +708,87 @@ std::tuple<Tensor, Tensor, Tensor> expertLinearAdjointAutograd(const Tensor& inp
     return {r[0], r[1], r[2]};
 }
 
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& input, const OptTensor& residual, double probability, int64_t seed, int64_t offset, const OptTensor& step)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({step.value_or(Tensor())});   // (refuses a step that was advanced in between)
+        ctx->saved_data["residual"] = residual.has_value() && residual->defined();
+        ctx->saved_data["probability"] = probability;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["offset"] = offset;
+        return QMLP_CALL("dropout_forward", dropoutForward).call(input, residual, probability, seed, offset, step);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grad)
+    {
+        const bool residual = ctx->saved_data["residual"].toBool();
+        variable_list g(6);
+        // linear in the input: its own adjoint, and differentiable like the operator itself
+        if (ctx->needs_input_grad(0))
+            g[0] = QMLP_CALL("dropout_forward", dropoutForward).call(grad[0], std::nullopt, ctx->saved_data["probability"].toDouble(), ctx->saved_data["seed"].toInt(),
+                                                                     ctx->saved_data["offset"].toInt(), optional(ctx->get_saved_variables()[0]));
+        if (residual && ctx->needs_input_grad(1)) g[1] = grad[0];
+        return g;
+    }
+};
+Tensor dropoutForwardAutograd(const Tensor& input, const OptTensor& residual, double probability, int64_t seed, int64_t offset, const OptTensor& step)
+{
+    refuseTangents("dropout_forward", input, residual);
+    if (wantsNode(input, residual)) return DropoutFunction::apply(input, residual, probability, seed, offset, step);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return QMLP_CALL("dropout_forward", dropoutForward).call(input, residual, probability, seed, offset, step);
+}
+
+// (codes have no gradient)
+std::tuple<Tensor, Tensor> mxQuantizeAutograd(const Tensor& input)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    return QMLP_CALL("mx_quantize", mxQuantize).call(input);
+}
+Tensor mxDequantizeAutograd(const Tensor& codes, const Tensor& scales, int64_t channels, c10::ScalarType type)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    return QMLP_CALL("mx_dequantize", mxDequantize).call(codes, scales, channels, type);
+}
+
+struct MxLinearFunction : torch::autograd::Function<MxLinearFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& input, const Tensor& codes, const Tensor& scales, const OptTensor& offsets, const OptTensor& bias)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({codes, scales, offsets.value_or(Tensor())});
+        ctx->saved_data["channels"] = input.size(-1);
+        ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+        return QMLP_CALL("mx_linear_forward", mxLinearForward).call(input, codes, scales, offsets, bias);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grad)
+    {
+        const auto s = ctx->get_saved_variables();
+        const bool wx = ctx->needs_input_grad(0), wb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(s[2].defined() ? 4 : 3);
+        auto g = QMLP_CALL("mx_linear_adjoint", mxLinearAdjoint).call(grad[0], s[0], s[1], ctx->saved_data["channels"].toInt(), optional(s[2]), wx, wb);
+        return {wx ? std::get<0>(g) : Tensor(), Tensor(), Tensor(), Tensor(), wb ? std::get<1>(g) : Tensor()};
+    }
+};
+Tensor mxLinearForwardAutograd(const Tensor& input, const Tensor& codes, const Tensor& scales, const OptTensor& offsets, const OptTensor& bias)
+{
+    refuseTangents("mx_linear_forward", input, bias);
+    if (wantsNode(input, bias)) return MxLinearFunction::apply(input, codes, scales, offsets, bias);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return QMLP_CALL("mx_linear_forward", mxLinearForward).call(input, codes, scales, offsets, bias);
+}
+std::tuple<Tensor, Tensor> mxLinearAdjointAutograd(const Tensor& adjOutput, const Tensor& codes, const Tensor& scales, int64_t channels, const OptTensor& offsets, bool wantInput,
+                                                   bool wantBias)
+{
+    refuseTangents("mx_linear_adjoint", adjOutput);
+    variable_list r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto g = QMLP_CALL("mx_linear_adjoint", mxLinearAdjoint).call(adjOutput, codes, scales, channels, offsets, wantInput, wantBias);
+        r = {std::get<0>(g), std::get<1>(g)};
+    }
+    r = once("mx_linear_adjoint", r, {adjOutput});
+    return {r[0], r[1]};
+}
+
 // ---- shapes (meta tensors) ---------------------------------------------------------------------------------------------------
 Tensor emptyOf(const Tensor& like, c10::SymIntArrayRef sizes) { return at::empty_symint(sizes, like.options().memory_format(c10::MemoryFormat::Contiguous)); }
 Tensor emptyOf(const Tensor& like, c10::SymIntArrayRef sizes, c10::ScalarType type) { return at::empty_symint(sizes, like.options().dtype(type)); }
@@ -630,13 +850,55 @@ std::tuple<Tensor, Tensor, Tensor> expertLinearAdjointMeta(const Tensor& input, 
             wantBias ? emptyOf(weight, {weight.sym_size(0), weight.sym_size(1)}) : nothing(weight)};
 }
 
+Tensor dropoutForwardMeta(const Tensor& input, const OptTensor& residual, double probability, int64_t, int64_t, const OptTensor& step)
+{
+    rowsIn(input);
+    checkDropout(input, residual, probability, step);
+    return emptyOf(input, input.sym_sizes());
+}
+std::tuple<Tensor, Tensor> mxQuantizeMeta(const Tensor& input)
+{
+    const auto sizes = mxSizes(input.sym_sizes());
+    rowsIn(input);
+    return {emptyOf(input, sizes.first, torch::kUInt8), emptyOf(input, sizes.second, torch::kUInt8)};
+}
+Tensor mxDequantizeMeta(const Tensor& codes, const Tensor& scales, int64_t channels, c10::ScalarType type)
+{
+    checkMx(codes, scales, channels);
+    c10::SymDimVector sizes(codes.sym_sizes().begin(), codes.sym_sizes().end());
+    sizes.back() = channels;
+    return emptyOf(codes, sizes, type);
+}
+Tensor mxLinearForwardMeta(const Tensor& input, const Tensor& codes, const Tensor& scales, const OptTensor& offsets, const OptTensor& bias)
+{
+    rowsIn(input);
+    checkMx(codes, scales, input.size(-1));
+    checkMxLinear(codes, offsets, bias);
+    c10::SymDimVector sizes(input.sym_sizes().begin(), input.sym_sizes().end());
+    sizes.back() = codes.sym_size(-2);
+    return emptyOf(input, sizes);
+}
+std::tuple<Tensor, Tensor> mxLinearAdjointMeta(const Tensor& adjOutput, const Tensor& codes, const Tensor& scales, int64_t channels, const OptTensor& offsets, bool wantInput,
+                                               bool wantBias)
+{
+    rowsIn(adjOutput);
+    checkMx(codes, scales, channels);
+    checkMxLinear(codes, offsets, std::nullopt);
+    c10::SymDimVector sizes(adjOutput.sym_sizes().begin(), adjOutput.sym_sizes().end()), biasSizes(codes.sym_sizes().begin(), codes.sym_sizes().end() - 1);
+    sizes.back() = channels;
+    return {wantInput ? emptyOf(adjOutput, sizes) : nothing(adjOutput), wantBias ? emptyOf(adjOutput, biasSizes) : nothing(adjOutput)};
+}
+
 #define QMLP_ROW_OPERATORS(X, suffix)                                                                                          \
     X("layer_norm_forward", layerNormForward##suffix) X("layer_norm_adjoint", layerNormAdjoint##suffix)                         \
     X("embedding_forward", embeddingForward##suffix) X("embedding_adjoint", embeddingAdjoint##suffix)                           \
     X("route_forward", routeForward##suffix) X("route_adjoint", routeAdjoint##suffix)                                           \
     X("dispatch_forward", dispatchForward##suffix) X("dispatch_adjoint", dispatchAdjoint##suffix)                               \
     X("combine_forward", combineForward##suffix) X("combine_adjoint", combineAdjoint##suffix)                                   \
-    X("expert_linear_forward", expertLinearForward##suffix) X("expert_linear_adjoint", expertLinearAdjoint##suffix)
+    X("expert_linear_forward", expertLinearForward##suffix) X("expert_linear_adjoint", expertLinearAdjoint##suffix)             \
+    X("dropout_forward", dropoutForward##suffix)                                                                                \
+    X("mx_quantize", mxQuantize##suffix) X("mx_dequantize", mxDequantize##suffix)                                               \
+    X("mx_linear_forward", mxLinearForward##suffix) X("mx_linear_adjoint", mxLinearAdjoint##suffix)
 #define QMLP_IMPL(name, function) m->impl(name, function);
 
 void registerRowOperators(c10::DispatchKey key)
@@ -665,4 +927,13 @@ Tensor combineRows(const Tensor& rows, const Tensor& weights, const Tensor& orde
 Tensor expertLinear(const Tensor& input, const Tensor& weight, const Tensor& offsets, const OptTensor& bias)
 {
     return QMLP_CALL("expert_linear_forward", expertLinearForward).call(input, weight, offsets, bias);
+}
+Tensor dropoutRows(const Tensor& input, double probability, int64_t seed, int64_t offset, const OptTensor& residual, const OptTensor& step)
+{
+    return QMLP_CALL("dropout_forward", dropoutForward).call(input, residual, probability, seed, offset, step);
+}
+std::tuple<Tensor, Tensor> mxQuantized(const Tensor& input) { return QMLP_CALL("mx_quantize", mxQuantize).call(input); }
+Tensor mxLinear(const Tensor& input, const Tensor& codes, const Tensor& scales, const OptTensor& offsets, const OptTensor& bias)
+{
+    return QMLP_CALL("mx_linear_forward", mxLinearForward).call(input, codes, scales, offsets, bias);
 }

@@ -33,6 +33,11 @@ class TrainerConfig(C.Structure):
                 ("grid_half_copy", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Mx(C.Structure):
+    """qmlp_mx_t"""
+    _fields_ = [("matrices", C.c_int64), ("rows", C.c_int64), ("channels", C.c_int32), ("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
 class Routing(C.Structure):
     """qmlp_routing_t"""
     _fields_ = [("tokens", C.c_int64), ("num_experts", C.c_int32), ("chosen", C.c_int32), ("weights", C.c_void_p),
@@ -52,6 +57,7 @@ _lib = None
 # name -> (restype, argtypes); every symbol include/qmlp_b200.h declares
 _P = C.c_void_p
 _TP = C.POINTER(Tensor)
+_MP = C.POINTER(Mx)
 _RP = C.POINTER(Routing)
 _SIZE = C.POINTER(C.c_size_t)
 SIGNATURES = {
@@ -155,6 +161,14 @@ SIGNATURES = {
     "qmlp_expert_linear_forward": (C.c_int, [_TP, _TP, _P, C.c_int, _TP, _TP, _P, _P, C.c_size_t]),
     "qmlp_expert_linear_adjoint_memory": (C.c_int, [_TP, _TP, _TP, C.c_int, C.c_int, _SIZE]),
     "qmlp_expert_linear_adjoint": (C.c_int, [_TP, _TP, _TP, _P, C.c_int, _TP, _TP, _TP, _P, _P, C.c_size_t]),
+    "qmlp_dropout": (C.c_int, [_TP, _TP, C.c_double, C.c_uint64, C.c_uint64, _P, _TP, _P]),
+    "qmlp_mx_memory": (C.c_int, [C.c_int64, C.c_int64, C.c_int, _SIZE, _SIZE]),
+    "qmlp_mx_quantize": (C.c_int, [_TP, _MP, _P]),
+    "qmlp_mx_dequantize": (C.c_int, [_MP, _TP, _P]),
+    "qmlp_mx_linear_forward_memory": (C.c_int, [_TP, _MP, _SIZE]),
+    "qmlp_mx_linear_forward": (C.c_int, [_TP, _MP, _P, _TP, _TP, _P, _P, C.c_size_t]),
+    "qmlp_mx_linear_adjoint_memory": (C.c_int, [_TP, _MP, C.c_int, _SIZE]),
+    "qmlp_mx_linear_adjoint": (C.c_int, [_TP, _MP, _P, _TP, _TP, _P, _P, C.c_size_t]),
 }
 
 

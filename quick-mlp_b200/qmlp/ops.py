@@ -13,8 +13,8 @@ and loading it needs nothing but this package imported. The operator looks the c
     encoding_adjoint(Tensor input, Tensor? parameters, Tensor adj_output, bool want_input, bool want_parameters,
                      str cfg) -> (Tensor, Tensor)
 
-The operators on feature rows (qmlp/rows.py: layer norm, embedding lookup, routing to experts, products grouped by expert)
-are registered in the same way: X_forward, differentiable, and X_adjoint, its gradients.
+The operators on feature rows (qmlp/rows.py: layer norm, embedding lookup, routing to experts, products grouped by expert, dropout,
+4-bit matrices) are registered in the same way: X_forward, differentiable, and X_adjoint, its gradients.
 
 The schemas are registered here; the kernels and the autograd nodes come with the native call path (csrc/torch/calls.cpp),
 which registers them for CUDA and meta tensors when it is loaded. The first object of the package loads it, not the import:
@@ -45,6 +45,11 @@ SCHEMAS = {
     "combine_adjoint": "(Tensor rows, Tensor adj_output, Tensor weights, Tensor order, Tensor positions, bool want_rows, bool want_weights) -> (Tensor, Tensor)",
     "expert_linear_forward": "(Tensor input, Tensor weight, Tensor offsets, Tensor? bias) -> Tensor",
     "expert_linear_adjoint": "(Tensor input, Tensor adj_output, Tensor weight, Tensor offsets, bool want_input, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)",
+    "dropout_forward": "(Tensor input, Tensor? residual, float probability, int seed, int offset, Tensor? step) -> Tensor",
+    "mx_quantize": "(Tensor input) -> (Tensor, Tensor)",
+    "mx_dequantize": "(Tensor codes, Tensor scales, int channels, ScalarType dtype) -> Tensor",
+    "mx_linear_forward": "(Tensor input, Tensor codes, Tensor scales, Tensor? offsets, Tensor? bias) -> Tensor",
+    "mx_linear_adjoint": "(Tensor adj_output, Tensor codes, Tensor scales, int channels, Tensor? offsets, bool want_input, bool want_bias) -> (Tensor, Tensor)",
 }
 
 _library = torch.library.Library("qmlp_b200", "DEF")

@@ -1,5 +1,5 @@
 """Operators on feature rows, for what stands between an encoding and a network or around several networks: layer norm, lookup of
-latent codes, routing of rows to experts, matrix products grouped by expert.
+latent codes, routing of rows to experts, matrix products grouped by expert, dropout, matrices in 4 bits and products with them.
 
 The reference leaves these to PyTorch. Here they are kernels of the library behind registered operators
 (torch.ops.qmlp_b200.layer_norm_forward, ... in qmlp/ops.py), differentiable once. Features are float32, float16 or
@@ -79,6 +79,52 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
     if is_compiling() and _loaded():
         return torch.ops.qmlp_b200.expert_linear_forward(x, weight, offsets, bias)
     return _capi.calls().expert_linear(x, weight, offsets, bias)
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, residual: Optional[torch.Tensor] = None, step: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """residual + x / (1 - p) where an element is kept, residual (or 0) where it is dropped, with probability p (in units of 2^-16).
+
+    Which are dropped follows from seed and offset (int64) and an element's place: 16 bits of Philox4x32-10 with the key `seed` and the counter
+    (element // 8, offset + step). No mask is stored; another call with the same numbers drops the same. step: an int64 tensor of one element
+    on the device that is added to the offset when the kernel runs, so that a captured graph draws new numbers when its program advances it."""
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.dropout_forward(x, residual, p, seed, offset, step)
+    return _capi.calls().dropout(x, p, seed, offset, residual, step)
+
+
+class MXTensor(NamedTuple):
+    """A matrix (rows, channels) or matrices (matrices, rows, channels) in microscaled 4-bit floating point (MXFP4): 32 channels of a row share a power of two,
+    elements are e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign)."""
+    codes: torch.Tensor     # (..., rows, 16 * ceil(channels / 32)) uint8: two elements a byte, the first in the low bits, zeros behind the last channel
+    scales: torch.Tensor    # (..., ceil(rows / 128), ceil(channels / 128), 32, 4, 4) uint8: [t, c, i, q, j] is the exponent + 127 (255: NaN) of row
+    channels: int           # 128 t + 32 q + i and of the channels from 128 c + 32 j on, zero where there is no such block
+
+
+def mx_quantize(x: torch.Tensor) -> MXTensor:
+    """x (rows, channels) or (matrices, rows, channels) in 4 bits. A block's power of two is floor(log2(largest magnitude)) - 2, elements are rounded to the
+    nearest (ties to the even code, at most 6 in magnitude); a block with an infinity or NaN becomes NaN. No gradient."""
+    if is_compiling() and _loaded():
+        return MXTensor(*torch.ops.qmlp_b200.mx_quantize(x), x.shape[-1])
+    return MXTensor(*_capi.calls().mx_quantize(x), x.shape[-1])
+
+
+def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The values of q in float32, float16 or bfloat16 (exact in the first and the last, in float16 within its range)."""
+    _capi.calls()
+    return torch.ops.qmlp_b200.mx_dequantize(q.codes, q.scales, q.channels, dtype)
+
+
+def mx_linear(x: torch.Tensor, weight: MXTensor, offsets: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows times 4-bit matrices, as expert_linear: y[r] = weight[e] @ q(x[r]) + bias[e] for the rows r in [offsets[e], offsets[e + 1]), with q(x[r]) the row
+    in 4 bits too (mx_quantize); rows of no expert are zeros. A single matrix (channels out, channels in) takes no offsets and a bias (channels out).
+
+    x: (..., channels in) float16 or bfloat16, bias of the same type. Gradients of x and bias: the quantisation of x counts as the identity, the weights are
+    constants."""
+    if x.shape[-1:] != (weight.channels,):
+        raise _capi.QmlpError(f"x must have the weight's {weight.channels} channels")
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.mx_linear_forward(x, weight.codes, weight.scales, offsets, bias)
+    return _capi.calls().mx_linear(x, weight.codes, weight.scales, offsets, bias)
 
 
 class FusedLayerNorm(torch.nn.Module):
