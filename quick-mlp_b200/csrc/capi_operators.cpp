@@ -200,6 +200,7 @@ kernel::MxLinearArgs mxLinear(const qmlp_tensor_t* rows, const qmlp_mx_t* weight
     if (a.rows / kernel::MX_TILE + 2 * kernel::EXPERTS_MAX > 0x7fffffffll / kernel::mxTiles(weight->channels))
         throw std::runtime_error(format("%s has too many rows (%lld) of %d channels", name, static_cast<long long>(a.rows), weight->channels));
     a.type = rows->precision;
+    a.x = rowsOf(rows);   // (forward; the adjoint's rows are gradY)
     a.weight = matrixOf(weight);
     a.numSMs = Library::instance().smCount();
     a.status = Library::instance().statusWord();
@@ -608,7 +609,6 @@ int qmlp_mx_linear_forward(const qmlp_tensor_t* input, const qmlp_mx_t* weight, 
     checkSize(output, 0, a.rows, "output");
     checkSize(output, 1, weight->rows, "output");
     a.offsets = offsets;
-    a.x = rowsOf(input);
     a.y = rowsOf(output);
     checkScratch(tmp_memory, tmp_bytes, kernel::mxLinearBytes(a));
     a.scratch = tmp_memory;

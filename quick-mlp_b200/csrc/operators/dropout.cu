@@ -69,47 +69,52 @@ __global__ void __launch_bounds__(THREADS) dropout_kernel(const __grid_constant_
     const unsigned long long offset = a.offset + (a.step != nullptr ? static_cast<unsigned long long>(*a.step) : 0ull);
     const Key key = {static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32)};
     const long long first = static_cast<long long>(blockIdx.x) * (THREADS * UNROLL) + threadIdx.x;
-    Eight<T> vx[UNROLL], vr[UNROLL];
-    long long at[UNROLL], atResidual[UNROLL], atY[UNROLL];
     if constexpr (ACCESS != SINGLE) {
+        // blocks whose groups are all whole: every load is under way before the first is used
+        if ((static_cast<long long>(blockIdx.x) + 1) * (THREADS * UNROLL * GROUP) <= elements) {
+            Eight<T> vx[UNROLL], vr[UNROLL];
+            T* to[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const long long i = (first + u * THREADS) * GROUP;
-            if (i + GROUP > elements) continue;
-            at[u] = atResidual[u] = atY[u] = i;
-            if constexpr (ACCESS == ROWS) {
-                const long long row = (elements >> 32) == 0 ? static_cast<unsigned>(i) / static_cast<unsigned>(a.channels) : i / a.channels;
-                const int column = static_cast<int>(i - row * a.channels);
-                at[u] = row * a.x.stride + column;
-                atResidual[u] = row * a.residual.stride + column;
-                atY[u] = row * a.y.stride + column;
+            for (int u = 0; u < UNROLL; ++u) {
+                const long long i = (first + u * THREADS) * GROUP;
+                long long at = i, atResidual = i, atY = i;
+                if constexpr (ACCESS == ROWS) {
+                    const long long row = (elements >> 32) == 0 ? static_cast<unsigned>(i) / static_cast<unsigned>(a.channels) : i / a.channels;
+                    const int column = static_cast<int>(i - row * a.channels);
+                    at = row * a.x.stride + column;
+                    atResidual = row * a.residual.stride + column;
+                    atY = row * a.y.stride + column;
+                }
+                vx[u] = loadEight<T>(x + at);
+                if constexpr (RESIDUAL) vr[u] = loadEight<T>(residual + atResidual);
+                to[u] = y + atY;
             }
-            vx[u] = loadEight<T>(x + at[u]);
-            if constexpr (RESIDUAL) vr[u] = loadEight<T>(residual + atResidual[u]);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                uint32_t word[4];
+                philox(first + u * THREADS, offset, key, word);
+                float f[GROUP], r[GROUP];
+                unpackEight<T>(vx[u], f);
+                if constexpr (RESIDUAL) unpackEight<T>(vr[u], r);
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    const uint32_t number = j & 1 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
+                    // (selected, not multiplied: a dropped infinity or NaN is a zero)
+                    f[j] = number >= a.cut ? f[j] * scale : 0.f;
+                    if constexpr (RESIDUAL) f[j] += r[j];
+                }
+#pragma unroll
+                for (int k = 0; k < GROUP / WIDE<T>; ++k)
+                    store<T, WIDE<T>>(to[u] + k * WIDE<T>, pack<T, WIDE<T>>(*reinterpret_cast<const float (*)[WIDE<T>]>(&f[k * WIDE<T>])));
+            }
+            return;
         }
     }
-#pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const long long group = first + u * THREADS, i = group * GROUP;
         if (i >= elements) break;
         uint32_t word[4];
         philox(group, offset, key, word);
-        if (ACCESS != SINGLE && i + GROUP <= elements) {
-            float f[GROUP], r[GROUP];
-            unpackEight<T>(vx[u], f);
-            if constexpr (RESIDUAL) unpackEight<T>(vr[u], r);
-#pragma unroll
-            for (int j = 0; j < GROUP; ++j) {
-                const uint32_t number = j & 1 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
-                // (selected, not multiplied: a dropped infinity or NaN is a zero)
-                f[j] = number >= a.cut ? f[j] * scale : 0.f;
-                if constexpr (RESIDUAL) f[j] += r[j];
-            }
-#pragma unroll
-            for (int k = 0; k < GROUP / WIDE<T>; ++k)
-                store<T, WIDE<T>>(y + atY[u] + k * WIDE<T>, pack<T, WIDE<T>>(*reinterpret_cast<const float (*)[WIDE<T>]>(&f[k * WIDE<T>])));
-            continue;
-        }
         long long row = i / a.channels;
         int column = static_cast<int>(i - row * a.channels);
 #pragma unroll

@@ -13,9 +13,10 @@ struct RowTile {
     long long row;
     int rows;
 };
-__device__ __forceinline__ RowTile rowTile(const MxMatrix& q, int tilesPerMatrix, long long tile)
+__device__ __forceinline__ RowTile rowTile(const MxMatrix& q, int tilesPerMatrix, unsigned tile)
 {
-    const long long matrix = tile / tilesPerMatrix, within = (tile - matrix * tilesPerMatrix) * MX_TILE;
+    const unsigned matrix = static_cast<unsigned>(tile) / static_cast<unsigned>(tilesPerMatrix);
+    const long long within = static_cast<long long>(static_cast<unsigned>(tile) - matrix * tilesPerMatrix) * MX_TILE;
     return {matrix * q.rows + within, static_cast<int>(min(static_cast<long long>(MX_TILE), q.rows - within))};
 }
 
@@ -24,88 +25,98 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_quantize_kernel(const __grid_
                                                                    int codeBytes)
 {
     chained();
-    __shared__ uint4 words[MX_TILE / 4];
-    const long long tile = blockIdx.x / chunks;
-    const int chunk = blockIdx.x - static_cast<int>(tile) * chunks;
+    __shared__ __align__(16) unsigned char tileScales[MX_TILE_BYTES];
+    const unsigned tile = blockIdx.x / static_cast<unsigned>(chunks);
+    const int chunk = static_cast<int>(blockIdx.x - tile * chunks);
     const RowTile t = rowTile(q, tilesPerMatrix, tile);
     quantizeTile<T, LANES, ALIGNED>(x + t.row * stride, stride, t.rows, chunk, q.channels, q.codes + t.row * codeBytes, codeBytes,
-                                    q.scales + (tile * chunks + chunk) * MX_TILE_BYTES, reinterpret_cast<uint32_t*>(words));
+                                    q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES, tileScales);
 }
 
+// Rows that 16-byte accesses cannot write: a warp per row, a lane per channel of a block, element by element side by side (20011 rows of 777 floats: 16 elements
+// of a row per thread 75 us, so 25).
 template <class T, int LANES, bool ALIGNED>
 __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __grid_constant__ MxMatrix q, T* __restrict__ y, long long stride, int tilesPerMatrix, int chunks,
                                                                      int codeBytes)
 {
     chained();
-    constexpr int PASSES = TILE_PASSES<LANES>, STEP = TILE_THREADS / LANES;
-    const long long tile = blockIdx.x / chunks;
-    const int chunk = blockIdx.x - static_cast<int>(tile) * chunks;
+    const unsigned tile = blockIdx.x / static_cast<unsigned>(chunks);
+    const int chunk = static_cast<int>(blockIdx.x - tile * chunks);
     const RowTile t = rowTile(q, tilesPerMatrix, tile);
-    const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, c = chunk * MX_TILE + lane * 8;
-    if (c >= q.channels) return;
-    const unsigned char *codes = q.codes + t.row * codeBytes + c / 2, *scales = q.scales + (tile * chunks + chunk) * MX_TILE_BYTES + lane / 4;
-    uint32_t code[PASSES], scale[PASSES];
+    const unsigned char *codes = q.codes + t.row * codeBytes, *scales = q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES;
+    if constexpr (!ALIGNED) {
+        constexpr int AT_ONCE = 4, BLOCKS = MX_TILE / MX_BLOCK;
+        const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, c = chunk * MX_TILE + lane;
+        for (int i = warp; i < t.rows; i += TILE_WARPS * AT_ONCE) {
+            uint32_t code[AT_ONCE][BLOCKS], scale[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = i * STEP + first;
-        code[i] = scale[i] = 0;
-        if (r >= t.rows) continue;
-        code[i] = *reinterpret_cast<const uint32_t*>(codes + static_cast<long long>(r) * codeBytes);
-        scale[i] = scales[(r & 31) * 16 + (r >> 5) * 4];
-    }
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int r = min(i + k * TILE_WARPS, t.rows - 1);
+                scale[k] = *reinterpret_cast<const uint32_t*>(scales + (r & 31) * 16 + (r >> 5) * 4);
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = i * STEP + first;
-        if (r >= t.rows) break;
-        float f[8];
-        decodeEight(code[i], f);
-        const float power = powerOf(scale[i]);
+                for (int b = 0; b < BLOCKS; ++b)
+                    code[k][b] = c + b * MX_BLOCK < q.channels ? codes[static_cast<long long>(r) * codeBytes + (c + b * MX_BLOCK) / 2] : 0u;
+            }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= power;
-        T* at = y + (t.row + r) * stride + c;
-        if constexpr (ALIGNED) {
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int r = i + k * TILE_WARPS;
+                if (r >= t.rows) break;
 #pragma unroll
-            for (int k = 0; k < 8 / WIDE<T>; ++k) store<T, WIDE<T>>(at + k * WIDE<T>, pack<T, WIDE<T>>(*reinterpret_cast<const float (*)[WIDE<T>]>(&f[k * WIDE<T>])));
-        } else {
+                for (int b = 0; b < BLOCKS; ++b)
+                    if (c + b * MX_BLOCK < q.channels)
+                        y[(t.row + r) * stride + c + b * MX_BLOCK] = Element<T>::from(decodeOne(code[k][b] >> (lane & 1) * 4) * powerOf(scale[k] >> b * 8 & 255u));
+            }
+        }
+    } else {
+        // 16 bytes of a row a thread, neighbours side by side
+        constexpr int W = WIDE<T>, ROW = LANES * SIXTEEN / W, STEP = TILE_THREADS / ROW, PASSES = MX_TILE / STEP, AT_ONCE = PASSES < 8 ? PASSES : 8;
+        const int lane = threadIdx.x % ROW, first = threadIdx.x / ROW, c = chunk * MX_TILE + lane * W;
+        if (c >= q.channels) return;
+        codes += c / 2;
+        T* at = y + (t.row + first) * stride + c;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c + j < q.channels) at[j] = Element<T>::from(f[j]);
+        for (int begin = 0; begin < PASSES; begin += AT_ONCE) {
+            uint32_t code[AT_ONCE], scale[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int r = min((begin + i) * STEP + first, t.rows - 1);
+                if constexpr (W == 8) code[i] = *reinterpret_cast<const uint32_t*>(codes + static_cast<long long>(r) * codeBytes);
+                else code[i] = *reinterpret_cast<const uint16_t*>(codes + static_cast<long long>(r) * codeBytes);
+                scale[i] = scales[(r & 31) * 16 + (r >> 5) * 4 + lane * W / MX_BLOCK];
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                float f[8], out[W];
+                if constexpr (W == 8) decodeEight(code[i], f);
+                else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) f[j] = decodeOne(code[i] >> 4 * j);
+                }
+                const float power = powerOf(scale[i]);
+#pragma unroll
+                for (int j = 0; j < W; ++j) out[j] = f[j] * power;
+                if ((begin + i) * STEP + first < t.rows) store<T, W>(at, pack<T, W>(out));
+                at += STEP * stride;
+            }
         }
     }
 }
 
-// whether rows allow accesses of eight elements
 template <class T>
-bool aligned(const Rows& r, int channels)
+cudaError_t quantize(const MxMatrix& q, int type, const Rows& x, unsigned blocks, cudaStream_t stream)
 {
-    return (reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.stride % WIDE<T> == 0 && channels % 8 == 0;
-}
-// calls f(lanes, aligned) with both as constants
-template <class F>
-cudaError_t byShape(int channels, bool aligned, F&& f)
-{
-    auto lanes = [&](auto n) { return aligned ? f(n, std::true_type()) : f(n, std::false_type()); };
-    switch (lanesOf(channels)) {
-    case 4: return lanes(std::integral_constant<int, 4>());
-    case 8: return lanes(std::integral_constant<int, 8>());
-    default: return lanes(std::integral_constant<int, 16>());
-    }
-}
-template <class T>
-cudaError_t quantize(const MxMatrix& q, const Rows& x, unsigned blocks, cudaStream_t stream)
-{
-    return byShape(q.channels, aligned<T>(x, q.channels), [&](auto lanes, auto whole) {
-        launchChained(mx_quantize_kernel<T, decltype(lanes)::value, decltype(whole)::value>, blocks, TILE_THREADS, 0, stream, 1, q, static_cast<const T*>(x.data), x.stride,
-                      mxTiles(q.rows), mxTiles(q.channels), mxCodeBytes(q.channels));
+    return byLanes(x, type, q.channels, [&](auto lanes, auto aligned) {
+        launchChained(mx_quantize_kernel<T, decltype(lanes)::value, decltype(aligned)::value>, blocks, TILE_THREADS, 0, stream, 1, q, static_cast<const T*>(x.data), x.stride, mxTiles(q.rows),
+                      mxTiles(q.channels), mxCodeBytes(q.channels));
         return cudaGetLastError();
     });
 }
 template <class T>
-cudaError_t dequantize(const MxMatrix& q, const Rows& y, unsigned blocks, cudaStream_t stream)
+cudaError_t dequantize(const MxMatrix& q, int type, const Rows& y, unsigned blocks, cudaStream_t stream)
 {
-    return byShape(q.channels, aligned<T>(y, q.channels), [&](auto lanes, auto whole) {
-        launchChained(mx_dequantize_kernel<T, decltype(lanes)::value, decltype(whole)::value>, blocks, TILE_THREADS, 0, stream, 1, q, static_cast<T*>(y.data), y.stride,
-                      mxTiles(q.rows), mxTiles(q.channels), mxCodeBytes(q.channels));
+    return byLanes(y, type, q.channels, [&](auto lanes, auto aligned) {
+        launchChained(mx_dequantize_kernel<T, decltype(aligned)::value ? decltype(lanes)::value : 8, decltype(aligned)::value>, blocks, TILE_THREADS, 0, stream, 1, q, static_cast<T*>(y.data), y.stride, mxTiles(q.rows),
+                      mxTiles(q.channels), mxCodeBytes(q.channels));
         return cudaGetLastError();
     });
 }
@@ -123,14 +134,14 @@ cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStr
     unsigned blocks;
     if (!blocksOf(q, blocks)) return cudaErrorInvalidConfiguration;
     if (blocks == 0) return cudaSuccess;
-    return type == TYPE_FLOAT ? quantize<float>(q, x, blocks, stream) : type == TYPE_HALF ? quantize<__half>(q, x, blocks, stream) : quantize<__nv_bfloat16>(q, x, blocks, stream);
+    return type == TYPE_FLOAT ? quantize<float>(q, type, x, blocks, stream) : type == TYPE_HALF ? quantize<__half>(q, type, x, blocks, stream) : quantize<__nv_bfloat16>(q, type, x, blocks, stream);
 }
 cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream)
 {
     unsigned blocks;
     if (!blocksOf(q, blocks)) return cudaErrorInvalidConfiguration;
     if (blocks == 0) return cudaSuccess;
-    return type == TYPE_FLOAT ? dequantize<float>(q, y, blocks, stream) : type == TYPE_HALF ? dequantize<__half>(q, y, blocks, stream) : dequantize<__nv_bfloat16>(q, y, blocks, stream);
+    return type == TYPE_FLOAT ? dequantize<float>(q, type, y, blocks, stream) : type == TYPE_HALF ? dequantize<__half>(q, type, y, blocks, stream) : dequantize<__nv_bfloat16>(q, type, y, blocks, stream);
 }
 
 } // namespace kernel

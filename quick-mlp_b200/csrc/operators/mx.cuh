@@ -34,6 +34,8 @@ __device__ __forceinline__ uint32_t encodeEight(const float (&f)[8])
         : "=r"(r) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
     return r;
 }
+// a code to its value: an fp32 number with one bit of mantissa, whose exponent is off by 126
+__device__ __forceinline__ float decodeOne(uint32_t code) { return __uint_as_float((code & 7) << 22 | (code & 8) << 28) * 0x1p126f; }
 // eight codes to their values
 __device__ __forceinline__ void decodeEight(uint32_t codes, float (&f)[8])
 {
@@ -49,77 +51,131 @@ __device__ __forceinline__ void decodeEight(uint32_t codes, float (&f)[8])
     }
 }
 
-// eight elements of a row from channel c on, zeros behind the last
+// SIXTEEN channels of a row as they lie in memory; ALIGNED: by accesses of 16 bytes, else one by one
+constexpr int SIXTEEN = 16;
 template <class T>
-struct Eight {
-    Pack<T, WIDE<T>> v[8 / WIDE<T>];
+struct Sixteen {
+    Pack<T, WIDE<T>> v[SIXTEEN / WIDE<T>];
 };
+// of which `left` (at least one) are there. Asked for unconditionally, what is not there as the first again: a load that depends on a condition is waited for
+// where it is issued (131072 rows of 1024 bfloat16 quantised in 83 us, without conditions in 57). trim() makes zeros of what is not there.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ Eight<T> loadEight(const T* row, int c, int channels)
+__device__ __forceinline__ Sixteen<T> loadSixteen(const T* at, int left)
 {
-    Eight<T> r;
+    Sixteen<T> r;
     if constexpr (ALIGNED) {
 #pragma unroll
-        for (int i = 0; i < 8 / WIDE<T>; ++i) r.v[i] = load<T, WIDE<T>>(row + c + i * WIDE<T>);
+        for (int i = 0; i < SIXTEEN / WIDE<T>; ++i) r.v[i] = load<T, WIDE<T>>(at + (i * WIDE<T> < left ? i * WIDE<T> : 0));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r.v[i / WIDE<T>].v[i % WIDE<T>] = c + i < channels ? row[c + i] : Element<T>::from(0.f);
+        for (int i = 0; i < SIXTEEN; ++i) r.v[i / WIDE<T>].v[i % WIDE<T>] = at[i < left ? i : 0];
     }
     return r;
 }
-template <class T>
-__device__ __forceinline__ void unpackEight(const Eight<T>& p, float (&f)[8])
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void trim(Sixteen<T>& v, int left)
 {
+    if (left >= SIXTEEN) return;
+    constexpr int STEP = ALIGNED ? WIDE<T> : 1;
 #pragma unroll
-    for (int i = 0; i < 8 / WIDE<T>; ++i) unpack<T, WIDE<T>>(p.v[i], *reinterpret_cast<float (*)[WIDE<T>]>(&f[i * WIDE<T>]));
+    for (int i = 0; i < SIXTEEN; i += STEP)
+        if (i >= left) {
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) v.v[i / WIDE<T>].v[(i + j) % WIDE<T>] = Element<T>::from(0.f);
+        }
+}
+// bits of the largest magnitude as fp32, a NaN's if there is one; 16-bit elements are compared in pairs
+template <class T>
+__device__ __forceinline__ uint32_t largestOf(const Sixteen<T>& p)
+{
+    if constexpr (std::is_same<T, float>::value) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < SIXTEEN; ++i) m = max(m, __float_as_uint(p.v[i / WIDE<T>].v[i % WIDE<T>]) & 0x7fffffffu);
+        return m;
+    } else {
+        using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        Pair m[4];
+        Pair w[SIXTEEN / 2];
+        memcpy(w, &p, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = __hmax2_nan(__habs2(w[i]), __habs2(w[i + 4]));
+        m[0] = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
+        return __float_as_uint(Element<T>::to(__hmax_nan(m[0].x, m[0].y))) & 0x7fffffffu;
+    }
+}
+// codes of sixteen elements whose block has this scale
+template <class T>
+__device__ __forceinline__ uint2 encodeSixteen(const Sixteen<T>& p, uint32_t scale)
+{
+    float f[SIXTEEN];
+    const float inverse = inverseOf(scale);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        // (a power of two that bfloat16 has: products of pairs are exact, or too small to matter)
+        const __nv_bfloat162 pair = __float2bfloat162_rn(inverse);
+        __nv_bfloat162 w[SIXTEEN / 2];
+        memcpy(w, &p, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < SIXTEEN / 2; ++i) {
+            w[i] = __hmul2(w[i], pair);
+            f[2 * i] = __low2float(w[i]);
+            f[2 * i + 1] = __high2float(w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < SIXTEEN / WIDE<T>; ++i) unpack<T, WIDE<T>>(p.v[i], *reinterpret_cast<float (*)[WIDE<T>]>(&f[i * WIDE<T>]));
+#pragma unroll
+        for (int i = 0; i < SIXTEEN; ++i) f[i] *= inverse;
+    }
+    uint2 r = {encodeEight(*reinterpret_cast<const float (*)[8]>(&f[0])), encodeEight(*reinterpret_cast<const float (*)[8]>(&f[8]))};
+    if (scale == 255) r = make_uint2(0, 0);
+    return r;
 }
 
-// A block of TILE_THREADS threads works on a tile of 128 rows x 128 channels; LANES threads share a row, 8 channels each (16 of them for 128 channels, fewer
-// for matrices that are narrower).
-constexpr int TILE_THREADS = 256;
-template <int LANES> constexpr int TILE_PASSES = MX_TILE * LANES / TILE_THREADS;
+// A block of TILE_THREADS threads works on a tile of 128 rows x 128 channels. LANES threads share a row, 16 channels each (8 of them for 128 channels,
+// fewer for matrices that are narrower), two neighbours a block of 32.
+constexpr int TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32;
 
-// `rows` rows of x from `x` on, channels from 128 * chunk on, to codes (rows of codeBytes) and a tile of scales. `words`: 128 words of shared memory, which
-// the caller may use again after its next barrier.
+// `rows` rows of x, channels from 128 * chunk on, to codes (rows of codeBytes) and a tile of scales; tileScales: 512 bytes of shared memory.
 template <class T, int LANES, bool ALIGNED>
 __device__ __forceinline__ void quantizeTile(const T* x, long long stride, int rows, int chunk, int channels, unsigned char* codes, int codeBytes, unsigned char* scales,
-                                             uint32_t* words)
+                                             unsigned char* tileScales)
 {
-    constexpr int PASSES = TILE_PASSES<LANES>, STEP = TILE_THREADS / LANES;
-    const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, c = chunk * MX_TILE + lane * 8;
-    Eight<T> v[PASSES];
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = i * STEP + first;
-        v[i] = {};
-        if (r < rows && c < channels) v[i] = loadEight<T, ALIGNED>(x + r * stride, c, channels);
+    if constexpr (LANES < 8) {   // the blocks that are not there
+        if (threadIdx.x < MX_TILE) *reinterpret_cast<uint32_t*>(tileScales + threadIdx.x * 4) = 0;
+        __syncthreads();
     }
+    constexpr int PASSES = MX_TILE * LANES / TILE_THREADS, STEP = TILE_THREADS / LANES;
+    const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, c = chunk * MX_TILE + lane * SIXTEEN, left = channels - c;
+    const T* from = x + (left > 0 ? c : 0);
+    Sixteen<T> v[PASSES];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) v[i] = loadSixteen<T, ALIGNED>(from + min(i * STEP + first, rows - 1) * stride, left);
+    unsigned char* to = codes + static_cast<long long>(first) * codeBytes + c / 2;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int r = i * STEP + first;
-        float f[8];
-        unpackEight<T>(v[i], f);
-        uint32_t largest = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) largest = max(largest, __float_as_uint(f[j]) & 0x7fffffffu);
+        trim<T, ALIGNED>(v[i], r < rows ? left : 0);
+        uint32_t largest = largestOf<T>(v[i]);
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const uint32_t scale = scaleOf(largest);
-        const float inverse = inverseOf(scale);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = scale == 255 ? 0.f : f[j] * inverse;
-        const uint32_t code = encodeEight(f);
-        if (r < rows && c / 2 < codeBytes) *reinterpret_cast<uint32_t*>(codes + static_cast<long long>(r) * codeBytes + c / 2) = code;
-        uint32_t word = scale << (lane / 4 * 8);
-        if constexpr (LANES > 4) word |= __shfl_xor_sync(0xffffffffu, word, 4);
-        if constexpr (LANES > 8) word |= __shfl_xor_sync(0xffffffffu, word, 8);
-        if (lane == 0) words[(r & 31) * 4 + (r >> 5)] = word;
+        const uint2 code = encodeSixteen<T>(v[i], scale);
+        if (r < rows && c / 2 < codeBytes) *reinterpret_cast<uint2*>(to) = code;
+        to += STEP * codeBytes;
+        if ((lane & 1) == 0) tileScales[(r & 31) * 16 + (r >> 5) * 4 + lane / 2] = static_cast<unsigned char>(scale);
     }
     __syncthreads();
-    if (threadIdx.x < MX_TILE_BYTES / 16) *reinterpret_cast<uint4*>(scales + threadIdx.x * 16) = *reinterpret_cast<const uint4*>(words + threadIdx.x * 4);
+    if (threadIdx.x < MX_TILE_BYTES / 16) *reinterpret_cast<uint4*>(scales + threadIdx.x * 16) = *reinterpret_cast<const uint4*>(tileScales + threadIdx.x * 16);
 }
-// lanes that a row of `channels` channels takes
-inline int lanesOf(int channels) { return channels > 64 ? 16 : channels > 32 ? 8 : 4; }
+// calls f(integral_constant of LANES, of ALIGNED) for rows of `channels` elements of `type`
+template <class F>
+cudaError_t byLanes(const Rows& rows, int type, int channels, F&& f)
+{
+    auto aligned = [&](auto lanes) { return wide(rows, type, channels) ? f(lanes, std::true_type()) : f(lanes, std::false_type()); };
+    if (channels > 64) return aligned(std::integral_constant<int, 8>());
+    if (channels > 32) return aligned(std::integral_constant<int, 4>());
+    return aligned(std::integral_constant<int, 2>());
+}
 
 } // namespace mx
 } // namespace kernel

@@ -27,28 +27,32 @@ using namespace products;
 
 constexpr int STEP_CHANNELS = 256, SCALE_BYTES = 2 * MX_TILE_BYTES;   // channels of a step (128 bytes of codes), scales of 128 rows of a step
 
+constexpr int PAIR_EXPERTS = 1024;   // whose lists leave shared memory for five stages
+constexpr int MX_THREADS = (2 + EPILOGUE_WARPS) * 32, OUT_BYTES = 32 * 128;   // OUT_BYTES: 32 rows x 64 columns of D, per warp of the epilogue
+
 // BN: columns of D; CTAS: blocks that share a tile, each with BM rows of D and BN / CTAS of the columns of B
 template <int BN, int CTAS>
 struct MxLayout {
     static constexpr int BCOLS = BN / CTAS, ABYTES = BM * 128, BBYTES = BCOLS * 128;
     static constexpr int BTILES = (BN + MX_TILE - 1) / MX_TILE;       // tiles of scales of the columns (each block has all of them)
     static constexpr int SCALES = ABYTES + BBYTES, STAGE = SCALES + SCALE_BYTES * (1 + BTILES);
-    static constexpr int STAGES = std::min(8, 192 * 1024 / STAGE);
+    // Two blocks per SM for narrow layers: a tile of 128 x 64 and a step or two costs the warp that issues its products more time (1250 clocks to walk on, wait
+    // four times and issue) than anything else.
+    static constexpr int BLOCKS = BN == 64 ? 2 : 1, STAGES = BN == 64 ? 2 : BN == 128 ? 4 : 5, EXPERTS = CTAS == 2 ? PAIR_EXPERTS : EXPERTS_MAX;
     // tensor memory: accumulators, then two sets of scales, used in turn: of 128 rows (4 columns) for two times 128 channels, of the columns likewise
     static constexpr bool OVERLAP = BN == 256;
     static constexpr int SECOND = OVERLAP ? BN - 64 : BN;             // column of the second accumulator
     static constexpr int SCALE_AT = SECOND + BN, SCALE_SET = 32, SCALE_B = 8, SCALE_B_STEP = 4 * BTILES;
     static constexpr int TMEM = SCALE_AT + 2 * SCALE_SET <= 256 ? 256 : 512;
-    static constexpr int EPILOGUE = 32 * 64 + BN * 4, OUT = EPILOGUE_WARPS * EPILOGUE;   // per warp: 32 rows x 32 elements of 16 bits, a bias
+    static constexpr int OUT = STAGES * STAGE, BIAS = OUT + EPILOGUE_WARPS * OUT_BYTES, CONTROL = BIAS + EPILOGUE_WARPS * BN * 4;
     // barriers: full, empty (STAGES each), accumulator full, empty, overlap free (2 each), drain; then flag and tensor memory
     static constexpr int FULL = 0, EMPTY = 64, ACC_FULL = 128, ACC_EMPTY = 144, SHARED_FREE = 160, DRAIN = 176, FAILED = 184, BASE = 188, BARS = 192;
     // 1 KB for the alignment of the ring
-    static constexpr int bytes(int experts) { return 1024 + STAGES * STAGE + OUT + BARS + listInts(experts) * 4; }
+    static constexpr int bytes(int experts) { return 1024 + CONTROL + BARS + listInts(experts) * 4; }
     static_assert(SCALE_AT + 2 * SCALE_SET <= TMEM && SCALE_B + 2 * SCALE_B_STEP <= SCALE_SET, "tensor memory");
-    static_assert(STAGE % 1024 == 0 && STAGES >= 3, "ring");
-    static_assert(bytes(EXPERTS_MAX) + 512 <= 227 * 1024, "shared memory");
+    static_assert(STAGE % 1024 == 0 && STAGES <= 8, "ring");
+    static_assert(BLOCKS * (bytes(EXPERTS) + 1536) <= 228 * 1024, "shared memory");
 };
-constexpr int MX_THREADS = (2 + EPILOGUE_WARPS) * 32;
 
 // ---- PTX ---------------------------------------------------------------------------------------------------------------
 // a product of 64 channels; the instruction descriptor names the scales' places within their words
@@ -73,58 +77,149 @@ __device__ __forceinline__ void copyScales(uint32_t lead, uint32_t to, uint64_t 
     else
         asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(to), "l"(from), "r"(lead) : "memory");
 }
+// Tells the leader that tensor memory was read. Relaxed: what was read is in registers (tcgen05.wait::ld), and a release would wait for the warp's stores of
+// D as well, which took a microsecond per tile (16 experts, 32768 rows, 1024 -> 1024 bfloat16: 35 us for the product, RELAXED us so).
+__device__ __forceinline__ void clusterArriveRelaxed(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // descriptor of a tile of scales: no swizzle, groups of 8 rows of 16 bytes lie 128 bytes apart
 __device__ __forceinline__ uint64_t scaleDescriptor(uint32_t address) { return static_cast<uint64_t>((address >> 4) & 0x3FFFu) | (8ull << 32) | (1ull << 46); }
 
 // ---- the rows in 4 bits ----------------------------------------------------------------------------------------------------
 // Tiles of 128 rows of one expert, in the order of the product's units (of tileRows rows): tile t of all is part t % (tileRows / 128) of unit t / (tileRows / 128).
-template <class T, int LANES, bool ALIGNED>
-__global__ void __launch_bounds__(TILE_THREADS) mx_rows_kernel(const __grid_constant__ ProductArgs p, const T* __restrict__ x, long long stride, unsigned char* __restrict__ codes,
-                                                               unsigned char* __restrict__ scales, int chunks, int codeBytes)
+// First row and rows of every tile (`piece` rows, or what is left), a thread each; where the experts' units begin, if `unitsBefore` is given. (A block of the quantisation that looks for its tile's expert itself has to add up the offsets first: as
+// persistent blocks, which do it once, that kernel took 103 us for 131072 rows of 1024 bfloat16, a block per tile with this list ROWS us.)
+__global__ void __launch_bounds__(TILE_THREADS) mx_tiles_kernel(const __grid_constant__ ProductArgs p, int2* __restrict__ list, int tiles, int piece,
+                                                                int* __restrict__ unitsBefore)
 {
     extern __shared__ int lists[];
-    __shared__ uint4 words[2][MX_TILE / 4];
     chained();
     int *bounds = lists, *before = lists + listStride(p.experts);
     planExperts<FORWARD>(p, bounds, before, nullptr, TILE_THREADS);
     __syncthreads();
-    const int parts = p.tileRows / MX_TILE;
-    const long long items = static_cast<long long>(before[p.experts]) * parts * chunks;
-    int flip = 0;
-    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-        const long long tile = item / chunks;
-        const int chunk = static_cast<int>(item - tile * chunks), unit = static_cast<int>(tile / parts), part = static_cast<int>(tile - static_cast<long long>(unit) * parts);
+    const int tile = blockIdx.x * TILE_THREADS + threadIdx.x, parts = p.tileRows / piece, unit = tile / parts;
+    if (unitsBefore != nullptr && blockIdx.x == 0)
+        for (int e = threadIdx.x; e <= p.experts; e += TILE_THREADS) unitsBefore[e] = before[e];
+    if (tile >= tiles) return;
+    int2 found = {0, 0};
+    if (unit < before[p.experts]) {
         int low = 0, high = p.experts;   // the last expert whose units begin at or before this one (experts without units end up in front of it)
         while (high - low > 1) {
             const int middle = (low + high) / 2;
             if (before[middle] <= unit) low = middle;
             else high = middle;
         }
-        const long long begin = bounds[low] + static_cast<long long>(unit - before[low]) * p.tileRows + part * MX_TILE;
-        const long long left = bounds[low + 1] - begin;
-        if (left <= 0) continue;   // the second half of a unit's rows may be empty
-        quantizeTile<T, LANES, ALIGNED>(x + begin * stride, stride, static_cast<int>(min(left, static_cast<long long>(MX_TILE))), chunk, p.sum, codes + begin * codeBytes, codeBytes,
-                                        scales + item * MX_TILE_BYTES, reinterpret_cast<uint32_t*>(words[flip]));
-        flip ^= 1;   // (the next barrier lies between this use and the next of the same words)
+        const long long begin = bounds[low] + static_cast<long long>(unit - before[low]) * p.tileRows + (tile - unit * parts) * piece;
+        const long long left = bounds[low + 1] - begin;   // (the second part of a unit may be empty)
+        if (left > 0) found = make_int2(static_cast<int>(begin), static_cast<int>(min(left, static_cast<long long>(piece))));
+    }
+    list[tile] = found;
+}
+// A block per tile of 128 rows x 128 channels. `list`: mx_tiles_kernel's, or null where the rows are one expert's.
+template <class T, int LANES, bool ALIGNED>
+__global__ void __launch_bounds__(TILE_THREADS) mx_rows_kernel(const int2* __restrict__ list, const T* __restrict__ x, long long stride, long long rows, int channels,
+                                                               unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int chunks, int codeBytes)
+{
+    __shared__ __align__(16) unsigned char tileScales[MX_TILE_BYTES];
+    const unsigned tile = blockIdx.x / static_cast<unsigned>(chunks);
+    const int chunk = static_cast<int>(blockIdx.x - tile * chunks);
+    chained();
+    int2 t;
+    if (list != nullptr) t = list[tile];
+    else {
+        const long long begin = static_cast<long long>(tile) * MX_TILE;
+        t = make_int2(static_cast<int>(begin), static_cast<int>(max(0ll, min(static_cast<long long>(MX_TILE), rows - begin))));
+    }
+    if (t.y == 0) return;
+    quantizeTile<T, LANES, ALIGNED>(x + t.x * stride, stride, t.y, chunk, channels, codes + static_cast<long long>(t.x) * codeBytes, codeBytes,
+                           scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES, tileScales);
+}
+
+// ---- epilogue ------------------------------------------------------------------------------------------------------------------
+// Writes of D go by TMA, 32 rows x 64 columns (128 bytes of a row) at a time, from shared memory: 131072 rows of 1024 columns through the warps, 64 bytes of a
+// row at a time, were written at 3.1 TB/s. Runs that end within 32 rows, and rows that the TMA cannot write, take the other way.
+__device__ __forceinline__ void tmaStore(const CUtensorMap* map, int x, int y, uint32_t from)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(from) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tmaStoresRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tmaStoresDone() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void tmemWait32(float (&v)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
+struct OutTile {
+    int row, rows, column, columns;   // first row of the warp's 32, how many are to be written; first column, how many are left
+    long long stride;
+    bool wide;
+};
+// A warp's 32 lanes of an accumulator of BN columns from `from` on, plus a bias. `sharedLast`: the last 64 columns first (those that the other accumulator begins
+// with); `read` is called when the first 64 are.
+template <class T, int BN, class F>
+__device__ __forceinline__ void storeAccumulator(uint32_t from, bool sharedLast, const CUtensorMap* map, T* out, const OutTile& o, unsigned char* mine, const float* bias, F&& read)
+{
+    const int lane = threadIdx.x & 31;
+    const bool whole = o.wide && o.rows >= 32;
+#pragma unroll 1
+    for (int i = 0; i < BN / 64; ++i) {
+        const int c = (sharedLast ? (i + BN / 64 - 1) % (BN / 64) : i) * 64;
+        const bool used = c < o.columns && o.rows > 0;
+        if (used) {
+            if (lane == 0) tmaStoresRead();   // what was written from this memory last
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[32];
+                tmemLoad32(from + c + h * 32, v);
+                tmemWait32(v);
+                if (h == 1 && i == 0) read();
+                const int c0 = c + h * 32;
+                if (bias != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(bias + c0 + j);
+                        v[j] += f.x;
+                        v[j + 1] += f.y;
+                        v[j + 2] += f.z;
+                        v[j + 3] += f.w;
+                    }
+                }
+                if (whole) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        store<T, 8>(reinterpret_cast<T*>(mine + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)), pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[j * 8])));
+                } else if (c0 < o.columns) {
+                    storeTile<T>(v, mine, out + static_cast<long long>(o.row) * o.stride + o.column, o.stride, o.rows, c0, o.columns, o.wide);
+                }
+            }
+            if (whole) {
+                fenceProxyAsync();
+                __syncwarp();
+                if (lane == 0) tmaStore(map, o.column + c, o.row, smemAddress(mine));
+            }
+        } else if (i == 0) {
+            read();
+        }
     }
 }
 
 // ---- the product -------------------------------------------------------------------------------------------------------------
 template <class T, int BN, int CTAS>
-__global__ void __launch_bounds__(MX_THREADS, 1)
+__global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
     mx_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapScaleA,
-                      const __grid_constant__ CUtensorMap mapScaleB, const __grid_constant__ ProductArgs p, int chunks)
+                      const __grid_constant__ CUtensorMap mapScaleB, const __grid_constant__ CUtensorMap mapOut, const __grid_constant__ ProductArgs p, int chunks)
 {
     using L = MxLayout<BN, CTAS>;
     extern __shared__ unsigned char dynamic[];
     const uint32_t raw = smemAddress(dynamic), ring = (raw + 1023u) & ~1023u;
     unsigned char* base = dynamic + (ring - raw);
-    unsigned char* outStage = base + L::STAGES * L::STAGE;
-    const uint32_t bars = ring + L::STAGES * L::STAGE + L::OUT;
+    unsigned char* control = base + L::CONTROL;
+    const uint32_t bars = ring + L::CONTROL;
     const uint32_t full = bars + L::FULL, empty = bars + L::EMPTY, accFull = bars + L::ACC_FULL, accEmpty = bars + L::ACC_EMPTY, sharedFree = bars + L::SHARED_FREE;
-    volatile int* failed = reinterpret_cast<volatile int*>(outStage + L::OUT + L::FAILED);
-    uint32_t* tmemBase = reinterpret_cast<uint32_t*>(outStage + L::OUT + L::BASE);
-    int *bounds = reinterpret_cast<int*>(outStage + L::OUT + L::BARS), *before = bounds + listStride(p.experts);
+    volatile int* failed = reinterpret_cast<volatile int*>(control + L::FAILED);
+    uint32_t* tmemBase = reinterpret_cast<uint32_t*>(control + L::BASE);
+    int *bounds = reinterpret_cast<int*>(control + L::BARS), *before = bounds + listStride(p.experts);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = CTAS == 1 ? 0u : clusterRank();
 
@@ -242,8 +337,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1)
     } else {
         // ---- epilogue: two groups of four warps, one per accumulator -------------------------------------------------------
         const int group = (warp - 2) / 4, quarter = warp & 3;   // quarter: lanes of tensor memory this warp may read
-        unsigned char* mine = outStage + (warp - 2) * L::EPILOGUE;
-        float* mineBias = reinterpret_cast<float*>(mine + 32 * 64);
+        unsigned char* mine = base + L::OUT + (warp - 2) * OUT_BYTES;
+        float* mineBias = reinterpret_cast<float*>(base + L::BIAS) + (warp - 2) * BN;
         const uint32_t released = CTAS == 1 ? accEmpty + group * 8 : inBlock(accEmpty + group * 8, 0);
         const uint32_t sharedReleased = CTAS == 1 ? sharedFree + group * 8 : inBlock(sharedFree + group * 8, 0);
         auto release = [&](uint32_t bar) {
@@ -251,7 +346,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1)
             __syncwarp();
             if (lane == 0) {
                 if constexpr (CTAS == 1) barrierArrive(bar);
-                else clusterArriveBarrier(bar);
+                else clusterArriveRelaxed(bar);
             }
         };
         T* out = static_cast<T*>(p.out);
@@ -269,40 +364,9 @@ __global__ void __launch_bounds__(MX_THREADS, 1)
             if (!await(accFull + group * 8, accPhase, failed)) break;
             accPhase ^= 1;
             fenceAfter();
-            const uint32_t from = tmem + group * L::SECOND + (static_cast<uint32_t>(quarter * 32) << 16);
-            const int rowsLeft = t.end - tileRow - quarter * 32;
-            const long long firstRow = tileRow + quarter * 32;
-            // 64 columns of the accumulator at a time, 32 through shared memory; the columns that the accumulators share first: the last of one, the
-            // first of the other
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i) {
-                const int pair = L::OVERLAP && group == 0 ? (i + BN / 64 - 1) % (BN / 64) : i;
-                const bool used = t.column + pair * 64 < p.columns && rowsLeft > 0;
-                float v[2][32];
-                if (used) {
-                    tmemLoad32(from + pair * 64, v[0]);
-                    tmemLoad32(from + pair * 64 + 32, v[1]);
-                    tmemWait(v[0], v[1]);
-                }
-                if (L::OVERLAP && i == 0) release(sharedReleased);
-                if (!used) continue;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c0 = pair * 64 + h * 32;
-                    if (t.column + c0 >= p.columns) break;
-                    if (p.bias != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(mineBias + c0 + j);
-                            v[h][j] += f.x;
-                            v[h][j + 1] += f.y;
-                            v[h][j + 2] += f.z;
-                            v[h][j + 3] += f.w;
-                        }
-                    }
-                    storeTile<T>(v[h], mine, out + firstRow * p.outStride + t.column, p.outStride, rowsLeft, c0, p.columns - t.column, p.wideStore);
-                }
-            }
+            storeAccumulator<T, BN>(tmem + group * L::SECOND + (static_cast<uint32_t>(quarter * 32) << 16), L::OVERLAP && group == 0, &mapOut, out,
+                                    {tileRow + quarter * 32, t.end - tileRow - quarter * 32, t.column, p.columns - t.column, p.outStride, p.wideStore}, mine,
+                                    p.bias != nullptr ? mineBias : nullptr, [&] { if (L::OVERLAP) release(sharedReleased); });
             release(released);
         }
         // rows before the first and behind the last expert belong to nobody
@@ -312,6 +376,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1)
             T* row = out + (r < first ? r : last + (r - first)) * p.outStride;
             for (int c = lane; c < p.columns; c += 32) row[c] = Element<T>::from(0.f);
         }
+        if (lane == 0) tmaStoresDone();
+        __syncwarp();
     }
     fenceBefore();
     __syncthreads();
@@ -333,21 +399,231 @@ __global__ void __launch_bounds__(MX_THREADS, 1)
     if (warp == 1) tmemFree<CTAS>(tmem, L::TMEM);
 }
 
-// ---- host ------------------------------------------------------------------------------------------------------------------
-// `matrices` matrices of `rows` rows of `bytes` bytes, one behind the other (0: one, for a 2-D map), boxes of boxRows x boxBytes
-cudaError_t encodeBytes(CUtensorMap& map, const void* data, long long matrices, long long rows, int bytes, int boxBytes, int boxRows, bool swizzle)
+// ---- few rows: matrix-vector products -----------------------------------------------------------------------------------------
+// The product of a handful of rows is bound by reading their experts' matrices once. blockIdx.y is a row; a block takes up to 4 consecutive rows of one
+// expert (the first of every 4 does the work) and, a warp each, 4 times 4 channels out, those whose scales share 16 bytes of a tile: n, n + 32, n + 64, n + 96. A
+// lane takes blocks of 32 channels: 16 bytes of codes; `split` warps share a row of the matrix where it has more than 32. Twice an e2m1 number is an integer of -12 to 12, so a block's sum is exact in four dp4a per 16 numbers; then
+// two powers of two and an fp32 sum. The first codes are asked for before the rows are quantised.
+constexpr int FEW_ROWS = 4, FEW_WARPS = 4, FEW_OUT = 4;
+// four codes, in the low 16 bits, to four bytes of twice their values
+__device__ __forceinline__ uint32_t decodeBytes(uint32_t codes, uint32_t signs)
 {
-    const EncodeFn encode = encoder();
-    if (encode == nullptr) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(bytes / 4), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(matrices)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(bytes), static_cast<cuuint64_t>(bytes) * rows};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(boxBytes / 4), static_cast<cuuint32_t>(boxRows), 1}, one[3] = {1, 1, 1};
-    auto run = [&] {
-        return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, matrices > 0 ? 3 : 2, const_cast<void*>(data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const uint32_t number = codes & 0x7777u;
+    const uint32_t up = __byte_perm(0x03020100u, 0x0c080604u, number), down = __byte_perm(0xfdfeff00u, 0xf4f8fafcu, number), mask = __byte_perm(0x0000ff00u, 0u, signs & 0x1111u);
+    return (up & ~mask) | (down & mask);
+}
+// eight codes to two words
+__device__ __forceinline__ uint2 decodeWords(uint32_t codes)
+{
+    const uint32_t signs = codes >> 3;
+    return make_uint2(decodeBytes(codes, signs), decodeBytes(codes >> 16, signs >> 16));
+}
+// sum * 2^(a + b - 254) for scales a and b, NaN if one of them is. In two steps: a power alone may be out of range where the product is not.
+__device__ __forceinline__ float scaled(float sum, uint32_t a, uint32_t b)
+{
+    const int e = max(static_cast<int>(a + b), 4);   // (below, nothing is left of any sum)
+    const float first = __uint_as_float(static_cast<uint32_t>(e / 2) << 23), second = __uint_as_float(static_cast<uint32_t>(e - e / 2) << 23);
+    return max(a, b) == 255 ? __uint_as_float(0x7fffffffu) : sum * first * second;
+}
+
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(FEW_WARPS * 32) mx_few_rows_kernel(const __grid_constant__ MxLinearArgs a, int codeBytes, int chunks, int split)
+{
+    extern __shared__ uint4 quantized[];   // FEW_ROWS x 2 planes of half blocks x blocks; then the blocks' scales
+    __shared__ int found[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y, experts = static_cast<int>(a.weight.matrices), columns = static_cast<int>(a.weight.rows);
+    const int channels = a.weight.channels, blocks = codeBytes / 16;
+    const int group = blockIdx.x * (FEW_WARPS / split) + warp / split, within = group % 32, first = group / 32 * MX_TILE + within;   // channels out: first + 32 q
+    T* y = static_cast<T*>(a.y.data);
+    chained();
+    int expert = 0, count = min(FEW_ROWS, static_cast<int>(a.rows) - row);
+    if (a.offsets == nullptr) {
+        if (row % FEW_ROWS != 0) return;
+    } else {
+        if (threadIdx.x == 0) {
+            found[0] = experts + 1;
+            found[1] = 0;
+        }
+        __syncthreads();
+        // the first offset behind the row ends its expert's run (offsets are their running maximum): that expert is the one before it
+        int behind = experts + 1;
+        for (int e = threadIdx.x; e <= experts; e += FEW_WARPS * 32)
+            if (a.offsets[e] > row) { behind = e; break; }
+        if (behind <= experts) atomicMin(&found[0], behind);
+        __syncthreads();
+        behind = found[0];
+        if (behind == 0 || behind > experts) {   // nobody's row
+            if (warp % split == 0 && lane < FEW_OUT && first + lane * 32 < columns) y[row * a.y.stride + first + lane * 32] = Element<T>::from(0.f);
+            return;
+        }
+        int reached = 0;
+        for (int e = threadIdx.x; e < behind; e += FEW_WARPS * 32) reached = max(reached, a.offsets[e]);
+        if (reached > 0) atomicMax(&found[1], reached);
+        __syncthreads();
+        if ((row - found[1]) % FEW_ROWS != 0) return;
+        expert = behind - 1;
+        count = min(FEW_ROWS, static_cast<int>(min(a.rows, static_cast<long long>(a.offsets[behind]))) - row);
+    }
+    // codes and scales of a block of the warp's channels out (channels and blocks that are not there: the last ones again, and not used)
+    const int tile = blockIdx.x * FEW_WARPS / split / 32;
+    const unsigned char* codes[FEW_OUT];
+#pragma unroll
+    for (int q = 0; q < FEW_OUT; ++q) codes[q] = a.weight.codes + (static_cast<long long>(expert) * columns + min(first + q * 32, columns - 1)) * codeBytes;
+    const unsigned char* scales = a.weight.scales + (static_cast<long long>(expert) * ((columns + MX_TILE - 1) / MX_TILE) + tile) * chunks * MX_TILE_BYTES + within * 16;
+    auto fetch = [&](int block, uint4 (&code)[FEW_OUT], uint4& scale) {
+        const int b = min(block, blocks - 1);
+        scale = *reinterpret_cast<const uint4*>(scales + static_cast<long long>(b / 4) * MX_TILE_BYTES);
+#pragma unroll
+        for (int q = 0; q < FEW_OUT; ++q) code[q] = *reinterpret_cast<const uint4*>(codes[q] + b * 16);
     };
+    const int begin = warp % split * 32 + lane, step = split * 32;
+    uint4 code[FEW_OUT], scale;
+    fetch(begin, code, scale);
+    // the rows: half a block a thread
+    unsigned char* rowScales = reinterpret_cast<unsigned char*>(quantized + FEW_ROWS * 2 * blocks);
+    for (int r = 0; r < count; ++r) {
+        const T* x = static_cast<const T*>(a.x.data) + (row + r) * a.x.stride;
+        for (int h = threadIdx.x; h - lane < blocks * 2; h += FEW_WARPS * 32) {
+            const int left = channels - h * SIXTEEN;
+            Sixteen<T> v = loadSixteen<T, ALIGNED>(x + (left > 0 ? h * SIXTEEN : 0), left);
+            trim<T, ALIGNED>(v, left);
+            uint32_t largest = largestOf<T>(v);
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            const uint32_t s = scaleOf(largest);
+            const uint2 c = encodeSixteen<T>(v, s);
+            if (h >= blocks * 2) continue;
+            const uint2 low = decodeWords(c.x), high = decodeWords(c.y);
+            quantized[(r * 2 + (h & 1)) * blocks + h / 2] = make_uint4(low.x, low.y, high.x, high.y);
+            if ((h & 1) == 0) rowScales[r * blocks + h / 2] = static_cast<unsigned char>(s);
+        }
+    }
+    __syncthreads();
+    float sum[FEW_OUT][FEW_ROWS] = {};
+    for (int block = begin; block - lane < blocks; block += step) {
+        uint4 nextCode[FEW_OUT], nextScale;
+        if (block - lane + step < blocks) fetch(block + step, nextCode, nextScale);
+        if (block < blocks) {
+            const int at = (block & 3) * 8;
+            const uint32_t s[FEW_OUT] = {scale.x >> at & 255u, scale.y >> at & 255u, scale.z >> at & 255u, scale.w >> at & 255u};
+#pragma unroll
+            for (int q = 0; q < FEW_OUT; ++q) {
+                const uint2 w[4] = {decodeWords(code[q].x), decodeWords(code[q].y), decodeWords(code[q].z), decodeWords(code[q].w)};
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; ++r) {
+                    if (r >= count) break;
+                    const uint4 low = quantized[r * 2 * blocks + block], high = quantized[(r * 2 + 1) * blocks + block];
+                    int d = __dp4a(static_cast<int>(low.x), static_cast<int>(w[0].x), 0);
+                    d = __dp4a(static_cast<int>(low.y), static_cast<int>(w[0].y), d);
+                    d = __dp4a(static_cast<int>(low.z), static_cast<int>(w[1].x), d);
+                    d = __dp4a(static_cast<int>(low.w), static_cast<int>(w[1].y), d);
+                    d = __dp4a(static_cast<int>(high.x), static_cast<int>(w[2].x), d);
+                    d = __dp4a(static_cast<int>(high.y), static_cast<int>(w[2].y), d);
+                    d = __dp4a(static_cast<int>(high.z), static_cast<int>(w[3].x), d);
+                    d = __dp4a(static_cast<int>(high.w), static_cast<int>(w[3].y), d);
+                    sum[q][r] += scaled(0.25f * static_cast<float>(d), rowScales[r * blocks + block], s[q]);
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < FEW_OUT; ++q) code[q] = nextCode[q];
+        scale = nextScale;
+    }
+    // lane q * FEW_ROWS + r keeps that sum; then the warps that share channels out join theirs
+    float mine = 0.f;
+#pragma unroll
+    for (int q = 0; q < FEW_OUT; ++q)
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; ++r) {
+            if (r >= count) break;
+            const float all = groupSum<32>(sum[q][r]);
+            mine = lane == q * FEW_ROWS + r ? all : mine;
+        }
+    __shared__ float sums[FEW_WARPS][FEW_OUT * FEW_ROWS];
+    if (split > 1) {
+        if (lane < FEW_OUT * FEW_ROWS) sums[warp][lane] = mine;
+        __syncthreads();
+        if (warp % split != 0) return;
+        mine = 0.f;
+        if (lane < FEW_OUT * FEW_ROWS)
+            for (int w = 0; w < split; ++w) mine += sums[warp + w][lane];
+    }
+    const int n = first + lane / FEW_ROWS * 32, r = lane % FEW_ROWS;
+    if (lane < FEW_OUT * FEW_ROWS && r < count && n < columns) {
+        const float b = a.bias != nullptr ? Element<T>::to(static_cast<const T*>(a.bias)[static_cast<long long>(expert) * columns + n]) : 0.f;
+        y[(row + r) * a.y.stride + n] = Element<T>::from(mine + b);
+    }
+}
+
+// ---- bias gradient: column sums of an expert's rows --------------------------------------------------------------------------------
+// Pieces of BIAS_ROWS rows of one expert and 64 columns (32 element by element) a block, joined in order. 131072 rows of 1024 bfloat16, 16 experts: BIAS us (a block
+// per expert and 32 columns 199 us).
+constexpr int BIAS_ROWS = 512, BIAS_THREADS = 256;
+template <int VEC> constexpr int BIAS_LANES = VEC == 8 ? 8 : 32;
+template <class T, int VEC>
+__global__ void __launch_bounds__(BIAS_THREADS) mx_bias_kernel(const int2* __restrict__ list, const T* __restrict__ dy, long long stride, int columns, float* __restrict__ partial)
+{
+    constexpr int LANES = BIAS_LANES<VEC>, STEP = BIAS_THREADS / LANES, COLUMNS = LANES * VEC, AT_ONCE = 8;
+    __shared__ float sums[STEP][COLUMNS];
+    chained();
+    const unsigned groups = (columns + COLUMNS - 1) / COLUMNS, piece = blockIdx.x / groups;   // (blocks side by side read the rows' neighbouring columns)
+    const int firstColumn = static_cast<int>(blockIdx.x - piece * groups) * COLUMNS;
+    const int2 t = list[piece];
+    if (t.y == 0) return;
+    const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, c = firstColumn + lane * VEC;
+    float sum[VEC] = {};
+    if (c < columns) {
+        const T* at = dy + (static_cast<long long>(t.x) + first) * stride + c;
+        auto add = [&](const Pack<T, VEC>& v) {
+            float f[VEC];
+            unpack<T, VEC>(v, f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sum[j] += f[j];
+        };
+        int r = first;
+        for (; r + (AT_ONCE - 1) * STEP < t.y; r += STEP * AT_ONCE) {
+            Pack<T, VEC> v[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) v[i] = load<T, VEC>(at + i * STEP * stride);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) add(v[i]);
+            at += STEP * AT_ONCE * stride;
+        }
+        for (; r < t.y; r += STEP) {
+            add(load<T, VEC>(at));
+            at += STEP * stride;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sums[first][lane * VEC + j] = sum[j];
+    __syncthreads();
+    const int column = firstColumn + threadIdx.x;
+    if (threadIdx.x < COLUMNS && column < columns) {
+        float all = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < STEP; ++i) all += sums[i][threadIdx.x];
+        partial[static_cast<long long>(piece) * columns + column] = all;
+    }
+}
+template <class T>
+__global__ void __launch_bounds__(128) mx_bias_join_kernel(const int* __restrict__ unitsBefore, const float* __restrict__ partial, int columns, T* __restrict__ out)
+{
+    chained();
+    const int expert = blockIdx.x, c = blockIdx.y * 128 + threadIdx.x;
+    if (c >= columns) return;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int u = unitsBefore[expert]; u < unitsBefore[expert + 1]; ++u) sum += partial[static_cast<long long>(u) * columns + c];
+    out[static_cast<long long>(expert) * columns + c] = Element<T>::from(sum);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+// an encoding, once more with a context: in a thread's first call the driver wants one, which the runtime binds
+template <class F>
+cudaError_t encoded(F&& run)
+{
+    if (encoder() == nullptr) return cudaErrorNotSupported;
     CUresult r = run();
-    if (r == CUDA_ERROR_INVALID_CONTEXT) {   // a thread's first call: the driver wants a context, which the runtime binds
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
         int device = 0;
         cudaError_t e = cudaGetDevice(&device);
         if (e == cudaSuccess) e = cudaSetDevice(device);
@@ -355,6 +631,27 @@ cudaError_t encodeBytes(CUtensorMap& map, const void* data, long long matrices, 
         r = run();
     }
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+// `matrices` matrices of `rows` rows of `bytes` bytes, one behind the other (0: one, for a 2-D map), boxes of boxRows x boxBytes
+cudaError_t encodeBytes(CUtensorMap& map, const void* data, long long matrices, long long rows, int bytes, int boxBytes, int boxRows, bool swizzle)
+{
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(bytes / 4), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(matrices)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(bytes), static_cast<cuuint64_t>(bytes) * rows};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(boxBytes / 4), static_cast<cuuint32_t>(boxRows), 1}, one[3] = {1, 1, 1};
+    return encoded([&] {
+        return encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, matrices > 0 ? 3 : 2, const_cast<void*>(data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+}
+// rows of D, boxes of 32 x 64 elements of 16 bits
+cudaError_t encodeOut(CUtensorMap& map, void* data, long long rows, int columns, long long stride)
+{
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+    const cuuint32_t box[2] = {64, 32}, one[2] = {1, 1};
+    return encoded([&] {
+        return encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
@@ -366,7 +663,7 @@ Shape shapeOf(const MxLinearArgs& a)
 {
     const int columns = static_cast<int>(a.weight.rows);
     if (columns <= 64) return {64, 1};
-    if (columns <= 128 || a.rows / a.weight.matrices < 512) return {128, 1};
+    if (columns <= 128 || a.rows / a.weight.matrices < 512 || a.weight.matrices > PAIR_EXPERTS) return {128, 1};
     return {256, 2};
 }
 // tiles of 128 rows, none with rows of two experts, a multiple of ctas per expert: an upper bound
@@ -375,49 +672,68 @@ long long rowTiles(const MxLinearArgs& a, int ctas)
     return (a.rows / (MX_TILE * ctas) + std::min<long long>(a.rows, a.weight.matrices)) * ctas;
 }
 struct MxScratch {
-    size_t scales, bytes;   // codes lie at the start
+    size_t scales, list, bytes;   // codes lie at the start
     MxScratch(const MxLinearArgs& a)
     {
+        const size_t tiles = static_cast<size_t>(rowTiles(a, shapeOf(a).ctas));
         scales = align256(static_cast<size_t>(a.rows) * mxCodeBytes(a.weight.channels));
-        bytes = scales + align256(static_cast<size_t>(rowTiles(a, shapeOf(a).ctas)) * mxTiles(a.weight.channels) * MX_TILE_BYTES);
+        list = scales + align256(tiles * mxTiles(a.weight.channels) * MX_TILE_BYTES);
+        bytes = list + align256(tiles * sizeof(int2));
     }
 };
 
-template <class T, int LANES, bool ALIGNED>
-cudaError_t launchRows(const MxLinearArgs& a, const ProductArgs& p, unsigned char* codes, unsigned char* scales, cudaStream_t stream)
-{
-    auto* kernel = mx_rows_kernel<T, LANES, ALIGNED>;
-    const long long items = rowTiles(a, p.tileRows / MX_TILE) * mxTiles(p.sum);
-    launchChained(kernel, static_cast<unsigned>(std::min<long long>(items, a.numSMs * 6)), TILE_THREADS, 2 * listStride(p.experts) * sizeof(int), stream, 1, p,
-                  static_cast<const T*>(a.x.data), a.x.stride, codes, scales, mxTiles(p.sum), mxCodeBytes(p.sum));
-    return cudaGetLastError();
-}
 template <class T>
-cudaError_t quantizeRows(const MxLinearArgs& a, const ProductArgs& p, unsigned char* codes, unsigned char* scales, cudaStream_t stream)
+cudaError_t quantizeRows(const MxLinearArgs& a, const ProductArgs& p, unsigned char* codes, unsigned char* scales, int2* list, cudaStream_t stream)
 {
-    const bool aligned = (reinterpret_cast<uintptr_t>(a.x.data) & 15) == 0 && a.x.stride % 8 == 0 && p.sum % 8 == 0;
-    switch (lanesOf(p.sum)) {
-    case 4: return aligned ? launchRows<T, 4, true>(a, p, codes, scales, stream) : launchRows<T, 4, false>(a, p, codes, scales, stream);
-    case 8: return aligned ? launchRows<T, 8, true>(a, p, codes, scales, stream) : launchRows<T, 8, false>(a, p, codes, scales, stream);
-    default: return aligned ? launchRows<T, 16, true>(a, p, codes, scales, stream) : launchRows<T, 16, false>(a, p, codes, scales, stream);
-    }
+    const int tiles = static_cast<int>(rowTiles(a, p.tileRows / MX_TILE)), chunks = mxTiles(p.sum);
+    if (p.offsets != nullptr)
+        launchChained(mx_tiles_kernel, (tiles + TILE_THREADS - 1) / TILE_THREADS, TILE_THREADS, 2 * listStride(p.experts) * sizeof(int), stream, 1, p, list, tiles, MX_TILE, static_cast<int*>(nullptr));
+    else list = nullptr;
+    return byLanes(a.x, a.type, p.sum, [&](auto lanes, auto aligned) {
+        launchChained(mx_rows_kernel<T, decltype(lanes)::value, decltype(aligned)::value>, static_cast<unsigned>(tiles) * chunks, TILE_THREADS, 0, stream, 1, list, static_cast<const T*>(a.x.data), a.x.stride,
+                      a.rows, p.sum, codes, scales, chunks, mxCodeBytes(p.sum));
+        return cudaGetLastError();
+    });
 }
 
 template <class T, int BN, int CTAS>
-cudaError_t launchMx(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const ProductArgs& p, int numSMs, cudaStream_t stream)
+cudaError_t launchMx(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const CUtensorMap& out, const ProductArgs& p, int numSMs,
+                     cudaStream_t stream)
 {
     auto* kernel = mx_product_kernel<T, BN, CTAS>;
-    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), MxLayout<BN, CTAS>::bytes(EXPERTS_MAX));
+    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), MxLayout<BN, CTAS>::bytes(MxLayout<BN, CTAS>::EXPERTS));
     if (e != cudaSuccess) return e;
-    return launchChained(kernel, numSMs / CTAS * CTAS, MX_THREADS, MxLayout<BN, CTAS>::bytes(p.experts), stream, CTAS, a, b, sa, sb, p, mxTiles(p.sum));
+    return launchChained(kernel, numSMs / CTAS * CTAS * MxLayout<BN, CTAS>::BLOCKS, MX_THREADS, MxLayout<BN, CTAS>::bytes(p.experts), stream, CTAS, a, b, sa, sb, out, p, mxTiles(p.sum));
 }
 
-template <class T>
-cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
+// Rows that the matrix-vector kernel takes
+int fewBytes(int channels) { return FEW_ROWS * mxBlocks(channels) * (MX_BLOCK + 1); }
+bool fewRows(const MxLinearArgs& a)
 {
-    const Shape shape = shapeOf(a);
-    const MxScratch s(a);
-    unsigned char *codes = static_cast<unsigned char*>(a.scratch), *scales = codes + s.scales;
+    return a.rows <= 64 && a.rows * a.weight.channels * a.weight.rows <= 1ll << 27 && fewBytes(a.weight.channels) <= 200 * 1024;
+}
+template <class T>
+cudaError_t forwardFewRows(const MxLinearArgs& a, cudaStream_t stream)
+{
+    // warps that share a row of the matrix: as many as it has work for, while all blocks are resident (five on an SM)
+    const int blocks = mxBlocks(a.weight.channels), groups = mxTiles(a.weight.rows) * (32 / FEW_WARPS);
+    int split = 1;
+    while (split < FEW_WARPS && split * 32 < blocks && groups * split * 2 * a.rows <= a.numSMs * 5) split *= 2;
+    const dim3 grid(groups * split, static_cast<unsigned>(a.rows));
+    auto go = [&](auto* kernel) {
+        const int bytes = fewBytes(a.weight.channels);
+        if (bytes > 47 * 1024) {   // (48 KB without asking, which the kernel's static shared memory counts towards)
+            const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), 200 * 1024);
+            if (e != cudaSuccess) return e;
+        }
+        launchChained(kernel, grid, FEW_WARPS * 32, bytes, stream, 1, a, mxCodeBytes(a.weight.channels), mxTiles(a.weight.channels), split);
+        return cudaGetLastError();
+    };
+    return wide(a.x, a.type, a.weight.channels) ? go(mx_few_rows_kernel<T, true>) : go(mx_few_rows_kernel<T, false>);
+}
+
+ProductArgs productArgs(const MxLinearArgs& a, const Shape& shape)
+{
     ProductArgs p{};
     p.rows = a.rows;
     p.experts = static_cast<int>(a.weight.matrices);
@@ -431,46 +747,95 @@ cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
     p.bias = a.bias;
     p.status = a.status;
     p.wideStore = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.outStride % 8 == 0 && p.columns % 8 == 0;
+    return p;
+}
+cudaError_t encodeWeight(const MxLinearArgs& a, CUtensorMap& map, CUtensorMap& scales)
+{
+    const long long tiles = a.weight.matrices * mxTiles(a.weight.rows) * mxTiles(a.weight.channels);
+    const cudaError_t e = encodeBytes(map, a.weight.codes, a.weight.matrices, a.weight.rows, mxCodeBytes(a.weight.channels), 128, 64, true);
+    return e != cudaSuccess ? e : encodeBytes(scales, a.weight.scales, 0, tiles, MX_TILE_BYTES, MX_TILE_BYTES, 2, false);
+}
+template <class T>
+cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
+{
+    if (fewRows(a)) return forwardFewRows<T>(a, stream);
+    const Shape shape = shapeOf(a);
+    const MxScratch s(a);
+    unsigned char *codes = static_cast<unsigned char*>(a.scratch), *scales = codes + s.scales;
+    const ProductArgs p = productArgs(a, shape);
     const int chunks = mxTiles(p.sum), codeBytes = mxCodeBytes(p.sum);
-    CUtensorMap mapA, mapB, mapScaleA, mapScaleB;
+    CUtensorMap mapA, mapB, mapScaleA, mapScaleB, mapOut = {};
     cudaError_t e = encodeBytes(mapA, codes, 0, a.rows, codeBytes, 128, 64, true);
-    if (e == cudaSuccess) e = encodeBytes(mapB, a.weight.codes, a.weight.matrices, p.columns, codeBytes, 128, 64, true);
+    if (e == cudaSuccess) e = encodeWeight(a, mapB, mapScaleB);
     if (e == cudaSuccess) e = encodeBytes(mapScaleA, scales, 0, rowTiles(a, shape.ctas) * chunks, MX_TILE_BYTES, MX_TILE_BYTES, 2, false);
-    if (e == cudaSuccess) e = encodeBytes(mapScaleB, a.weight.scales, 0, a.weight.matrices * mxTiles(p.columns) * chunks, MX_TILE_BYTES, MX_TILE_BYTES, 2, false);
-    if (e == cudaSuccess) e = quantizeRows<T>(a, p, codes, scales, stream);
+    if (e == cudaSuccess && p.wideStore) e = encodeOut(mapOut, p.out, a.rows, p.columns, p.outStride);
+    if (e == cudaSuccess) e = quantizeRows<T>(a, p, codes, scales, reinterpret_cast<int2*>(codes + s.list), stream);
     if (e != cudaSuccess) return e;
-    if (shape.width == 64) return launchMx<T, 64, 1>(mapA, mapB, mapScaleA, mapScaleB, p, a.numSMs, stream);
-    if (shape.width == 128) return launchMx<T, 128, 1>(mapA, mapB, mapScaleA, mapScaleB, p, a.numSMs, stream);
-    return launchMx<T, 256, 2>(mapA, mapB, mapScaleA, mapScaleB, p, a.numSMs, stream);
+    if (shape.width == 64) return launchMx<T, 64, 1>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a.numSMs, stream);
+    if (shape.width == 128) return launchMx<T, 128, 1>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a.numSMs, stream);
+    return launchMx<T, 256, 2>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a.numSMs, stream);
 }
 
-// the matrices in 16 bits, then the input gradient's and the bias gradient's scratch
-size_t decodedBytes(const MxLinearArgs& a)
+// scratch of the adjoint: [the matrices in 16 bits | scratch of the input gradient's product] or [pieces of the bias gradient | their sums], one after the other
+struct MxAdjointScratch {
+    size_t product, before, partial, bytes;
+    int pieces;
+    explicit MxAdjointScratch(const MxLinearArgs& a)
+    {
+        product = a.gradX.data == nullptr || a.rows == 0 ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * a.weight.channels * 2);
+        pieces = static_cast<int>(a.rows / BIAS_ROWS + std::min<long long>(a.rows, a.weight.matrices));
+        before = align256(static_cast<size_t>(pieces) * sizeof(int2));
+        partial = before + align256((static_cast<size_t>(a.weight.matrices) + 1) * sizeof(int));
+        bytes = std::max(product + (a.gradX.data == nullptr ? 0 : expertBytes(inputGradient(a), true)), partial + static_cast<size_t>(pieces) * static_cast<size_t>(a.weight.rows) * sizeof(float));
+    }
+    // the product with the matrices in 16 bits at the start of the scratch
+    static ExpertArgs inputGradient(const MxLinearArgs& a)
+    {
+        ExpertArgs r{};
+        r.rows = a.rows;
+        r.experts = static_cast<int>(a.weight.matrices);
+        r.channelsIn = a.weight.channels;
+        r.channelsOut = static_cast<int>(a.weight.rows);
+        r.type = a.type;
+        r.numSMs = a.numSMs;
+        r.weight = a.scratch;
+        r.offsets = a.offsets;
+        r.gradY = a.gradY;
+        r.gradX = a.gradX;
+        r.status = a.status;
+        return r;
+    }
+};
+template <class T>
+cudaError_t biasGradient(const MxLinearArgs& a, const MxAdjointScratch& s, cudaStream_t stream)
 {
-    return a.gradX.data == nullptr || a.rows == 0 ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * a.weight.channels * 2);
-}
-ExpertArgs decoded(const MxLinearArgs& a)
-{
-    ExpertArgs r{};
-    r.rows = a.rows;
-    r.experts = static_cast<int>(a.weight.matrices);
-    r.channelsIn = a.weight.channels;
-    r.channelsOut = static_cast<int>(a.weight.rows);
-    r.type = a.type;
-    r.numSMs = a.numSMs;
-    r.weight = a.scratch;
-    r.offsets = a.offsets;
-    r.gradY = a.gradY;
-    r.gradX = a.gradX;
-    r.gradBias = a.gradBias;
-    r.status = a.status;
-    return r;
+    const int columns = static_cast<int>(a.weight.rows), experts = static_cast<int>(a.weight.matrices);
+    if (a.rows == 0) return cudaMemsetAsync(a.gradBias, 0, static_cast<size_t>(experts) * columns * sizeof(T), stream);
+    unsigned char* base = static_cast<unsigned char*>(a.scratch);
+    auto *list = reinterpret_cast<int2*>(base);
+    auto *before = reinterpret_cast<int*>(base + s.before);
+    auto *partial = reinterpret_cast<float*>(base + s.partial);
+    ProductArgs p{};
+    p.rows = a.rows;
+    p.experts = experts;
+    p.offsets = a.offsets;
+    p.tileRows = BIAS_ROWS;
+    launchChained(mx_tiles_kernel, (s.pieces + TILE_THREADS - 1) / TILE_THREADS, TILE_THREADS, 2 * listStride(experts) * sizeof(int), stream, 1, p, list, s.pieces, BIAS_ROWS, before);
+    const cudaError_t e = byAccess<T>({&a.gradY}, a.type, columns, [&](auto vec) {
+        constexpr int VEC = decltype(vec)::value, COLUMNS = BIAS_LANES<VEC> * VEC;
+        launchChained(mx_bias_kernel<T, VEC>, static_cast<unsigned>(s.pieces) * ((columns + COLUMNS - 1) / COLUMNS), BIAS_THREADS, 0, stream, 1, list, static_cast<const T*>(a.gradY.data), a.gradY.stride,
+                      columns, partial);
+        return cudaGetLastError();
+    });
+    if (e != cudaSuccess) return e;
+    launchChained(mx_bias_join_kernel<T>, dim3(experts, (columns + 127) / 128), 128, 0, stream, 1, before, partial, columns, static_cast<T*>(a.gradBias));
+    return cudaGetLastError();
 }
 
 } // namespace
 
-size_t mxLinearBytes(const MxLinearArgs& a) { return a.rows == 0 ? 0 : MxScratch(a).bytes; }
-size_t mxLinearAdjointBytes(const MxLinearArgs& a) { return decodedBytes(a) + expertBytes(decoded(a), true); }
+size_t mxLinearBytes(const MxLinearArgs& a) { return a.rows == 0 || fewRows(a) ? 0 : MxScratch(a).bytes; }
+size_t mxLinearAdjointBytes(const MxLinearArgs& a) { return a.rows == 0 ? 0 : MxAdjointScratch(a).bytes; }
 
 cudaError_t launchMxLinear(const MxLinearArgs& a, cudaStream_t stream)
 {
@@ -479,12 +844,14 @@ cudaError_t launchMxLinear(const MxLinearArgs& a, cudaStream_t stream)
 }
 cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream)
 {
-    ExpertArgs r = decoded(a);
-    r.scratch = static_cast<unsigned char*>(a.scratch) + decodedBytes(a);
-    if (decodedBytes(a) > 0) {
-        const cudaError_t e = launchMxDequantize(a.weight, a.type, {a.scratch, a.weight.channels}, stream);
-        if (e != cudaSuccess) return e;
-    }
+    const MxAdjointScratch s(a);
+    cudaError_t e = cudaSuccess;
+    if (a.gradBias != nullptr) e = a.type == TYPE_HALF ? biasGradient<__half>(a, s, stream) : biasGradient<__nv_bfloat16>(a, s, stream);
+    if (e != cudaSuccess || a.gradX.data == nullptr || a.rows == 0) return e;
+    e = launchMxDequantize(a.weight, a.type, {a.scratch, a.weight.channels}, stream);
+    if (e != cudaSuccess) return e;
+    ExpertArgs r = MxAdjointScratch::inputGradient(a);
+    r.scratch = static_cast<unsigned char*>(a.scratch) + s.product;
     return launchExpertAdjoint(r, stream);
 }
 
