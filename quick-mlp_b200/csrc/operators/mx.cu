@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __gri
                 scale[k] = *reinterpret_cast<const uint32_t*>(scales + (r & 31) * 16 + (r >> 5) * 4);
 #pragma unroll
                 for (int b = 0; b < BLOCKS; ++b)
-                    code[k][b] = c + b * MX_BLOCK < q.channels ? codes[static_cast<long long>(r) * codeBytes + (c + b * MX_BLOCK) / 2] : 0u;
+                    code[k][b] = codes[static_cast<long long>(r) * codeBytes + min(c + b * MX_BLOCK, q.channels - 1) / 2];
             }
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {

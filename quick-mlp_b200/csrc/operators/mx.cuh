@@ -133,7 +133,8 @@ __device__ __forceinline__ uint2 encodeSixteen(const Sixteen<T>& p, uint32_t sca
 }
 
 // A block of TILE_THREADS threads works on a tile of 128 rows x 128 channels. LANES threads share a row, 16 channels each (8 of them for 128 channels,
-// fewer for matrices that are narrower), two neighbours a block of 32.
+// fewer for matrices that are narrower), two neighbours a block of 32. Rows that 16-byte accesses cannot read go through shared memory, read side by side (20011
+// rows of 777 floats: 27 us with 16 elements of a row per thread, which meet the same sectors 16 times; 46 us with a warp per row and its maximum by redux; QUANT us so).
 constexpr int TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32;
 
 // `rows` rows of x, channels from 128 * chunk on, to codes (rows of codeBytes) and a tile of scales; tileScales: 512 bytes of shared memory.
@@ -141,28 +142,61 @@ template <class T, int LANES, bool ALIGNED>
 __device__ __forceinline__ void quantizeTile(const T* x, long long stride, int rows, int chunk, int channels, unsigned char* codes, int codeBytes, unsigned char* scales,
                                              unsigned char* tileScales)
 {
-    if constexpr (LANES < 8) {   // the blocks that are not there
+    if constexpr (LANES < 8 || !ALIGNED) {   // the blocks and rows that are not there
         if (threadIdx.x < MX_TILE) *reinterpret_cast<uint32_t*>(tileScales + threadIdx.x * 4) = 0;
         __syncthreads();
     }
-    constexpr int PASSES = MX_TILE * LANES / TILE_THREADS, STEP = TILE_THREADS / LANES;
-    const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, c = chunk * MX_TILE + lane * SIXTEEN, left = channels - c;
-    const T* from = x + (left > 0 ? c : 0);
-    Sixteen<T> v[PASSES];
+    if constexpr (ALIGNED) {
+        constexpr int PASSES = MX_TILE * LANES / TILE_THREADS, STEP = TILE_THREADS / LANES;
+        const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, c = chunk * MX_TILE + lane * SIXTEEN, left = channels - c;
+        const T* from = x + (left > 0 ? c : 0);
+        Sixteen<T> v[PASSES];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) v[i] = loadSixteen<T, ALIGNED>(from + min(i * STEP + first, rows - 1) * stride, left);
-    unsigned char* to = codes + static_cast<long long>(first) * codeBytes + c / 2;
+        for (int i = 0; i < PASSES; ++i) v[i] = loadSixteen<T, true>(from + min(i * STEP + first, rows - 1) * stride, left);
+        unsigned char* to = codes + static_cast<long long>(first) * codeBytes + c / 2;
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = i * STEP + first;
-        trim<T, ALIGNED>(v[i], r < rows ? left : 0);
-        uint32_t largest = largestOf<T>(v[i]);
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        const uint32_t scale = scaleOf(largest);
-        const uint2 code = encodeSixteen<T>(v[i], scale);
-        if (r < rows && c / 2 < codeBytes) *reinterpret_cast<uint2*>(to) = code;
-        to += STEP * codeBytes;
-        if ((lane & 1) == 0) tileScales[(r & 31) * 16 + (r >> 5) * 4 + lane / 2] = static_cast<unsigned char>(scale);
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = i * STEP + first;
+            trim<T, true>(v[i], r < rows ? left : 0);
+            uint32_t largest = largestOf<T>(v[i]);
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            const uint32_t scale = scaleOf(largest);
+            const uint2 code = encodeSixteen<T>(v[i], scale);
+            if (r < rows && c / 2 < codeBytes) *reinterpret_cast<uint2*>(to) = code;
+            to += STEP * codeBytes;
+            if ((lane & 1) == 0) tileScales[(r & 31) * 16 + (r >> 5) * 4 + lane / 2] = static_cast<unsigned char>(scale);
+        }
+    } else {
+        // through shared memory: 32 rows at a time, read side by side, taken up again 16 channels a thread
+        constexpr int CHANNELS = LANES * SIXTEEN, ROWS = TILE_THREADS / LANES, PER = ROWS * CHANNELS / TILE_THREADS, PITCH = CHANNELS + 16 / static_cast<int>(sizeof(T));
+        __shared__ __align__(16) T staged[ROWS * PITCH];
+        const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES, c = chunk * MX_TILE + lane * SIXTEEN, left = channels - c;
+        const int column = threadIdx.x % CHANNELS, line = threadIdx.x / CHANNELS, channel = min(chunk * MX_TILE + column, channels - 1);
+        constexpr int LINES = TILE_THREADS / CHANNELS;
+        T v[PER];
+        auto ask = [&](int begin) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = x[min(begin + i * LINES + line, rows - 1) * stride + channel];
+        };
+        ask(0);
+        for (int begin = 0; begin < rows; begin += ROWS) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) staged[(i * LINES + line) * PITCH + column] = v[i];
+            __syncthreads();
+            ask(begin + ROWS);
+            const int r = begin + mine;
+            Sixteen<T> part;
+#pragma unroll
+            for (int i = 0; i < SIXTEEN / WIDE<T>; ++i) part.v[i] = load<T, WIDE<T>>(&staged[mine * PITCH + lane * SIXTEEN + i * WIDE<T>]);
+            trim<T, false>(part, r < rows ? left : 0);
+            uint32_t largest = largestOf<T>(part);
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            const uint32_t scale = scaleOf(largest);
+            const uint2 code = encodeSixteen<T>(part, scale);
+            if (r < rows && c / 2 < codeBytes) *reinterpret_cast<uint2*>(codes + static_cast<long long>(r) * codeBytes + c / 2) = code;
+            if (r < MX_TILE && (lane & 1) == 0) tileScales[(r & 31) * 16 + (r >> 5) * 4 + lane / 2] = static_cast<unsigned char>(scale);
+            __syncthreads();
+        }
     }
     __syncthreads();
     if (threadIdx.x < MX_TILE_BYTES / 16) *reinterpret_cast<uint4*>(scales + threadIdx.x * 16) = *reinterpret_cast<const uint4*>(tileScales + threadIdx.x * 16);

@@ -30,15 +30,16 @@ constexpr int STEP_CHANNELS = 256, SCALE_BYTES = 2 * MX_TILE_BYTES;   // channel
 constexpr int PAIR_EXPERTS = 1024;   // whose lists leave shared memory for five stages
 constexpr int MX_THREADS = (2 + EPILOGUE_WARPS) * 32, OUT_BYTES = 32 * 128;   // OUT_BYTES: 32 rows x 64 columns of D, per warp of the epilogue
 
-// BN: columns of D; CTAS: blocks that share a tile, each with BM rows of D and BN / CTAS of the columns of B
-template <int BN, int CTAS>
+// BN: columns of D; CTAS: blocks that share a tile, each with BM rows of D and BN / CTAS of the columns of B. WHOLE: the kernel quantises its rows itself.
+// KB: bytes of a row's codes in a step, 128 (256 channels) or, for matrices of up to 64 channels, 32: stages of a quarter, and more of them.
+template <int BN, int CTAS, bool WHOLE, int KB>
 struct MxLayout {
-    static constexpr int BCOLS = BN / CTAS, ABYTES = BM * 128, BBYTES = BCOLS * 128;
+    static constexpr int BCOLS = BN / CTAS, ABYTES = BM * KB, BBYTES = BCOLS * KB, BOXBYTES = 64 * KB;
     static constexpr int BTILES = (BN + MX_TILE - 1) / MX_TILE;       // tiles of scales of the columns (each block has all of them)
     static constexpr int SCALES = ABYTES + BBYTES, STAGE = SCALES + SCALE_BYTES * (1 + BTILES);
     // Two blocks per SM for narrow layers: a tile of 128 x 64 and a step or two costs the warp that issues its products more time (1250 clocks to walk on, wait
     // four times and issue) than anything else.
-    static constexpr int BLOCKS = BN == 64 ? 2 : 1, STAGES = BN == 64 ? 2 : BN == 128 ? 4 : 5, EXPERTS = CTAS == 2 ? PAIR_EXPERTS : EXPERTS_MAX;
+    static constexpr int BLOCKS = BN == 64 && !WHOLE ? 2 : 1, STAGES = KB == 32 ? (BN == 64 ? 7 : 8) : BN == 64 ? (WHOLE ? 6 : 2) : BN == 128 ? 4 : 5, EXPERTS = CTAS == 2 ? PAIR_EXPERTS : EXPERTS_MAX;
     // tensor memory: accumulators, then two sets of scales, used in turn: of 128 rows (4 columns) for two times 128 channels, of the columns likewise
     static constexpr bool OVERLAP = BN == 256;
     static constexpr int SECOND = OVERLAP ? BN - 64 : BN;             // column of the second accumulator
@@ -80,6 +81,11 @@ __device__ __forceinline__ void copyScales(uint32_t lead, uint32_t to, uint64_t 
 // Tells the leader that tensor memory was read. Relaxed: what was read is in registers (tcgen05.wait::ld), and a release would wait for the warp's stores of
 // D as well, which took a microsecond per tile (16 experts, 32768 rows, 1024 -> 1024 bfloat16: 35 us for the product, RELAXED us so).
 __device__ __forceinline__ void clusterArriveRelaxed(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// descriptor of a 32-byte swizzled K-major operand: groups of 8 rows of 32 bytes
+__device__ __forceinline__ uint64_t narrowDescriptor(uint32_t address)
+{
+    return static_cast<uint64_t>((address >> 4) & 0x3FFFu) | (1ull << 16) | (16ull << 32) | (1ull << 46) | (6ull << 61);
+}
 // descriptor of a tile of scales: no swizzle, groups of 8 rows of 16 bytes lie 128 bytes apart
 __device__ __forceinline__ uint64_t scaleDescriptor(uint32_t address) { return static_cast<uint64_t>((address >> 4) & 0x3FFFu) | (8ull << 32) | (1ull << 46); }
 
@@ -205,12 +211,45 @@ __device__ __forceinline__ void storeAccumulator(uint32_t from, bool sharedLast,
 }
 
 // ---- the product -------------------------------------------------------------------------------------------------------------
-template <class T, int BN, int CTAS>
-__global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
-    mx_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapScaleA,
-                      const __grid_constant__ CUtensorMap mapScaleB, const __grid_constant__ CUtensorMap mapOut, const __grid_constant__ ProductArgs p, int chunks)
+// Rows that the kernel quantises itself (see forward()): x, its row stride, whether 16-byte accesses read it
+template <class T>
+struct RawRows {
+    const T* x;
+    long long stride;
+    bool aligned;
+};
+// 128 rows x 256 channels of a step by the epilogue's warps, to a stage's codes (128-byte swizzled) and scales
+// (LANES threads to a row: 16, fewer where a row has no more than 128 or 64 channels)
+template <class T, bool ALIGNED, int LANES>
+__device__ __forceinline__ void quantizeStep(const T* x, long long stride, int rows, int channels, int step, unsigned char* codes, unsigned char* scales)
 {
-    using L = MxLayout<BN, CTAS>;
+    constexpr int THREADS = EPILOGUE_WARPS * 32, ROWS = THREADS / LANES, AT_ONCE = BM / ROWS < 4 ? BM / ROWS : 4;
+    const int thread = threadIdx.x - 64, part = thread % LANES, first = thread / LANES, c = step * STEP_CHANNELS + part * SIXTEEN, left = channels - c;
+    for (int begin = 0; begin < rows; begin += ROWS * AT_ONCE) {   // (rows that are not there: whatever, their rows of D are not stored)
+        Sixteen<T> v[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) v[i] = loadSixteen<T, ALIGNED>(x + min(begin + i * ROWS + first, rows - 1) * stride + (left > 0 ? c : 0), left);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = begin + i * ROWS + first;
+            if (begin + i * ROWS >= rows) break;
+            trim<T, ALIGNED>(v[i], left);
+            uint32_t largest = largestOf<T>(v[i]);
+            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            const uint32_t scale = scaleOf(largest);
+            *reinterpret_cast<uint2*>(codes + r * 128 + ((part / 2 ^ (r & 7)) << 4) + (part & 1) * 8) = encodeSixteen<T>(v[i], scale);
+            if ((part & 1) == 0) scales[part / 8 * MX_TILE_BYTES + (r & 31) * 16 + (r >> 5) * 4 + part / 2 % 4] = static_cast<unsigned char>(scale);
+        }
+    }
+}
+
+template <class T, int BN, int CTAS, bool WHOLE, int KB>
+__global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS, WHOLE, KB>::BLOCKS)
+    mx_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const __grid_constant__ CUtensorMap mapScaleA,
+                      const __grid_constant__ CUtensorMap mapScaleB, const __grid_constant__ CUtensorMap mapOut, const __grid_constant__ ProductArgs p, int chunks, const __grid_constant__ RawRows<T> raws)
+{
+    static_assert(!WHOLE || (CTAS == 1 && KB == 128), "");
+    using L = MxLayout<BN, CTAS, WHOLE, KB>;
     extern __shared__ unsigned char dynamic[];
     const uint32_t raw = smemAddress(dynamic), ring = (raw + 1023u) & ~1023u;
     unsigned char* base = dynamic + (ring - raw);
@@ -225,7 +264,7 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::STAGES; ++s) {
-            barrierInit(full + s * 8, CTAS);
+            barrierInit(full + s * 8, WHOLE ? 1 + EPILOGUE_WARPS : CTAS);
             barrierInit(empty + s * 8, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -245,7 +284,7 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
     if constexpr (CTAS > 1) clusterSync();   // the other block's barriers are set
     fenceAfter();
     const uint32_t tmem = *tmemBase;
-    const int steps = (p.sum + STEP_CHANNELS - 1) / STEP_CHANNELS;
+    const int steps = KB == 32 ? 1 : (p.sum + STEP_CHANNELS - 1) / STEP_CHANNELS;
     Walk<FORWARD, BN, CTAS> walk(p, bounds, before, nullptr, 0, 1);
     Tile t;
     InFlight copies;   // of warp 0
@@ -260,9 +299,9 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
         while (ok && walk.next(t)) {
             if (__all_sync(0xffffffffu, t.expert < 0)) continue;   // no tile for this block in the last round
             const int row = t.row + rank * BM, column = t.column + rank * L::BCOLS;
-            const int boxesA = boxes(t.end - row, BM / 64), boxesB = boxes(p.columns - column, L::BCOLS / 64);
-            const uint32_t bytes = (boxesA + boxesB) * BOX + SCALE_BYTES * (1 + L::BTILES);   // of this block; of both blocks:
-            const uint32_t allBytes = CTAS == 1 ? bytes : bytes + (boxes(t.end - row - BM, BM / 64) + boxes(p.columns - column - L::BCOLS, L::BCOLS / 64)) * BOX + SCALE_BYTES * (1 + L::BTILES);
+            const int boxesA = WHOLE ? 0 : boxes(t.end - row, BM / 64), boxesB = boxes(p.columns - column, L::BCOLS / 64);
+            const uint32_t bytes = (boxesA + boxesB) * L::BOXBYTES + SCALE_BYTES * ((WHOLE ? 0 : 1) + L::BTILES);   // of this block; of both blocks:
+            const uint32_t allBytes = CTAS == 1 ? bytes : bytes + (boxes(t.end - row - BM, BM / 64) + boxes(p.columns - column - L::BCOLS, L::BCOLS / 64)) * L::BOXBYTES + SCALE_BYTES * (1 + L::BTILES);
             // tiles of scales, each a row of the scales' maps (the expert's tiles of 128 columns: one behind the last is the next expert's, or zeros)
             const int scaleA = (t.slot * CTAS + static_cast<int>(rank)) * chunks, scaleB = (t.expert * columnScaleTiles + t.column / MX_TILE) * chunks;
             for (int k = 0; __all_sync(0xffffffffu, k < steps); ++k) {
@@ -275,11 +314,13 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
                     if (CTAS > 1) barrierArrive(full + stage * 8);
                 }
                 __syncwarp();
+                if constexpr (!WHOLE) {
 #pragma unroll
-                for (int i = 0; i < BM / 64; ++i) tmaLoad2<CTAS>(lead && i < boxesA, a + i * BOX, &mapA, k * 32, row + i * 64, ready);
+                    for (int i = 0; i < BM / 64; ++i) tmaLoad2<CTAS>(lead && i < boxesA, a + i * L::BOXBYTES, &mapA, k * 32, row + i * 64, ready);
+                    tmaLoad2<CTAS>(lead, s, &mapScaleA, 0, scaleA + k * 2, ready);
+                }
 #pragma unroll
-                for (int i = 0; i < L::BCOLS / 64; ++i) tmaLoad3<CTAS>(lead && i < boxesB, b + i * BOX, &mapB, k * 32, column + i * 64, t.expert, ready);
-                tmaLoad2<CTAS>(lead, s, &mapScaleA, 0, scaleA + k * 2, ready);
+                for (int i = 0; i < L::BCOLS / 64; ++i) tmaLoad3<CTAS>(lead && i < boxesB, b + i * L::BOXBYTES, &mapB, k * 32, column + i * 64, t.expert, ready);
 #pragma unroll
                 for (int i = 0; i < L::BTILES; ++i) tmaLoad2<CTAS>(lead, s + SCALE_BYTES * (1 + i), &mapScaleB, 0, scaleB + i * chunks + k * 2, ready);
                 ++issued;
@@ -306,6 +347,7 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
             accPhases ^= 1u << acc;
             fenceAfter();
             const uint32_t d = tmem + acc * L::SECOND;
+            const uint32_t columnsAt = BN < MX_TILE ? t.column % MX_TILE / 32 : 0;   // (a tile of 64 columns has half a tile of scales)
             for (int k = 0; __all_sync(0xffffffffu, k < steps); ++k) {
                 if (!await(full + stage * 8, phase, failed)) { ok = false; break; }
                 // the products that read this set of scales are done (those of the step before keep the tensor core busy meanwhile)
@@ -313,9 +355,9 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
                 fenceAfter();
                 const uint32_t a = ring + stage * L::STAGE, b = a + L::ABYTES, s = a + L::SCALES, scales = tmem + L::SCALE_AT + set * L::SCALE_SET;
                 const int parts = min(STEP_CHANNELS, p.sum - k * STEP_CHANNELS + 63) / 64;
-                const uint64_t descA = operandDescriptor(a, 16), descB = operandDescriptor(b, 16), descS = scaleDescriptor(s);
+                const uint64_t descA = KB == 32 ? narrowDescriptor(a) : operandDescriptor(a, 16), descB = KB == 32 ? narrowDescriptor(b) : operandDescriptor(b, 16), descS = scaleDescriptor(s);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < (KB == 32 ? 1 : 2); ++c) {
                     copyScales<CTAS>(lead && parts > 2 * c, scales + c * 4, descS + c * (MX_TILE_BYTES >> 4));
 #pragma unroll
                     for (int i = 0; i < L::BTILES; ++i)
@@ -323,9 +365,9 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
                 }
                 // 64 channels: 32 bytes of a row, two scales of a word of four
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < (KB == 32 ? 1 : 4); ++i)
                     mmaMx<CTAS>(lead && i < parts, d, descA + i * (32 >> 4), descB + i * (32 >> 4), instruction | (i & 1 ? (2u << 29) | (2u << 4) : 0u), scales + i / 2 * 4,
-                                scales + L::SCALE_B + i / 2 * L::SCALE_B_STEP, i > 0 ? 1u : k > 0 ? 1u : 0u);
+                                scales + L::SCALE_B + i / 2 * L::SCALE_B_STEP + columnsAt, i > 0 ? 1u : k > 0 ? 1u : 0u);
                 mmaCommit<CTAS>(lead, empty + stage * 8);
                 mmaCommit<CTAS>(lead && k == steps - 1, accFull + acc * 8);
                 before2 = before1;
@@ -350,10 +392,31 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
             }
         };
         T* out = static_cast<T*>(p.out);
-        uint32_t accPhase = 0;
-        walk = Walk<FORWARD, BN, CTAS>(p, bounds, before, nullptr, group, EPILOGUE_GROUPS);
-        while (walk.next(t)) {
+        uint32_t accPhase = 0, stage = 0, phase = 0, turn = 0;
+        if constexpr (!WHOLE) walk = Walk<FORWARD, BN, CTAS>(p, bounds, before, nullptr, group, EPILOGUE_GROUPS);
+        bool ok = true;
+        while (ok && walk.next(t)) {
             if (t.expert < 0) break;
+            if constexpr (WHOLE) {   // the tile's rows, by both groups; then its epilogue, by one
+                for (int k = 0; k < steps; ++k) {
+                    if (!await(empty + stage * 8, phase ^ 1, failed)) { ok = false; break; }
+                    unsigned char* codes = base + stage * L::STAGE;
+                    const T* x = raws.x + static_cast<long long>(t.begin) * raws.stride;
+                    auto quantize = [&](auto aligned) {
+                        constexpr bool A = decltype(aligned)::value;
+                        if (p.sum <= 64) quantizeStep<T, A, 4>(x, raws.stride, t.end - t.begin, p.sum, k, codes, codes + L::SCALES);
+                        else if (p.sum <= 128) quantizeStep<T, A, 8>(x, raws.stride, t.end - t.begin, p.sum, k, codes, codes + L::SCALES);
+                        else quantizeStep<T, A, 16>(x, raws.stride, t.end - t.begin, p.sum, k, codes, codes + L::SCALES);
+                    };
+                    if (raws.aligned) quantize(std::true_type());
+                    else quantize(std::false_type());
+                    fenceProxyAsync();
+                    __syncwarp();
+                    if (lane == 0) barrierArrive(full + stage * 8);
+                    if (++stage == L::STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (!ok || (turn++ & 1) != static_cast<uint32_t>(group)) continue;
+            }
             const int tileRow = t.row + rank * BM;
             if (p.bias != nullptr) {
                 const T* row = static_cast<const T*>(p.bias) + static_cast<long long>(t.expert) * p.columns + t.column;
@@ -400,72 +463,64 @@ __global__ void __launch_bounds__(MX_THREADS, MxLayout<BN, CTAS>::BLOCKS)
 }
 
 // ---- few rows: matrix-vector products -----------------------------------------------------------------------------------------
-// The product of a handful of rows is bound by reading their experts' matrices once. blockIdx.y is a row; a block takes up to 4 consecutive rows of one
-// expert (the first of every 4 does the work) and, a warp each, 4 times 4 channels out, those whose scales share 16 bytes of a tile: n, n + 32, n + 64, n + 96. A
-// lane takes blocks of 32 channels: 16 bytes of codes; `split` warps share a row of the matrix where it has more than 32. Twice an e2m1 number is an integer of -12 to 12, so a block's sum is exact in four dp4a per 16 numbers; then
-// two powers of two and an fp32 sum. The first codes are asked for before the rows are quantised.
-constexpr int FEW_ROWS = 4, FEW_WARPS = 4, FEW_OUT = 4;
-// four codes, in the low 16 bits, to four bytes of twice their values
-__device__ __forceinline__ uint32_t decodeBytes(uint32_t codes, uint32_t signs)
+// The product of a handful of rows is bound by reading their experts' matrices. blockIdx.y is a row; its warps take 4 channels out each, those whose scales share 16
+// bytes of a tile: n, n + 32, n + 64, n + 96; `split` of them share these where the matrix' rows are long. A lane takes blocks of 32 channels: 16 bytes of codes.
+// Codes become pairs of halves, one instruction a pair, and so did the row's: products of e2m1 numbers are multiples of 1/4 up to 36, so that 8 of them are added up in
+// half without a rounding; from there on in fp32, times two powers of two. The first codes are asked for before the row is quantised. Rows of one expert read its matrix
+// each for itself (from L2, but for the first): blocks of up to 4 rows that share their reads took longer, 16 rows of 1024 -> 1024 9.5 us, now 6.9, 4 of 4096 -> 4096 14.6 us,
+// now 13.1. One row of 4096 -> 4096, 9 MB from memory: 6.6 us, 4 of them before the first byte comes; a way over bytes, twice a code's value looked up in registers, and
+// dp4a 8.3 us.
+constexpr int FEW_WARPS = 8, FEW_OUT = 4, PLANES = MX_BLOCK / 8;   // PLANES: of 8 channels, 16 bytes as halves
+// eight codes to four pairs of halves
+__device__ __forceinline__ void decodePairs(uint32_t codes, __half2* h)
 {
-    const uint32_t number = codes & 0x7777u;
-    const uint32_t up = __byte_perm(0x03020100u, 0x0c080604u, number), down = __byte_perm(0xfdfeff00u, 0xf4f8fafcu, number), mask = __byte_perm(0x0000ff00u, 0u, signs & 0x1111u);
-    return (up & ~mask) | (down & mask);
+    uint32_t u[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(codes));
+    memcpy(h, u, sizeof(u));
 }
-// eight codes to two words
-__device__ __forceinline__ uint2 decodeWords(uint32_t codes)
+constexpr int NO_SCALE = 1 << 12;   // in the place of a row's scale 255
+// sum * 2^(a + b - 254) for a row's scale a and a matrix' b, NaN if one of them is
+__device__ __forceinline__ float scaled(float sum, int a, uint32_t b)
 {
-    const uint32_t signs = codes >> 3;
-    return make_uint2(decodeBytes(codes, signs), decodeBytes(codes >> 16, signs >> 16));
-}
-// sum * 2^(a + b - 254) for scales a and b, NaN if one of them is. In two steps: a power alone may be out of range where the product is not.
-__device__ __forceinline__ float scaled(float sum, uint32_t a, uint32_t b)
-{
-    const int e = max(static_cast<int>(a + b), 4);   // (below, nothing is left of any sum)
-    const float first = __uint_as_float(static_cast<uint32_t>(e / 2) << 23), second = __uint_as_float(static_cast<uint32_t>(e - e / 2) << 23);
-    return max(a, b) == 255 ? __uint_as_float(0x7fffffffu) : sum * first * second;
+    const int e = a + static_cast<int>(b) - 127;
+    if (static_cast<unsigned>(e - 1) < 254u && b != 255) return sum * __uint_as_float(static_cast<uint32_t>(e) << 23);
+    if (a == NO_SCALE || b == 255) return __uint_as_float(0x7fffffffu);
+    // in two steps: a power alone is out of range where the product need not be (below 4, nothing is left of any sum)
+    const int two = max(e + 127, 4);
+    return sum * __uint_as_float(static_cast<uint32_t>(two / 2) << 23) * __uint_as_float(static_cast<uint32_t>(two - two / 2) << 23);
 }
 
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(FEW_WARPS * 32) mx_few_rows_kernel(const __grid_constant__ MxLinearArgs a, int codeBytes, int chunks, int split)
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) mx_few_rows_kernel(const __grid_constant__ MxLinearArgs a, int codeBytes, int chunks, int split)
 {
-    extern __shared__ uint4 quantized[];   // FEW_ROWS x 2 planes of half blocks x blocks; then the blocks' scales
-    __shared__ int found[2];
+    extern __shared__ uint4 quantized[];   // planes x blocks, 8 halves each; then the blocks' scales
+    __shared__ int found;
+    __shared__ float sums[FEW_WARPS][FEW_OUT];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y, experts = static_cast<int>(a.weight.matrices), columns = static_cast<int>(a.weight.rows);
     const int channels = a.weight.channels, blocks = codeBytes / 16;
-    const int group = blockIdx.x * (FEW_WARPS / split) + warp / split, within = group % 32, first = group / 32 * MX_TILE + within;   // channels out: first + 32 q
+    const int group = blockIdx.x * (FEW_WARPS / split) + warp / split, within = group % 32, tile = group / 32, first = tile * MX_TILE + within;   // channels out: first + 32 q
     T* y = static_cast<T*>(a.y.data);
     chained();
-    int expert = 0, count = min(FEW_ROWS, static_cast<int>(a.rows) - row);
-    if (a.offsets == nullptr) {
-        if (row % FEW_ROWS != 0) return;
-    } else {
-        if (threadIdx.x == 0) {
-            found[0] = experts + 1;
-            found[1] = 0;
-        }
+    int expert = 0;
+    if (a.offsets != nullptr) {
+        if (threadIdx.x == 0) found = experts + 1;
         __syncthreads();
         // the first offset behind the row ends its expert's run (offsets are their running maximum): that expert is the one before it
         int behind = experts + 1;
         for (int e = threadIdx.x; e <= experts; e += FEW_WARPS * 32)
             if (a.offsets[e] > row) { behind = e; break; }
-        if (behind <= experts) atomicMin(&found[0], behind);
+        if (behind <= experts) atomicMin(&found, behind);
         __syncthreads();
-        behind = found[0];
+        behind = found;
         if (behind == 0 || behind > experts) {   // nobody's row
             if (warp % split == 0 && lane < FEW_OUT && first + lane * 32 < columns) y[row * a.y.stride + first + lane * 32] = Element<T>::from(0.f);
             return;
         }
-        int reached = 0;
-        for (int e = threadIdx.x; e < behind; e += FEW_WARPS * 32) reached = max(reached, a.offsets[e]);
-        if (reached > 0) atomicMax(&found[1], reached);
-        __syncthreads();
-        if ((row - found[1]) % FEW_ROWS != 0) return;
         expert = behind - 1;
-        count = min(FEW_ROWS, static_cast<int>(min(a.rows, static_cast<long long>(a.offsets[behind]))) - row);
     }
     // codes and scales of a block of the warp's channels out (channels and blocks that are not there: the last ones again, and not used)
-    const int tile = blockIdx.x * FEW_WARPS / split / 32;
     const unsigned char* codes[FEW_OUT];
 #pragma unroll
     for (int q = 0; q < FEW_OUT; ++q) codes[q] = a.weight.codes + (static_cast<long long>(expert) * columns + min(first + q * 32, columns - 1)) * codeBytes;
@@ -477,93 +532,97 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) mx_few_rows_kernel(const __gri
         for (int q = 0; q < FEW_OUT; ++q) code[q] = *reinterpret_cast<const uint4*>(codes[q] + b * 16);
     };
     const int begin = warp % split * 32 + lane, step = split * 32;
-    uint4 code[FEW_OUT], scale;
-    fetch(begin, code, scale);
-    // the rows: half a block a thread
-    unsigned char* rowScales = reinterpret_cast<unsigned char*>(quantized + FEW_ROWS * 2 * blocks);
-    for (int r = 0; r < count; ++r) {
-        const T* x = static_cast<const T*>(a.x.data) + (row + r) * a.x.stride;
-        for (int h = threadIdx.x; h - lane < blocks * 2; h += FEW_WARPS * 32) {
-            const int left = channels - h * SIXTEEN;
-            Sixteen<T> v = loadSixteen<T, ALIGNED>(x + (left > 0 ? h * SIXTEEN : 0), left);
-            trim<T, ALIGNED>(v, left);
-            uint32_t largest = largestOf<T>(v);
-            largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-            const uint32_t s = scaleOf(largest);
-            const uint2 c = encodeSixteen<T>(v, s);
-            if (h >= blocks * 2) continue;
-            const uint2 low = decodeWords(c.x), high = decodeWords(c.y);
-            quantized[(r * 2 + (h & 1)) * blocks + h / 2] = make_uint4(low.x, low.y, high.x, high.y);
-            if ((h & 1) == 0) rowScales[r * blocks + h / 2] = static_cast<unsigned char>(s);
-        }
+    uint4 code[2][FEW_OUT], scale[2];   // of this turn and the next
+    fetch(begin, code[0], scale[0]);
+    fetch(begin + step, code[1], scale[1]);
+    // the row: half a block a thread
+    int16_t* rowScales = reinterpret_cast<int16_t*>(quantized + PLANES * blocks);
+    const T* x = static_cast<const T*>(a.x.data) + row * a.x.stride;
+    for (int h = threadIdx.x; h - lane < blocks * 2; h += FEW_WARPS * 32) {
+        const int left = channels - h * SIXTEEN;
+        Sixteen<T> v = loadSixteen<T, ALIGNED>(x + (left > 0 ? h * SIXTEEN : 0), left);
+        trim<T, ALIGNED>(v, left);
+        uint32_t largest = largestOf<T>(v);
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        const uint32_t s = scaleOf(largest);
+        const uint2 c = encodeSixteen<T>(v, s);
+        if (h >= blocks * 2) continue;
+        __half2 pairs[8];
+        decodePairs(c.x, pairs);
+        decodePairs(c.y, pairs + 4);
+        uint4 u[2];
+        memcpy(u, pairs, sizeof(u));
+        quantized[(h & 1) * 2 * blocks + h / 2] = u[0];
+        quantized[((h & 1) * 2 + 1) * blocks + h / 2] = u[1];
+        if ((h & 1) == 0) rowScales[h / 2] = static_cast<int16_t>(s == 255 ? NO_SCALE : static_cast<int>(s));
     }
     __syncthreads();
-    float sum[FEW_OUT][FEW_ROWS] = {};
-    for (int block = begin; block - lane < blocks; block += step) {
-        uint4 nextCode[FEW_OUT], nextScale;
-        if (block - lane + step < blocks) fetch(block + step, nextCode, nextScale);
-        if (block < blocks) {
-            const int at = (block & 3) * 8;
-            const uint32_t s[FEW_OUT] = {scale.x >> at & 255u, scale.y >> at & 255u, scale.z >> at & 255u, scale.w >> at & 255u};
+    float sum[FEW_OUT] = {};
+    auto add = [&](int block, const uint4 (&code)[FEW_OUT], const uint4& scale) {
+        const int at = (block & 3) * 8, rowScale = rowScales[block];
+        const uint32_t s[FEW_OUT] = {scale.x >> at & 255u, scale.y >> at & 255u, scale.z >> at & 255u, scale.w >> at & 255u};
+        float all[FEW_OUT] = {};
+#pragma unroll
+        for (int p = 0; p < PLANES; p += 2) {   // 16 channels
+            const uint4 u[2] = {quantized[p * blocks + block], quantized[(p + 1) * blocks + block]};
+            __half2 xs[8];
+            memcpy(xs, u, sizeof(u));
 #pragma unroll
             for (int q = 0; q < FEW_OUT; ++q) {
-                const uint2 w[4] = {decodeWords(code[q].x), decodeWords(code[q].y), decodeWords(code[q].z), decodeWords(code[q].w)};
+                const uint32_t words[PLANES] = {code[q].x, code[q].y, code[q].z, code[q].w};
+                __half2 w[8];
+                decodePairs(words[p], w);
+                decodePairs(words[p + 1], w + 4);
+                __half2 h = __hmul2(w[0], xs[0]);
 #pragma unroll
-                for (int r = 0; r < FEW_ROWS; ++r) {
-                    if (r >= count) break;
-                    const uint4 low = quantized[r * 2 * blocks + block], high = quantized[(r * 2 + 1) * blocks + block];
-                    int d = __dp4a(static_cast<int>(low.x), static_cast<int>(w[0].x), 0);
-                    d = __dp4a(static_cast<int>(low.y), static_cast<int>(w[0].y), d);
-                    d = __dp4a(static_cast<int>(low.z), static_cast<int>(w[1].x), d);
-                    d = __dp4a(static_cast<int>(low.w), static_cast<int>(w[1].y), d);
-                    d = __dp4a(static_cast<int>(high.x), static_cast<int>(w[2].x), d);
-                    d = __dp4a(static_cast<int>(high.y), static_cast<int>(w[2].y), d);
-                    d = __dp4a(static_cast<int>(high.z), static_cast<int>(w[3].x), d);
-                    d = __dp4a(static_cast<int>(high.w), static_cast<int>(w[3].y), d);
-                    sum[q][r] += scaled(0.25f * static_cast<float>(d), rowScales[r * blocks + block], s[q]);
-                }
+                for (int i = 1; i < 8; ++i) h = __hfma2(w[i], xs[i], h);
+                const float2 f = __half22float2(h);
+                all[q] += f.x + f.y;
             }
         }
 #pragma unroll
-        for (int q = 0; q < FEW_OUT; ++q) code[q] = nextCode[q];
-        scale = nextScale;
+        for (int q = 0; q < FEW_OUT; ++q) sum[q] += scaled(all[q], rowScale, s[q]);
+    };
+    for (int block = begin; block - lane < blocks; block += 2 * step) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int b = block + i * step;
+            if (b < blocks) add(b, code[i], scale[i]);
+            if (b - lane + 2 * step < blocks) fetch(b + 2 * step, code[i], scale[i]);
+        }
     }
-    // lane q * FEW_ROWS + r keeps that sum; then the warps that share channels out join theirs
+    // lane q keeps that sum; then the warps that share channels out join theirs
     float mine = 0.f;
 #pragma unroll
-    for (int q = 0; q < FEW_OUT; ++q)
-#pragma unroll
-        for (int r = 0; r < FEW_ROWS; ++r) {
-            if (r >= count) break;
-            const float all = groupSum<32>(sum[q][r]);
-            mine = lane == q * FEW_ROWS + r ? all : mine;
-        }
-    __shared__ float sums[FEW_WARPS][FEW_OUT * FEW_ROWS];
+    for (int q = 0; q < FEW_OUT; ++q) {
+        const float all = groupSum<32>(sum[q]);
+        mine = lane == q ? all : mine;
+    }
     if (split > 1) {
-        if (lane < FEW_OUT * FEW_ROWS) sums[warp][lane] = mine;
+        if (lane < FEW_OUT) sums[warp][lane] = mine;
         __syncthreads();
         if (warp % split != 0) return;
         mine = 0.f;
-        if (lane < FEW_OUT * FEW_ROWS)
+        if (lane < FEW_OUT)
             for (int w = 0; w < split; ++w) mine += sums[warp + w][lane];
     }
-    const int n = first + lane / FEW_ROWS * 32, r = lane % FEW_ROWS;
-    if (lane < FEW_OUT * FEW_ROWS && r < count && n < columns) {
+    const int n = first + lane * 32;
+    if (lane < FEW_OUT && n < columns) {
         const float b = a.bias != nullptr ? Element<T>::to(static_cast<const T*>(a.bias)[static_cast<long long>(expert) * columns + n]) : 0.f;
-        y[(row + r) * a.y.stride + n] = Element<T>::from(mine + b);
+        y[row * a.y.stride + n] = Element<T>::from(mine + b);
     }
 }
 
 // ---- bias gradient: column sums of an expert's rows --------------------------------------------------------------------------------
 // Pieces of BIAS_ROWS rows of one expert and 64 columns (32 element by element) a block, joined in order. 131072 rows of 1024 bfloat16, 16 experts: BIAS us (a block
 // per expert and 32 columns 199 us).
-constexpr int BIAS_ROWS = 512, BIAS_THREADS = 256;
+constexpr int BIAS_ROWS = 1024, BIAS_THREADS = 256;
 template <int VEC> constexpr int BIAS_LANES = VEC == 8 ? 8 : 32;
 template <class T, int VEC>
 __global__ void __launch_bounds__(BIAS_THREADS) mx_bias_kernel(const int2* __restrict__ list, const T* __restrict__ dy, long long stride, int columns, float* __restrict__ partial)
 {
     constexpr int LANES = BIAS_LANES<VEC>, STEP = BIAS_THREADS / LANES, COLUMNS = LANES * VEC, AT_ONCE = 8;
-    __shared__ float sums[STEP][COLUMNS];
+    __shared__ float sums[BIAS_THREADS / 32][COLUMNS];
     chained();
     const unsigned groups = (columns + COLUMNS - 1) / COLUMNS, piece = blockIdx.x / groups;   // (blocks side by side read the rows' neighbouring columns)
     const int firstColumn = static_cast<int>(blockIdx.x - piece * groups) * COLUMNS;
@@ -593,14 +652,21 @@ __global__ void __launch_bounds__(BIAS_THREADS) mx_bias_kernel(const int2* __res
             at += STEP * stride;
         }
     }
+    // the rows of a warp, then the warps
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sums[first][lane * VEC + j] = sum[j];
+    for (int o = LANES; o < 32; o *= 2)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+    if ((threadIdx.x & 31) < LANES) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sums[threadIdx.x / 32][lane * VEC + j] = sum[j];
+    }
     __syncthreads();
     const int column = firstColumn + threadIdx.x;
     if (threadIdx.x < COLUMNS && column < columns) {
         float all = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < STEP; ++i) all += sums[i][threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < BIAS_THREADS / 32; ++i) all += sums[i][threadIdx.x];
         partial[static_cast<long long>(piece) * columns + column] = all;
     }
 }
@@ -633,14 +699,14 @@ cudaError_t encoded(F&& run)
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 // `matrices` matrices of `rows` rows of `bytes` bytes, one behind the other (0: one, for a 2-D map), boxes of boxRows x boxBytes
-cudaError_t encodeBytes(CUtensorMap& map, const void* data, long long matrices, long long rows, int bytes, int boxBytes, int boxRows, bool swizzle)
+cudaError_t encodeBytes(CUtensorMap& map, const void* data, long long matrices, long long rows, int bytes, int boxBytes, int boxRows, CUtensorMapSwizzle swizzle)
 {
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(bytes / 4), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(matrices)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(bytes), static_cast<cuuint64_t>(bytes) * rows};
     const cuuint32_t box[3] = {static_cast<cuuint32_t>(boxBytes / 4), static_cast<cuuint32_t>(boxRows), 1}, one[3] = {1, 1, 1};
     return encoded([&] {
         return encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, matrices > 0 ? 3 : 2, const_cast<void*>(data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     });
 }
 // rows of D, boxes of 32 x 64 elements of 16 bits
@@ -656,15 +722,32 @@ cudaError_t encodeOut(CUtensorMap& map, void* data, long long rows, int columns,
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
+// One kernel, which quantises a tile's rows itself, where there are no more tiles than SMs and a tile's rows are a few batches of what its threads take at once (64
+// rows of 256 channels): a batch costs about a microsecond, the kernels that list and quantise the rows first 4 us with offsets and 2 us without. us, so / with
+// those kernels: 16 experts of 256 -> 256, 4 to 512 rows 7.2 to 7.7 / 11.1 to 11.7; 16 of 1024 -> 1024, 4 rows 9.7 / 12.2, 512 rows 12.7 / 12.7; 8 of 4096 -> 1024, 4
+// rows 19.5 / 16.2; one of 512 -> 2048, 4 rows 7.7 / 8.7, 128 rows 10.8 / 8.7.
+bool wholeRows(const MxLinearArgs& a)
+{
+    const int lanes = a.weight.channels <= 64 ? 4 : a.weight.channels <= 128 ? 8 : 16, batch = 1024 / lanes, steps = (a.weight.channels + STEP_CHANNELS - 1) / STEP_CHANNELS;
+    const long long rows = std::min<long long>((a.rows + a.weight.matrices - 1) / a.weight.matrices, MX_TILE);
+    return steps * ((rows + batch - 1) / batch) <= (a.weight.matrices > 1 ? 4 : 2);
+}
 struct Shape {
     int width, ctas;
+    bool whole;   // the product's kernel quantises the rows
 };
+long long rowTiles(const MxLinearArgs& a, int ctas);
 Shape shapeOf(const MxLinearArgs& a)
 {
     const int columns = static_cast<int>(a.weight.rows);
-    if (columns <= 64) return {64, 1};
-    if (columns <= 128 || a.rows / a.weight.matrices < 512 || a.weight.matrices > PAIR_EXPERTS) return {128, 1};
-    return {256, 2};
+    const long long tiles = rowTiles(a, 1);
+    if (wholeRows(a)) {
+        if (tiles * ((columns + 63) / 64) <= a.numSMs) return {64, 1, true};
+        if (tiles * ((columns + 127) / 128) <= a.numSMs) return {128, 1, true};
+    }
+    if (columns <= 64) return {64, 1, false};
+    if (columns <= 128 || a.rows / a.weight.matrices < 512 || a.weight.matrices > PAIR_EXPERTS) return {128, 1, false};
+    return {256, 2, false};
 }
 // tiles of 128 rows, none with rows of two experts, a multiple of ctas per expert: an upper bound
 long long rowTiles(const MxLinearArgs& a, int ctas)
@@ -696,37 +779,41 @@ cudaError_t quantizeRows(const MxLinearArgs& a, const ProductArgs& p, unsigned c
     });
 }
 
-template <class T, int BN, int CTAS>
-cudaError_t launchMx(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const CUtensorMap& out, const ProductArgs& p, int numSMs,
+template <class T, int BN, int CTAS, bool WHOLE, int KB>
+cudaError_t launchMx(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const CUtensorMap& out, const ProductArgs& p, const MxLinearArgs& m,
                      cudaStream_t stream)
 {
-    auto* kernel = mx_product_kernel<T, BN, CTAS>;
-    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), MxLayout<BN, CTAS>::bytes(MxLayout<BN, CTAS>::EXPERTS));
+    using L = MxLayout<BN, CTAS, WHOLE, KB>;
+    auto* kernel = mx_product_kernel<T, BN, CTAS, WHOLE, KB>;
+    const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), L::bytes(L::EXPERTS));
     if (e != cudaSuccess) return e;
-    return launchChained(kernel, numSMs / CTAS * CTAS * MxLayout<BN, CTAS>::BLOCKS, MX_THREADS, MxLayout<BN, CTAS>::bytes(p.experts), stream, CTAS, a, b, sa, sb, out, p, mxTiles(p.sum));
+    const RawRows<T> rows = {static_cast<const T*>(m.x.data), m.x.stride, wide(m.x, m.type, p.sum)};
+    return launchChained(kernel, m.numSMs / CTAS * CTAS * L::BLOCKS, MX_THREADS, L::bytes(p.experts), stream, CTAS, a, b, sa, sb, out, p, mxTiles(p.sum), rows);
 }
 
-// Rows that the matrix-vector kernel takes
-int fewBytes(int channels) { return FEW_ROWS * mxBlocks(channels) * (MX_BLOCK + 1); }
+// Rows that the matrix-vector kernel takes: as long as its blocks (8 warps, 32 channels out) go over the machine about twice. us, so / by the tensor cores: 1024 ->
+// 1024, 16 rows 6.9 / 9.1, 32 rows 11.5 / 9.0; 4096 -> 4096, 3 rows 12.0 / 13.1, 6 rows 18.2 / 13.1; 64 experts of 1024 -> 2048, 12 rows 11.5 / 15.2, 24 rows 19.2 / 16.7;
+// 16 of 1024 -> 1024, 24 rows 11.0 / 12.0, 32 rows 14.1 / 12.3; 64 of 256 -> 256, 64 rows 8.4 / 9.1.
+int fewGroups(const MxLinearArgs& a) { return mxTiles(a.weight.rows) * 32 / FEW_WARPS; }
+int fewBytes(int channels) { return mxBlocks(channels) * (PLANES * 16 + 2); }
 bool fewRows(const MxLinearArgs& a)
 {
-    return a.rows <= 64 && a.rows * a.weight.channels * a.weight.rows <= 1ll << 27 && fewBytes(a.weight.channels) <= 200 * 1024;
+    return a.rows <= 64 && (a.rows == 1 || fewGroups(a) * a.rows <= (a.weight.matrices > 1 ? 768 : 512)) && fewBytes(a.weight.channels) <= 200 * 1024;
 }
 template <class T>
 cudaError_t forwardFewRows(const MxLinearArgs& a, cudaStream_t stream)
 {
-    // warps that share a row of the matrix: as many as it has work for, while all blocks are resident (five on an SM)
-    const int blocks = mxBlocks(a.weight.channels), groups = mxTiles(a.weight.rows) * (32 / FEW_WARPS);
+    // warps that share channels out: as many as there is work for, while all blocks are resident
+    const int blocks = mxBlocks(a.weight.channels), groups = fewGroups(a);
     int split = 1;
-    while (split < FEW_WARPS && split * 32 < blocks && groups * split * 2 * a.rows <= a.numSMs * 5) split *= 2;
-    const dim3 grid(groups * split, static_cast<unsigned>(a.rows));
+    while (split < FEW_WARPS && split * 32 < blocks && groups * split * 2 * a.rows <= a.numSMs * 2) split *= 2;
     auto go = [&](auto* kernel) {
         const int bytes = fewBytes(a.weight.channels);
         if (bytes > 47 * 1024) {   // (48 KB without asking, which the kernel's static shared memory counts towards)
             const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), 200 * 1024);
             if (e != cudaSuccess) return e;
         }
-        launchChained(kernel, grid, FEW_WARPS * 32, bytes, stream, 1, a, mxCodeBytes(a.weight.channels), mxTiles(a.weight.channels), split);
+        launchChained(kernel, dim3(groups * split, static_cast<unsigned>(a.rows)), FEW_WARPS * 32, bytes, stream, 1, a, mxCodeBytes(a.weight.channels), mxTiles(a.weight.channels), split);
         return cudaGetLastError();
     };
     return wide(a.x, a.type, a.weight.channels) ? go(mx_few_rows_kernel<T, true>) : go(mx_few_rows_kernel<T, false>);
@@ -749,11 +836,16 @@ ProductArgs productArgs(const MxLinearArgs& a, const Shape& shape)
     p.wideStore = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.outStride % 8 == 0 && p.columns % 8 == 0;
     return p;
 }
-cudaError_t encodeWeight(const MxLinearArgs& a, CUtensorMap& map, CUtensorMap& scales)
+// codes, 128 or 32 bytes of a row per box
+cudaError_t encodeCodes(CUtensorMap& map, const void* data, long long matrices, long long rows, int bytes, int boxBytes)
+{
+    return encodeBytes(map, data, matrices, rows, bytes, boxBytes, 64, boxBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_32B);
+}
+cudaError_t encodeWeight(const MxLinearArgs& a, CUtensorMap& map, CUtensorMap& scales, int boxBytes)
 {
     const long long tiles = a.weight.matrices * mxTiles(a.weight.rows) * mxTiles(a.weight.channels);
-    const cudaError_t e = encodeBytes(map, a.weight.codes, a.weight.matrices, a.weight.rows, mxCodeBytes(a.weight.channels), 128, 64, true);
-    return e != cudaSuccess ? e : encodeBytes(scales, a.weight.scales, 0, tiles, MX_TILE_BYTES, MX_TILE_BYTES, 2, false);
+    const cudaError_t e = encodeCodes(map, a.weight.codes, a.weight.matrices, a.weight.rows, mxCodeBytes(a.weight.channels), boxBytes);
+    return e != cudaSuccess ? e : encodeBytes(scales, a.weight.scales, 0, tiles, MX_TILE_BYTES, MX_TILE_BYTES, 2, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 template <class T>
 cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
@@ -764,16 +856,25 @@ cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
     unsigned char *codes = static_cast<unsigned char*>(a.scratch), *scales = codes + s.scales;
     const ProductArgs p = productArgs(a, shape);
     const int chunks = mxTiles(p.sum), codeBytes = mxCodeBytes(p.sum);
-    CUtensorMap mapA, mapB, mapScaleA, mapScaleB, mapOut = {};
-    cudaError_t e = encodeBytes(mapA, codes, 0, a.rows, codeBytes, 128, 64, true);
-    if (e == cudaSuccess) e = encodeWeight(a, mapB, mapScaleB);
-    if (e == cudaSuccess) e = encodeBytes(mapScaleA, scales, 0, rowTiles(a, shape.ctas) * chunks, MX_TILE_BYTES, MX_TILE_BYTES, 2, false);
+    CUtensorMap mapA = {}, mapB, mapScaleA = {}, mapScaleB, mapOut = {};
+    const int boxBytes = !shape.whole && p.sum <= 64 ? 32 : 128;
+    cudaError_t e = encodeWeight(a, mapB, mapScaleB, boxBytes);
     if (e == cudaSuccess && p.wideStore) e = encodeOut(mapOut, p.out, a.rows, p.columns, p.outStride);
+    if (e != cudaSuccess) return e;
+    if (shape.whole)
+        return shape.width == 64 ? launchMx<T, 64, 1, true, 128>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a, stream)
+                                 : launchMx<T, 128, 1, true, 128>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a, stream);
+    e = encodeCodes(mapA, codes, 0, a.rows, codeBytes, boxBytes);
+    if (e == cudaSuccess) e = encodeBytes(mapScaleA, scales, 0, rowTiles(a, shape.ctas) * chunks, MX_TILE_BYTES, MX_TILE_BYTES, 2, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (e == cudaSuccess) e = quantizeRows<T>(a, p, codes, scales, reinterpret_cast<int2*>(codes + s.list), stream);
     if (e != cudaSuccess) return e;
-    if (shape.width == 64) return launchMx<T, 64, 1>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a.numSMs, stream);
-    if (shape.width == 128) return launchMx<T, 128, 1>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a.numSMs, stream);
-    return launchMx<T, 256, 2>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a.numSMs, stream);
+    auto go = [&](auto bytes) {
+        constexpr int KB = decltype(bytes)::value;
+        if (shape.width == 64) return launchMx<T, 64, 1, false, KB>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a, stream);
+        if (shape.width == 128) return launchMx<T, 128, 1, false, KB>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a, stream);
+        return launchMx<T, 256, 2, false, KB>(mapA, mapB, mapScaleA, mapScaleB, mapOut, p, a, stream);
+    };
+    return boxBytes == 32 ? go(std::integral_constant<int, 32>()) : go(std::integral_constant<int, 128>());
 }
 
 // scratch of the adjoint: [the matrices in 16 bits | scratch of the input gradient's product] or [pieces of the bias gradient | their sums], one after the other
@@ -834,7 +935,7 @@ cudaError_t biasGradient(const MxLinearArgs& a, const MxAdjointScratch& s, cudaS
 
 } // namespace
 
-size_t mxLinearBytes(const MxLinearArgs& a) { return a.rows == 0 || fewRows(a) ? 0 : MxScratch(a).bytes; }
+size_t mxLinearBytes(const MxLinearArgs& a) { return a.rows == 0 || fewRows(a) || shapeOf(a).whole ? 0 : MxScratch(a).bytes; }
 size_t mxLinearAdjointBytes(const MxLinearArgs& a) { return a.rows == 0 ? 0 : MxAdjointScratch(a).bytes; }
 
 cudaError_t launchMxLinear(const MxLinearArgs& a, cudaStream_t stream)
