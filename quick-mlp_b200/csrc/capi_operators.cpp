@@ -202,9 +202,14 @@ kernel::MxLinearArgs mxLinear(const qmlp_tensor_t* rows, const qmlp_mx_t* weight
     a.type = rows->precision;
     a.x = rowsOf(rows);   // (forward; the adjoint's rows are gradY)
     a.weight = matrixOf(weight);
+    return a;
+}
+// what asks the device comes behind the checks
+size_t onDevice(kernel::MxLinearArgs& a, bool adjoint)
+{
     a.numSMs = Library::instance().smCount();
     a.status = Library::instance().statusWord();
-    return a;
+    return adjoint ? kernel::mxLinearAdjointBytes(a) : kernel::mxLinearBytes(a);
 }
 void checkMxOffsets(const kernel::MxLinearArgs& a, const int32_t* offsets)
 {
@@ -593,7 +598,8 @@ int qmlp_mx_linear_forward_memory(const qmlp_tensor_t* input, const qmlp_mx_t* w
     QMLP_TRY
     checkPointer(bytes, "bytes");
     checkPointer(weight, "weight");
-    *bytes = kernel::mxLinearBytes(mxLinear(input, weight, weight->channels, "input"));
+    kernel::MxLinearArgs a = mxLinear(input, weight, weight->channels, "input");
+    *bytes = onDevice(a, false);
     QMLP_CATCH
 }
 int qmlp_mx_linear_forward(const qmlp_tensor_t* input, const qmlp_mx_t* weight, const int32_t* offsets, const qmlp_tensor_t* bias, qmlp_tensor_t* output,
@@ -610,7 +616,7 @@ int qmlp_mx_linear_forward(const qmlp_tensor_t* input, const qmlp_mx_t* weight, 
     checkSize(output, 1, weight->rows, "output");
     a.offsets = offsets;
     a.y = rowsOf(output);
-    checkScratch(tmp_memory, tmp_bytes, kernel::mxLinearBytes(a));
+    checkScratch(tmp_memory, tmp_bytes, onDevice(a, false));
     a.scratch = tmp_memory;
     launch(KERNEL_ID_MX_LINEAR_FORWARD, stream, [&](cudaStream_t s) { return kernel::launchMxLinear(a, s); });
     QMLP_CATCH
@@ -624,7 +630,7 @@ int qmlp_mx_linear_adjoint_memory(const qmlp_tensor_t* adj_output, const qmlp_mx
     a.gradY = rowsOf(adj_output);
     char wanted = 0;   // (only whether a gradient is wanted enters the size)
     if (adjoint_flags & QMLP_GRADIENTS_INPUT) a.gradX.data = &wanted;
-    *bytes = kernel::mxLinearAdjointBytes(a);
+    *bytes = onDevice(a, true);
     QMLP_CATCH
 }
 int qmlp_mx_linear_adjoint(const qmlp_tensor_t* adj_output, const qmlp_mx_t* weight, const int32_t* offsets, qmlp_tensor_t* adj_input, qmlp_tensor_t* adj_bias,
@@ -644,7 +650,7 @@ int qmlp_mx_linear_adjoint(const qmlp_tensor_t* adj_output, const qmlp_mx_t* wei
         a.gradX = rowsOf(adj_input);
     }
     a.gradBias = const_cast<void*>(mxBias(adj_bias, a, "adj_bias"));
-    checkScratch(tmp_memory, tmp_bytes, kernel::mxLinearAdjointBytes(a));
+    checkScratch(tmp_memory, tmp_bytes, onDevice(a, true));
     a.scratch = tmp_memory;
     launch(KERNEL_ID_MX_LINEAR_ADJOINT, stream, [&](cudaStream_t s) { return kernel::launchMxLinearAdjoint(a, s); });
     QMLP_CATCH

@@ -134,7 +134,7 @@ __device__ __forceinline__ uint2 encodeSixteen(const Sixteen<T>& p, uint32_t sca
 
 // A block of TILE_THREADS threads works on a tile of 128 rows x 128 channels. LANES threads share a row, 16 channels each (8 of them for 128 channels,
 // fewer for matrices that are narrower), two neighbours a block of 32. Rows that 16-byte accesses cannot read go through shared memory, read side by side (20011
-// rows of 777 floats: 27 us with 16 elements of a row per thread, which meet the same sectors 16 times; 46 us with a warp per row and its maximum by redux; QUANT us so).
+// rows of 777 floats: 27 us with 16 elements of a row per thread, which meet the same sectors 16 times; 46 us with a warp per row and its maximum by redux; 26 us so).
 constexpr int TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32;
 
 // `rows` rows of x, channels from 128 * chunk on, to codes (rows of codeBytes) and a tile of scales; tileScales: 512 bytes of shared memory.

@@ -570,5 +570,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("expert_linear", wrap_pybind_function_no_gil(expertLinear));
     m.def("dropout", wrap_pybind_function_no_gil(dropoutRows));
     m.def("mx_quantize", wrap_pybind_function_no_gil(mxQuantized));
+    m.def("mx_dequantize", wrap_pybind_function_no_gil(mxDequantized));
     m.def("mx_linear", wrap_pybind_function_no_gil(mxLinear));
 }

@@ -933,6 +933,10 @@ Tensor dropoutRows(const Tensor& input, double probability, int64_t seed, int64_
     return QMLP_CALL("dropout_forward", dropoutForward).call(input, residual, probability, seed, offset, step);
 }
 std::tuple<Tensor, Tensor> mxQuantized(const Tensor& input) { return QMLP_CALL("mx_quantize", mxQuantize).call(input); }
+Tensor mxDequantized(const Tensor& codes, const Tensor& scales, int64_t channels, c10::ScalarType type)
+{
+    return QMLP_CALL("mx_dequantize", mxDequantize).call(codes, scales, channels, type);
+}
 Tensor mxLinear(const Tensor& input, const Tensor& codes, const Tensor& scales, const OptTensor& offsets, const OptTensor& bias)
 {
     return QMLP_CALL("mx_linear_forward", mxLinearForward).call(input, codes, scales, offsets, bias);

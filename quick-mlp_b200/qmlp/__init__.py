@@ -5,8 +5,8 @@ from .import_library import load_library, load_torch_classes
 from .activation import FusedActivation
 from .encoding import FusedEncoding
 from .network import SimulatedNetwork, FusedNetwork, copy_torch_to_fused
-from .rows import (FusedEmbedding, FusedExperts, FusedLayerNorm, MXTensor, Routing, combine, dispatch, dropout, embedding,
-                   expert_linear, layer_norm, mx_dequantize, mx_linear, mx_quantize, route)
+from .rows import (FusedDropout, FusedEmbedding, FusedExperts, FusedLayerNorm, MXTensor, QuantizedExperts, Routing, combine, dispatch,
+                   dropout, embedding, expert_linear, layer_norm, mx_dequantize, mx_linear, mx_quantize, route)
 from .trainer import FusedTrainer, shard_points
 
 __all__ = [
@@ -20,10 +20,12 @@ __all__ = [
     "copy_torch_to_fused",
     "FusedTrainer",
     "shard_points",
+    "FusedDropout",
     "FusedEmbedding",
     "FusedExperts",
     "FusedLayerNorm",
     "MXTensor",
+    "QuantizedExperts",
     "Routing",
     "combine",
     "dispatch",

@@ -110,8 +110,9 @@ def mx_quantize(x: torch.Tensor) -> MXTensor:
 
 def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values of q in float32, float16 or bfloat16 (exact in the first and the last, in float16 within its range)."""
-    _capi.calls()
-    return torch.ops.qmlp_b200.mx_dequantize(q.codes, q.scales, q.channels, dtype)
+    if is_compiling() and _loaded():
+        return torch.ops.qmlp_b200.mx_dequantize(q.codes, q.scales, q.channels, dtype)
+    return _capi.calls().mx_dequantize(q.codes, q.scales, q.channels, dtype)
 
 
 def mx_linear(x: torch.Tensor, weight: MXTensor, offsets: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -159,14 +160,38 @@ class FusedEmbedding(torch.nn.Module):
         return f"{tuple(self.table.shape)}, scale={self.scale}"
 
 
+class FusedDropout(torch.nn.Module):
+    """Dropout in training, nothing but the residual's addition in evaluation. `step` counts the calls on the device, so that a step captured in a graph
+    drops other elements every time it is replayed, and a state_dict that is loaded goes on where it was saved."""
+
+    def __init__(self, p: float, seed: int = 0, device="cuda"):
+        super().__init__()
+        if not 0 <= p <= 1:
+            raise ValueError("p must be between 0 and 1")
+        self.p, self.seed = p, seed
+        self.register_buffer("step", torch.zeros(1, dtype=torch.int64, device=device))
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if not self.training:
+            return x if residual is None else x + residual
+        step = self.step.clone()      # what the gradient's call reads too
+        self.step.add_(1)
+        return dropout(x, self.p, self.seed, 0, residual, step)
+
+    def extra_repr(self):
+        return f"p={self.p}, seed={self.seed}"
+
+
 class FusedExperts(torch.nn.Module):
     """A layer of experts: a router picks k of them for every row, each is a two-layer network with an activation of the
     package between its layers, and their outputs are added up with the router's weights.
 
-    Parameters are kept in `weight_dtype` and cast to `dtype` (the type of the products) per call, like FusedNetwork's."""
+    Parameters are kept in `weight_dtype` and cast to `dtype` (the type of the products) per call, like FusedNetwork's.
+    dropout: share of the hidden channels dropped in training (behind the activation), by numbers that follow from `seed`.
+    quantized() gives the layer with its matrices in 4 bits."""
 
     def __init__(self, channels_in: int, channels_hidden: int, channels_out: int, experts: int, k: int = 2, activation: str = "relu",
-                 normalize: bool = True, weight_dtype=torch.float32, dtype=torch.float16, device="cuda"):
+                 normalize: bool = True, weight_dtype=torch.float32, dtype=torch.float16, device="cuda", dropout: float = 0.0, seed: int = 0):
         super().__init__()
         from .activation import FusedActivation
         if dtype not in (torch.float16, torch.bfloat16):
@@ -184,16 +209,52 @@ class FusedExperts(torch.nn.Module):
         self.bias1 = torch.nn.Parameter(torch.zeros((experts, channels_hidden), dtype=weight_dtype, device=device))
         self.weight2 = uniform(experts, channels_out, channels_hidden, fan_in=channels_hidden)
         self.bias2 = torch.nn.Parameter(torch.zeros((experts, channels_out), dtype=weight_dtype, device=device))
+        self.dropout = FusedDropout(dropout, seed, device) if dropout > 0 else None
+
+    def quantized(self) -> "QuantizedExperts":
+        """A copy whose matrices are kept and multiplied in 4 bits, for serving."""
+        return QuantizedExperts(self)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape, x = x.shape, x.reshape(-1, x.shape[-1])
         routing = route(torch.nn.functional.linear(x.float(), self.router.float()), self.k, self.normalize)
         h = dispatch(x.to(self.dtype), routing)
         h = expert_linear(h, self.weight1.to(self.dtype), routing.offsets, self.bias1.to(self.dtype))
-        h = expert_linear(self.activation(h), self.weight2.to(self.dtype), routing.offsets, self.bias2.to(self.dtype))
+        h = self.activation(h)
+        if self.dropout is not None:
+            h = self.dropout(h)
+        h = expert_linear(h, self.weight2.to(self.dtype), routing.offsets, self.bias2.to(self.dtype))
         y = combine(h, routing)
         return y.reshape(*shape[:-1], y.shape[-1])
 
     def extra_repr(self):
         e, hidden, n_in = self.weight1.shape
         return f"{n_in} -> {hidden} -> {self.weight2.shape[1]}, experts={e}, k={self.k}"
+
+
+class QuantizedExperts(torch.nn.Module):
+    """A layer of experts (FusedExperts) with its matrices in 4 bits; the rows of both products are quantised in their calls. Nothing of it is trained; gradients
+    of the rows pass through (mx_linear), for what is in front of it."""
+
+    def __init__(self, layer: FusedExperts):
+        super().__init__()
+        self.k, self.normalize, self.dtype, self.activation = layer.k, layer.normalize, layer.dtype, layer.activation
+        self.channels_in, self.channels_hidden = layer.weight1.shape[2], layer.weight2.shape[2]
+        with torch.no_grad():
+            tensors = {"router": layer.router.detach().float().clone(), "bias1": layer.bias1.to(self.dtype), "bias2": layer.bias2.to(self.dtype)}
+            for name, weight in (("1", layer.weight1), ("2", layer.weight2)):
+                tensors["codes" + name], tensors["scales" + name], _ = mx_quantize(weight.detach())
+        for name, t in tensors.items():
+            self.register_buffer(name, t.detach())
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        shape, x = x.shape, x.reshape(-1, x.shape[-1])
+        routing = route(torch.nn.functional.linear(x.float(), self.router), self.k, self.normalize)
+        h = dispatch(x.to(self.dtype), routing)
+        h = self.activation(mx_linear(h, MXTensor(self.codes1, self.scales1, self.channels_in), routing.offsets, self.bias1))
+        h = mx_linear(h, MXTensor(self.codes2, self.scales2, self.channels_hidden), routing.offsets, self.bias2)
+        y = combine(h, routing)
+        return y.reshape(*shape[:-1], y.shape[-1])
+
+    def extra_repr(self):
+        return f"{self.channels_in} -> {self.channels_hidden} -> {self.bias2.shape[1]}, experts={self.bias1.shape[0]}, k={self.k}, 4 bits"
