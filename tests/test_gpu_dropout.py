@@ -99,6 +99,10 @@ def test_dropout_probabilities(qmlp):
     assert not qmlp.dropout(x, 1.0, 5).any() and torch.equal(qmlp.dropout(x, 1.0, 5, residual=r), r)
     leaf = x.clone().requires_grad_()
     assert not torch.autograd.grad(qmlp.dropout(leaf, 1.0, 5), leaf, r)[0].any()
+    bad = torch.full_like(x, float("nan"))
+    for residual in (r, r[:1].expand(500, 64), r.t().contiguous().t(), rand(16, (500, 70))[:, 3:67]):
+        assert torch.equal(qmlp.dropout(bad, 1.0, 5, residual=residual), residual)
+    assert not qmlp.dropout(bad[:, 1:50], 1.0, 5).any()
     case(qmlp, x, r, 1 - 2.0 ** -16, x)
     for bad in (float("inf"), float("nan")):
         y = qmlp.dropout(torch.full_like(x, bad), 0.5, SEED, OFFSET, residual=r)
