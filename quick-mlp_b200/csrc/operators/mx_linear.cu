@@ -167,6 +167,7 @@ __device__ __forceinline__ void storeAccumulator(uint32_t from, bool sharedLast,
 {
     const int lane = threadIdx.x & 31;
     const bool whole = o.wide && o.rows >= 32;
+    constexpr bool EARLY = BN == 256;   // all 64 columns at once, so that `read` comes early (of 64 columns in all, nothing waits for it, and registers are short)
 #pragma unroll 1
     for (int i = 0; i < BN / 64; ++i) {
         const int c = (sharedLast ? (i + BN / 64 - 1) % (BN / 64) : i) * 64;
@@ -174,12 +175,24 @@ __device__ __forceinline__ void storeAccumulator(uint32_t from, bool sharedLast,
         if (used) {
             if (lane == 0) tmaStoresRead();   // what was written from this memory last
             __syncwarp();
+            float both64[2][32];
+            if constexpr (EARLY) {
+                tmemLoad32(from + c, both64[0]);
+                tmemLoad32(from + c + 32, both64[1]);
+                tmemWait(both64[0], both64[1]);
+                if (i == 0) read();
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float v[32];
-                tmemLoad32(from + c + h * 32, v);
-                tmemWait32(v);
-                if (h == 1 && i == 0) read();
+                if constexpr (EARLY) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = both64[h][j];
+                } else {
+                    tmemLoad32(from + c + h * 32, v);
+                    tmemWait32(v);
+                    if (h == 1 && i == 0) read();
+                }
                 const int c0 = c + h * 32;
                 if (bias != nullptr) {
 #pragma unroll
