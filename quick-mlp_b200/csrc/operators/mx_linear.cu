@@ -160,6 +160,48 @@ struct OutTile {
     long long stride;
     bool wide;
 };
+// 64 columns of `rows` rows from a warp's memory (rows of 128 bytes, their 16-byte chunks swizzled as the TMA's) to D where the TMA cannot write: 16 bytes at a time, or
+// pairs of elements that begin on 4 bytes, which in rows of an odd address are the second and third, fourth and fifth, ... (20000 rows of 64 experts of 300 -> 777:
+// element by element 58 us for the call, so 48 us; 23 us for 776 columns, by TMA.)
+template <class T>
+__device__ __forceinline__ void storeChunk(const unsigned char* mine, T* out, long long stride, int rows, int columns, bool wide)
+{
+    const int lane = threadIdx.x & 31;
+    auto at = [&](int r, int c) { return mine + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2; };
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + lane / 8, c = lane % 8 * 8;
+            if (r < rows && c < columns) store<T, 8>(out + r * stride + c, load<T, 8>(reinterpret_cast<const T*>(at(r, c))));
+        }
+        return;
+    }
+    constexpr int AT_ONCE = 8;   // (all read before the first is written: the compiler has to take either memory for the other)
+    for (int first = 0; first < rows; first += AT_ONCE) {
+        uint32_t pair[AT_ONCE], before[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = first + i, odd = static_cast<int>((reinterpret_cast<uintptr_t>(out + r * stride) >> 1) & 1), c = 2 * lane + odd;
+            const uint32_t low = *reinterpret_cast<const unsigned short*>(at(r, c)), high = *reinterpret_cast<const unsigned short*>(at(r, (c + 1) & 63));
+            pair[i] = low | high << 16;
+            before[i] = *reinterpret_cast<const unsigned short*>(at(r, 0));
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = first + i;
+            if (r >= rows) break;
+            T* row = out + r * stride;
+            const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(row) >> 1) & 1), c = 2 * lane + odd;
+            // (predicates: the branches that a condition becomes took 150 clocks a row)
+            const bool both = c + 1 < min(columns, 64);
+            asm volatile("{\n\t.reg .pred p, q, s;\n\t.reg .b16 u, v;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 s, %6, 0;\n\t"
+                         "cvt.u16.u32 u, %2;\n\tcvt.u16.u32 v, %3;\n\t@p st.global.b32 [%0], %2;\n\t@q st.global.b16 [%0], u;\n\t@s st.global.b16 [%1], v;\n\t}"
+                         ::"l"(row + c), "l"(row), "r"(pair[i]), "r"(before[i]), "r"(static_cast<int>(both)), "r"(static_cast<int>(!both && c < columns)),
+                         "r"(static_cast<int>(odd != 0 && lane == 0)) : "memory");
+        }
+    }
+}
+
 // A warp's 32 lanes of an accumulator of BN columns from `from` on, plus a bias. `sharedLast`: the last 64 columns first (those that the other accumulator begins
 // with); `read` is called when the first 64 are.
 template <class T, int BN, class F>
@@ -204,18 +246,18 @@ __device__ __forceinline__ void storeAccumulator(uint32_t from, bool sharedLast,
                         v[j + 3] += f.w;
                     }
                 }
-                if (whole) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        store<T, 8>(reinterpret_cast<T*>(mine + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)), pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[j * 8])));
-                } else if (c0 < o.columns) {
-                    storeTile<T>(v, mine, out + static_cast<long long>(o.row) * o.stride + o.column, o.stride, o.rows, c0, o.columns, o.wide);
-                }
+                for (int j = 0; j < 4; ++j)
+                    store<T, 8>(reinterpret_cast<T*>(mine + lane * 128 + (((h * 4 + j) ^ (lane & 7)) << 4)), pack<T, 8>(*reinterpret_cast<const float (*)[8]>(&v[j * 8])));
             }
             if (whole) {
                 fenceProxyAsync();
                 __syncwarp();
                 if (lane == 0) tmaStore(map, o.column + c, o.row, smemAddress(mine));
+            } else {
+                __syncwarp();
+                storeChunk<T>(mine, out + static_cast<long long>(o.row) * o.stride + o.column + c, o.stride, min(o.rows, 32), o.columns - c, o.wide);
+                __syncwarp();
             }
         } else if (i == 0) {
             read();

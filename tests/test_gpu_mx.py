@@ -173,6 +173,32 @@ def test_linear_outside(qmlp):
         linear_case(qmlp, x, q, exact, torch.tensor(bad, dtype=torch.int32, device="cuda"), b, g)
 
 
+@pytest.mark.parametrize("rows", [7, 40, 64])
+def test_linear_few_rows_offsets(qmlp, rows):
+    """a handful of rows: experts without rows, rows of nobody, offsets out of range or out of order, one expert with offsets"""
+    q, exact = weights(qmlp, 46, (4, 72, 100))
+    x, b, g = rand(47, (rows, 100), torch.float16), rand(48, (4, 72), torch.float16), rand(49, (rows, 72), torch.float16)
+    for bad in ([0, 3, 3, 5, rows], [2, 2, 4, 4, 5], [-5, 6, 4, 5, 3], [rows, 3, 2, 1, 0], [0, rows, 0, rows, 0], [2 ** 31 - 1] * 5, [-2 ** 31] * 5, [-1, 1, 2, 3, 10 * rows], [1, 1, 1, 1, 1]):
+        linear_case(qmlp, x, q, exact, torch.tensor(bad, dtype=torch.int32, device="cuda"), b, g)
+    one = q._replace(codes=q.codes[:1], scales=q.scales[:1])
+    for ends in ([0, rows], [2, 5], [3, 1], [0, 0]):
+        linear_case(qmlp, x, one, exact[:1], torch.tensor(ends, dtype=torch.int32, device="cuda"), b[:1], g)
+
+
+def test_linear_long(qmlp):
+    """codes that pass 2^32 bytes: rows at both ends"""
+    rows, n_in = 600000, 16384
+    base = rand(52, (3, n_in), torch.float16)
+    q, exact = weights(qmlp, 53, (40, n_in))
+    offsets = None
+    for at in (0, 2):
+        y = qmlp.mx_linear(base[at:at + 1].expand(rows, n_in), q, offsets)
+        want, slack = mx.mx_linear(base[at:at + 1], exact, None, None)[0]
+        for r in (0, 131072, 262143, 524289, rows - 1):
+            ref.check(y[r:r + 1], want, slack, f"row {r}")
+        assert torch.equal(y[1:], y[:-1])
+
+
 @pytest.mark.parametrize("rows,n_in,n_out", [(1, 96, 40), (9, 96, 40), (200, 96, 40), (700, 300, 300)])
 def test_linear_not_finite(qmlp, rows, n_in, n_out):
     """an infinity or NaN in a row makes that row NaN, one in a row of the matrix that channel, and nothing else"""
