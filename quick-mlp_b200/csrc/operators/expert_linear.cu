@@ -16,7 +16,7 @@
 //
 // One persistent block per SM, or a pair of blocks that share tiles of 256 x 256 (cta_group::2; each block loads half of either operand):
 // a TMA warp, an MMA warp, two groups of four epilogue warps, one per accumulator, so that the products of a tile run under the
-// epilogues of the two before; in the weight product four more warps add up the columns of dy for the bias gradient, from the
+// epilogues of the two before; in the weight product (and on request in the input gradient's) four more warps add up the columns of dy for the bias gradient, from the
 // stages that are in shared memory anyway. Which tile is whose follows from the offsets, which every block adds up for itself: the group
 // sizes never travel to the host. 16 experts, 131072 rows, 1024 -> 1024 bfloat16: 200, 196 and 205 us for the three products, 3 us more
 // with the bias gradient (1.34 to 1.40 PFLOP/s; a library product of one matrix of that size 198 us, at clocks that the power limit holds
@@ -327,6 +327,45 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
             for (long long r = me; r < first + (p.rows - last); r += threads) {
                 T* row = out + (r < first ? r : last + (r - first)) * p.outStride;
                 for (int c = lane; c < p.columns; c += 32) row[c] = Element<T>::from(0.f);
+            }
+        }
+    } else if constexpr (SUMS && MODE == INPUT) {
+        // ---- column sums of dy beside the input gradient, of 32 rows a warp, left for a kernel that joins them -------------------
+        const int group = warp - (2 + EPILOGUE_WARPS);
+        uint32_t stage = 0, phases = 0;                      // phases: one bit per stage
+        bool ok = true;
+        if (blockIdx.x == 0)
+            for (int e = threadIdx.x - (2 + EPILOGUE_WARPS) * 32; e <= p.experts; e += SUM_WARPS * 32) reinterpret_cast<int*>(p.plan)[e] = before[e];
+        while (ok && walk.next(t)) {
+            const int steps = walk.steps(t);
+            if (t.expert < 0) break;
+            if (t.column != 0) {
+                stage = (stage + steps) % L::STAGES;
+                continue;
+            }
+            const int rows = max(0, min(32, t.end - t.row - static_cast<int>(rank) * BM - group * 32));
+            float* to = p.partialBias + ((static_cast<long long>(t.slot) * CTAS + rank) * SUM_WARPS + group) * p.sum;
+            for (int k = 0; k < steps; ++k) {
+                // (the four warps leave together: none may wait for another below)
+                if (!sumWarpsAgree(await(landed + stage * 8, phases >> stage & 1, failed))) { ok = false; break; }
+                phases ^= 1u << stage;
+                const unsigned char* box = base + stage * L::STAGE + (group >> 1) * BOX + (group & 1) * 32 * 128;
+                auto pair = [&](int r) { return toPair(reinterpret_cast<const Pack<T, 2>*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)->v); };
+                float2 sum[4] = {};
+                if (rows == 32) {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) sum[r & 3] = add2(sum[r & 3], pair(r));
+                } else {
+                    for (int r = 0; r < rows; ++r) sum[0] = add2(sum[0], pair(r));
+                }
+                __syncwarp();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (threadIdx.x == (2 + EPILOGUE_WARPS) * 32) barrierArrive(empty + stage * 8);
+                const float2 all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                const int channel = k * BK + lane * 2;
+                if (channel < p.sum) to[channel] = all.x;
+                if (channel + 1 < p.sum) to[channel + 1] = all.y;
+                if (++stage == L::STAGES) stage = 0;
             }
         }
     } else if constexpr (SUMS) {
@@ -1311,7 +1350,9 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         p.out = a.gradX.data;
         p.outStride = a.gradX.stride;
         p.wideStore = wideOut(p.out, p.outStride, p.columns);
-        e = launchShape<T, INPUT>(shape, mapY, mapW, p, a.numSMs, stream);
+        p.partialBias = a.columnSums;
+        p.plan = reinterpret_cast<int2*>(a.unitsBefore);
+        e = a.columnSums != nullptr ? launchShape<T, INPUT, true>(shape, mapY, mapW, p, a.numSMs, stream) : launchShape<T, INPUT>(shape, mapY, mapW, p, a.numSMs, stream);
     }
     if (e == cudaSuccess && a.gradWeight != nullptr) {
         e = readable<T>(x, xStride, a.rows, a.channelsIn, base + s.x, stream);
@@ -1346,6 +1387,11 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
 
 } // namespace
 
+int expertSumsPerUnit(const ExpertArgs& a) { return rowShape(a, a.channelsIn).ctas * SUM_WARPS; }
+long long expertSums(const ExpertArgs& a)
+{
+    return (a.rows / (BM * rowShape(a, a.channelsIn).ctas) + std::min<long long>(a.rows, a.experts)) * expertSumsPerUnit(a);
+}
 size_t expertBytes(const ExpertArgs& a, bool adjoint) { return a.rows == 0 || (!adjoint && fewRows(a)) ? 0 : Scratch(a, adjoint).bytes; }
 
 cudaError_t launchExpertForward(const ExpertArgs& a, cudaStream_t stream)

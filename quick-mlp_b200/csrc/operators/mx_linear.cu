@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) mx_few_rows_kernel(const __
     }
 }
 
-// ---- bias gradient: column sums of an expert's rows --------------------------------------------------------------------------------
+// ---- bias gradient without an input gradient: column sums of an expert's rows --------------------------------------------------------------------------------
 // Pieces of BIAS_ROWS rows of one expert and 64 columns (32 element by element) a block, joined in order. 131072 rows of 1024 bfloat16, 16 experts: 57 us (a block
 // per expert and 32 columns 199 us).
 constexpr int BIAS_ROWS = 1024, BIAS_THREADS = 256;
@@ -725,16 +725,28 @@ __global__ void __launch_bounds__(BIAS_THREADS) mx_bias_kernel(const int2* __res
         partial[static_cast<long long>(piece) * columns + column] = all;
     }
 }
+// the sums of an expert's pieces, perUnit of them for each of its units, of 32 columns: JOIN_ROWS threads to a column
+constexpr int JOIN_ROWS = 16;
 template <class T>
-__global__ void __launch_bounds__(128) mx_bias_join_kernel(const int* __restrict__ unitsBefore, const float* __restrict__ partial, int columns, T* __restrict__ out)
+__global__ void __launch_bounds__(32 * JOIN_ROWS) mx_bias_join_kernel(const int* __restrict__ unitsBefore, int perUnit, const float* __restrict__ partial, int columns, T* __restrict__ out)
 {
+    __shared__ float sums[JOIN_ROWS][32];
     chained();
-    const int expert = blockIdx.x, c = blockIdx.y * 128 + threadIdx.x;
-    if (c >= columns) return;
+    const int expert = blockIdx.x, lane = threadIdx.x & 31, part = threadIdx.x / 32, c = blockIdx.y * 32 + lane;
+    const long long end = static_cast<long long>(unitsBefore[expert + 1]) * perUnit;
     float sum = 0.f;
+    if (c < columns) {
 #pragma unroll 8
-    for (int u = unitsBefore[expert]; u < unitsBefore[expert + 1]; ++u) sum += partial[static_cast<long long>(u) * columns + c];
-    out[static_cast<long long>(expert) * columns + c] = Element<T>::from(sum);
+        for (long long u = static_cast<long long>(unitsBefore[expert]) * perUnit + part; u < end; u += JOIN_ROWS) sum += partial[u * columns + c];
+    }
+    sums[part][lane] = sum;
+    __syncthreads();
+    if (part == 0 && c < columns) {
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < JOIN_ROWS; ++i) sum += sums[i][lane];
+        out[static_cast<long long>(expert) * columns + c] = Element<T>::from(sum);
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -932,19 +944,21 @@ cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
     return boxBytes == 32 ? go(std::integral_constant<int, 32>()) : go(std::integral_constant<int, 128>());
 }
 
-// scratch of the adjoint: [the matrices in 16 bits | scratch of the input gradient's product] or [pieces of the bias gradient | their sums], one after the other
+// scratch of the adjoint: [units before the experts | the bias gradient's sums | the matrices in 16 bits | scratch of the input gradient's product], or, where the bias
+// gradient is all that is wanted, [units | sums | list of its pieces]
 struct MxAdjointScratch {
-    size_t product, before, partial, bytes;
+    size_t partial, matrices, product, list, bytes;
     int pieces;
     explicit MxAdjointScratch(const MxLinearArgs& a)
     {
-        product = a.gradX.data == nullptr || a.rows == 0 ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * a.weight.channels * 2);
+        const ExpertArgs r = inputGradient(a);
         pieces = static_cast<int>(a.rows / BIAS_ROWS + std::min<long long>(a.rows, a.weight.matrices));
-        before = align256(static_cast<size_t>(pieces) * sizeof(int2));
-        partial = before + align256((static_cast<size_t>(a.weight.matrices) + 1) * sizeof(int));
-        bytes = std::max(product + (a.gradX.data == nullptr ? 0 : expertBytes(inputGradient(a), true)), partial + static_cast<size_t>(pieces) * static_cast<size_t>(a.weight.rows) * sizeof(float));
+        partial = align256((static_cast<size_t>(a.weight.matrices) + 1) * sizeof(int));
+        matrices = list = partial + align256(static_cast<size_t>(a.gradX.data != nullptr ? expertSums(r) : pieces) * static_cast<size_t>(a.weight.rows) * sizeof(float));
+        product = matrices + (a.gradX.data == nullptr ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * a.weight.channels * 2));
+        bytes = a.gradX.data != nullptr ? product + expertBytes(r, true) : list + align256(static_cast<size_t>(pieces) * sizeof(int2));
     }
-    // the product with the matrices in 16 bits at the start of the scratch
+    // the product with the matrices in 16 bits
     static ExpertArgs inputGradient(const MxLinearArgs& a)
     {
         ExpertArgs r{};
@@ -954,7 +968,6 @@ struct MxAdjointScratch {
         r.channelsOut = static_cast<int>(a.weight.rows);
         r.type = a.type;
         r.numSMs = a.numSMs;
-        r.weight = a.scratch;
         r.offsets = a.offsets;
         r.gradY = a.gradY;
         r.gradX = a.gradX;
@@ -963,13 +976,22 @@ struct MxAdjointScratch {
     }
 };
 template <class T>
+cudaError_t joinBias(const MxLinearArgs& a, const MxAdjointScratch& s, int perUnit, cudaStream_t stream)
+{
+    const int columns = static_cast<int>(a.weight.rows);
+    const unsigned char* base = static_cast<const unsigned char*>(a.scratch);
+    launchChained(mx_bias_join_kernel<T>, dim3(static_cast<unsigned>(a.weight.matrices), (columns + 31) / 32), 32 * JOIN_ROWS, 0, stream, 1, reinterpret_cast<const int*>(base), perUnit,
+                  reinterpret_cast<const float*>(base + s.partial), columns, static_cast<T*>(a.gradBias));
+    return cudaGetLastError();
+}
+// the bias gradient alone
+template <class T>
 cudaError_t biasGradient(const MxLinearArgs& a, const MxAdjointScratch& s, cudaStream_t stream)
 {
     const int columns = static_cast<int>(a.weight.rows), experts = static_cast<int>(a.weight.matrices);
-    if (a.rows == 0) return cudaMemsetAsync(a.gradBias, 0, static_cast<size_t>(experts) * columns * sizeof(T), stream);
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
-    auto *list = reinterpret_cast<int2*>(base);
-    auto *before = reinterpret_cast<int*>(base + s.before);
+    auto *list = reinterpret_cast<int2*>(base + s.list);
+    auto *before = reinterpret_cast<int*>(base);
     auto *partial = reinterpret_cast<float*>(base + s.partial);
     ProductArgs p{};
     p.rows = a.rows;
@@ -983,9 +1005,7 @@ cudaError_t biasGradient(const MxLinearArgs& a, const MxAdjointScratch& s, cudaS
                       columns, partial);
         return cudaGetLastError();
     });
-    if (e != cudaSuccess) return e;
-    launchChained(mx_bias_join_kernel<T>, dim3(experts, (columns + 127) / 128), 128, 0, stream, 1, before, partial, columns, static_cast<T*>(a.gradBias));
-    return cudaGetLastError();
+    return e != cudaSuccess ? e : joinBias<T>(a, s, 1, stream);
 }
 
 } // namespace
@@ -1000,15 +1020,26 @@ cudaError_t launchMxLinear(const MxLinearArgs& a, cudaStream_t stream)
 }
 cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream)
 {
+    if (a.rows == 0) return a.gradBias == nullptr ? cudaSuccess : cudaMemsetAsync(a.gradBias, 0, static_cast<size_t>(a.weight.matrices) * a.weight.rows * 2, stream);
     const MxAdjointScratch s(a);
-    cudaError_t e = cudaSuccess;
-    if (a.gradBias != nullptr) e = a.type == TYPE_HALF ? biasGradient<__half>(a, s, stream) : biasGradient<__nv_bfloat16>(a, s, stream);
-    if (e != cudaSuccess || a.gradX.data == nullptr || a.rows == 0) return e;
-    e = launchMxDequantize(a.weight, a.type, {a.scratch, a.weight.channels}, stream);
+    if (a.gradX.data == nullptr) {
+        if (a.gradBias == nullptr) return cudaSuccess;
+        return a.type == TYPE_HALF ? biasGradient<__half>(a, s, stream) : biasGradient<__nv_bfloat16>(a, s, stream);
+    }
+    unsigned char* base = static_cast<unsigned char*>(a.scratch);
+    cudaError_t e = launchMxDequantize(a.weight, a.type, {base + s.matrices, a.weight.channels}, stream);
     if (e != cudaSuccess) return e;
+    // the product's tiles of dy lie in shared memory: their columns are added up there
     ExpertArgs r = MxAdjointScratch::inputGradient(a);
-    r.scratch = static_cast<unsigned char*>(a.scratch) + s.product;
-    return launchExpertAdjoint(r, stream);
+    r.weight = base + s.matrices;
+    r.scratch = base + s.product;
+    if (a.gradBias != nullptr) {
+        r.columnSums = reinterpret_cast<float*>(base + s.partial);
+        r.unitsBefore = reinterpret_cast<int*>(base);
+    }
+    e = launchExpertAdjoint(r, stream);
+    if (e != cudaSuccess || a.gradBias == nullptr) return e;
+    return a.type == TYPE_HALF ? joinBias<__half>(a, s, expertSumsPerUnit(r), stream) : joinBias<__nv_bfloat16>(a, s, expertSumsPerUnit(r), stream);
 }
 
 } // namespace kernel

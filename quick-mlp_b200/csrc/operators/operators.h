@@ -105,7 +105,13 @@ struct ExpertArgs {
     void *gradWeight, *gradBias;   // may be null
     void* scratch;
     int* status;
+    // column sums of gradY beside an input gradient alone (null: none): expertSums rows of channelsOut floats, expertSumsPerUnit for every unit of rows of an
+    // expert, one expert's behind another's; units of the experts in front of each (experts + 1)
+    float* columnSums;
+    int* unitsBefore;
 };
+int expertSumsPerUnit(const ExpertArgs& a);
+long long expertSums(const ExpertArgs& a);   // an upper bound
 // scratch of a forward call (adjoint = false) or an adjoint call
 size_t expertBytes(const ExpertArgs& a, bool adjoint);
 cudaError_t launchExpertForward(const ExpertArgs& a, cudaStream_t stream);

@@ -260,6 +260,27 @@ def test_linear_layouts(qmlp):
     assert y.shape == (4, 5, 6, 80) and torch.equal(y.view(120, 80), flat) and dx.shape == leaf.shape
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["half", "bfloat16"])
+@pytest.mark.parametrize("counts,n_in,n_out", [(None, 40, 7), (None, 300, 130), ([3000, 0, 1, 2049], 512, 200), ([33, 31, 700], 96, 65), ([5] * 100, 130, 333), ([70000], 32, 66)])
+def test_linear_gradients_apart(qmlp, counts, n_in, n_out, dtype):
+    """the gradients of the rows, of the bias, and of both: each for itself what the formula says, and the rows' the same either way"""
+    e, rows = (1, 777) if counts is None else (len(counts), sum(counts))
+    q, exact = weights(qmlp, 85, (n_out, n_in) if counts is None else (e, n_out, n_in))
+    x, b, g = rand(86, (rows, n_in), dtype), rand(87, (n_out,) if counts is None else (e, n_out), dtype), rand(88, (rows, n_out), dtype)
+    offsets = None if counts is None else offsets_of(counts)
+    want = mx.mx_linear(x, exact, offsets, b, g)
+    got = []
+    for rows_too, bias_too in ((True, True), (True, False), (False, True)):
+        leaves = [x.clone().requires_grad_(rows_too), b.clone().requires_grad_(bias_too)]
+        grads = list(torch.autograd.grad(qmlp.mx_linear(leaves[0], q, offsets, leaves[1]), [t for t in leaves if t.requires_grad], g))
+        got.append(grads.pop(0) if rows_too else None)
+        if rows_too:
+            ref.check(got[-1], *want[1], "rows")
+        if bias_too:
+            ref.check(grads[0].view(want[2][0].shape), *want[2], "bias")
+    assert torch.equal(got[0], got[1])
+
+
 def test_linear_empty(qmlp):
     q, _ = weights(qmlp, 80, (3, 8, 16))
     x, b = (torch.ones(s, dtype=torch.float16, device="cuda", requires_grad=True) for s in ((0, 16), (3, 8)))
