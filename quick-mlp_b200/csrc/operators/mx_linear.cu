@@ -3,15 +3,19 @@
 //   y_r = W_e q(x_r) + b_e          W_e: (channels out, channels in) in 4 bits; q: the row in 4 bits (mx.cuh)
 //   dx_r = W_e^T dy_r               (straight through q), W_e decoded to 16 bits, which is exact, and the product of expert_linear.cu
 //
-// Two kernels. The first quantises the rows, tile by tile of 128 rows of one expert, so that a tile's scales lie as the tensor core wants them. The second
-// is the product D (128 x BN, fp32 in tensor memory) += A B, 256 channels in a step: codes by TMA in boxes of 64 rows x 128 bytes (256 channels), 128-byte
+// Two kernels (one for small calls, and another for a few rows; the rules stand at the end). The first quantises the rows, tile by tile of 128 rows of one expert,
+// so that a tile's scales lie as the tensor core wants them. The second is the product D (128 x BN, fp32 in tensor memory) += A B, 256 channels in a step: codes by TMA in boxes of 64 rows x 128 bytes (256 channels), 128-byte
 // swizzled, both operands K-major; scales by TMA in tiles of 512 bytes, copied to tensor memory by tcgen05.cp in front of the products that use them. A
 // product multiplies 64 channels, blocks of 32 with their two scales (kind::mxf4), exactly, and adds them up in fp32. What lies outside a matrix arrives as zeros.
 // A tile that reaches behind its expert's last row reads rows of the next one, which only fill rows of D that are not stored.
 //
 // One persistent block per SM, or a pair of blocks that share tiles of 256 x 256: a TMA warp, an MMA warp, two groups of four epilogue warps,
 // one per accumulator. Tensor memory has no room for two accumulators of 256 columns and the scales: there the second begins 64 columns before
-// the first one's end, and the epilogue reads the shared columns first.
+// the first one's end, and the epilogue reads the shared columns first. 16384 rows of 4096 -> 4096 bfloat16: 31 us and 93 us (5.9 PFLOP/s); 16 experts, 131072 rows,
+// 1024 -> 1024: 55 and 76 us, of which the shared columns cost about a third (a tile's 4 steps take 2050 clocks, until the next one's first product goes out 1200 more pass:
+// accumulator complete, 64 columns read, released, issued). All eight warps of the epilogue on every tile, or a tile looked up ahead, did not change that. 512 experts,
+// 1000003 rows, 64 -> 64 half: 24 and 32 us. Quantising the rows in the product's kernel by eight more warps (no second pass over them) took 109 us for that and 258 us for
+// the experts before: conversions want the warps of a whole SM.
 // Waits are bounded: on a timeout the block drains, gives its tensor memory back and sets the library's status word.
 #include "mx.cuh"
 #include "products.cuh"
@@ -91,8 +95,9 @@ __device__ __forceinline__ uint64_t scaleDescriptor(uint32_t address) { return s
 
 // ---- the rows in 4 bits ----------------------------------------------------------------------------------------------------
 // Tiles of 128 rows of one expert, in the order of the product's units (of tileRows rows): tile t of all is part t % (tileRows / 128) of unit t / (tileRows / 128).
-// First row and rows of every tile (`piece` rows, or what is left), a thread each; where the experts' units begin, if `unitsBefore` is given. (A block of the quantisation that looks for its tile's expert itself has to add up the offsets first: as
-// persistent blocks, which do it once, that kernel took 103 us for 131072 rows of 1024 bfloat16, a block per tile with this list 73 us, and 60 us with all its loads unconditional.)
+// First row and rows of every tile (`piece` rows, or what is left), a thread each; where the experts' units begin, if `unitsBefore` is given. (A block of the
+// quantisation that looks for its tile's expert itself has to add up the offsets first: as persistent blocks, which do it once, that kernel took 103 us for 131072
+// rows of 1024 bfloat16, a block per tile with this list 73 us, and 55 us with loads that depend on no condition.)
 __global__ void __launch_bounds__(TILE_THREADS) mx_tiles_kernel(const __grid_constant__ ProductArgs p, int2* __restrict__ list, int tiles, int piece,
                                                                 int* __restrict__ unitsBefore)
 {
