@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_quantize_kernel(const __grid_
 }
 
 // Rows that 16-byte accesses cannot write: a warp per row, a lane per channel of a block, element by element side by side (20011 rows of 777 floats: 16 elements
-// of a row per thread 75 us, so 25).
+// of a row per thread 75 us, so 20).
 template <class T, int LANES, bool ALIGNED>
 __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __grid_constant__ MxMatrix q, T* __restrict__ y, long long stride, int tilesPerMatrix, int chunks,
                                                                      int codeBytes)
@@ -46,25 +46,31 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __gri
     const unsigned char *codes = q.codes + t.row * codeBytes, *scales = q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES;
     if constexpr (!ALIGNED) {
         constexpr int AT_ONCE = 4, BLOCKS = MX_TILE / MX_BLOCK;
-        const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, c = chunk * MX_TILE + lane;
+        const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, c = chunk * MX_TILE + lane, shift = (lane & 1) * 4;
+        int at[BLOCKS];   // of a lane's code in a row
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) at[b] = min(c + b * MX_BLOCK, q.channels - 1) / 2;
         for (int i = warp; i < t.rows; i += TILE_WARPS * AT_ONCE) {
             uint32_t code[AT_ONCE][BLOCKS], scale[AT_ONCE];
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 const int r = min(i + k * TILE_WARPS, t.rows - 1);
-                scale[k] = *reinterpret_cast<const uint32_t*>(scales + (r & 31) * 16 + (r >> 5) * 4);
+                const unsigned char* row = codes + static_cast<long long>(r) * codeBytes;
+                scale[k] = scales[(r & 31) * 16 + (r >> 5) * 4 + (lane & 3)];   // a lane per block
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b)
-                    code[k][b] = codes[static_cast<long long>(r) * codeBytes + min(c + b * MX_BLOCK, q.channels - 1) / 2];
+                for (int b = 0; b < BLOCKS; ++b) code[k][b] = row[at[b]];
             }
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 const int r = i + k * TILE_WARPS;
                 if (r >= t.rows) break;
+                const float power = powerOf(scale[k]);
+                T* row = y + (t.row + r) * stride + c;
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b)
-                    if (c + b * MX_BLOCK < q.channels)
-                        y[(t.row + r) * stride + c + b * MX_BLOCK] = Element<T>::from(decodeOne(code[k][b] >> (lane & 1) * 4) * powerOf(scale[k] >> b * 8 & 255u));
+                for (int b = 0; b < BLOCKS; ++b) {
+                    const float v = decodeOne(code[k][b] >> shift) * __shfl_sync(0xffffffffu, power, b);
+                    if (c + b * MX_BLOCK < q.channels) row[b * MX_BLOCK] = Element<T>::from(v);
+                }
             }
         }
     } else {

@@ -139,7 +139,7 @@ __device__ __forceinline__ uint2 encodeSixteen(const Sixteen<T>& p, uint32_t sca
 
 // A block of TILE_THREADS threads works on a tile of 128 rows x 128 channels. LANES threads share a row, 16 channels each (8 of them for 128 channels,
 // fewer for matrices that are narrower), two neighbours a block of 32. Rows that 16-byte accesses cannot read go through shared memory, read side by side (20011
-// rows of 777 floats: 27 us with 16 elements of a row per thread, which meet the same sectors 16 times; 46 us with a warp per row and its maximum by redux; 26 us so).
+// rows of 777 floats: 27 us with 16 elements of a row per thread, which meet the same sectors 16 times; 46 us with a warp per row and its maximum by redux; 23 us so).
 constexpr int TILE_THREADS = 256, TILE_WARPS = TILE_THREADS / 32;
 
 // `rows` rows of x, channels from 128 * chunk on, to codes (rows of codeBytes) and a tile of scales; tileScales: 512 bytes of shared memory.
@@ -179,9 +179,19 @@ __device__ __forceinline__ void quantizeTile(const T* x, long long stride, int r
         const int column = threadIdx.x % CHANNELS, line = threadIdx.x / CHANNELS, channel = min(chunk * MX_TILE + column, channels - 1);
         constexpr int LINES = TILE_THREADS / CHANNELS;
         T v[PER];
+        const T* from = x + channel;
         auto ask = [&](int begin) {
+            if (begin + ROWS <= rows) {
+                const T* row = from + (begin + line) * stride;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] = x[min(begin + i * LINES + line, rows - 1) * stride + channel];
+                for (int i = 0; i < PER; ++i) {
+                    v[i] = *row;
+                    row += LINES * stride;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[i] = from[min(begin + i * LINES + line, rows - 1) * stride];
+            }
         };
         ask(0);
         for (int begin = 0; begin < rows; begin += ROWS) {
