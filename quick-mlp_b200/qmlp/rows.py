@@ -241,11 +241,12 @@ class QuantizedExperts(torch.nn.Module):
         self.k, self.normalize, self.dtype, self.activation = layer.k, layer.normalize, layer.dtype, layer.activation
         self.channels_in, self.channels_hidden = layer.weight1.shape[2], layer.weight2.shape[2]
         with torch.no_grad():
-            tensors = {"router": layer.router.detach().float().clone(), "bias1": layer.bias1.to(self.dtype), "bias2": layer.bias2.to(self.dtype)}
+            tensors = {"router": layer.router.float(), "bias1": layer.bias1.to(self.dtype), "bias2": layer.bias2.to(self.dtype)}
+            tensors = {name: t.detach().clone() for name, t in tensors.items()}      # (of the type it should be, `to` gives the parameter itself)
             for name, weight in (("1", layer.weight1), ("2", layer.weight2)):
                 tensors["codes" + name], tensors["scales" + name], _ = mx_quantize(weight.detach())
         for name, t in tensors.items():
-            self.register_buffer(name, t.detach())
+            self.register_buffer(name, t)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape, x = x.shape, x.reshape(-1, x.shape[-1])

@@ -76,6 +76,12 @@ def test_experts(qmlp, dtype):
         for rows in (1, 3, 64, 700):      # single rows, small calls, larger ones
             assert torch.equal(again(x[:rows]), served(x[:rows]))
             assert torch.allclose(served(x[:rows]).float(), y[:rows].detach().float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+        exact = qmlp.FusedExperts(48, 100, 24, experts=6, k=2, dtype=dtype, weight_dtype=dtype)      # (parameters of the products' type)
+        copied = exact.quantized()
+        before = copied(x)
+        for p in exact.parameters():
+            p.add_(1)
+        assert torch.equal(copied(x), before)
 
 
 def test_training_step_captured(qmlp):
