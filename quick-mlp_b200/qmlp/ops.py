@@ -74,6 +74,24 @@ for _name, _schema in SCHEMAS.items():
     for _key in ("CompositeExplicitAutograd", "Autograd"):
         _library.impl(_name, _load(_name), _key)
 
+
+
+def dropout_step(step):
+    """a copy of a layer's count of calls, which is then advanced. Refused inside a backward pass: a forward pass that is recomputed there
+    (activation checkpointing) has to repeat its numbers, and which call of the count it repeats cannot be known."""
+    if torch._C._current_graph_task_id() != -1:
+        raise _capi.QmlpError("dropout with a seed counts its calls and cannot be recomputed in a backward pass (activation checkpointing): the recomputed call would "
+                              "drop other elements. Call qmlp.dropout with a step of your own")
+    before = step.clone()
+    step.add_(1)
+    return before
+
+
+# (an operator, so that a call that was compiled before it is checkpointed is refused too)
+_library.define("dropout_step(Tensor(a!) step) -> Tensor", tags=(torch.Tag.pt2_compliant_tag,))
+for _key in ("CUDA", "CPU", "Meta"):
+    _library.impl("dropout_step", dropout_step, _key)
+
 activation_forward = torch.ops.qmlp_b200.activation_forward
 activation_adjoint = torch.ops.qmlp_b200.activation_adjoint
 encoding_forward = torch.ops.qmlp_b200.encoding_forward

@@ -14,7 +14,7 @@ import torch
 from torch.compiler import assume_constant_result, is_compiling
 
 from . import _capi
-from . import ops  # noqa: F401  (registers torch.ops.qmlp_b200.*)
+from . import ops  # (registers torch.ops.qmlp_b200.*)
 
 
 @assume_constant_result
@@ -162,7 +162,8 @@ class FusedEmbedding(torch.nn.Module):
 
 class FusedDropout(torch.nn.Module):
     """Dropout in training, nothing but the residual's addition in evaluation. `step` counts the calls on the device, so that a step captured in a graph
-    drops other elements every time it is replayed, and a state_dict that is loaded goes on where it was saved."""
+    drops other elements every time it is replayed, and a state_dict that is loaded goes on where it was saved. A call that is recomputed in a
+    backward pass (activation checkpointing) is refused: the count does not say which call it repeats."""
 
     def __init__(self, p: float, seed: int = 0, device="cuda"):
         super().__init__()
@@ -174,8 +175,7 @@ class FusedDropout(torch.nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training:
             return x if residual is None else x + residual
-        step = self.step.clone()      # what the gradient's call reads too
-        self.step.add_(1)
+        step = (torch.ops.qmlp_b200 if is_compiling() else ops).dropout_step(self.step)      # what the gradient's call reads too
         return dropout(x, self.p, self.seed, 0, residual, step)
 
     def extra_repr(self):
