@@ -81,7 +81,7 @@ def dropout_step(step):
     (activation checkpointing) has to repeat its numbers, and which call of the count it repeats cannot be known."""
     if torch._C._current_graph_task_id() != -1:
         raise _capi.QmlpError("dropout with a seed counts its calls and cannot be recomputed in a backward pass (activation checkpointing): the recomputed call would "
-                              "drop other elements. Call qmlp.dropout with a step of your own")
+                              "drop other elements. A layer without a seed takes its numbers from torch's generator, which is restored then")
     before = step.clone()
     step.add_(1)
     return before

@@ -161,11 +161,16 @@ class FusedEmbedding(torch.nn.Module):
 
 
 class FusedDropout(torch.nn.Module):
-    """Dropout in training, nothing but the residual's addition in evaluation. `step` counts the calls on the device, so that a step captured in a graph
-    drops other elements every time it is replayed, and a state_dict that is loaded goes on where it was saved. A call that is recomputed in a
-    backward pass (activation checkpointing) is refused: the count does not say which call it repeats."""
+    """Dropout in training, nothing but the residual's addition in evaluation.
 
-    def __init__(self, p: float, seed: int = 0, device="cuda"):
+    Without a seed every call takes its numbers from a draw of torch's generator of x's device, as torch's own dropout: layers drop different elements, a
+    captured step other ones every time it is replayed, torch.manual_seed repeats them (ranks that are to differ seed differently), and a call
+    that is recomputed in a backward pass (activation checkpointing, which restores the generator) drops the same ones.
+
+    With a seed the numbers follow from it and from `step`, which counts the calls on the device: layers of equal seeds drop equal elements, a captured step counts on
+    in every replay, and a state_dict that is loaded goes on where it was saved. A recomputed call is refused then: the count does not say which call it repeats."""
+
+    def __init__(self, p: float, seed: Optional[int] = None, device="cuda"):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError("p must be between 0 and 1")
@@ -175,6 +180,8 @@ class FusedDropout(torch.nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training:
             return x if residual is None else x + residual
+        if self.seed is None:
+            return dropout(x, self.p, 0, 0, residual, torch.randint(2 ** 63 - 1, (1,), device=x.device))
         step = (torch.ops.qmlp_b200 if is_compiling() else ops).dropout_step(self.step)      # what the gradient's call reads too
         return dropout(x, self.p, self.seed, 0, residual, step)
 
@@ -187,11 +194,11 @@ class FusedExperts(torch.nn.Module):
     package between its layers, and their outputs are added up with the router's weights.
 
     Parameters are kept in `weight_dtype` and cast to `dtype` (the type of the products) per call, like FusedNetwork's.
-    dropout: share of the hidden channels dropped in training (behind the activation), by numbers that follow from `seed`.
+    dropout: share of the hidden channels dropped in training (behind the activation), with or without a `seed` as FusedDropout.
     quantized() gives the layer with its matrices in 4 bits."""
 
     def __init__(self, channels_in: int, channels_hidden: int, channels_out: int, experts: int, k: int = 2, activation: str = "relu",
-                 normalize: bool = True, weight_dtype=torch.float32, dtype=torch.float16, device="cuda", dropout: float = 0.0, seed: int = 0):
+                 normalize: bool = True, weight_dtype=torch.float32, dtype=torch.float16, device="cuda", dropout: float = 0.0, seed: Optional[int] = None):
         super().__init__()
         from .activation import FusedActivation
         if dtype not in (torch.float16, torch.bfloat16):

@@ -74,3 +74,44 @@ def test_checkpoint_in_a_compiled_call(qmlp):
     with pytest.raises(RuntimeError, match="recomputed"):
         call(meta(6, 16).requires_grad_()).sum().backward()
     torch._dynamo.reset()
+
+
+def test_layers_without_a_seed(qmlp, monkeypatch):
+    """every call of every layer takes a number of its own from torch's generator, which repeats it; a seed that is given stays what it is, 0 too"""
+    seen = []
+    real = torch.randint
+    monkeypatch.setattr(torch, "randint", lambda high, size, device: real(high, size))      # (numbers, where meta tensors have none)
+    monkeypatch.setattr(qmlp.rows, "dropout", lambda x, p, seed, offset, residual, step: seen.append((seed, offset, int(step))) or x)
+    layers = [qmlp.FusedDropout(0.5, device="meta") for _ in range(2)] + [qmlp.FusedExperts(16, 32, 8, experts=4, device="meta", dropout=0.5).dropout]
+
+    def run():
+        seen.clear()
+        torch.manual_seed(9)
+        for _ in range(3):
+            for layer in layers:
+                layer(meta(4, 8))
+        return list(seen)
+    first = run()
+    assert len(set(first)) == 9 and run() == first
+    seen.clear()
+    torch.manual_seed(10)
+    layers[0](meta(4, 8))
+    assert seen[0] != first[0]
+    for seed in (0, 7):
+        counted = qmlp.FusedDropout(0.5, seed, device="cpu")
+        seen.clear()
+        for _ in range(3):
+            counted(meta(4, 8))
+        assert seen == [(seed, 0, i) for i in range(3)]
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+@pytest.mark.parametrize("compiled", [False, True])
+def test_checkpointed_without_a_seed(qmlp, reentrant, compiled):
+    torch._dynamo.reset()
+    block = Block(qmlp.FusedDropout(0.3, device="meta"))
+    call = torch.compile(block, fullgraph=True, backend="aot_eager") if compiled else block
+    x = meta(6, 16).requires_grad_()
+    checkpoint(call, x, use_reentrant=reentrant).sum().backward()
+    assert x.grad.shape == x.shape
+    torch._dynamo.reset()
