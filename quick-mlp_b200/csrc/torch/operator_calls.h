@@ -739,9 +739,10 @@ Tensor dropoutForwardAutograd(const Tensor& input, const OptTensor& residual, do
     return QMLP_CALL("dropout_forward", dropoutForward).call(input, residual, probability, seed, offset, step);
 }
 
-// (codes have no gradient)
+// (codes have no gradient, and as whole numbers no tangent)
 std::tuple<Tensor, Tensor> mxQuantizeAutograd(const Tensor& input)
 {
+    refuseTangents("mx_quantize", input);
     at::AutoDispatchBelowADInplaceOrView below;
     return QMLP_CALL("mx_quantize", mxQuantize).call(input);
 }
