@@ -241,7 +241,8 @@ class FusedExperts(torch.nn.Module):
 
 class QuantizedExperts(torch.nn.Module):
     """A layer of experts (FusedExperts) with its matrices in 4 bits; the rows of both products are quantised in their calls. Nothing of it is trained; gradients
-    of the rows pass through (mx_linear), for what is in front of it."""
+    of the rows pass through (mx_linear), for what is in front of it.
+    The router and the biases are cast per call, like FusedExperts', so that a model may be cast as a whole."""
 
     def __init__(self, layer: FusedExperts):
         super().__init__()
@@ -257,10 +258,10 @@ class QuantizedExperts(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape, x = x.shape, x.reshape(-1, x.shape[-1])
-        routing = route(torch.nn.functional.linear(x.float(), self.router), self.k, self.normalize)
+        routing = route(torch.nn.functional.linear(x.float(), self.router.float()), self.k, self.normalize)
         h = dispatch(x.to(self.dtype), routing)
-        h = self.activation(mx_linear(h, MXTensor(self.codes1, self.scales1, self.channels_in), routing.offsets, self.bias1))
-        h = mx_linear(h, MXTensor(self.codes2, self.scales2, self.channels_hidden), routing.offsets, self.bias2)
+        h = self.activation(mx_linear(h, MXTensor(self.codes1, self.scales1, self.channels_in), routing.offsets, self.bias1.to(self.dtype)))
+        h = mx_linear(h, MXTensor(self.codes2, self.scales2, self.channels_hidden), routing.offsets, self.bias2.to(self.dtype))
         y = combine(h, routing)
         return y.reshape(*shape[:-1], y.shape[-1])
 

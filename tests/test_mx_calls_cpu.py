@@ -24,3 +24,23 @@ def test_quantize_refuses_tangents(qmlp):
     codes = qmlp.mx_quantize(meta(8, 40)).codes
     with fwad.dual_level(), pytest.raises(ValueError, match="floating"):
         fwad.make_dual(codes, codes)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_served_layers_are_cast(qmlp, dtype, monkeypatch):
+    """a model with a served layer that is cast as a whole still runs: what the products are given has their type (meta tensors do not see to that)"""
+    linear, mx_linear = torch.nn.functional.linear, qmlp.rows.mx_linear
+
+    def checked_linear(x, w):
+        assert x.dtype == w.dtype == torch.float32
+        return linear(x, w)
+
+    def checked_mx_linear(x, weight, offsets, bias):
+        assert x.dtype == bias.dtype == dtype
+        return mx_linear(x, weight, offsets, bias)
+    monkeypatch.setattr(torch.nn.functional, "linear", checked_linear)
+    monkeypatch.setattr(qmlp.rows, "mx_linear", checked_mx_linear)
+    for cast in (torch.float16, torch.bfloat16, torch.float32, torch.float64):
+        served = qmlp.FusedExperts(16, 32, 8, experts=4, dtype=dtype, device="meta").quantized().to(cast)
+        y = served(meta(7, 16, dtype=cast))
+        assert served.bias1.dtype == cast and served.codes1.dtype == torch.uint8 and y.shape == (7, 8) and y.dtype == dtype
