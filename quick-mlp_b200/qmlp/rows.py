@@ -216,7 +216,7 @@ class FusedExperts(torch.nn.Module):
         self.bias1 = torch.nn.Parameter(torch.zeros((experts, channels_hidden), dtype=weight_dtype, device=device))
         self.weight2 = uniform(experts, channels_out, channels_hidden, fan_in=channels_hidden)
         self.bias2 = torch.nn.Parameter(torch.zeros((experts, channels_out), dtype=weight_dtype, device=device))
-        self.dropout = FusedDropout(dropout, seed, device) if dropout > 0 else None
+        self.dropout = FusedDropout(dropout, seed, device) if dropout != 0 else None      # (which refuses what is no probability)
 
     def quantized(self) -> "QuantizedExperts":
         """A copy whose matrices are kept and multiplied in 4 bits, for serving."""

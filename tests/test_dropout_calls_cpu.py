@@ -115,3 +115,9 @@ def test_checkpointed_without_a_seed(qmlp, reentrant, compiled):
     checkpoint(call, x, use_reentrant=reentrant).sum().backward()
     assert x.grad.shape == x.shape
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("dropout", [-0.1, 1.5, float("nan")])
+def test_experts_refuse_what_is_no_probability(qmlp, dropout):
+    with pytest.raises(ValueError, match="between 0 and 1"):
+        qmlp.FusedExperts(16, 32, 8, experts=4, device="meta", dropout=dropout)
