@@ -252,7 +252,8 @@ class QuantizedExperts(torch.nn.Module):
             tensors = {"router": layer.router.float(), "bias1": layer.bias1.to(self.dtype), "bias2": layer.bias2.to(self.dtype)}
             tensors = {name: t.detach().clone() for name, t in tensors.items()}      # (of the type it should be, `to` gives the parameter itself)
             for name, weight in (("1", layer.weight1), ("2", layer.weight2)):
-                tensors["codes" + name], tensors["scales" + name], _ = mx_quantize(weight.detach())
+                weight = weight.detach()
+                tensors["codes" + name], tensors["scales" + name], _ = mx_quantize(weight.float() if weight.dtype == torch.float64 else weight)
         for name, t in tensors.items():
             self.register_buffer(name, t)
 

@@ -31,3 +31,11 @@ def test_served_layers_are_cast(qmlp, dtype):
             for name in ("router", "bias1", "bias2"):
                 getattr(layer, name).copy_(getattr(layer, name).to(cast).to(dtype).to(cast))
             assert torch.equal(layer.quantized().to(cast)(x), layer.quantized()(x))
+
+
+def test_layers_in_64_bits_are_served(qmlp):
+    torch.manual_seed(3)
+    layer = qmlp.FusedExperts(48, 96, 24, experts=4)
+    x = rand(4, (100, 48))
+    with torch.no_grad():
+        assert torch.equal(layer.double().quantized()(x), layer.float().quantized()(x))

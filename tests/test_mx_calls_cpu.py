@@ -44,3 +44,15 @@ def test_served_layers_are_cast(qmlp, dtype, monkeypatch):
         served = qmlp.FusedExperts(16, 32, 8, experts=4, dtype=dtype, device="meta").quantized().to(cast)
         y = served(meta(7, 16, dtype=cast))
         assert served.bias1.dtype == cast and served.codes1.dtype == torch.uint8 and y.shape == (7, 8) and y.dtype == dtype
+
+
+def test_layers_in_64_bits_are_served(qmlp, monkeypatch):
+    """parameters in float64, which a layer casts per call, are rounded to float32 first (meta tensors would take any type)"""
+    seen = []
+    quantize = qmlp.rows.mx_quantize
+    monkeypatch.setattr(qmlp.rows, "mx_quantize", lambda w: seen.append(w.dtype) or quantize(w))
+    for given, taken in ((torch.float64, torch.float32), (torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)):
+        layer = qmlp.FusedExperts(16, 32, 8, experts=4, weight_dtype=given, device="meta")
+        served = layer.quantized()
+        assert seen == [taken] * 2 and served(meta(7, 16)).shape == layer(meta(7, 16)).shape
+        seen.clear()
