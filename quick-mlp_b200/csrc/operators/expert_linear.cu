@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
 #pragma unroll
                 for (int i = 0; i < BN / 32; ++i) bias[i] = p.bias != nullptr && t.column + i * 32 + lane < p.columns ? Element<T>::to(row[i * 32 + lane]) : 0.f;
             }
+            const float power = MODE == INPUT && p.powers != nullptr ? p.powers[t.expert] : 1.f;
             if (!await(accFull + group * 8, accPhase, failed)) break;
             accPhase ^= 1;
             fenceAfter();
@@ -308,6 +309,12 @@ __global__ void __launch_bounds__(blockThreads(SUMS), 1)
                                 v[h][i + 2] += f.z;
                                 v[h][i + 3] += f.w;
                             }
+                        }
+                    }
+                    if constexpr (MODE == INPUT) {
+                        if (p.powers != nullptr) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[h][i] *= power;
                         }
                     }
                     storeTile<T>(v[h], mine, out + firstRow * p.outStride + t.column, p.outStride, rowsLeft, c0, p.columns - t.column, p.wideStore);
@@ -1352,6 +1359,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         p.wideStore = wideOut(p.out, p.outStride, p.columns);
         p.partialBias = a.columnSums;
         p.plan = reinterpret_cast<int2*>(a.unitsBefore);
+        p.powers = a.powers;
         e = a.columnSums != nullptr ? launchShape<T, INPUT, true>(shape, mapY, mapW, p, a.numSMs, stream) : launchShape<T, INPUT>(shape, mapY, mapW, p, a.numSMs, stream);
     }
     if (e == cudaSuccess && a.gradWeight != nullptr) {

@@ -33,16 +33,86 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_quantize_kernel(const __grid_
                                     q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES, tileScales);
 }
 
+// The lowest and highest power of two of a matrix' blocks, from its scales; blocks of zeros, whose scale is the lowest, do not count.
+__global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_constant__ MxMatrix q, int2* __restrict__ found, int parts, int tiles, int chunks, int codeBytes)
+{
+    static_assert(TILE_WARPS == MX_RANGE_TILES, "");
+    __shared__ int2 ofWarp[TILE_WARPS];
+    chained();
+    const int matrix = blockIdx.x / parts, part = blockIdx.x - matrix * parts, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const unsigned char *scales = q.scales + static_cast<long long>(matrix) * tiles * MX_TILE_BYTES, *codes = q.codes + matrix * q.rows * codeBytes;
+    uint32_t low = 255, high = 0, low4 = 0xffffffffu, high4 = 0;   // the latter: of four bytes each
+    for (int tile = part * TILE_WARPS + warp; tile < tiles; tile += parts * TILE_WARPS) {
+        const uint4 u = *reinterpret_cast<const uint4*>(scales + static_cast<long long>(tile) * MX_TILE_BYTES + lane * 16);
+        const uint32_t words[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((__vcmpeq4(words[i], 0) | __vcmpeq4(words[i], 0xffffffffu)) == 0) {
+                low4 = __vminu4(low4, words[i]);
+                high4 = __vmaxu4(high4, words[i]);
+                continue;
+            }
+            const long long row = static_cast<long long>(tile / chunks) * MX_TILE + i * 32 + lane;
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t scale = words[i] >> 8 * j & 255u;
+                const int at = (tile % chunks * 4 + j) * 16;
+                if (scale == 255) continue;   // (NaN, whatever it is divided by)
+                if (scale == 0) {
+                    if (row >= q.rows || at >= codeBytes) continue;
+                    const uint4 c = *reinterpret_cast<const uint4*>(codes + row * codeBytes + at);
+                    if (((c.x | c.y | c.z | c.w) & 0x77777777u) == 0) continue;
+                }
+                low = min(low, scale);
+                high = max(high, scale);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        low = min(low, low4 >> 8 * j & 255u);
+        high = max(high, high4 >> 8 * j & 255u);
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0) ofWarp[warp] = make_int2(static_cast<int>(low), static_cast<int>(high));
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int2 all = ofWarp[0];
+        for (int w = 1; w < TILE_WARPS; ++w) all = make_int2(min(all.x, ofWarp[w].x), max(all.y, ofWarp[w].y));
+        found[blockIdx.x] = all;
+    }
+}
+// What a matrix is divided by, 2^s, as 2^-s, for a whole warp; written down (with whether its powers lie too far apart) by the block that has its first tile.
+__device__ __forceinline__ float dividedBy(const MxRanges& ranges, unsigned matrix, bool first)
+{
+    constexpr int LOWEST = 127 - 23, HIGHEST = 127 + 13;   // of a block in half: 0.5 * 2^-23 is its smallest number, 6 * 2^13 below its largest
+    const int lane = threadIdx.x & 31;
+    const int2 f = lane < ranges.parts ? ranges.found[matrix * ranges.parts + lane] : make_int2(255, 0);
+    const int low = __reduce_min_sync(0xffffffffu, f.x), high = __reduce_max_sync(0xffffffffu, f.y);
+    // (-110: the power and its inverse are normal numbers, and the lowest scale still is in reach)
+    const int s = low >= LOWEST && high <= HIGHEST ? 0 : max(high - HIGHEST, -110);
+    if (first && threadIdx.x == 0) {
+        ranges.power[matrix] = powerOf(127 + s);
+        ranges.apart[matrix] = low < LOWEST + s;
+    }
+    return powerOf(127 - s);
+}
+
 // Rows that 16-byte accesses cannot write: a warp per row, a lane per channel of a block, element by element side by side (20011 rows of 777 floats: 16 elements
 // of a row per thread 75 us, so 20).
-template <class T, int LANES, bool ALIGNED>
+template <class T, int LANES, bool ALIGNED, bool DIVIDED>
 __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __grid_constant__ MxMatrix q, T* __restrict__ y, long long stride, int tilesPerMatrix, int chunks,
-                                                                     int codeBytes)
+                                                                     int codeBytes, const __grid_constant__ MxRanges ranges)
 {
     chained();
     const unsigned tile = blockIdx.x / static_cast<unsigned>(chunks);
     const int chunk = static_cast<int>(blockIdx.x - tile * chunks);
     const RowTile t = rowTile(q, tilesPerMatrix, tile);
+    float down = 1.f;
+    if constexpr (DIVIDED) {
+        const unsigned matrix = tile / static_cast<unsigned>(tilesPerMatrix);
+        down = dividedBy(ranges, matrix, chunk == 0 && tile == matrix * tilesPerMatrix);
+    }
     const unsigned char *codes = q.codes + t.row * codeBytes, *scales = q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES;
     if constexpr (!ALIGNED) {
         constexpr int AT_ONCE = 4, BLOCKS = MX_TILE / MX_BLOCK;
@@ -64,7 +134,7 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __gri
             for (int k = 0; k < AT_ONCE; ++k) {
                 const int r = i + k * TILE_WARPS;
                 if (r >= t.rows) break;
-                const float power = powerOf(scale[k]);
+                const float power = powerOf(scale[k]) * down;
                 T* row = y + (t.row + r) * stride + c;
 #pragma unroll
                 for (int b = 0; b < BLOCKS; ++b) {
@@ -98,7 +168,7 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < W; ++j) f[j] = decodeOne(code[i] >> 4 * j);
                 }
-                const float power = powerOf(scale[i]);
+                const float power = powerOf(scale[i]) * down;
 #pragma unroll
                 for (int j = 0; j < W; ++j) out[j] = f[j] * power;
                 if ((begin + i) * STEP + first < t.rows) store<T, W>(at, pack<T, W>(out));
@@ -117,12 +187,12 @@ cudaError_t quantize(const MxMatrix& q, int type, const Rows& x, unsigned blocks
         return cudaGetLastError();
     });
 }
-template <class T>
-cudaError_t dequantize(const MxMatrix& q, int type, const Rows& y, unsigned blocks, cudaStream_t stream)
+template <class T, bool DIVIDED = false>
+cudaError_t dequantize(const MxMatrix& q, int type, const Rows& y, unsigned blocks, cudaStream_t stream, const MxRanges& ranges = {})
 {
     return byLanes(y, type, q.channels, [&](auto lanes, auto aligned) {
-        launchChained(mx_dequantize_kernel<T, decltype(aligned)::value ? decltype(lanes)::value : 8, decltype(aligned)::value>, blocks, TILE_THREADS, 0, stream, 1, q, static_cast<T*>(y.data), y.stride, mxTiles(q.rows),
-                      mxTiles(q.channels), mxCodeBytes(q.channels));
+        launchChained(mx_dequantize_kernel<T, decltype(aligned)::value ? decltype(lanes)::value : 8, decltype(aligned)::value, DIVIDED>, blocks, TILE_THREADS, 0, stream, 1, q,
+                      static_cast<T*>(y.data), y.stride, mxTiles(q.rows), mxTiles(q.channels), mxCodeBytes(q.channels), ranges);
         return cudaGetLastError();
     });
 }
@@ -142,11 +212,20 @@ cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStr
     if (blocks == 0) return cudaSuccess;
     return type == TYPE_FLOAT ? quantize<float>(q, type, x, blocks, stream) : type == TYPE_HALF ? quantize<__half>(q, type, x, blocks, stream) : quantize<__nv_bfloat16>(q, type, x, blocks, stream);
 }
-cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream)
+cudaError_t launchMxRanges(const MxMatrix& q, const MxRanges& ranges, cudaStream_t stream)
+{
+    const int chunks = mxTiles(q.channels);
+    launchChained(mx_ranges_kernel, static_cast<unsigned>(q.matrices * ranges.parts), TILE_THREADS, 0, stream, 1, q, ranges.found, ranges.parts, mxTiles(q.rows) * chunks, chunks,
+                  mxCodeBytes(q.channels));
+    return cudaGetLastError();
+}
+cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream, const MxRanges* ranges)
 {
     unsigned blocks;
     if (!blocksOf(q, blocks)) return cudaErrorInvalidConfiguration;
     if (blocks == 0) return cudaSuccess;
+    if (ranges != nullptr && type != TYPE_HALF) return cudaErrorInvalidValue;
+    if (ranges != nullptr) return dequantize<__half, true>(q, type, y, blocks, stream, *ranges);
     return type == TYPE_FLOAT ? dequantize<float>(q, type, y, blocks, stream) : type == TYPE_HALF ? dequantize<__half>(q, type, y, blocks, stream) : dequantize<__nv_bfloat16>(q, type, y, blocks, stream);
 }
 

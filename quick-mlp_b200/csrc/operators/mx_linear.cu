@@ -1,7 +1,8 @@
 // Products of feature rows with microscaled 4-bit matrices, one matrix per expert: rows [offsets[e], offsets[e + 1]) of x belong to expert e.
 //
 //   y_r = W_e q(x_r) + b_e          W_e: (channels out, channels in) in 4 bits; q: the row in 4 bits (mx.cuh)
-//   dx_r = W_e^T dy_r               (straight through q), W_e decoded to 16 bits, which is exact, and the product of expert_linear.cu
+//   dx_r = W_e^T dy_r               (straight through q), W_e decoded to 16 bits and the product of expert_linear.cu. bfloat16 holds every 4-bit number; half holds
+//                                   37 neighbouring powers of two, so that W_e goes there divided by one where it leaves half's own (see mx_apart_kernel)
 //
 // Two kernels (one for small calls, and another for a few rows; the rules stand at the end). The first quantises the rows, tile by tile of 128 rows of one expert,
 // so that a tile's scales lie as the tensor core wants them. The second is the product D (128 x BN, fp32 in tensor memory) += A B, 256 channels in a step: codes by TMA in boxes of 64 rows x 128 bytes (256 channels), 128-byte
@@ -754,6 +755,79 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) mx_bias_join_kernel(const int*
     }
 }
 
+// ---- input gradient of half rows where half does not hold a matrix -------------------------------------------------------------
+// Matrices whose powers of two reach from -23 to 13 are decoded to half as they are; others are divided by a power of two, which the product's sums are multiplied
+// with in fp32 (mx_ranges_kernel, dividedBy). What remains are matrices whose blocks lie more than 2^36 apart: their rows of dx are computed once more here,
+// dx_rc = sum over n of dy_rn (W_nc 2^E), codes decoded to fp32, sums in fp32. Few weights look like that, so this kernel is plain: a tile of 128 rows x 64 channels in
+// a block, 32 channels out at a time through shared memory. 131072 rows of half, 16 experts of 1024 -> 1024: 182 us where no matrix is apart, 815 with one of the 16, 8.6 ms with all;
+// finding it out costs every call 5 to 8 us, two launches (2.5 to 4.5 and 2).
+constexpr int APART_COLUMNS = 64, APART_STEP = 32, APART_THREADS = 256;
+__global__ void __launch_bounds__(APART_THREADS) mx_apart_kernel(const __grid_constant__ ProductArgs p, const __grid_constant__ MxMatrix w, const int* __restrict__ apart,
+                                                                 const __half* __restrict__ dy, long long stride, int codeBytes, int chunks)
+{
+    extern __shared__ int lists[];
+    __shared__ float rows[APART_STEP][BM + 1];
+    __shared__ __align__(16) float columns[APART_STEP][APART_COLUMNS];
+    chained();
+    int any = 0;
+    for (int e = threadIdx.x; e < p.experts; e += APART_THREADS) any |= apart[e];
+    if (!__syncthreads_or(any)) return;
+    int *bounds = lists, *before = lists + listStride(p.experts);
+    planExperts<FORWARD>(p, bounds, before, nullptr, APART_THREADS);
+    __syncthreads();
+    Walk<FORWARD, APART_COLUMNS, 1> walk(p, bounds, before, nullptr, 0, 1);
+    Tile t;
+    const int line = threadIdx.x / 32, lane = threadIdx.x & 31, mine = threadIdx.x / 16 * 8, column = threadIdx.x % 16 * 4;   // 8 rows x 4 channels of a thread
+    const int channelsOut = static_cast<int>(w.rows), tilesOut = (channelsOut + MX_TILE - 1) / MX_TILE;
+    while (walk.next(t)) {
+        if (t.expert < 0) break;
+        if (apart[t.expert] == 0) continue;
+        float sum[8][4] = {};
+        for (int begin = 0; begin < channelsOut; begin += APART_STEP) {
+#pragma unroll 4
+            for (int r = line; r < BM; r += APART_THREADS / 32) {
+                const bool there = r < t.end - t.begin && begin + lane < channelsOut;
+                rows[lane][r] = there ? __half2float(dy[(static_cast<long long>(t.begin) + r) * stride + begin + lane]) : 0.f;
+            }
+            {   // 8 channels of a channel out
+                const int k = threadIdx.x / 8, n = begin + k, c = t.column + threadIdx.x % 8 * 8;
+                float f[8] = {};
+                if (n < channelsOut && c / 2 < codeBytes) {
+                    const long long matrix = t.expert;
+                    const unsigned char scale = w.scales[((matrix * tilesOut + n / MX_TILE) * chunks + c / MX_TILE) * MX_TILE_BYTES + n % 32 * 16 + n % MX_TILE / 32 * 4 + c % MX_TILE / MX_BLOCK];
+                    decodeEight(*reinterpret_cast<const uint32_t*>(w.codes + (matrix * channelsOut + n) * codeBytes + c / 2), f);
+                    const float power = powerOf(scale);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] *= power;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) columns[k][threadIdx.x % 8 * 8 + i] = f[i];
+            }
+            __syncthreads();
+#pragma unroll 4
+            for (int k = 0; k < APART_STEP; ++k) {
+                const float4 b = *reinterpret_cast<const float4*>(&columns[k][column]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float a = rows[k][mine + i];
+                    sum[i][0] += a * b.x;
+                    sum[i][1] += a * b.y;
+                    sum[i][2] += a * b.z;
+                    sum[i][3] += a * b.w;
+                }
+            }
+            __syncthreads();
+        }
+        __half* out = static_cast<__half*>(p.out);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (mine + i < t.end - t.begin && t.column + column + j < p.columns)
+                    out[(static_cast<long long>(t.begin) + mine + i) * p.outStride + t.column + column + j] = __float2half_rn(sum[i][j]);
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------
 // an encoding, once more with a context: in a thread's first call the driver wants one, which the runtime binds
 template <class F>
@@ -949,17 +1023,21 @@ cudaError_t forward(const MxLinearArgs& a, cudaStream_t stream)
     return boxBytes == 32 ? go(std::integral_constant<int, 32>()) : go(std::integral_constant<int, 128>());
 }
 
-// scratch of the adjoint: [units before the experts | the bias gradient's sums | the matrices in 16 bits | scratch of the input gradient's product], or, where the bias
-// gradient is all that is wanted, [units | sums | list of its pieces]
+// scratch of the adjoint: [units before the experts | the bias gradient's sums | half: how far the matrices' powers of two reach | the matrices in 16 bits | scratch of
+// the input gradient's product], or, where the bias gradient is all that is wanted, [units | sums | list of its pieces]
 struct MxAdjointScratch {
-    size_t partial, matrices, product, list, bytes;
+    size_t partial, found, power, apart, matrices, product, list, bytes;
     int pieces;
     explicit MxAdjointScratch(const MxLinearArgs& a)
     {
         const ExpertArgs r = inputGradient(a);
         pieces = static_cast<int>(a.rows / BIAS_ROWS + std::min<long long>(a.rows, a.weight.matrices));
         partial = align256((static_cast<size_t>(a.weight.matrices) + 1) * sizeof(int));
-        matrices = list = partial + align256(static_cast<size_t>(a.gradX.data != nullptr ? expertSums(r) : pieces) * static_cast<size_t>(a.weight.rows) * sizeof(float));
+        found = list = partial + align256(static_cast<size_t>(a.gradX.data != nullptr ? expertSums(r) : pieces) * static_cast<size_t>(a.weight.rows) * sizeof(float));
+        const size_t ranges = a.type == TYPE_HALF ? static_cast<size_t>(a.weight.matrices) : 0;
+        power = found + align256(ranges * mxRangeParts(a.weight) * sizeof(int2));
+        apart = power + align256(ranges * sizeof(float));
+        matrices = apart + align256(ranges * sizeof(int));
         product = matrices + (a.gradX.data == nullptr ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * a.weight.channels * 2));
         bytes = a.gradX.data != nullptr ? product + expertBytes(r, true) : list + align256(static_cast<size_t>(pieces) * sizeof(int2));
     }
@@ -980,6 +1058,21 @@ struct MxAdjointScratch {
         return r;
     }
 };
+cudaError_t launchApart(const MxLinearArgs& a, const MxRanges& ranges, cudaStream_t stream)
+{
+    ProductArgs p{};
+    p.rows = a.rows;
+    p.experts = static_cast<int>(a.weight.matrices);
+    p.columns = a.weight.channels;
+    p.columnTiles = (p.columns + APART_COLUMNS - 1) / APART_COLUMNS;
+    p.tileRows = BM;
+    p.offsets = a.offsets;
+    p.out = a.gradX.data;
+    p.outStride = a.gradX.stride;
+    launchChained(mx_apart_kernel, 2 * a.numSMs, APART_THREADS, 2 * listStride(p.experts) * sizeof(int), stream, 1, p, a.weight, ranges.apart, static_cast<const __half*>(a.gradY.data),
+                  a.gradY.stride, mxCodeBytes(p.columns), mxTiles(p.columns));
+    return cudaGetLastError();
+}
 template <class T>
 cudaError_t joinBias(const MxLinearArgs& a, const MxAdjointScratch& s, int perUnit, cudaStream_t stream)
 {
@@ -1032,7 +1125,10 @@ cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream)
         return a.type == TYPE_HALF ? biasGradient<__half>(a, s, stream) : biasGradient<__nv_bfloat16>(a, s, stream);
     }
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
-    cudaError_t e = launchMxDequantize(a.weight, a.type, {base + s.matrices, a.weight.channels}, stream);
+    const bool half = a.type == TYPE_HALF;
+    const MxRanges ranges = {mxRangeParts(a.weight), reinterpret_cast<int2*>(base + s.found), reinterpret_cast<float*>(base + s.power), reinterpret_cast<int*>(base + s.apart)};
+    cudaError_t e = half ? launchMxRanges(a.weight, ranges, stream) : cudaSuccess;
+    if (e == cudaSuccess) e = launchMxDequantize(a.weight, a.type, {base + s.matrices, a.weight.channels}, stream, half ? &ranges : nullptr);
     if (e != cudaSuccess) return e;
     // the product's tiles of dy lie in shared memory: their columns are added up there
     ExpertArgs r = MxAdjointScratch::inputGradient(a);
@@ -1042,7 +1138,9 @@ cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream)
         r.columnSums = reinterpret_cast<float*>(base + s.partial);
         r.unitsBefore = reinterpret_cast<int*>(base);
     }
+    if (half) r.powers = ranges.power;
     e = launchExpertAdjoint(r, stream);
+    if (e == cudaSuccess && half) e = launchApart(a, ranges, stream);
     if (e != cudaSuccess || a.gradBias == nullptr) return e;
     return a.type == TYPE_HALF ? joinBias<__half>(a, s, expertSumsPerUnit(r), stream) : joinBias<__nv_bfloat16>(a, s, expertSumsPerUnit(r), stream);
 }

@@ -109,6 +109,7 @@ struct ExpertArgs {
     // expert, one expert's behind another's; units of the experts in front of each (experts + 1)
     float* columnSums;
     int* unitsBefore;
+    const float* powers;   // of each expert, what its rows of an input gradient alone are multiplied with before they are rounded (null: one)
 };
 int expertSumsPerUnit(const ExpertArgs& a);
 long long expertSums(const ExpertArgs& a);   // an upper bound
@@ -142,7 +143,24 @@ struct MxMatrix {
     unsigned char *codes, *scales;
 };
 cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStream_t stream);
-cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream);
+// How far the powers of two of each matrix reach. Half holds the numbers of 37 neighbouring powers (of two, those of its elements from 0.5 to 6) exactly, its
+// own range being -23 to 13: a matrix that leaves it is divided by a power of two, `power`, so that its largest numbers come to the upper end; `apart`: its powers
+// lie farther apart than half holds. found: the lowest and highest power (+ 127) that a `parts`-th of a matrix has; (255, 0) for none.
+struct MxRanges {
+    int parts;
+    int2* found;     // matrices x parts
+    float* power;    // matrices; written with the decoded matrices, as
+    int* apart;      // matrices
+};
+constexpr int MX_RANGE_PARTS = 32, MX_RANGE_TILES = 8;   // most parts of a matrix; tiles of scales that a block takes at once
+inline int mxRangeParts(const MxMatrix& q)
+{
+    const long long n = static_cast<long long>(mxTiles(q.rows)) * mxTiles(q.channels) / MX_RANGE_TILES;
+    return n < 1 ? 1 : n < MX_RANGE_PARTS ? static_cast<int>(n) : MX_RANGE_PARTS;
+}
+cudaError_t launchMxRanges(const MxMatrix& q, const MxRanges& ranges, cudaStream_t stream);
+// `ranges`: of half y, whose matrices are divided by their powers; null: as they are
+cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream, const MxRanges* ranges = nullptr);
 
 // products of rows with such matrices (weight.matrices experts, weight.rows channels out)
 struct MxLinearArgs {

@@ -162,6 +162,7 @@ struct ProductArgs {
     void* out;
     long long outStride;          // elements between rows of D in memory
     const void* bias;             // forward: (experts, columns) or null
+    const float* powers;          // input: what the sums of an expert's rows are multiplied with, or null
     int2* plan;                   // weights: first slot and items of an expert, written for the join; null where no expert can have two
     float* partial;               // weights: slots x tiles x tileRows x BN sums; the items of experts with more than one have a slot each
     int* status;
