@@ -33,13 +33,22 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_quantize_kernel(const __grid_
                                     q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES, tileScales);
 }
 
+// An expert whose offsets, taken as they are used (within [0, rows], their running maximum), do not rise has no rows. (They rise only where they rise here.)
+__device__ __forceinline__ bool hasRows(const MxWanted& w, unsigned matrix)
+{
+    if (w.offsets == nullptr) return true;
+    const long long begin = max(w.offsets[matrix], 0), end = w.offsets[matrix + 1];
+    return min(end, w.rows) > min(begin, w.rows);
+}
+
 // The lowest and highest power of two of a matrix' blocks, from its scales; blocks of zeros, whose scale is the lowest, do not count.
-__global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_constant__ MxMatrix q, int2* __restrict__ found, int parts, int tiles, int chunks, int codeBytes)
+__global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_constant__ MxMatrix q, const __grid_constant__ MxWanted wanted, int2* __restrict__ found, int parts, int tiles, int chunks, int codeBytes)
 {
     static_assert(TILE_WARPS == MX_RANGE_TILES, "");
     __shared__ int2 ofWarp[TILE_WARPS];
     chained();
     const int matrix = blockIdx.x / parts, part = blockIdx.x - matrix * parts, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (!hasRows(wanted, matrix)) return;
     const unsigned char *scales = q.scales + static_cast<long long>(matrix) * tiles * MX_TILE_BYTES, *codes = q.codes + matrix * q.rows * codeBytes;
     uint32_t low = 255, high = 0, low4 = 0xffffffffu, high4 = 0;   // the latter: of four bytes each
     for (int tile = part * TILE_WARPS + warp; tile < tiles; tile += parts * TILE_WARPS) {
@@ -102,17 +111,23 @@ __device__ __forceinline__ float dividedBy(const MxRanges& ranges, unsigned matr
 // of a row per thread 75 us, so 20).
 template <class T, int LANES, bool ALIGNED, bool DIVIDED>
 __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __grid_constant__ MxMatrix q, T* __restrict__ y, long long stride, int tilesPerMatrix, int chunks,
-                                                                     int codeBytes, const __grid_constant__ MxRanges ranges)
+                                                                     int codeBytes, const __grid_constant__ MxWanted wanted, const __grid_constant__ MxRanges ranges)
 {
     chained();
     const unsigned tile = blockIdx.x / static_cast<unsigned>(chunks);
     const int chunk = static_cast<int>(blockIdx.x - tile * chunks);
     const RowTile t = rowTile(q, tilesPerMatrix, tile);
-    float down = 1.f;
-    if constexpr (DIVIDED) {
-        const unsigned matrix = tile / static_cast<unsigned>(tilesPerMatrix);
-        down = dividedBy(ranges, matrix, chunk == 0 && tile == matrix * tilesPerMatrix);
+    const unsigned matrix = tile / static_cast<unsigned>(tilesPerMatrix);
+    const bool first = chunk == 0 && tile == matrix * tilesPerMatrix;
+    if (!hasRows(wanted, matrix)) {
+        if (DIVIDED && first && threadIdx.x == 0) {
+            ranges.power[matrix] = 1.f;
+            ranges.apart[matrix] = 0;
+        }
+        return;
     }
+    float down = 1.f;
+    if constexpr (DIVIDED) down = dividedBy(ranges, matrix, first);
     const unsigned char *codes = q.codes + t.row * codeBytes, *scales = q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES;
     if constexpr (!ALIGNED) {
         constexpr int AT_ONCE = 4, BLOCKS = MX_TILE / MX_BLOCK;
@@ -188,11 +203,11 @@ cudaError_t quantize(const MxMatrix& q, int type, const Rows& x, unsigned blocks
     });
 }
 template <class T, bool DIVIDED = false>
-cudaError_t dequantize(const MxMatrix& q, int type, const Rows& y, unsigned blocks, cudaStream_t stream, const MxRanges& ranges = {})
+cudaError_t dequantize(const MxMatrix& q, int type, const Rows& y, unsigned blocks, cudaStream_t stream, const MxWanted& wanted, const MxRanges& ranges = {})
 {
     return byLanes(y, type, q.channels, [&](auto lanes, auto aligned) {
         launchChained(mx_dequantize_kernel<T, decltype(aligned)::value ? decltype(lanes)::value : 8, decltype(aligned)::value, DIVIDED>, blocks, TILE_THREADS, 0, stream, 1, q,
-                      static_cast<T*>(y.data), y.stride, mxTiles(q.rows), mxTiles(q.channels), mxCodeBytes(q.channels), ranges);
+                      static_cast<T*>(y.data), y.stride, mxTiles(q.rows), mxTiles(q.channels), mxCodeBytes(q.channels), wanted, ranges);
         return cudaGetLastError();
     });
 }
@@ -212,21 +227,21 @@ cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStr
     if (blocks == 0) return cudaSuccess;
     return type == TYPE_FLOAT ? quantize<float>(q, type, x, blocks, stream) : type == TYPE_HALF ? quantize<__half>(q, type, x, blocks, stream) : quantize<__nv_bfloat16>(q, type, x, blocks, stream);
 }
-cudaError_t launchMxRanges(const MxMatrix& q, const MxRanges& ranges, cudaStream_t stream)
+cudaError_t launchMxRanges(const MxMatrix& q, const MxWanted& wanted, const MxRanges& ranges, cudaStream_t stream)
 {
     const int chunks = mxTiles(q.channels);
-    launchChained(mx_ranges_kernel, static_cast<unsigned>(q.matrices * ranges.parts), TILE_THREADS, 0, stream, 1, q, ranges.found, ranges.parts, mxTiles(q.rows) * chunks, chunks,
+    launchChained(mx_ranges_kernel, static_cast<unsigned>(q.matrices * ranges.parts), TILE_THREADS, 0, stream, 1, q, wanted, ranges.found, ranges.parts, mxTiles(q.rows) * chunks, chunks,
                   mxCodeBytes(q.channels));
     return cudaGetLastError();
 }
-cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream, const MxRanges* ranges)
+cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream, const MxWanted& wanted, const MxRanges* ranges)
 {
     unsigned blocks;
     if (!blocksOf(q, blocks)) return cudaErrorInvalidConfiguration;
     if (blocks == 0) return cudaSuccess;
     if (ranges != nullptr && type != TYPE_HALF) return cudaErrorInvalidValue;
-    if (ranges != nullptr) return dequantize<__half, true>(q, type, y, blocks, stream, *ranges);
-    return type == TYPE_FLOAT ? dequantize<float>(q, type, y, blocks, stream) : type == TYPE_HALF ? dequantize<__half>(q, type, y, blocks, stream) : dequantize<__nv_bfloat16>(q, type, y, blocks, stream);
+    if (ranges != nullptr) return dequantize<__half, true>(q, type, y, blocks, stream, wanted, *ranges);
+    return type == TYPE_FLOAT ? dequantize<float>(q, type, y, blocks, stream, wanted) : type == TYPE_HALF ? dequantize<__half>(q, type, y, blocks, stream, wanted) : dequantize<__nv_bfloat16>(q, type, y, blocks, stream, wanted);
 }
 
 } // namespace kernel

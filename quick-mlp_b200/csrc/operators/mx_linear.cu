@@ -1127,8 +1127,9 @@ cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream)
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
     const bool half = a.type == TYPE_HALF;
     const MxRanges ranges = {mxRangeParts(a.weight), reinterpret_cast<int2*>(base + s.found), reinterpret_cast<float*>(base + s.power), reinterpret_cast<int*>(base + s.apart)};
-    cudaError_t e = half ? launchMxRanges(a.weight, ranges, stream) : cudaSuccess;
-    if (e == cudaSuccess) e = launchMxDequantize(a.weight, a.type, {base + s.matrices, a.weight.channels}, stream, half ? &ranges : nullptr);
+    const MxWanted wanted = {a.offsets, a.rows};
+    cudaError_t e = half ? launchMxRanges(a.weight, wanted, ranges, stream) : cudaSuccess;
+    if (e == cudaSuccess) e = launchMxDequantize(a.weight, a.type, {base + s.matrices, a.weight.channels}, stream, wanted, half ? &ranges : nullptr);
     if (e != cudaSuccess) return e;
     // the product's tiles of dy lie in shared memory: their columns are added up there
     ExpertArgs r = MxAdjointScratch::inputGradient(a);

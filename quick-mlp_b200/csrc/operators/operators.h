@@ -158,9 +158,15 @@ inline int mxRangeParts(const MxMatrix& q)
     const long long n = static_cast<long long>(mxTiles(q.rows)) * mxTiles(q.channels) / MX_RANGE_TILES;
     return n < 1 ? 1 : n < MX_RANGE_PARTS ? static_cast<int>(n) : MX_RANGE_PARTS;
 }
-cudaError_t launchMxRanges(const MxMatrix& q, const MxRanges& ranges, cudaStream_t stream);
+// Of matrices of experts, those that are wanted: of experts that have rows, or all (offsets null). (Gradient of 2 rows of 64 experts of 1024 -> 2048 bfloat16: all
+// matrices decoded 75 us, those of the two 27 us.)
+struct MxWanted {
+    const int* offsets;   // matrices + 1
+    long long rows;
+};
+cudaError_t launchMxRanges(const MxMatrix& q, const MxWanted& wanted, const MxRanges& ranges, cudaStream_t stream);
 // `ranges`: of half y, whose matrices are divided by their powers; null: as they are
-cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream, const MxRanges* ranges = nullptr);
+cudaError_t launchMxDequantize(const MxMatrix& q, int type, const Rows& y, cudaStream_t stream, const MxWanted& wanted = {}, const MxRanges* ranges = nullptr);
 
 // products of rows with such matrices (weight.matrices experts, weight.rows channels out)
 struct MxLinearArgs {

@@ -158,3 +158,33 @@ def test_gradient_scales_captured(qmlp):
         scales.copy_(sets[i].scales)
         graph.replay()
         assert torch.equal(dx, want[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["half", "bfloat16"])
+@pytest.mark.parametrize("n_in", [256, 130])
+def test_gradient_leaves_matrices_without_rows(qmlp, dtype, n_in):
+    """matrices of experts without rows are not decoded: most of the scratch memory is as it was; offsets out of order count as they are used"""
+    import ctypes as C
+    from qmlp import _capi
+    lib, e, n_out, rows = _capi.lib(), 64, 200, 30
+    w = rand(50, (e, n_out, n_in))
+    q, grad = qmlp.mx_quantize(w), rand(51, (rows, n_out), dtype)
+    m = _capi.Mx(matrices=e, rows=n_out, channels=n_in, codes=q.codes.data_ptr(), scales=q.scales.data_ptr())
+
+    def view(t):
+        v = _capi.Tensor(data=t.data_ptr(), precision=_capi.QMLP_HALF if t.dtype == torch.float16 else _capi.QMLP_BFLOAT16, ndim=2)
+        v.sizes[0], v.sizes[1], v.strides[0], v.strides[1] = *t.shape, *t.stride()
+        return C.byref(v)
+    size = C.c_size_t()
+    assert lib.qmlp_mx_linear_adjoint_memory(view(grad), C.byref(m), 1, C.byref(size)) == 0
+    for used in ([0] * 6 + [10] * 40 + [30] * 19, [5] * 3 + [12] * 20 + [-1] * 20 + [7] * 20 + [99] * 2, [0] * 65, [-5] * 64 + [30]):
+        offsets = torch.tensor(used, dtype=torch.int32, device="cuda")
+        scratch = torch.full((size.value,), 0xA5, dtype=torch.uint8, device="cuda")
+        dx = torch.full((rows, n_in), 7.0, dtype=dtype, device="cuda")
+        assert lib.qmlp_mx_linear_adjoint(view(grad), C.byref(m), C.c_void_p(offsets.data_ptr()), view(dx), None, _capi.current_stream(), scratch.data_ptr(), size.value) == 0
+        want, slack = mx.mx_linear(torch.zeros((rows, n_in), dtype=dtype, device="cuda"), mx.nearest(w), offsets, None, grad)[1]
+        ref.check(dx, want, slack, "input gradient")
+        rising = sum(min(max(b, 0), rows) > min(max(a, 0), rows) for a, b in zip(used, used[1:]))
+        # what is written: their matrices, once more with padded rows where the channels ask for it, and what goes with rows and experts alone
+        bound = rising * n_out * 2 * (n_in + (n_in + 7) // 8 * 8 if n_in % 8 else n_in) + rows * (n_out + 8) * 2 + e * 32 + 4096
+        assert int((scratch != 0xA5).sum()) <= bound < size.value // 4
