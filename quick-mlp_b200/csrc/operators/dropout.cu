@@ -6,6 +6,7 @@
 //
 // A thread takes groups of 8 elements, one generator call each. Bound by memory, with a third of the machine's instructions left: 32768 rows of 4096 bfloat16 forward with a
 // residual and the gradient 233 us (5.8 TB/s); 1000003 rows of 64 half 41 us either way (6.2 TB/s; 49 us with loads that depend on a condition and keys added up).
+// Rows that are neither dense nor apart by 16 bytes go element by element, at a quarter of the rate: 32768 rows of 4095 half, 4096 apart, 344 us, dense 86.
 #include "common.cuh"
 
 #include <algorithm>

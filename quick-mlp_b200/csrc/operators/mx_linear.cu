@@ -883,6 +883,8 @@ struct Shape {
     bool whole;   // the product's kernel quantises the rows
 };
 long long rowTiles(const MxLinearArgs& a, int ctas);
+// Pairs of blocks from 512 rows an expert on. us for the call, in pairs / single blocks of 128 columns: 16 experts of 1024 -> 1024, 256 rows each 23.6 / 21.5, 512 rows 25.6 / 25.6, 768 rows
+// 29.7 / 31.7, 2048 rows 46 / 52; one of 4096 -> 4096, 512 rows 21.5 / 19.5, 768 rows 21.5 / 25.6; 64 of 512 -> 512, 256 rows 25.6 / 23.6, 512 rows 31.7 / 31.7, 2048 rows 71 / 73.
 Shape shapeOf(const MxLinearArgs& a)
 {
     const int columns = static_cast<int>(a.weight.rows);
