@@ -41,17 +41,16 @@ __device__ __forceinline__ bool hasRows(const MxWanted& w, unsigned matrix)
     return min(end, w.rows) > min(begin, w.rows);
 }
 
-// The lowest and highest power of two of a matrix' blocks, from its scales; blocks of zeros, whose scale is the lowest, do not count.
-__global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_constant__ MxMatrix q, const __grid_constant__ MxWanted wanted, int2* __restrict__ found, int parts, int tiles, int chunks, int codeBytes)
+// The lowest and highest power of two (+ 127) of blocks of a matrix, from their scales: those of the tiles first, first + step, ..., a warp a tile. For a whole block.
+// Blocks of zeros, whose scale is the lowest, do not count.
+__device__ __forceinline__ int2 rangeOf(const MxMatrix& q, int matrix, int first, int step, int tiles, int chunks, int codeBytes)
 {
     static_assert(TILE_WARPS == MX_RANGE_TILES, "");
     __shared__ int2 ofWarp[TILE_WARPS];
-    chained();
-    const int matrix = blockIdx.x / parts, part = blockIdx.x - matrix * parts, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    if (!hasRows(wanted, matrix)) return;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const unsigned char *scales = q.scales + static_cast<long long>(matrix) * tiles * MX_TILE_BYTES, *codes = q.codes + matrix * q.rows * codeBytes;
     uint32_t low = 255, high = 0, low4 = 0xffffffffu, high4 = 0;   // the latter: of four bytes each
-    for (int tile = part * TILE_WARPS + warp; tile < tiles; tile += parts * TILE_WARPS) {
+    for (int tile = first + warp; tile < tiles; tile += step) {
         const uint4 u = *reinterpret_cast<const uint4*>(scales + static_cast<long long>(tile) * MX_TILE_BYTES + lane * 16);
         const uint32_t words[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -85,19 +84,35 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_co
     high = __reduce_max_sync(0xffffffffu, high);
     if (lane == 0) ofWarp[warp] = make_int2(static_cast<int>(low), static_cast<int>(high));
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int2 all = ofWarp[0];
-        for (int w = 1; w < TILE_WARPS; ++w) all = make_int2(min(all.x, ofWarp[w].x), max(all.y, ofWarp[w].y));
-        found[blockIdx.x] = all;
-    }
+    int2 all = ofWarp[0];
+#pragma unroll
+    for (int w = 1; w < TILE_WARPS; ++w) all = make_int2(min(all.x, ofWarp[w].x), max(all.y, ofWarp[w].y));
+    return all;
 }
-// What a matrix is divided by, 2^s, as 2^-s, for a whole warp; written down (with whether its powers lie too far apart) by the block that has its first tile.
-__device__ __forceinline__ float dividedBy(const MxRanges& ranges, unsigned matrix, bool first)
+__global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_constant__ MxMatrix q, const __grid_constant__ MxWanted wanted, int2* __restrict__ found, int parts, int tiles,
+                                                                 int chunks, int codeBytes)
+{
+    chained();
+    const int matrix = blockIdx.x / parts, part = blockIdx.x - matrix * parts;
+    if (!hasRows(wanted, matrix)) return;
+    const int2 all = rangeOf(q, matrix, part * TILE_WARPS, parts * TILE_WARPS, tiles, chunks, codeBytes);
+    if (threadIdx.x == 0) found[blockIdx.x] = all;
+}
+// What a matrix is divided by, 2^s, as 2^-s, for a whole block; written down (with whether its powers lie too far apart) by the block that has its first tile.
+__device__ __forceinline__ float dividedBy(const MxMatrix& q, const MxRanges& ranges, unsigned matrix, bool first, int tiles, int chunks, int codeBytes)
 {
     constexpr int LOWEST = 127 - 23, HIGHEST = 127 + 13;   // of a block in half: 0.5 * 2^-23 is its smallest number, 6 * 2^13 below its largest
-    const int lane = threadIdx.x & 31;
-    const int2 f = lane < ranges.parts ? ranges.found[matrix * ranges.parts + lane] : make_int2(255, 0);
-    const int low = __reduce_min_sync(0xffffffffu, f.x), high = __reduce_max_sync(0xffffffffu, f.y);
+    int low, high;
+    if (ranges.parts == 0) {
+        const int2 all = rangeOf(q, static_cast<int>(matrix), 0, TILE_WARPS, tiles, chunks, codeBytes);
+        low = all.x;
+        high = all.y;
+    } else {
+        const int lane = threadIdx.x & 31;
+        const int2 f = lane < ranges.parts ? ranges.found[matrix * ranges.parts + lane] : make_int2(255, 0);
+        low = __reduce_min_sync(0xffffffffu, f.x);
+        high = __reduce_max_sync(0xffffffffu, f.y);
+    }
     // (-110: the power and its inverse are normal numbers, and the lowest scale still is in reach)
     const int s = low >= LOWEST && high <= HIGHEST ? 0 : max(high - HIGHEST, -110);
     if (first && threadIdx.x == 0) {
@@ -127,7 +142,7 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_dequantize_kernel(const __gri
         return;
     }
     float down = 1.f;
-    if constexpr (DIVIDED) down = dividedBy(ranges, matrix, first);
+    if constexpr (DIVIDED) down = dividedBy(q, ranges, matrix, first, tilesPerMatrix * chunks, chunks, codeBytes);
     const unsigned char *codes = q.codes + t.row * codeBytes, *scales = q.scales + static_cast<long long>(blockIdx.x) * MX_TILE_BYTES;
     if constexpr (!ALIGNED) {
         constexpr int AT_ONCE = 4, BLOCKS = MX_TILE / MX_BLOCK;
@@ -229,6 +244,7 @@ cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStr
 }
 cudaError_t launchMxRanges(const MxMatrix& q, const MxWanted& wanted, const MxRanges& ranges, cudaStream_t stream)
 {
+    if (ranges.parts == 0) return cudaSuccess;
     const int chunks = mxTiles(q.channels);
     launchChained(mx_ranges_kernel, static_cast<unsigned>(q.matrices * ranges.parts), TILE_THREADS, 0, stream, 1, q, wanted, ranges.found, ranges.parts, mxTiles(q.rows) * chunks, chunks,
                   mxCodeBytes(q.channels));
