@@ -1150,6 +1150,8 @@ int weightChunk(const ExpertArgs& a, int tiles, int tileElements, int blocks)
     return static_cast<int>(std::min<double>(std::max<double>(std::ceil(rows / BK) * BK, 512), 1 << 16));
 }
 
+long long weightStride(const ExpertArgs& a) { return a.weightStride != 0 ? a.weightStride : a.channelsIn; }
+
 // scratch: [x | weight | dy in a form the TMA reads, where needed | partial sums of the weight and bias gradients | their plan]
 struct Scratch {
     size_t x, weight, gradY, partial, partialBias, plan, bytes;
@@ -1168,7 +1170,7 @@ struct Scratch {
         };
         const bool weights = adjoint && a.gradWeight != nullptr;
         x = take((forward || weights) && !direct(a.x.data, a.x.stride, a.channelsIn), rows * pad8(a.channelsIn) * 2);
-        weight = take((forward || a.gradX.data != nullptr) && !direct(a.weight, a.channelsIn, a.channelsIn), matrices * pad8(a.channelsIn) * 2);
+        weight = take((forward || a.gradX.data != nullptr) && !direct(a.weight, weightStride(a), a.channelsIn), matrices * pad8(a.channelsIn) * 2);
         gradY = take(adjoint && !direct(a.gradY.data, a.gradY.stride, a.channelsOut), rows * pad8(a.channelsOut) * 2);
         shape = weightShape(a);
         tileRows = BM * shape.ctas;
@@ -1321,7 +1323,7 @@ cudaError_t adjoint(const ExpertArgs& a, cudaStream_t stream)
         return e;
     }
     const void *x = a.x.data, *w = a.weight, *dy = a.gradY.data;
-    long long xStride = a.x.stride, wStride = a.channelsIn, dyStride = a.gradY.stride;
+    long long xStride = a.x.stride, wStride = weightStride(a), dyStride = a.gradY.stride;
     CUtensorMap mapX, mapW, mapY;
     if (e == cudaSuccess) e = readable<T>(dy, dyStride, a.rows, a.channelsOut, base + s.gradY, stream);
     if (e == cudaSuccess) e = encodeMap(mapY, a.type, dy, 0, a.rows, a.channelsOut, dyStride);

@@ -220,7 +220,7 @@ cudaError_t quantize(const MxMatrix& q, int type, const Rows& x, unsigned blocks
 template <class T, bool DIVIDED = false>
 cudaError_t dequantize(const MxMatrix& q, int type, const Rows& y, unsigned blocks, cudaStream_t stream, const MxWanted& wanted, const MxRanges& ranges = {})
 {
-    return byLanes(y, type, q.channels, [&](auto lanes, auto aligned) {
+    return byLanes(y, type, wanted.padded ? (q.channels + 7) / 8 * 8 : q.channels, [&](auto lanes, auto aligned) {
         launchChained(mx_dequantize_kernel<T, decltype(aligned)::value ? decltype(lanes)::value : 8, decltype(aligned)::value, DIVIDED>, blocks, TILE_THREADS, 0, stream, 1, q,
                       static_cast<T*>(y.data), y.stride, mxTiles(q.rows), mxTiles(q.channels), mxCodeBytes(q.channels), wanted, ranges);
         return cudaGetLastError();

@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) mx_bias_join_kernel(const int*
 // with in fp32 (mx_ranges_kernel, dividedBy). What remains are matrices whose blocks lie more than 2^36 apart: their rows of dx are computed once more here,
 // dx_rc = sum over n of dy_rn (W_nc 2^E), codes decoded to fp32, sums in fp32. Few weights look like that, so this kernel is plain: a tile of 128 rows x 64 channels in
 // a block, 32 channels out at a time through shared memory. 131072 rows of half, 16 experts of 1024 -> 1024: 182 us where no matrix is apart, 815 with one of the 16, 8.6 ms with all;
-// finding it out costs every call 5 to 8 us, two launches (2.5 to 4.5 and 2).
+// finding it out costs every call of half rows 3 to 6 us (2.5 to 5 in front, less for small matrices, and 2 for this kernel's launch).
 constexpr int APART_COLUMNS = 64, APART_STEP = 32, APART_THREADS = 256;
 __global__ void __launch_bounds__(APART_THREADS) mx_apart_kernel(const __grid_constant__ ProductArgs p, const __grid_constant__ MxMatrix w, const int* __restrict__ apart,
                                                                  const __half* __restrict__ dy, long long stride, int codeBytes, int chunks)
@@ -1040,7 +1040,7 @@ struct MxAdjointScratch {
         power = found + align256(ranges * mxRangeParts(a.weight) * sizeof(int2));
         apart = power + align256(ranges * sizeof(float));
         matrices = apart + align256(ranges * sizeof(int));
-        product = matrices + (a.gradX.data == nullptr ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * a.weight.channels * 2));
+        product = matrices + (a.gradX.data == nullptr ? 0 : align256(static_cast<size_t>(a.weight.matrices) * a.weight.rows * r.weightStride * 2));
         bytes = a.gradX.data != nullptr ? product + expertBytes(r, true) : list + align256(static_cast<size_t>(pieces) * sizeof(int2));
     }
     // the product with the matrices in 16 bits
@@ -1057,6 +1057,7 @@ struct MxAdjointScratch {
         r.gradY = a.gradY;
         r.gradX = a.gradX;
         r.status = a.status;
+        r.weightStride = (r.channelsIn + 7) / 8 * 8;   // (rows that the product's TMA reads as they are: 32 matrices of 300 x 777 decoded in 7 us, else 14 and 9 more for a copy)
         return r;
     }
 };
@@ -1129,12 +1130,12 @@ cudaError_t launchMxLinearAdjoint(const MxLinearArgs& a, cudaStream_t stream)
     unsigned char* base = static_cast<unsigned char*>(a.scratch);
     const bool half = a.type == TYPE_HALF;
     const MxRanges ranges = {mxRangeParts(a.weight), reinterpret_cast<int2*>(base + s.found), reinterpret_cast<float*>(base + s.power), reinterpret_cast<int*>(base + s.apart)};
-    const MxWanted wanted = {a.offsets, a.rows};
+    ExpertArgs r = MxAdjointScratch::inputGradient(a);
+    const MxWanted wanted = {a.offsets, a.rows, true};
     cudaError_t e = half ? launchMxRanges(a.weight, wanted, ranges, stream) : cudaSuccess;
-    if (e == cudaSuccess) e = launchMxDequantize(a.weight, a.type, {base + s.matrices, a.weight.channels}, stream, wanted, half ? &ranges : nullptr);
+    if (e == cudaSuccess) e = launchMxDequantize(a.weight, a.type, {base + s.matrices, r.weightStride}, stream, wanted, half ? &ranges : nullptr);
     if (e != cudaSuccess) return e;
     // the product's tiles of dy lie in shared memory: their columns are added up there
-    ExpertArgs r = MxAdjointScratch::inputGradient(a);
     r.weight = base + s.matrices;
     r.scratch = base + s.product;
     if (a.gradBias != nullptr) {

@@ -110,6 +110,7 @@ struct ExpertArgs {
     float* columnSums;
     int* unitsBefore;
     const float* powers;   // of each expert, what its rows of an input gradient alone are multiplied with before they are rounded (null: one)
+    int weightStride;      // adjoint: elements between rows of weight (0: channelsIn)
 };
 int expertSumsPerUnit(const ExpertArgs& a);
 long long expertSums(const ExpertArgs& a);   // an upper bound
@@ -165,6 +166,7 @@ inline int mxRangeParts(const MxMatrix& q)
 struct MxWanted {
     const int* offsets;   // matrices + 1
     long long rows;
+    bool padded;          // of 16-bit y: what lies behind a row up to a multiple of 8 channels may be written (zeros)
 };
 cudaError_t launchMxRanges(const MxMatrix& q, const MxWanted& wanted, const MxRanges& ranges, cudaStream_t stream);
 // `ranges`: of half y, whose matrices are divided by their powers; null: as they are

@@ -188,3 +188,22 @@ def test_gradient_leaves_matrices_without_rows(qmlp, dtype, n_in):
         # what is written: their matrices, once more with padded rows where the channels ask for it, and what goes with rows and experts alone
         bound = rising * n_out * 2 * (n_in + (n_in + 7) // 8 * 8 if n_in % 8 else n_in) + rows * (n_out + 8) * 2 + e * 32 + 4096
         assert int((scratch != 0xA5).sum()) <= bound < size.value // 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["half", "bfloat16"])
+def test_gradient_of_odd_widths(qmlp, dtype):
+    """matrices of any width are decoded once, to rows of a multiple of 8 channels: no more memory than for that multiple; what lies behind a row counts for nothing"""
+    import ctypes as C
+    from qmlp import _capi
+    lib, e, n_out, rows = _capi.lib(), 5, 72, 700
+    offsets, grad = torch.tensor([0, 100, 100, 420, 699, 700], dtype=torch.int32, device="cuda"), rand(60, (rows, n_out), dtype)
+    view = _capi.Tensor(data=grad.data_ptr(), precision=_capi.QMLP_HALF if dtype == torch.float16 else _capi.QMLP_BFLOAT16, ndim=2)
+    view.sizes[0], view.sizes[1], view.strides[0], view.strides[1] = rows, n_out, n_out, 1
+
+    def memory(n_in):
+        size, m = C.c_size_t(), _capi.Mx(matrices=e, rows=n_out, channels=n_in, codes=grad.data_ptr(), scales=grad.data_ptr())
+        assert lib.qmlp_mx_linear_adjoint_memory(C.byref(view), C.byref(m), 1, C.byref(size)) == 0
+        return size.value
+    for n_in in (1, 7, 9, 33, 63, 65, 127, 130, 255, 777):
+        assert memory(n_in) == memory((n_in + 7) // 8 * 8)
+        gradient_case(qmlp, rand(61 + n_in, (e, n_out, n_in)), grad, offsets)
