@@ -101,7 +101,10 @@ __global__ void __launch_bounds__(TILE_THREADS) mx_ranges_kernel(const __grid_co
 // What a matrix is divided by, 2^s, as 2^-s, for a whole block; written down (with whether its powers lie too far apart) by the block that has its first tile.
 __device__ __forceinline__ float dividedBy(const MxMatrix& q, const MxRanges& ranges, unsigned matrix, bool first, int tiles, int chunks, int codeBytes)
 {
-    constexpr int LOWEST = 127 - 23, HIGHEST = 127 + 13;   // of a block in half: 0.5 * 2^-23 is its smallest number, 6 * 2^13 below its largest
+    // Of a block in half: 0.5 * 2^-13 is its smallest normal number, 6 * 2^13 below its largest. Its subnormal ones reach down to -23, but a tensor core lines products up by their
+    // operands' exponents, of which a subnormal one has the lowest whatever its bits are, and cuts off what lies 2^25 below the largest: sums of numbers 2^-9 below it lose as many bits.
+    // (As they do from subnormal numbers of dy, in these products as in the 16-bit ones.)
+    constexpr int LOWEST = 127 - 13, HIGHEST = 127 + 13;
     int low, high;
     if (ranges.parts == 0) {
         const int2 all = rangeOf(q, static_cast<int>(matrix), 0, TILE_WARPS, tiles, chunks, codeBytes);
@@ -113,8 +116,8 @@ __device__ __forceinline__ float dividedBy(const MxMatrix& q, const MxRanges& ra
         low = __reduce_min_sync(0xffffffffu, f.x);
         high = __reduce_max_sync(0xffffffffu, f.y);
     }
-    // (-110: the power and its inverse are normal numbers, and the lowest scale still is in reach)
-    const int s = low >= LOWEST && high <= HIGHEST ? 0 : max(high - HIGHEST, -110);
+    // (-114: the power and its inverse are normal numbers, and the lowest scale still is in reach)
+    const int s = low >= LOWEST && high <= HIGHEST ? 0 : max(high - HIGHEST, -114);
     if (first && threadIdx.x == 0) {
         ranges.power[matrix] = powerOf(127 + s);
         ranges.apart[matrix] = low < LOWEST + s;

@@ -2,7 +2,7 @@
 //
 //   y_r = W_e q(x_r) + b_e          W_e: (channels out, channels in) in 4 bits; q: the row in 4 bits (mx.cuh)
 //   dx_r = W_e^T dy_r               (straight through q), W_e decoded to 16 bits and the product of expert_linear.cu. bfloat16 holds every 4-bit number; half holds
-//                                   37 neighbouring powers of two, so that W_e goes there divided by one where it leaves half's own (see mx_apart_kernel)
+//                                   27 neighbouring powers of two, so that W_e goes there divided by one where it leaves half's own (see mx_apart_kernel)
 //
 // Two kernels (one for small calls, and another for a few rows; the rules stand at the end). The first quantises the rows, tile by tile of 128 rows of one expert,
 // so that a tile's scales lie as the tensor core wants them. The second is the product D (128 x BN, fp32 in tensor memory) += A B, 256 channels in a step: codes by TMA in boxes of 64 rows x 128 bytes (256 channels), 128-byte
@@ -756,8 +756,8 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) mx_bias_join_kernel(const int*
 }
 
 // ---- input gradient of half rows where half does not hold a matrix -------------------------------------------------------------
-// Matrices whose powers of two reach from -23 to 13 are decoded to half as they are; others are divided by a power of two, which the product's sums are multiplied
-// with in fp32 (mx_ranges_kernel, dividedBy). What remains are matrices whose blocks lie more than 2^36 apart: their rows of dx are computed once more here,
+// Matrices whose powers of two lie between -13 and 13 are decoded to half as they are; others are divided by a power of two, which the product's sums are multiplied
+// with in fp32 (mx_ranges_kernel, dividedBy). What remains are matrices whose blocks lie more than 2^26 apart: their rows of dx are computed once more here,
 // dx_rc = sum over n of dy_rn (W_nc 2^E), codes decoded to fp32, sums in fp32. Few weights look like that, so this kernel is plain: a tile of 128 rows x 64 channels in
 // a block, 32 channels out at a time through shared memory. 131072 rows of half, 16 experts of 1024 -> 1024: 182 us where no matrix is apart, 815 with one of the 16, 8.6 ms with all;
 // finding it out costs every call of half rows 3 to 6 us (2.5 to 5 in front, less for small matrices, and 2 for this kernel's launch).

@@ -144,8 +144,8 @@ struct MxMatrix {
     unsigned char *codes, *scales;
 };
 cudaError_t launchMxQuantize(const MxMatrix& q, int type, const Rows& x, cudaStream_t stream);
-// How far the powers of two of each matrix reach. Half holds the numbers of 37 neighbouring powers (of two, those of its elements from 0.5 to 6) exactly, its
-// own range being -23 to 13: a matrix that leaves it is divided by a power of two, `power`, so that its largest numbers come to the upper end; `apart`: its powers
+// How far the powers of two of each matrix reach. Half has the elements (0.5 to 6) of 27 neighbouring powers of two as normal numbers, its
+// own being -13 to 13: a matrix that leaves it is divided by a power of two, `power`, so that its largest numbers come to the upper end; `apart`: its powers
 // lie farther apart than half holds. found: the lowest and highest power (+ 127) that a `parts`-th of a matrix has; (255, 0) for none.
 struct MxRanges {
     int parts;

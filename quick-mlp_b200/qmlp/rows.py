@@ -120,7 +120,7 @@ def mx_linear(x: torch.Tensor, weight: MXTensor, offsets: Optional[torch.Tensor]
     in 4 bits too (mx_quantize); rows of no expert are zeros. A single matrix (channels out, channels in) takes no offsets and a bias (channels out).
 
     x: (..., channels in) float16 or bfloat16, bias of the same type. Gradients of x and bias: the quantisation of x counts as the identity, the weights are
-    constants, exact over the whole range that mx_quantize gives (float16 gradients of matrices whose blocks lie more than 2^36 apart take many times as long)."""
+    constants, exact over the whole range that mx_quantize gives (float16 gradients of matrices whose blocks lie more than 2^26 apart take many times as long)."""
     if x.shape[-1:] != (weight.channels,):
         raise _capi.QmlpError(f"x must have the weight's {weight.channels} channels")
     if is_compiling() and _loaded():

@@ -108,3 +108,19 @@ def test_captured(qmlp):
         assert torch.equal(y, dx)
         seen.append(y.clone())
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_compiled_with_a_seed(qmlp):
+    """compiled, a layer with a seed counts on: the elements of the eager calls, and their gradients"""
+    torch._dynamo.reset()
+    layer, x, r = qmlp.FusedDropout(0.4, seed=3), rand(6, (200, 24)), rand(7, (200, 24))
+    compiled = torch.compile(layer, fullgraph=True, backend="aot_eager")
+    outs = []
+    for i, call in enumerate((compiled, layer, compiled, compiled)):
+        leaf = x.clone().requires_grad_()
+        y = call(leaf, r)
+        assert torch.equal(y, qmlp.dropout(x, 0.4, 3, i, residual=r)) and int(layer.step) == i + 1
+        outs.append((y, leaf, i))
+    for y, leaf, i in outs:
+        assert torch.equal(torch.autograd.grad(y, leaf, r)[0], qmlp.dropout(r, 0.4, 3, i))
+    torch._dynamo.reset()

@@ -207,3 +207,19 @@ def test_gradient_of_odd_widths(qmlp, dtype):
     for n_in in (1, 7, 9, 33, 63, 65, 127, 130, 255, 777):
         assert memory(n_in) == memory((n_in + 7) // 8 * 8)
         gradient_case(qmlp, rand(61 + n_in, (e, n_out, n_in)), grad, offsets)
+
+
+@pytest.mark.parametrize("power", [-40, -23, -22, -20, -17, -14, -13, 0, 13, 14, 20])
+def test_gradient_sums_keep_their_bits(qmlp, power):
+    """large terms cancel and leave small ones, which count whatever the matrix' magnitude: sums of whole numbers of units, up to 2^21 of them, exact in fp32"""
+    n_in, rows = 64, 130
+    w = torch.zeros((4, n_in), device="cuda")
+    w[0], w[1], w[2], w[3] = 4.0, 4.0, 0.5, 1.0
+    w[2, ::32] = w[3, ::32] = 4.0      # (every block has the power `power`)
+    w = w * 2.0 ** power
+    unit = 2.0 ** min(max(-7, -power - 4), 4)
+    grad = torch.tensor([[1024.0, -1024.0, 3 / 256, 5 / 256]], device="cuda").expand(rows, 4) * unit
+    grad = grad.half()
+    assert (grad[0].abs() >= 2.0 ** -14).all()      # (normal numbers)
+    dx, want = gradient_case(qmlp, w, grad)
+    assert torch.equal(dx.double(), want.half().double())
